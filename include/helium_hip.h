@@ -454,6 +454,33 @@ int he_pool_end_scope(uint64_t scope);
 int he_pool_allocate(size_t bytes, uint64_t scope, void** ptr, he_block* block);
 int he_pool_release(void* ptr, const he_block* block, uint64_t scope);
 
+/* ==================================================================================================
+ * 8. Group norm with an activation - what a training step normalises with where its batches are too small for batch norm's
+ *    statistics (helium/src/modules/batch_norm.rs). No counterpart in the reference.
+ * ================================================================================================== */
+typedef struct he_group_norm_s* he_group_norm_t;
+enum { HE_ACT_NONE = 0, HE_ACT_RELU = 1, HE_ACT_SILU = 2 };
+
+/* x is [batch, pixels, channels] (NHWC), row-major and packed; `groups` divides the channels. Over the pixels * (channels / groups)
+ * values of a sample's group: xh = (x - mean) * rstd, rstd = 1 / sqrt(variance + epsilon), z = gamma[c] * xh + beta[c], y = act(z):
+ * z, max(z, 0) or z * sigmoid(z). dtype: HE_F32, HE_BF16 or HE_F16, of x, y and their gradients; param_dtype: of gamma and beta,
+ * HE_F32 or dtype. Arithmetic and sums are f32, y is rounded once. batch may be 0 (then a call writes nothing, but for the
+ * parameters' gradients, which are zero). Compiles the kernels; needs no device. */
+int he_group_norm_create(he_group_norm_t* norm, int64_t batch, int64_t pixels, int64_t channels, int64_t groups, int dtype, int param_dtype,
+                         int activation, float epsilon);
+/* mean and rstd [batch, groups] are what the backward pass reads; each may be NULL where there is none. y may be x. Tensors are
+ * aligned to 16 bytes, or to the largest power of two that divides a pixel's bytes where that is less. The first call on a
+ * stream allocates scratch for it, later ones allocate nothing; calls on several streams may overlap. */
+int he_group_norm_forward(he_group_norm_t norm, const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
+                          he_stream_t stream);
+/* The gradients of x (of its type; dx may be dy or x), gamma and beta ([channels], f32, summed over the batch in a fixed order). */
+int he_group_norm_backward(he_group_norm_t norm, const void* dy, const void* x, const void* gamma, const void* beta, const float* mean,
+                           const float* rstd, void* dx, float* dgamma, float* dbeta, he_stream_t stream);
+/* The generated HIP source, and how forward and backward are cut (a line each). */
+const char* he_group_norm_source(he_group_norm_t norm);
+const char* he_group_norm_describe(he_group_norm_t norm);
+int he_group_norm_destroy(he_group_norm_t norm);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,124 @@
+"""Group norm without a GPU: the oracle against differences, the generated kernels under emulation (host AddressSanitizer
+checks every access) against the oracle, and what the entry points refuse."""
+import ctypes
+import re
+
+import numpy as np
+import pytest
+
+import helium_amd as ha
+from cpu_emul import run_kernel
+from group_norm_cases import EPSILON, SHAPES, check_backward, check_forward, inputs, to_f32
+from helium_amd import _ffi
+from oracle import group_norm as oracle
+
+
+@pytest.mark.parametrize("activation", ["none", "silu", "relu"])
+def test_the_oracles_gradients_are_those_of_its_forward_pass(activation):
+    rng = np.random.default_rng(5)
+    n, p, c, groups = 2, 7, 12, 3
+    x, dy = rng.standard_normal((2, n, p, c))
+    gamma, beta = 1 + 0.3 * rng.standard_normal(c), 0.3 * rng.standard_normal(c)
+    mean, rstd = oracle.statistics(x, groups, EPSILON)
+    loss = lambda x, gamma, beta: (oracle.forward(x, gamma, beta, groups, activation, EPSILON)[0] * dy).sum()  # noqa: E731
+    got = oracle.backward(dy, x, gamma, beta, mean, rstd, activation)
+    h = 1e-6
+    for k, (v, gradient) in enumerate(zip((x, gamma, beta), got)):
+        for at in rng.choice(v.size, 12, replace=False):
+            step = np.zeros(v.size)
+            step[at] = h
+            step = step.reshape(v.shape)
+            up, down = [[x, gamma, beta] for _ in range(2)]
+            up[k], down[k] = v + step, v - step
+            # (the difference of two sums of 168 values near one, over 2 h: 1e-14 / 2e-6; curvature adds h^2)
+            assert abs((loss(*up) - loss(*down)) / (2 * h) - gradient.reshape(-1)[at]) < 1e-6
+
+
+def launch(norm, backward):
+    """Grid, threads, parts of a sample and text of the forward or the backward pass."""
+    line = norm.description.splitlines()[backward]
+    return [int(re.search(k + r"=(\d+)", line).group(1)) for k in ("grid", "threads", "chunks")] + ["#define BATCH" + norm.source.split("#define BATCH")[1 + backward]]
+
+
+def forward_emulated(norm, shape, host):
+    n, p, c, groups = shape
+    grid, threads, chunks, text = launch(norm, False)
+    y, stat = np.empty((n, p, c), host["x"].dtype), np.empty((n, groups), np.float32)
+    parts, = run_kernel(text, "group_norm_stats", grid, threads, [(host["x"], 0), (np.empty((n, groups, chunks, 2), np.float32), 1)])
+    stats, mean, rstd = run_kernel(text, "group_norm_merge", (n * groups + 3) // 4, 256,
+                                   [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)])
+    y, = run_kernel(text, "group_norm_apply", grid, threads, [(host["x"], 0), (host["gamma"], 0), (host["beta"], 0), (stats, 0), (y, 1)])
+    return y, mean, rstd
+
+
+def backward_emulated(norm, shape, host, mean, rstd):
+    n, p, c, groups = shape
+    grid, threads, chunks, text = launch(norm, True)
+    given = [(host[k], 0) for k in ("dy", "x", "gamma", "beta")] + [(mean, 0), (rstd, 0)]
+    parts, = run_kernel(text, "group_norm_sums", grid, threads, given + [(np.empty((n * chunks, 2, c), np.float32), 1)])
+    samples, sums = run_kernel(text, "group_norm_fold", (n * groups + 3) // 4, 256,
+                               [(parts, 0), (host["gamma"], 0), (np.empty((n, 2, c), np.float32), 1), (np.empty((n, groups, 2), np.float32), 1)])
+    return run_kernel(text, "group_norm_gradient", grid + (c + 63) // 64, threads,
+                      given + [(samples, 0), (sums, 0), (np.empty((n, p, c), host["x"].dtype), 1), (np.empty(c, np.float32), 1), (np.empty(c, np.float32), 1)])
+
+
+CASES = [(shape, ("f32", "bf16", "f16")[k % 3], ("none", "relu", "silu")[(k // 2) % 3]) for k, shape in enumerate(SHAPES)]
+
+
+@pytest.mark.parametrize("shape,dtype,activation", CASES)
+def test_the_kernels_match_the_oracle(shape, dtype, activation):
+    param_dtype = dtype if shape[1] % 2 else "f32"
+    norm = ha.GroupNorm(*shape, dtype, param_dtype=param_dtype, activation=activation, epsilon=EPSILON)
+    host, v, mean, rstd = inputs(shape, dtype, param_dtype, activation, seed=shape[1])
+    y, got_mean, got_rstd = forward_emulated(norm, shape, host)
+    check_forward(shape, dtype, activation, v, to_f32(y, dtype), got_mean, got_rstd)
+    dx, dgamma, dbeta = backward_emulated(norm, shape, host, mean, rstd)
+    check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
+@pytest.mark.parametrize("kwargs,says", [
+    (dict(channels=30, groups=4), "do not divide"),
+    (dict(groups=0), "groups 0"),
+    (dict(pixels=0), "pixels 0"),
+    (dict(batch=-1), "batch -1"),
+    (dict(epsilon=-1.0), "epsilon"),
+    (dict(epsilon=float("nan")), "epsilon"),
+    (dict(dtype="u32"), "dtype u32"),
+    (dict(dtype="bf16", param_dtype="f16"), "parameters are f32 or of the tensor's type"),
+    (dict(channels=32768, groups=1), "at most 16384"),
+])
+def test_what_cannot_be_normalised_is_refused(kwargs, says):
+    given = dict(batch=2, pixels=9, channels=32, groups=4, dtype="f32", epsilon=1e-5)
+    with pytest.raises(ha.HeliumError, match=says):
+        ha.GroupNorm(**{**given, **kwargs})
+
+
+def test_unknown_activations_and_null_handles_are_refused():
+    with pytest.raises(ValueError):
+        ha.GroupNorm(1, 1, 8, 1, "f32", activation="tanh")
+    h = ctypes.c_void_p()
+    assert _ffi.lib.he_group_norm_create(ctypes.byref(h), 1, 1, 8, 1, _ffi.F32, _ffi.F32, 7, 1e-5) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_group_norm_create(None, 1, 1, 8, 1, _ffi.F32, _ffi.F32, 0, 1e-5) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_group_norm_forward(None, *[None] * 7) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_group_norm_backward(None, *[None] * 10) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_group_norm_destroy(None) == _ffi.OK
+
+
+def test_null_and_misaligned_operands_are_refused_before_any_launch():
+    norm = ha.GroupNorm(1, 4, 16, 2, "bf16")
+    good = 4096  # (an address that nothing follows: every call below is refused)
+    for bad in (None, good + 8):
+        with pytest.raises(ha.HeliumError, match="aligned"):
+            norm.forward(bad, good, good, good)
+        with pytest.raises(ha.HeliumError, match="aligned"):
+            norm.backward(good, good, good, good, good, good, bad, good, good)
+    with pytest.raises(ha.HeliumError, match="gamma or beta"):
+        norm.forward(good, None, good, good)
+    with pytest.raises(ha.HeliumError, match="needs the statistics"):
+        norm.backward(good, good, good, good, None, good, good, good, good)
+    with pytest.raises(ha.HeliumError, match="gradients are null"):
+        norm.backward(good, good, good, good, good, good, good, None, good)
+
+
+def test_an_empty_batch_needs_no_operands():
+    ha.GroupNorm(0, 4, 16, 2, "bf16").forward(None, None, None, None)
