@@ -6,5 +6,6 @@ from .permute import PermuteDims  # noqa: F401
 from . import allocator, backend, configs, fusion, fusion_search, ir, kernels  # noqa: F401
 from .group_norm import GroupNorm  # noqa: F401
 from .kernels import TileKernel  # noqa: F401
+from .muon import Muon  # noqa: F401
 
-__all__ = ["HeliumError", "device", "DeviceBuffer", "Event", "Stream", "PermuteDims", "TileKernel", "GroupNorm", "ir", "fusion", "kernels", "backend", "configs", "fusion_search"]
+__all__ = ["HeliumError", "device", "DeviceBuffer", "Event", "Stream", "PermuteDims", "TileKernel", "GroupNorm", "Muon", "ir", "fusion", "kernels", "backend", "configs", "fusion_search"]

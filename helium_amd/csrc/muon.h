@@ -1,0 +1,75 @@
+// Orthogonalised updates of a group of matrices (Newton-Schulz products) and the optimizer step built on them.
+#pragma once
+#include <array>
+#include <map>
+#include <memory>
+#include <mutex>
+#include <string>
+#include <vector>
+
+#include "common.h"
+#include "rtc.h"
+
+namespace he {
+
+struct MuonProblem {
+    std::vector<std::array<int64_t, 2>> shapes;  // rows, columns
+    int dtype = HE_F32;                          // of the matrices that come in (and of orthogonalised ones that go out)
+    bool split = true;                           // f32_f32: f16 operands in two parts; otherwise in one
+    int steps = 5;
+};
+
+// What the kernels know of a matrix; the device holds an array of these. Offsets are bytes in the workspace. The smaller extent
+// is m, the larger n, both padded to whole tiles with zeros (which every product leaves zeros): X is [mp][np], XT its transpose.
+struct MuonMatrix {
+    uint32_t rows, cols, mp, np;
+    uint32_t tall, first_part, parts;  // parts: shares of the sum of squares
+    float shape_scale;                 // sqrt(max(1, rows / cols))
+    uint64_t x[2], xt[2][2], a[2], b[2];  // planes: [high, low]; xt twice, in turn
+};
+struct MuonTile {
+    uint32_t matrix, i, j;
+};
+
+struct MuonStep {
+    float learning_rate, momentum, weight_decay;
+    int32_t nesterov;
+};
+
+class Muon {
+public:
+    explicit Muon(const MuonProblem& pr);
+    ~Muon();
+    void orthogonalize(const void* const* in, void* const* out, hipStream_t stream);
+    void step(const void* const* grads, const float* const* momenta, const float* const* weights, float* const* new_momenta,
+              float* const* new_weights, const MuonStep& how, hipStream_t stream);
+    const std::string& source() const { return source_; }
+    const std::string& describe() const { return describe_; }
+    size_t count() const { return pr_.shapes.size(); }
+    // The tables the kernels read, as bytes: 0 matrices, 1 tiles of symmetric products, 2 tiles of whole ones, 3 shares of the
+    // sums of squares, 4 blocks of the conversions.
+    const std::vector<char>& table(int which) const { return tables_[which]; }
+    size_t workspace_bytes() const { return workspace_bytes_; }
+
+private:
+    struct Buffers {
+        char* tables = nullptr;
+        char* workspace = nullptr;
+    };
+    Buffers buffers(hipStream_t stream);
+    void step_or_not(const void* const* in, const float* const* momenta, const float* const* weights, float* const* new_momenta, void* const* out,
+                     const MuonStep* how, hipStream_t stream);
+    void products(char* ws, char* tables, hipStream_t stream);
+    MuonProblem pr_;
+    std::vector<MuonMatrix> matrices_;
+    std::vector<char> tables_[5];
+    size_t table_at_[5] = {}, table_bytes_ = 0, workspace_bytes_ = 0;
+    std::array<uint32_t, 5> table_size_{};
+    std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 3 and 4
+    std::string source_, describe_;
+    std::unique_ptr<JitKernel> norm_, convert_, gram_, square_, apply_, finish_, norm_step_, convert_step_, finish_step_;
+    std::mutex mu_;
+    std::map<hipStream_t, Buffers> per_stream_;
+};
+
+}  // namespace he

@@ -481,6 +481,36 @@ const char* he_group_norm_source(he_group_norm_t norm);
 const char* he_group_norm_describe(he_group_norm_t norm);
 int he_group_norm_destroy(he_group_norm_t norm);
 
+/* ==================================================================================================
+ * 9. Orthogonalised updates (the Muon optimizer) for the matrices of a model: layers as they are, a convolution's filter
+ *    [out, kh, kw, in] as out x (kh * kw * in). What Sgd (helium/src/optimizer/sgd.rs) is for every parameter alike. No counterpart
+ *    in the reference.
+ * ================================================================================================== */
+typedef struct he_muon_s* he_muon_t;
+
+/* A group of `count` matrices of any extents, shapes[2 k] x shapes[2 k + 1], row-major and packed; a call treats all of them with one
+ * launch per stage. dtype: HE_F32, HE_BF16 or HE_F16, of the matrices that come in. The orthogonalised form of U: X = U / (|U| + 1e-7)
+ * (Frobenius norm, transposed where there are more rows than columns), then `steps` times S = X X^T, X = a X + (b S + c S S) X with
+ * (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value to about 1 (0.7 to 1.2 in five steps where it was at least
+ * 1/100 of the norm; 0 stays 0). precision: HE_PREC_F32_F32 (results as of f32 products) or HE_PREC_F16_F32 (f16 operands,
+ * f32 sums; results good to about 3 digits, for gradients in 16 bits). Compiles the kernels; needs no device. */
+int he_muon_create(he_muon_t* muon, const int64_t* shapes, int count, int dtype, int precision, int steps);
+/* out[k] (of `dtype`) is the orthogonalised in[k]; it may be in[k]. Lists of `count` device addresses in host memory, aligned to 16
+ * bytes. The first call on a stream allocates workspace for it, later ones allocate nothing; calls on several streams may overlap. */
+int he_muon_orthogonalize(he_muon_t muon, const void* const* in, void* const* out, int count, he_stream_t stream);
+/* One optimizer step per matrix: M' = momentum M + G, U = nesterov ? G + momentum M' : M', O = U orthogonalised,
+ * W' = (1 - learning_rate weight_decay) W - learning_rate sqrt(max(1, rows / columns)) O. Gradients are of `dtype`, momenta and weights
+ * f32; new_momenta[k] may be momenta[k] and new_weights[k] weights[k]. */
+int he_muon_step(he_muon_t muon, const void* const* gradients, const float* const* momenta, const float* const* weights,
+                 float* const* new_momenta, float* const* new_weights, int count, float learning_rate, float momentum, float weight_decay,
+                 int nesterov, he_stream_t stream);
+/* The generated HIP source, how the products are cut, and the tables the kernels read (0 matrices, 1 tiles of the symmetric products,
+ * 2 of the whole ones, 3 shares of the sums of squares, 4 blocks of the conversions), for inspection and tests. */
+const char* he_muon_source(he_muon_t muon);
+const char* he_muon_describe(he_muon_t muon);
+int he_muon_table(he_muon_t muon, int which, void* data, size_t capacity, size_t* bytes);
+int he_muon_destroy(he_muon_t muon);
+
 #ifdef __cplusplus
 }
 #endif

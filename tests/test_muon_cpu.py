@@ -1,0 +1,167 @@
+"""Orthogonalised updates without a GPU: the oracle's properties, the kernels under emulation (host AddressSanitizer checks every
+access) against the oracle, and what the entry points refuse."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import helium_amd as ha
+from cpu_emul import run_kernel
+from helium_amd import _ffi
+from muon_cases import SHAPES, check, matrix, to_f32, to_storage
+from oracle import muon as oracle
+
+MATRIX = np.dtype([("rows", "u4"), ("cols", "u4"), ("mp", "u4"), ("np", "u4"), ("tall", "u4"), ("first_part", "u4"), ("parts", "u4"),
+                   ("shape_scale", "f4"), ("x", "u8", 2), ("xt", "u8", (2, 2)), ("a", "u8", 2), ("b", "u8", 2)])
+TILE = np.dtype([("matrix", "u4"), ("i", "u4"), ("j", "u4")])
+
+
+def test_singular_values_go_where_the_polynomial_takes_them():
+    rng = np.random.default_rng(1)
+    for shape in ((20, 33), (33, 20), (12, 12)):
+        u, s, vt = np.linalg.svd(rng.standard_normal(shape), full_matrices=False)
+        got = oracle.orthogonalize((u * s) @ vt)
+        want = (u * oracle.singular_values_after(s / (np.linalg.norm(s) + oracle.NORM_FLOOR))) @ vt
+        assert np.abs(got - want).max() < 1e-10
+
+
+def test_the_iteration_never_leaves_the_range_that_the_kernels_operands_are_scaled_for():
+    s = np.linspace(0, 1, 200001)
+    for _ in range(40):
+        s = oracle.singular_values_after(s, 1)
+        assert s.min() >= 0 and s.max() < 1.21
+    a, b, c = oracle.COEFFICIENTS
+    t = np.linspace(0, 1.21, 10001) ** 2
+    assert np.abs(b * t + c * t * t).max() < 2.82 and 2.82 * 8192 < 65504 and 1.21 * 4096 < 65504 and 1.4642 * 8192 < 65504
+
+
+def test_five_steps_bring_the_documented_range_near_one():
+    s = oracle.singular_values_after(np.linspace(0.01, 1, 100001))
+    assert s.min() > 0.65 and s.max() < 1.21
+
+
+@pytest.mark.parametrize("kind", ["normal", "low_rank", "one_entry", "zero"])
+@pytest.mark.parametrize("split", [True, False])
+def test_the_documented_arithmetic_is_within_the_tests_own_tolerance(kind, split):
+    for k, shape in enumerate(SHAPES):
+        u = matrix(shape, kind, 1 + k).astype(np.float32)
+        check(oracle.modelled(u, split), u, "f32", split)
+
+
+SHFL = r"""
+static double g_shfl64[1024];
+static inline double emu_shfl64(double v, int mask) {
+    unsigned tid = threadIdx.x;
+    g_shfl64[tid] = v;
+    WAVE_BAR();
+    double r = g_shfl64[(tid & ~63u) | ((tid & 63u) ^ (unsigned)mask)];
+    WAVE_BAR();
+    return r;
+}
+#define SHFL_XOR_F64(v, m) emu_shfl64(v, m)
+"""
+
+
+def emulated(shapes, dtype, split, steps, in_storage, step=None):
+    """The launches of a call, one after the other. `step`: (momenta, weights, learning rate, mu, decay, nesterov)."""
+    muon = ha.Muon(shapes, dtype, precision="f32_f32" if split else "f16_f32", steps=steps)
+    mats, lower, whole, parts, blocks = (np.frombuffer(muon.table(t), MATRIX if t == 0 else TILE) for t in range(5))
+    workspace = int(muon.description.split("workspace=")[1].split()[0])
+    threads = int(muon.description.split("threads=")[1].split()[0])
+    names = [f"in{k}" for k in range(len(shapes))]
+    fill = "".join(f"o.in[{k}] = in{k}; " for k in range(len(shapes)))
+    params = ", ".join(f"const elem_t* in{k}" for k in range(len(shapes)))
+    if step:
+        fill += "".join(f"o.momentum[{k}] = m{k}; o.new_momentum[{k}] = nm{k}; o.weight[{k}] = w{k}; " for k in range(len(shapes)))
+        fill += "o.learning_rate = %.9gf; o.mu = %.9gf; o.weight_decay = %.9gf; o.nesterov = %d; " % step[2:]
+        params += "".join(f", const float* m{k}, float* nm{k}, const float* w{k}" for k in range(len(shapes)))
+    out_type = "float" if step else "elem_t"
+    outs = ", ".join(f"{out_type}* out{k}" for k in range(len(shapes)))
+    fill_out = "".join(f"o.out[{k}] = out{k}; " for k in range(len(shapes)))
+    which = "true" if step else "false"
+    wrappers = f"""
+extern "C" void emu_norm(const Matrix* m, const Tile* t, double* s, {params}) {{ Operands o{{}}; {fill} norm_part<{which}>(m, t, s, o); }}
+extern "C" void emu_convert(const Matrix* m, const Tile* t, const double* s, char* ws, {params}) {{ Operands o{{}}; {fill} convert_block<{which}>(m, t, s, ws, o); }}
+extern "C" void emu_finish(const Matrix* m, const Tile* t, const char* ws, {params}, {outs}) {{ Operands o{{}}; {fill} {fill_out} finish_block<{which}>(m, t, ws, o); }}
+extern "C" void emu_gram(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<GRAM>(m, t, ws, *turn); }}
+extern "C" void emu_square(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<SQUARE>(m, t, ws, *turn); }}
+extern "C" void emu_apply(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<APPLY>(m, t, ws, *turn); }}
+"""
+    text = SHFL + muon.source + wrappers
+    given = [(a, 0) for a in in_storage]
+    sums = np.zeros(len(parts))
+    if step:
+        momenta, weights = step[0], step[1]
+        for m, w in zip(momenta, weights):
+            given += [(m, 0), (np.empty_like(m), 1), (w, 0)]
+    got = run_kernel(text, "emu_norm", len(parts), 256, [(mats, 0), (parts, 0), (sums, 1)] + given)
+    sums, new_momenta = got[0], got[1:]
+    if step:  # from here on the new momenta are inputs
+        given = [(a, 0) for a in in_storage] + [b for m, n, w in zip(momenta, new_momenta, weights) for b in ((m, 0), (n, 0), (w, 0))]
+    ws, = run_kernel(text, "emu_convert", len(blocks), 256, [(mats, 0), (blocks, 0), (sums, 0), (np.empty(workspace, np.uint8), 1)] + given)
+    for k in range(steps):
+        turn = np.array([k & 1], np.uint32)
+        for entry, tiles in (("emu_gram", lower), ("emu_square", lower), ("emu_apply", whole)):
+            ws, = run_kernel(text, entry, len(tiles), threads, [(mats, 0), (tiles, 0), (ws, 2), (turn, 0)])
+    outs = [np.empty(s, np.float32 if step else in_storage[0].dtype) for s in shapes]
+    return run_kernel(text, "emu_finish", len(blocks), 256, [(mats, 0), (blocks, 0), (ws, 0)] + given + [(o, 1) for o in outs]), new_momenta
+
+
+@pytest.mark.parametrize("dtype,split,steps", [("f32", True, 2), ("bf16", False, 2), ("f16", False, 1), ("f32", False, 3)])
+def test_the_kernels_match_the_oracle(dtype, split, steps):
+    shapes = [(5, 9), (70, 33), (1, 1), (40, 150)]
+    stored = [to_storage(matrix(s, "normal", 3), dtype) for s in shapes]
+    got, _ = emulated(shapes, dtype, split, steps, stored)
+    for g, s in zip(got, stored):
+        check(to_f32(g, dtype), to_f32(s, dtype), dtype, split, steps)
+
+
+@pytest.mark.parametrize("nesterov", [0, 1])
+def test_the_kernels_step_matches_the_oracles(nesterov):
+    shapes = [(6, 10), (20, 3)]
+    rng = np.random.default_rng(8)
+    grads = [to_storage(rng.standard_normal(s), "bf16") for s in shapes]
+    momenta, weights = ([rng.standard_normal(s).astype(np.float32) for s in shapes] for _ in range(2))
+    new_weights, new_momenta = emulated(shapes, "bf16", True, 2, grads, (momenta, weights, 0.1, 0.9, 0.02, nesterov))
+    for g, m, w, nw, nm in zip(grads, momenta, weights, new_weights, new_momenta):
+        want_w, want_m = oracle.step(to_f32(g, "bf16"), m, w, np.float32(0.1), np.float32(0.9), np.float32(0.02), nesterov, 2)
+        assert np.abs(nm - want_m).max() < 4 * 2.0 ** -24 * np.abs(want_m).max()
+        # the orthogonalised part is good to some 1e-6 of values up to 1.2, times 0.1 sqrt(rows / columns)
+        assert np.abs(nw - want_w).max() < 1e-5
+
+
+@pytest.mark.parametrize("shapes,dtype,precision,steps,says", [
+    ([(4, 0)], "f32", "f32_f32", 5, "matrix 0 is 4 x 0"),
+    ([(4, 4), (-1, 3)], "f32", "f32_f32", 5, "matrix 1 is -1 x 3"),
+    ([(40000, 40000)], "f32", "f32_f32", 5, "extents up to"),
+    ([(2 << 20, 4)], "f32", "f32_f32", 5, "extents up to"),
+    ([(4, 4)], "u32", "f32_f32", 5, "dtype u32"),
+    ([(4, 4)], "f32", "f32_f32", 0, "0 steps"),
+    ([(4, 4)], "f32", "f32_f32", 33, "33 steps"),
+    ([], "f32", "f32_f32", 5, "bad argument"),
+])
+def test_what_cannot_be_orthogonalised_is_refused(shapes, dtype, precision, steps, says):
+    with pytest.raises(ha.HeliumError, match=says):
+        ha.Muon(shapes, dtype, precision=precision, steps=steps)
+
+
+def test_operands_are_checked_before_any_launch():
+    muon = ha.Muon([(4, 4), (3, 5)], "f32")
+    good = 4096  # (an address that nothing follows: every call below is refused)
+    with pytest.raises(ha.HeliumError, match="takes 2 matrices, got 1"):
+        muon.orthogonalize([good], [good])
+    with pytest.raises(ValueError):
+        muon.orthogonalize([good, good], [good])
+    for bad in (None, good + 4):
+        with pytest.raises(ha.HeliumError, match="matrix 1 is null or not 16-byte aligned"):
+            muon.orthogonalize([good, bad], [good, good])
+        with pytest.raises(ha.HeliumError, match="matrix 0 is null or not 16-byte aligned"):
+            muon.step([good] * 2, [good] * 2, [good] * 2, [good] * 2, [bad, good], learning_rate=0.1)
+    with pytest.raises(ha.HeliumError, match="not finite"):
+        muon.step([good] * 2, [good] * 2, [good] * 2, [good] * 2, [good] * 2, learning_rate=float("nan"))
+    with pytest.raises(ValueError):
+        ha.Muon([(4, 4)], "f32", precision="bf16_f32")
+    h, shape = ctypes.c_void_p(), (ctypes.c_int64 * 2)(4, 4)
+    assert _ffi.lib.he_muon_create(ctypes.byref(h), shape, 1, _ffi.F32, 2, 5) == _ffi.ERR_INVALID   # bf16_f32
+    assert _ffi.lib.he_muon_orthogonalize(None, None, None, 0, None) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_muon_destroy(None) == _ffi.OK

@@ -1,0 +1,190 @@
+"""Orthogonalised updates and the optimizer step through the C ABI on the GPU, against the 64-bit oracle."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import helium_amd as ha
+from muon_cases import SHAPES, check, matrix, to_f32, to_storage
+from oracle import muon as oracle
+from test_group_norm_gpu import address, back, device
+
+pytestmark = pytest.mark.gpu
+
+LARGER = [(256, 256), (300, 1000), (1000, 300), (512, 4608), (777, 1203), (1024, 1024), (20, 5000), (5000, 20)]
+
+
+def orthogonalized(shapes, stored, dtype, precision, steps=5, in_place=False, muon=None, stream=None):
+    muon = muon or ha.Muon(shapes, dtype, precision=precision, steps=steps)
+    given = [device(s) for s in stored]
+    out = given if in_place else [device(np.zeros_like(s)) for s in stored]
+    muon.orthogonalize([address(g) for g in given], [address(o) for o in out], stream=stream)
+    if stream is not None:
+        stream.synchronize()
+    return [back(o, s) for o, s in zip(out, stored)]
+
+
+@pytest.mark.parametrize("dtype,precision", [("f32", "f32_f32"), ("f32", "f16_f32"), ("bf16", "f16_f32"), ("f16", "f16_f32"), ("bf16", "f32_f32")])
+@pytest.mark.parametrize("kind", ["normal", "low_rank", "one_entry", "zero"])
+def test_small_matrices_as_one_group(gpu, dtype, precision, kind):
+    stored = [to_storage(matrix(s, kind, 1 + k), dtype) for k, s in enumerate(SHAPES)]
+    for g, s in zip(orthogonalized(SHAPES, stored, dtype, precision), stored):
+        check(to_f32(g, dtype), to_f32(s, dtype), dtype, precision == "f32_f32")
+
+
+@pytest.mark.parametrize("dtype,precision", [("f32", "f32_f32"), ("f32", "f16_f32"), ("bf16", "f16_f32")])
+@pytest.mark.parametrize("shape", LARGER)
+def test_larger_matrices_by_themselves(gpu, shape, dtype, precision):
+    stored = [to_storage(matrix(shape, "normal", 2), dtype)]
+    got, = orthogonalized([shape], stored, dtype, precision)
+    check(to_f32(got, dtype), to_f32(stored[0], dtype), dtype, precision == "f32_f32")
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4])
+def test_any_number_of_steps(gpu, steps):
+    shapes = [(40, 70), (70, 40)]
+    stored = [to_storage(matrix(s, "normal", 3), "f32") for s in shapes]
+    for precision in ("f32_f32", "f16_f32"):
+        for g, s in zip(orthogonalized(shapes, stored, "f32", precision, steps), stored):
+            check(g, s, "f32", precision == "f32_f32", steps)
+
+
+def test_more_matrices_than_one_launch_takes_operands(gpu):
+    shapes = [(1 + 3 * k % 37, 1 + 7 * k % 41) for k in range(70)]
+    stored = [to_storage(matrix(s, "normal", k), "f32") for k, s in enumerate(shapes)]
+    for g, s in zip(orthogonalized(shapes, stored, "f32", "f32_f32"), stored):
+        check(g, s, "f32", True)
+
+
+def test_a_matrix_of_a_group_has_the_bits_it_has_by_itself(gpu):
+    shapes = [(64, 576), (100, 30), (257, 300)]
+    stored = [to_storage(matrix(s, "normal", 4), "f32") for s in shapes]
+    for g, shape, s in zip(orthogonalized(shapes, stored, "f32", "f32_f32"), shapes, stored):
+        check(g, s, "f32", True)
+        alone, = orthogonalized([shape], [s], "f32", "f32_f32")
+        check(alone, s, "f32", True)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e25])
+def test_the_norm_neither_vanishes_nor_overflows(gpu, scale):
+    """Squares of these are outside f32. (Norms far below the 1e-7 that is added leave a small multiple of U.)"""
+    u = (matrix((48, 60), "normal", 5) * scale).astype(np.float32)
+    got, = orthogonalized([u.shape], [u], "f32", "f32_f32")
+    want = oracle.orthogonalize(u)
+    if scale > 1:
+        check(got, u, "f32", True)
+    else:  # f16 parts of values scaled by 4096 end at 2^-24, so at 2^-37 of what comes out a few hundred times larger
+        assert np.abs(got - want).max() <= 1e-5 * np.abs(want).max() + 500 * 2.0 ** -37
+
+
+def test_what_is_not_finite_stays_in_its_matrix(gpu):
+    shapes = [(20, 30), (33, 20), (16, 16)]
+    stored = [to_storage(matrix(s, "normal", 6), "f32") for s in shapes]
+    clean = orthogonalized(shapes, stored, "f32", "f32_f32")
+    for bad in (np.nan, np.inf):
+        spoilt = [s.copy() for s in stored]
+        spoilt[1][4, 5] = bad
+        got = orthogonalized(shapes, spoilt, "f32", "f32_f32")
+        assert np.array_equal(got[0], clean[0]) and np.array_equal(got[2], clean[2])
+        assert np.isnan(got[1]).all()
+
+
+def test_results_may_take_the_operands_place_and_repeat(gpu):
+    shapes = [(64, 576), (100, 30)]
+    muon = ha.Muon(shapes, "bf16", precision="f16_f32")
+    stored = [to_storage(matrix(s, "normal", 7), "bf16") for s in shapes]
+    want = orthogonalized(shapes, stored, "bf16", None, muon=muon)
+    other = [to_storage(matrix(s, "low_rank", 8), "bf16") for s in shapes]
+    stream = ha.Stream()
+    for again in range(3):
+        orthogonalized(shapes, other, "bf16", None, muon=muon)   # whatever the workspace held before
+        for in_place in (False, True):
+            for a, b in zip(orthogonalized(shapes, stored, "bf16", None, muon=muon, in_place=in_place, stream=stream if again else None), want):
+                assert np.array_equal(a, b)
+
+
+def test_streams_that_overlap_have_workspace_of_their_own(gpu):
+    shapes = [(256, 300), (90, 90)]
+    muon = ha.Muon(shapes, "f32")
+    stored = [[to_storage(matrix(s, "normal", k), "f32") for s in shapes] for k in (9, 10)]
+    want = [orthogonalized(shapes, s, "f32", None, muon=muon) for s in stored]
+    streams = [ha.Stream(), ha.Stream()]
+    bufs = [([device(m) for m in s], [device(np.zeros_like(m)) for m in s]) for s in stored]
+    for _ in range(5):
+        for (given, out), stream in zip(bufs, streams):
+            muon.orthogonalize([address(g) for g in given], [address(o) for o in out], stream=stream)
+    for (_, out), stream, w, s in zip(bufs, streams, want, stored):
+        stream.synchronize()
+        for o, ww, m in zip(out, w, s):
+            assert np.array_equal(back(o, m), ww)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("nesterov", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_the_step_matches_the_oracles(gpu, dtype, nesterov, in_place):
+    shapes = [(64, 576), (1000, 100), (3, 5), (130, 130)] + [(20, 7)] * 40
+    rng = np.random.default_rng(11)
+    grads = [to_storage(rng.standard_normal(s), dtype) for s in shapes]
+    momenta, weights = ([rng.standard_normal(s).astype(np.float32) for s in shapes] for _ in range(2))
+    muon = ha.Muon(shapes, dtype)
+    g, m, w = ([device(a) for a in v] for v in (grads, momenta, weights))
+    nm, nw = (m, w) if in_place else ([device(np.zeros_like(a)) for a in v] for v in (momenta, weights))
+    lists = [[address(b) for b in v] for v in (g, m, w, nm, nw)]
+    muon.step(*lists, learning_rate=0.1, momentum=0.9, weight_decay=0.02, nesterov=nesterov)
+    for k, shape in enumerate(shapes):
+        want_w, want_m = oracle.step(to_f32(grads[k], dtype), momenta[k], weights[k], np.float32(0.1), np.float32(0.9), np.float32(0.02), nesterov)
+        got_m, got_w = back(nm[k], momenta[k]), back(nw[k], weights[k])
+        assert np.abs(got_m - want_m).max() <= 4 * 2.0 ** -24 * np.abs(want_m).max()
+        # what the orthogonalised update may be off (the tests above), times its factor, and f32 rounding of the weight
+        u = to_f32(grads[k], dtype).astype(np.float64) + 0.9 * want_m if nesterov else want_m
+        off = np.linalg.norm(oracle.modelled(u, True) - oracle.orthogonalize(u))
+        allowed = 0.1 * np.sqrt(max(1, shape[0] / shape[1])) * (4 * off + 1e-6 * np.sqrt(min(shape))) + 4 * 2.0 ** -24 * np.linalg.norm(want_w)
+        assert np.linalg.norm(got_w - want_w) <= allowed, (shape, np.linalg.norm(got_w - want_w), allowed)
+
+
+def test_a_captured_step_replays(gpu):
+    """A step in place, recorded into a HIP graph (after one call that allocates the stream's workspace), replayed with other work in
+    between: the same weights as eager steps."""
+    torch = pytest.importorskip("torch")
+    shapes = [(64, 576), (300, 40)]
+    rng = np.random.default_rng(12)
+    host = [[rng.standard_normal(s).astype(np.float32) for s in shapes] for _ in range(3)]
+    muon = ha.Muon(shapes, "f32")
+
+    def fresh():
+        return [[torch.from_numpy(a.copy()).cuda() for a in v] for v in host]
+
+    def one(g, m, w, stream=None):
+        at = lambda v: [x.data_ptr() for x in v]  # noqa: E731
+        muon.step(at(g), at(m), at(w), at(m), at(w), learning_rate=0.05, stream=stream)
+
+    g, m, w = fresh()
+    eager = []
+    for _ in range(4):
+        one(g, m, w)
+        torch.cuda.synchronize()
+        eager.append([x.cpu().numpy() for x in m + w])
+    s = ha.Stream()
+    stream = torch.cuda.ExternalStream(ha._ffi.lib.he_stream_raw(s.handle))
+    one(*fresh(), stream=s)
+    s.synchronize()
+    g, m, w = fresh()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        one(g, m, w, stream=s)
+    for k in range(4):
+        orthogonalized([(30, 30)], [np.ones((30, 30), np.float32)], "f32", "f32_f32")
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(m + w, eager[k]):
+            assert np.array_equal(a.cpu().numpy(), b)
+
+
+def test_addresses_come_from_any_kind_of_buffer(gpu):
+    u = matrix((12, 20), "normal", 13).astype(np.float32)
+    a, b = ha.DeviceBuffer.from_numpy(u), ha.DeviceBuffer(u.nbytes)
+    muon = ha.Muon([u.shape], "f32")
+    muon.orthogonalize([a], [ctypes.c_void_p(b.ptr.value).value])
+    check(b.to_numpy(np.float32, u.shape), u, "f32", True)
