@@ -39,13 +39,27 @@ typedef float elem_t;
 #define LDS_AS __attribute__((address_space(3)))
 #define GLOBAL_AS __attribute__((address_space(1)))
 #endif
+#ifndef WAIT_LOADS
+#define WAIT_LOADS(n) (0x0070 | ((n) & 15) | (((n) >> 4) << 14))   /* vmcnt(n), and lgkmcnt(0): this wave's reads of LDS are done */
+#endif
+#ifndef KERNEL_ATTRS
+#define KERNEL_ATTRS __attribute__((amdgpu_waves_per_eu(2, 2)))
+#endif
+#ifndef HE_WS_STORE
+// Partial results on their way to another workgroup: device-scope accesses go past the L2 of the XCD they come from, so what is
+// written this way and waited for before a ticket is taken is there for whoever sees the ticket.
+#define HE_WS_STORE(p, v) __hip_atomic_store((p), (v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+#define HE_WS_LOAD(p) __hip_atomic_load((p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+#define HE_WS_TICKET(p) __hip_atomic_fetch_add((p), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+#endif
 struct Matrix {
     u32 rows, cols, mp, np;
     u32 tall, first_part, parts;
     float shape_scale;
-    u64 x[2], xt[2][2], a[2], b[2];
+    u64 x, xt[2], a, b, x_low;
 };
-struct Tile { u32 matrix, i, j; };
+struct Block { u32 matrix, i, j; };
+struct Task { u32 matrix, i, j, k_begin, k_end, slot, share, shares; };
 struct Operands {
     const elem_t* in[GROUP];
     const float* momentum[GROUP];
@@ -63,31 +77,117 @@ struct Operands {
 #define NS_B -4.7750f
 #define NS_C 2.0315f
 
-// The matrix that is orthogonalised, element by element: the operand itself, or the step's update from the gradient and the new momentum.
-template <bool STEP> __device__ __forceinline__ float update_of(const Operands& o, u32 k, u64 e) {
-    const float g = (float)o.in[k][e];
-    if (!STEP) return g;
-    const float m = o.new_momentum[k][e];
-    return o.nesterov ? g + o.mu * m : m;
+// Matrices of the workspace are rows of chunks of 8 values: with PARTS == 2 the chunk's high parts, then its low ones, so that a row's
+// 128 bytes are 32 values in two parts or 64 in one and are moved alike.
+#define PARTS (SPLIT ? 2 : 1)
+__device__ __forceinline__ u64 chunk_at(u64 row, u32 col, u32 pitch) { return (row * pitch + col) * PARTS; }   // col: a multiple of 8
+
+__device__ __forceinline__ f16x8 high_of(const float (&v)[8]) {
+    f16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; e++) h[e] = (f16_t)v[e];
+    return h;
+}
+__device__ __forceinline__ f16x8 low_of(const float (&v)[8], f16x8 h) {
+    f16x8 l;
+#pragma unroll
+    for (int e = 0; e < 8; e++) l[e] = (f16_t)(v[e] - (float)h[e]);
+    return l;
+}
+// Eight values of a row. `low`: where the low parts go if the format has none (may be null).
+__device__ __forceinline__ void put(f16_t* __restrict__ to, u64 row, u32 col, u32 pitch, const float (&v)[8], f16_t* __restrict__ low) {
+    const f16x8 h = high_of(v);
+    f16_t* at = to + chunk_at(row, col, pitch);
+    *(f16x8*)at = h;
+    if (SPLIT) *(f16x8*)(at + 8) = low_of(v, h);
+    else if (low) *(f16x8*)(low + row * pitch + col) = low_of(v, h);
+}
+__device__ __forceinline__ void get(const f16_t* __restrict__ from, u64 row, u32 col, u32 pitch, float (&v)[8], const f16_t* __restrict__ low) {
+    const f16_t* at = from + chunk_at(row, col, pitch);
+    const f16x8 h = *(const f16x8*)at;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)h[e];
+    if (SPLIT || low) {
+        const f16x8 l = *(const f16x8*)(SPLIT ? at + 8 : low + row * pitch + col);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += (float)l[e];
+    }
+}
+
+// Up to eight neighbouring values of a caller's row; `whole`: all eight are there, at an address that a vector access may have.
+template <class E> __device__ __forceinline__ void row_of(const E* __restrict__ from, u32 left, bool whole, float (&v)[8]) {
+    typedef E vec_t __attribute__((ext_vector_type(16 / sizeof(E))));
+    if (whole) {
+#pragma unroll
+        for (u32 b = 0; b < 8 * sizeof(E) / 16; b++) {
+            const vec_t x = ((const vec_t*)from)[b];
+#pragma unroll
+            for (u32 e = 0; e < 16 / sizeof(E); e++) v[b * (16 / sizeof(E)) + e] = (float)x[e];
+        }
+    } else {
+#pragma unroll
+        for (u32 e = 0; e < 8; e++) v[e] = e < left ? (float)from[e] : 0.0f;
+    }
+}
+template <class E> __device__ __forceinline__ void row_to(E* __restrict__ to, u32 left, bool whole, const float (&v)[8]) {
+    typedef E vec_t __attribute__((ext_vector_type(16 / sizeof(E))));
+    if (whole) {
+#pragma unroll
+        for (u32 b = 0; b < 8 * sizeof(E) / 16; b++) {
+            vec_t x;
+#pragma unroll
+            for (u32 e = 0; e < 16 / sizeof(E); e++) x[e] = (E)v[b * (16 / sizeof(E)) + e];
+            ((vec_t*)to)[b] = x;
+        }
+    } else {
+#pragma unroll
+        for (u32 e = 0; e < 8; e++)
+            if (e < left) to[e] = (E)v[e];
+    }
+}
+
+// Eight neighbouring values of the matrix that is orthogonalised (zeros beyond it): of the operand itself, or of the step's update,
+// from the gradient and the new momentum.
+template <bool STEP> __device__ __forceinline__ void updates_of(const Operands& o, u32 k, u32 r, u32 c, u32 rows, u32 cols, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.0f;
+    if (r >= rows || c >= cols) return;
+    const u64 at = (u64)r * cols + c;
+    const bool whole = cols % 8 == 0;
+    if (!STEP || o.nesterov) row_of<elem_t>(o.in[k] + at, cols - c, whole, v);
+    if (STEP) {
+        float m[8];
+        row_of<float>(o.new_momentum[k] + at, cols - c, whole, m);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = o.nesterov ? v[e] + o.mu * m[e] : m[e];
+    }
 }
 )HIP";
 
 const char* kElements = R"HIP(
 // Shares of |U|^2, in 64 bits: squares of f32 neither overflow nor vanish there. The step's first pass also writes the new momenta.
-template <bool STEP> __device__ __forceinline__ void norm_part(const Matrix* __restrict__ mats, const Tile* __restrict__ parts, double* __restrict__ sums, const Operands& o) {
+template <bool STEP> __device__ __forceinline__ void norm_part(const Matrix* __restrict__ mats, const Block* __restrict__ parts, double* __restrict__ sums, const Operands& o) {
     __shared__ double wave_sums[4];
-    const Tile t = parts[blockIdx.x];
+    const Block t = parts[blockIdx.x];
     const u32 k = t.matrix - o.first;
     const u64 size = (u64)mats[t.matrix].rows * mats[t.matrix].cols, begin = (u64)t.i * PART, end = begin + PART < size ? begin + PART : size;
     double s = 0.0;
-    for (u64 e = begin + threadIdx.x; e < end; e += 256) {
-        float u = (float)o.in[k][e];
+    for (u64 e = begin + threadIdx.x * 8; e < end; e += 2048) {
+        const u32 left = end - e < 8 ? (u32)(end - e) : 8u;
+        float u[8];
+        row_of<elem_t>(o.in[k] + e, left, left == 8, u);
         if (STEP) {
-            const float m = o.mu * o.momentum[k][e] + u;
-            o.new_momentum[k][e] = m;
-            u = o.nesterov ? u + o.mu * m : m;
+            float m[8];
+            row_of<float>(o.momentum[k] + e, left, left == 8, m);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                m[i] = o.mu * m[i] + u[i];
+                u[i] = o.nesterov ? u[i] + o.mu * m[i] : m[i];
+            }
+            row_to<float>(o.new_momentum[k] + e, left, left == 8, m);
         }
-        s += (double)u * (double)u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s += (double)u[i] * (double)u[i];
     }
     for (int m = 32; m > 0; m /= 2) s += SHFL_XOR_F64(s, m);
     if ((threadIdx.x & 63u) == 0) wave_sums[threadIdx.x >> 6] = s;
@@ -95,17 +195,12 @@ template <bool STEP> __device__ __forceinline__ void norm_part(const Matrix* __r
     if (threadIdx.x == 0) sums[blockIdx.x + t.j] = wave_sums[0] + wave_sums[1] + wave_sums[2] + wave_sums[3];
 }
 
-__device__ __forceinline__ void store_split(f16_t* __restrict__ high, f16_t* __restrict__ low, u64 at, float v, bool with_low) {
-    const f16_t h = (f16_t)v;
-    high[at] = h;
-    if (with_low) low[at] = (f16_t)(v - (float)h);
-}
-
-// U / (|U| + floor) in f16 parts, in both orientations, zeros beyond the matrix. A block of 64 x 64.
-template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, const Operands& o) {
+// U / (|U| + floor) in f16 parts, in both orientations, zeros beyond the matrix. A block of 64 x 64: 8 lanes take the 64 columns of a
+// row, 8 values each.
+template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, const Operands& o) {
     __shared__ float tile[64][65];
     __shared__ double total;
-    const Tile t = blocks[blockIdx.x];
+    const Block t = blocks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
     const u32 k = t.matrix - o.first, rows_p = m.tall ? m.np : m.mp, cols_p = m.tall ? m.mp : m.np, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     if (wave == 0) {
@@ -116,47 +211,80 @@ template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix*
     }
     __syncthreads();
     const double scale = (double)X_SCALE / (sqrt(total) + (double)NORM_FLOOR);
-    f16_t *nh = (f16_t*)(ws + (m.tall ? m.xt[0][0] : m.x[0])), *nl = (f16_t*)(ws + (m.tall ? m.xt[0][1] : m.x[1]));
-    f16_t *th = (f16_t*)(ws + (m.tall ? m.x[0] : m.xt[0][0])), *tl = (f16_t*)(ws + (m.tall ? m.x[1] : m.xt[0][1]));
-    const u32 c = t.j * 64 + lane;
-    for (u32 i = wave; i < 64; i += 4) {
-        const u32 r = t.i * 64 + i;
-        float v = 0.0f;
-        if (r < m.rows && c < m.cols) v = (float)((double)update_of<STEP>(o, k, (u64)r * m.cols + c) * scale);
-        tile[i][lane] = v;
-        store_split(nh, nl, (u64)r * cols_p + c, v, SPLIT || !m.tall);
+    f16_t *natural = (f16_t*)(ws + (m.tall ? m.xt[0] : m.x)), *turned = (f16_t*)(ws + (m.tall ? m.x : m.xt[0])), *low = (f16_t*)(ws + m.x_low);
+    const u32 c = t.j * 64 + (lane & 7u) * 8;
+#pragma unroll
+    for (u32 pass = 0; pass < 2; pass++) {
+        const u32 i = pass * 32 + wave * 8 + (lane >> 3), r = t.i * 64 + i;
+        float v[8];
+        updates_of<STEP>(o, k, r, c, m.rows, m.cols, v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[e] = (float)((double)v[e] * scale);
+            tile[i][(lane & 7u) * 8 + e] = v[e];
+        }
+        put(natural, r, c, cols_p, v, SPLIT || m.tall ? nullptr : low);
     }
     __syncthreads();
-    for (u32 i = wave; i < 64; i += 4) store_split(th, tl, (u64)(t.j * 64 + i) * rows_p + t.i * 64 + lane, tile[lane][i], SPLIT || m.tall);
+#pragma unroll
+    for (u32 pass = 0; pass < 2; pass++) {
+        const u32 i = pass * 32 + wave * 8 + (lane >> 3);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = tile[(lane & 7u) * 8 + e][i];
+        put(turned, t.j * 64 + i, t.i * 64 + (lane & 7u) * 8, rows_p, v, SPLIT || !m.tall ? nullptr : low);
+    }
 }
 
-template <bool STEP> __device__ __forceinline__ void finish_block(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const char* __restrict__ ws, const Operands& o) {
-    const Tile t = blocks[blockIdx.x];
+// The last X to where it goes, by way of LDS where the matrix was iterated as its transpose.
+template <bool STEP> __device__ __forceinline__ void finish_block(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const char* __restrict__ ws, const Operands& o) {
+    __shared__ float tile[64][65];
+    const Block t = blocks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
-    const u32 k = t.matrix - o.first, cols_p = m.tall ? m.mp : m.np, c = t.j * 64 + (threadIdx.x & 63u);
-    const f16_t *h = (const f16_t*)(ws + (m.tall ? m.xt[STEPS & 1][0] : m.x[0])), *l = (const f16_t*)(ws + (m.tall ? m.xt[STEPS & 1][1] : m.x[1]));
-    for (u32 i = threadIdx.x >> 6; i < 64; i += 4) {
-        const u32 r = t.i * 64 + i;
+    const u32 k = t.matrix - o.first, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = t.j * 64 + (lane & 7u) * 8;
+    const f16_t *from = (const f16_t*)(ws + m.x), *low = SPLIT ? nullptr : (const f16_t*)(ws + m.x_low);
+    if (m.tall) {
+#pragma unroll
+        for (u32 pass = 0; pass < 2; pass++) {
+            const u32 i = pass * 32 + wave * 8 + (lane >> 3);
+            float v[8];
+            get(from, t.j * 64 + i, t.i * 64 + (lane & 7u) * 8, m.np, v, low);
+#pragma unroll
+            for (int e = 0; e < 8; e++) tile[(lane & 7u) * 8 + e][i] = v[e];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (u32 pass = 0; pass < 2; pass++) {
+        const u32 i = pass * 32 + wave * 8 + (lane >> 3), r = t.i * 64 + i;
         if (r >= m.rows || c >= m.cols) continue;
-        const u64 at = (u64)r * cols_p + c, e = (u64)r * m.cols + c;
-        float v = (float)h[at];
-        v += (float)l[at];
-        v *= 1.0f / X_SCALE;
+        float v[8];
+        if (m.tall)
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = tile[i][(lane & 7u) * 8 + e];
+        else get(from, r, c, m.np, v, low);
+        const u64 e0 = (u64)r * m.cols + c;
+        const bool whole = c + 8 <= m.cols && m.cols % 8 == 0;
         if (STEP) {
-            const float w = o.weight[k][e];
-            ((float*)o.out[k])[e] = (w - o.learning_rate * o.weight_decay * w) - o.learning_rate * m.shape_scale * v;
+            float w[8];
+            row_of<float>(o.weight[k] + e0, m.cols - c, whole, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = (w[e] - o.learning_rate * o.weight_decay * w[e]) - o.learning_rate * m.shape_scale * (v[e] * (1.0f / X_SCALE));
+            row_to<float>((float*)o.out[k] + e0, m.cols - c, whole, w);
         } else {
-            ((elem_t*)o.out[k])[e] = (elem_t)v;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] *= 1.0f / X_SCALE;
+            row_to<elem_t>((elem_t*)o.out[k] + e0, m.cols - c, whole, v);
         }
     }
 }
 
-extern "C" __global__ __launch_bounds__(256) void muon_norm(const Matrix* __restrict__ mats, const Tile* __restrict__ parts, double* __restrict__ sums, Operands o) { norm_part<false>(mats, parts, sums, o); }
-extern "C" __global__ __launch_bounds__(256) void muon_norm_step(const Matrix* __restrict__ mats, const Tile* __restrict__ parts, double* __restrict__ sums, Operands o) { norm_part<true>(mats, parts, sums, o); }
-extern "C" __global__ __launch_bounds__(256) void muon_convert(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, Operands o) { convert_block<false>(mats, blocks, sums, ws, o); }
-extern "C" __global__ __launch_bounds__(256) void muon_convert_step(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, Operands o) { convert_block<true>(mats, blocks, sums, ws, o); }
-extern "C" __global__ __launch_bounds__(256) void muon_finish(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const char* __restrict__ ws, Operands o) { finish_block<false>(mats, blocks, ws, o); }
-extern "C" __global__ __launch_bounds__(256) void muon_finish_step(const Matrix* __restrict__ mats, const Tile* __restrict__ blocks, const char* __restrict__ ws, Operands o) { finish_block<true>(mats, blocks, ws, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_norm(const Matrix* __restrict__ mats, const Block* __restrict__ parts, double* __restrict__ sums, Operands o) { norm_part<false>(mats, parts, sums, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_norm_step(const Matrix* __restrict__ mats, const Block* __restrict__ parts, double* __restrict__ sums, Operands o) { norm_part<true>(mats, parts, sums, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_convert(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, Operands o) { convert_block<false>(mats, blocks, sums, ws, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_convert_step(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, Operands o) { convert_block<true>(mats, blocks, sums, ws, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_finish(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const char* __restrict__ ws, Operands o) { finish_block<false>(mats, blocks, ws, o); }
+extern "C" __global__ __launch_bounds__(256) void muon_finish_step(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const char* __restrict__ ws, Operands o) { finish_block<true>(mats, blocks, ws, o); }
 )HIP";
 
 // One kernel for the three products of a step, each of the form R = alpha P Q^T + beta E with P, Q row-major and contiguous along the
@@ -167,49 +295,47 @@ extern "C" __global__ __launch_bounds__(256) void muon_finish_step(const Matrix*
 const char* kProduct = R"HIP(
 #define BM TILE
 #define BN TILE
-#define BK 64
 #define WAVES (WAVES_M * WAVES_N)
 #define WTM (BM / WAVES_M)
 #define WTN (BN / WAVES_N)
 #define MB (WTM / 32)
 #define NB (WTN / 32)
-#define STAGE_HALVES ((BM + BN) * BK)
+#define BK (64 / PARTS)                 /* values of a row in a k-tile: 128 bytes */
+#define KS (BK / 16)                    /* matrix instructions along a k-tile */
+#define STAGE_HALVES ((BM + BN) * 64)
 #define LOADS ((BM + BN) / 8 / WAVES)   /* direct loads of a wave per k-tile: 8 rows of 128 bytes each */
-#define STRIP_PITCH 72                  /* of a wave's 64 x 64 strip in LDS, in halves: rows stay 16-byte aligned */
+#define SROWS (WTM < 64 ? WTM : 64)     /* a wave's strip: rows and columns of results that go through LDS at a time */
+#define SCOLS (WTN < 64 ? WTN : 64)
+#define STRIP_PITCH (SCOLS + 1)         /* odd: rows and columns are both read without bank conflicts */
+#define STRIP_FLOATS (WAVES * SROWS * STRIP_PITCH)
+#define LDS_HALVES (STAGES * STAGE_HALVES > 2 * STRIP_FLOATS ? STAGES * STAGE_HALVES : 2 * STRIP_FLOATS)
 enum { GRAM, SQUARE, APPLY };
 
-// Waits until this wave's direct loads have landed, then for the other waves'.
-__device__ __forceinline__ void tile_ready() {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
+__device__ __forceinline__ void strip_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Tile* __restrict__ tiles, char* __restrict__ ws, u32 turn) {
-    __shared__ __attribute__((aligned(16))) f16_t lds[2 * STAGE_HALVES];
-    const Tile t = tiles[blockIdx.x];
+template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ shared_tiles, u32* __restrict__ tickets, u32 turn, u32 last_step) {
+    __shared__ __attribute__((aligned(16))) f16_t lds[LDS_HALVES];
+    __shared__ u32 last;
+    const Task t = tasks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
-    const u32 k_len = STAGE == GRAM ? m.np : m.mp, k_tiles = k_len / BK;
-    const f16_t *p_plane[2], *q_plane[2];
-#pragma unroll
-    for (int part = 0; part < 2; part++) {
-        p_plane[part] = (const f16_t*)(ws + (STAGE == GRAM ? m.x[part] : STAGE == SQUARE ? m.a[part] : m.b[part])) + (u64)t.i * BM * k_len;
-        q_plane[part] = (const f16_t*)(ws + (STAGE == GRAM ? m.x[part] : STAGE == SQUARE ? m.a[part] : m.xt[turn][part])) + (u64)t.j * BN * k_len;
-    }
+    const u32 k_len = (STAGE == GRAM ? m.np : m.mp) * PARTS;   // halves of a row
+    const f16_t* p_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b)) + (u64)t.i * BM * k_len;
+    const f16_t* q_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[turn])) + (u64)t.j * BN * k_len;
     // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows
     // meet 8 different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes.
     const u32 lane_off = (lane >> 3) * k_len + (((lane & 7u) ^ (lane >> 3)) << 3);
-    // (parts: high x high, high x low, low x high)
-    const u32 all = SPLIT ? 3 * k_tiles : k_tiles;
     auto fetch = [&](u32 kt, u32 slot) {
-        const u32 pass = SPLIT ? kt / k_tiles : 0, k0 = (kt - pass * k_tiles) * BK;
-        const f16_t *p = p_plane[pass == 2], *q = q_plane[pass == 1];
         f16_t* base = lds + slot * STAGE_HALVES;
 #pragma unroll
         for (int l = 0; l < LOADS; l++) {
             const u32 row = (wave * LOADS + l) * 8;   // of P's rows, then Q's
-            const f16_t* src = (row < BM ? p + (u64)row * k_len : q + (u64)(row - BM) * k_len) + k0 + lane_off;
-            __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * BK), 16, 0, 0);
+            const f16_t* src = (row < BM ? p_rows + (u64)row * k_len : q_rows + (u64)(row - BM) * k_len) + (u64)kt * 64 + lane_off;
+            __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * 64), 16, 0, 0);
         }
     };
     f32x16 acc[MB][NB];
@@ -220,92 +346,139 @@ template <int STAGE> __device__ __forceinline__ void product(const Matrix* __res
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
     const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane & 7u;
-    fetch(0, 0);
-    for (u32 kt = 0; kt < all; kt++) {
-        tile_ready();
-        if (kt + 1 < all) fetch(kt + 1, (kt + 1) & 1u);
-        const f16_t *p = lds + (kt & 1u) * STAGE_HALVES + (wave_m * WTM + frag_row) * BK, *q = lds + (kt & 1u) * STAGE_HALVES + (BM + wave_n * WTN + frag_row) * BK;
+    u32 slot = 0;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; kk++) {
-            f16x8 a[MB], b[NB];
-            const u32 chunk = ((kk * 2 + half) ^ swz) * 8;
+    for (int s = 0; s < STAGES - 1; s++)
+        if (t.k_begin + s < t.k_end) fetch(t.k_begin + s, s);
+    for (u32 kt = t.k_begin; kt < t.k_end; kt++) {
+        // this wave's loads of the k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'
+        if (kt + STAGES - 2 < t.k_end) __builtin_amdgcn_s_waitcnt(WAIT_LOADS((STAGES - 2) * LOADS));
+        else __builtin_amdgcn_s_waitcnt(WAIT_LOADS(0));
+        // (the bare barrier: __syncthreads() would wait for all loads; no wave still reads the stage that is filled next)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (kt + STAGES - 1 < t.k_end) fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1);
+        const f16_t *p = lds + slot * STAGE_HALVES + (wave_m * WTM + frag_row) * 64, *q = lds + slot * STAGE_HALVES + (BM + wave_n * WTN + frag_row) * 64;
 #pragma unroll
-            for (int i = 0; i < MB; i++) a[i] = *(const f16x8*)(p + i * 32 * BK + chunk);
+        for (int kk = 0; kk < KS; kk++) {
+            f16x8 a[PARTS][MB], b[PARTS][NB];
 #pragma unroll
-            for (int j = 0; j < NB; j++) b[j] = *(const f16x8*)(q + j * 32 * BK + chunk);
+            for (int part = 0; part < PARTS; part++) {
+                const u32 chunk = (((kk * 2 + half) * PARTS + part) ^ swz) * 8;
+#pragma unroll
+                for (int i = 0; i < MB; i++) a[part][i] = *(const f16x8*)(p + i * 32 * 64 + chunk);
+#pragma unroll
+                for (int j = 0; j < NB; j++) b[part][j] = *(const f16x8*)(q + j * 32 * 64 + chunk);
+            }
+            // high x high, high x low, low x high
+#pragma unroll
+            for (int c = 0; c < (SPLIT ? 3 : 1); c++)
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[c == 2][i], b[c == 1][j], acc[i][j], 0, 0, 0);
+        }
+        slot = slot + 1 < STAGES ? slot + 1 : 0;
+    }
+
+    // A tile whose sum several workgroups share: each parks its part, the last to arrive adds them up in their order and goes on.
+    if (t.shares > 1) {
+        u64* mine = (u64*)(shared_tiles + (u64)(t.slot + t.share) * (BM * BN)) + wave * (WTM * WTN / 2) + lane;
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float two[2] = {acc[i][j][2 * e], acc[i][j][2 * e + 1]};
+                    HE_WS_STORE(mine + ((i * NB + j) * 8 + e) * 64, __builtin_bit_cast(u64, two));
+                }
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (threadIdx.x == 0) last = HE_WS_TICKET(tickets + t.slot) + 1 == t.shares;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) HE_WS_STORE(tickets + t.slot, 0u);   // as the next launch wants it
+#pragma unroll
+        for (int i = 0; i < MB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+        for (u32 s = 0; s < t.shares; s++) {
+            const u64* from = (const u64*)(shared_tiles + (u64)(t.slot + s) * (BM * BN)) + wave * (WTM * WTN / 2) + lane;
 #pragma unroll
             for (int i = 0; i < MB; i++)
 #pragma unroll
-                for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i], b[j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < NB; j++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        struct Two { float v[2]; } two = __builtin_bit_cast(Two, HE_WS_LOAD(from + ((i * NB + j) * 8 + e) * 64));
+                        acc[i][j][2 * e] += two.v[0];
+                        acc[i][j][2 * e + 1] += two.v[1];
+                    }
         }
     }
     __syncthreads();   // the operand stages become the waves' strips
 
-    // Results: a lane holds rows (e / 4) * 8 + half * 4 + e % 4 of column lane % 32 of each 32 x 32 block. Strips of 64 x 64 go through
-    // LDS into whole rows, once as they are and once transposed.
-    const u32 out_pitch = STAGE == APPLY ? m.np : m.mp;
-    f16_t* strip = lds + wave * 64 * STRIP_PITCH;
-    const u64 row0 = (u64)t.i * BM + wave_m * WTM, col0 = (u64)t.j * BN + wave_n * WTN;
-    const bool mirrored = STAGE == APPLY || t.i != t.j;
+    // Results: a lane holds rows (e / 4) * 8 + half * 4 + e % 4 of column lane % 32 of each 32 x 32 block. Through a strip in LDS a lane gets
+    // 8 neighbours of a row, adds E, stores them, and puts them back for the transposed copy.
+    const u32 pitch = STAGE == APPLY ? m.np : m.mp;
+    const f16_t* e_rows = (const f16_t*)(ws + (STAGE == SQUARE ? m.a : m.x));
+    f16_t *plain = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.x)), *turned = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.xt[turn ^ 1u]));
+    // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
+    // singular values with it)
+    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.x_low) : nullptr;
+    float* strip = (float*)lds + wave * (SROWS * STRIP_PITCH);
+    const bool mirrored = STAGE == APPLY ? !last_step : t.i != t.j;
+    constexpr u32 row_lanes = SCOLS / 8, col_lanes = SROWS / 8;   // lanes along a row of the strip, and along a column
 #pragma unroll
-    for (int i = 0; i < MB; i += 2)
+    for (int i = 0; i < WTM / SROWS; i++)
 #pragma unroll
-        for (int j = 0; j < NB; j += 2) {
-            float v[2][2][16];
+        for (int j = 0; j < WTN / SCOLS; j++) {
+            const u32 row0 = t.i * BM + wave_m * WTM + i * SROWS, col0 = t.j * BN + wave_n * WTN + j * SCOLS;
 #pragma unroll
-            for (int di = 0; di < 2; di++)
+            for (int di = 0; di < SROWS / 32; di++)
 #pragma unroll
-                for (int dj = 0; dj < 2; dj++)
+                for (int dj = 0; dj < SCOLS / 32; dj++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float s = acc[i + di][j + dj][e];
-                        if (STAGE == GRAM) {
-                            v[di][dj][e] = s * (A_SCALE / (X_SCALE * X_SCALE));
-                            continue;
-                        }
-                        const u64 at = (row0 + (i + di) * 32 + (e / 4) * 8 + half * 4 + e % 4) * out_pitch + col0 + (j + dj) * 32 + frag_row;
-                        float other = (float)((const f16_t*)(ws + (STAGE == SQUARE ? m.a[0] : m.x[0])))[at];
-                        // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and
-                        // the small singular values with it)
-                        if (SPLIT || STAGE == APPLY) other += (float)((const f16_t*)(ws + (STAGE == SQUARE ? m.a[1] : m.x[1])))[at];
-                        v[di][dj][e] = STAGE == SQUARE ? NS_B * other + (NS_C * B_SCALE / (A_SCALE * A_SCALE)) * s : NS_A * other + (1.0f / B_SCALE) * s;
-                    }
+                    for (int e = 0; e < 16; e++)
+                        strip[(di * 32 + (e / 4) * 8 + half * 4 + e % 4) * STRIP_PITCH + dj * 32 + frag_row] = acc[i * (SROWS / 32) + di][j * (SCOLS / 32) + dj][e];
+            strip_sync();
 #pragma unroll
-            for (int part = 0; part < 2; part++) {
-                const bool keep_plain = SPLIT || part == 0 || STAGE == APPLY, keep_mirror = mirrored && (SPLIT || part == 0 || STAGE == APPLY);
-                if (!keep_plain) continue;
-                f16_t *plain = (f16_t*)(ws + (STAGE == GRAM ? m.a[part] : STAGE == SQUARE ? m.b[part] : m.x[part]));
-                f16_t *mirror = (f16_t*)(ws + (STAGE == GRAM ? m.a[part] : STAGE == SQUARE ? m.b[part] : m.xt[turn ^ 1u][part]));
+            for (u32 s = 0; s < SROWS * row_lanes / 64; s++) {
+                const u32 r = s * (64 / row_lanes) + lane / row_lanes, c = lane % row_lanes * 8;
+                float v[8], other[8];
+                if (STAGE != GRAM) get(e_rows, row0 + r, col0 + c, pitch, other, low);
 #pragma unroll
-                for (int way = 0; way < 2; way++) {
-                    if (way == 1 && !keep_mirror) continue;
-                    __syncthreads();
-#pragma unroll
-                    for (int di = 0; di < 2; di++)
-#pragma unroll
-                        for (int dj = 0; dj < 2; dj++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const u32 r = di * 32 + (e / 4) * 8 + half * 4 + e % 4, c = dj * 32 + frag_row;
-                                const f16_t high = (f16_t)v[di][dj][e];
-                                strip[way ? c * STRIP_PITCH + r : r * STRIP_PITCH + c] = part ? (f16_t)(v[di][dj][e] - (float)high) : high;
-                            }
-                    __syncthreads();
-                    f16_t* to = way ? mirror + (col0 + j * 32) * (STAGE == APPLY ? m.mp : m.mp) + row0 + i * 32 : plain + (row0 + i * 32) * out_pitch + col0 + j * 32;
-                    const u32 pitch = way ? m.mp : out_pitch;
-#pragma unroll
-                    for (int s = 0; s < 8; s++) {
-                        const u32 r = s * 8 + (lane >> 3), c = (lane & 7u) * 8;
-                        *(u32x4*)(to + (u64)r * pitch + c) = *(const u32x4*)(strip + r * STRIP_PITCH + c);
-                    }
+                for (int e = 0; e < 8; e++) {
+                    const float sum = strip[r * STRIP_PITCH + c + e];
+                    v[e] = STAGE == GRAM ? sum * (A_SCALE / (X_SCALE * X_SCALE))
+                         : STAGE == SQUARE ? NS_B * other[e] + (NS_C * B_SCALE / (A_SCALE * A_SCALE)) * sum
+                                           : NS_A * other[e] + (1.0f / B_SCALE) * sum;
+                    strip[r * STRIP_PITCH + c + e] = v[e];
                 }
+                put(plain, row0 + r, col0 + c, pitch, v, low);
             }
+            strip_sync();
+            if (mirrored)
+#pragma unroll
+                for (u32 s = 0; s < SCOLS * col_lanes / 64; s++) {
+                    const u32 c = s * (64 / col_lanes) + lane / col_lanes, r = lane % col_lanes * 8;
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = strip[(r + e) * STRIP_PITCH + c];
+                    put(turned, col0 + c, row0 + r, m.mp, v, nullptr);
+                }
+            strip_sync();
         }
 }
 
-extern "C" __global__ __launch_bounds__(WAVES * 64) void muon_gram(const Matrix* __restrict__ mats, const Tile* __restrict__ tiles, char* __restrict__ ws, u32 turn) { product<GRAM>(mats, tiles, ws, turn); }
-extern "C" __global__ __launch_bounds__(WAVES * 64) void muon_square(const Matrix* __restrict__ mats, const Tile* __restrict__ tiles, char* __restrict__ ws, u32 turn) { product<SQUARE>(mats, tiles, ws, turn); }
-extern "C" __global__ __launch_bounds__(WAVES * 64) void muon_apply(const Matrix* __restrict__ mats, const Tile* __restrict__ tiles, char* __restrict__ ws, u32 turn) { product<APPLY>(mats, tiles, ws, turn); }
+#define KERNEL(name, stage) extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ shared_tiles, u32* __restrict__ tickets, u32 turn, u32 last_step) { product<stage>(mats, tasks, ws, shared_tiles, tickets, turn, last_step); }
+KERNEL(muon_gram, GRAM)
+KERNEL(muon_square, SQUARE)
+KERNEL(muon_apply, APPLY)
 )HIP";
 
 struct OperandsArg {
@@ -319,17 +492,49 @@ struct OperandsArg {
     int32_t nesterov;
 };
 
-// Tiles in the order of their blocks: blocks are dealt round-robin to the 8 XCDs, each with an L2 of its own, so XCD x gets the
+// Tasks in the order of their blocks: blocks are dealt round-robin to the 8 XCDs, each with an L2 of its own, so XCD x gets the
 // x-th eighth of a sequence in which neighbours share rows and columns.
-void deal(std::vector<MuonTile>& tiles) {
-    const size_t n = tiles.size(), whole = n / 8, over = n % 8;
-    std::vector<MuonTile> out(n);
+void deal(std::vector<MuonTask>& tasks) {
+    const size_t n = tasks.size(), whole = n / 8, over = n % 8;
+    std::vector<MuonTask> out(n);
     for (size_t b = 0; b < n; b++) {
         const size_t x = b % 8;
-        out[b] = tiles[x * whole + std::min(x, over) + b / 8];
+        out[b] = tasks[x * whole + std::min(x, over) + b / 8];
     }
-    tiles.swap(out);
+    tasks.swap(out);
 }
+
+// The tasks of one product of every matrix: bands of four tile rows, column by column; a tile's sum is dealt to several workgroups
+// where there are too few tiles to fill the chip. `slots`: workgroups that it runs at once; `least`: k-tiles a share has at least.
+std::vector<MuonTask> tasks_of(const std::vector<MuonMatrix>& mats, uint32_t tile, bool lower, bool along_n, uint32_t bk, uint32_t slots, uint32_t least,
+                               uint32_t* shared) {
+    uint64_t units = 0, tiles = 0;
+    for (const MuonMatrix& m : mats) {
+        const uint64_t ti = m.mp / tile, count = lower ? ti * (ti + 1) / 2 : ti * (m.np / tile);
+        tiles += count;
+        units += count * ((along_n ? m.np : m.mp) / bk);
+    }
+    const uint64_t target = tiles >= slots ? units : std::max<uint64_t>(least, (units + slots - 1) / slots);
+    std::vector<MuonTask> out;
+    *shared = 0;
+    for (size_t k = 0; k < mats.size(); k++) {
+        const MuonMatrix& m = mats[k];
+        const uint32_t ti = m.mp / tile, tj = lower ? ti : m.np / tile, kt = (along_n ? m.np : m.mp) / bk;
+        const uint32_t shares = (uint32_t)std::max<uint64_t>(1, kt / target);
+        for (uint32_t g = 0; g < ti; g += 4)
+            for (uint32_t j = 0; j < tj; j++)
+                for (uint32_t i = g; i < std::min(g + 4, ti); i++) {
+                    if (lower && j > i) continue;
+                    for (uint32_t s = 0; s < shares; s++)
+                        out.push_back({(uint32_t)k, i, j, (uint32_t)((uint64_t)kt * s / shares), (uint32_t)((uint64_t)kt * (s + 1) / shares), *shared, s, shares});
+                    if (shares > 1) *shared += shares;
+                }
+    }
+    deal(out);
+    return out;
+}
+
+int env_int(const char* name, int dflt) { return tuning::get_int(name, dflt); }
 
 template <class T> std::vector<char> bytes_of(const std::vector<T>& v) {
     std::vector<char> out(v.size() * sizeof(T));
@@ -343,14 +548,16 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     HE_REQUIRE(!pr.shapes.empty() && pr.shapes.size() <= 65536, HE_ERR_INVALID, "muon: %zu matrices, 1 to 65536 are taken", pr.shapes.size());
     HE_REQUIRE(pr.dtype == HE_F16 || pr.dtype == HE_BF16 || pr.dtype == HE_F32, HE_ERR_INVALID, "muon does not take dtype %s", dtype_name(pr.dtype));
     HE_REQUIRE(pr.steps >= 1 && pr.steps <= 32, HE_ERR_INVALID, "muon: %d steps, 1 to 32 are taken", pr.steps);
-    const uint32_t tile = 128;
+    const uint32_t tile = (uint32_t)env_int("HELIUM_HIP_MUON_TILE", 128), stages = (uint32_t)env_int("HELIUM_HIP_MUON_STAGES", 2), bk = pr.split ? 32 : 64;
+    const uint32_t waves_m = tile == 64 ? 2 : 2, waves_n = tile == 256 ? 4 : 2;
+    threads_ = waves_m * waves_n * 64;
     uint64_t at = 0, parts = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    std::vector<MuonTile> lower, whole, shares, blocks;
+    std::vector<MuonBlock> shares, blocks;
     for (size_t k = 0; k < pr.shapes.size(); k++) {
         const int64_t rows = pr.shapes[k][0], cols = pr.shapes[k][1];
         HE_REQUIRE(rows >= 1 && cols >= 1, HE_ERR_INVALID, "muon: matrix %zu is %lld x %lld", k, (long long)rows, (long long)cols);
@@ -361,19 +568,9 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         auto padded = [&](int64_t v) { return (uint32_t)((v + tile - 1) / tile * tile); };
         m.mp = padded(std::min(rows, cols)), m.np = padded(std::max(rows, cols));
         m.shape_scale = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
-        const uint64_t x = (uint64_t)m.mp * m.np * 2, a = (uint64_t)m.mp * m.mp * 2;
-        for (int part = 0; part < 2; part++) {
-            m.x[part] = take(x);  // (its low part counts in either precision; the transpose's does where the result is tall)
-            for (int turn = 0; turn < 2; turn++) m.xt[turn][part] = take(x);
-            if (part == 0 || pr.split) m.a[part] = take(a), m.b[part] = take(a);
-        }
-        const uint32_t ti = m.mp / tile, tj = m.np / tile;
-        for (uint32_t g = 0; g < ti; g += 4)  // bands of four tile rows, column by column
-            for (uint32_t j = 0; j < std::max(ti, tj); j++)
-                for (uint32_t i = g; i < std::min(g + 4, ti); i++) {
-                    if (j < tj) whole.push_back({(uint32_t)k, i, j});
-                    if (j <= i) lower.push_back({(uint32_t)k, i, j});
-                }
+        const uint64_t bytes = pr.split ? 4 : 2, x = m.mp * bytes * m.np, a = m.mp * bytes * m.mp;
+        m.x = take(x), m.xt[0] = take(x), m.xt[1] = take(x), m.a = take(a), m.b = take(a);
+        if (!pr.split) m.x_low = take(x);
         const uint64_t size = (uint64_t)rows * cols;
         m.first_part = (uint32_t)parts;
         m.parts = (uint32_t)((size + kPart - 1) / kPart);
@@ -389,30 +586,38 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     }
     part_begin_.push_back((uint32_t)shares.size());
     block_begin_.push_back((uint32_t)blocks.size());
-    deal(lower);
-    deal(whole);
+    const uint32_t slots = 256 * (tile == 256 ? 1 : 2), least = (uint32_t)env_int("HELIUM_HIP_MUON_LEAST", 8);
+    uint32_t shared[3];
+    const std::vector<MuonTask> gram = tasks_of(matrices_, tile, true, true, bk, slots, least, &shared[0]),
+                                square = tasks_of(matrices_, tile, true, false, bk, slots, least, &shared[1]),
+                                apply = tasks_of(matrices_, tile, false, false, bk, slots, least, &shared[2]);
+    const uint32_t most = std::max({shared[0], shared[1], shared[2]});
+    tickets_ = most;
+    tickets_at_ = take((uint64_t)most * 4);
+    shared_at_ = take((uint64_t)most * tile * tile * 4);
     // (a share's place among the sums is its block's, plus where its launch begins)
     for (size_t k = 0; k < pr.shapes.size(); k++)
         for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) shares[p].j = part_begin_[k / kGroup * kGroup];
     workspace_bytes_ = take(parts * sizeof(double)) + parts * sizeof(double);
-    tables_[0] = bytes_of(matrices_), tables_[1] = bytes_of(lower), tables_[2] = bytes_of(whole), tables_[3] = bytes_of(shares), tables_[4] = bytes_of(blocks);
-    table_size_ = {(uint32_t)matrices_.size(), (uint32_t)lower.size(), (uint32_t)whole.size(), (uint32_t)shares.size(), (uint32_t)blocks.size()};
-    for (int t = 0; t < 5; t++) {
+    tables_[0] = bytes_of(matrices_), tables_[1] = bytes_of(gram), tables_[2] = bytes_of(square), tables_[3] = bytes_of(apply);
+    tables_[4] = bytes_of(shares), tables_[5] = bytes_of(blocks);
+    table_size_ = {(uint32_t)matrices_.size(), (uint32_t)gram.size(), (uint32_t)square.size(), (uint32_t)apply.size(), (uint32_t)shares.size(), (uint32_t)blocks.size()};
+    for (int t = 0; t < kTables; t++) {
         table_at_[t] = table_bytes_;
         table_bytes_ += (tables_[t].size() + 255) / 256 * 256;
     }
-    const int waves_m = 2, waves_n = 2;
     std::ostringstream s;
     s << "#define GROUP " << kGroup << "\n#define PART " << kPart << "ull\n#define STEPS " << pr.steps << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
       << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define NORM_FLOOR 1e-7\n#define TILE " << tile << "\n#define WAVES_M " << waves_m
-      << "\n#define WAVES_N " << waves_n << "\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
+      << "\n#define WAVES_N " << waves_n << "\n#define STAGES " << stages << "\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
     source_ = s.str() + kCommon + kElements + kProduct;
     auto make = [&](const char* entry) { return std::make_unique<JitKernel>(source_, entry); };
     norm_ = make("muon_norm"), convert_ = make("muon_convert"), finish_ = make("muon_finish");
     norm_step_ = make("muon_norm_step"), convert_step_ = make("muon_convert_step"), finish_step_ = make("muon_finish_step");
     gram_ = make("muon_gram"), square_ = make("muon_square"), apply_ = make("muon_apply");
-    describe_ = strfmt("muon matrices=%zu steps=%d parts=%d tile=%u threads=%d lower=%u whole=%u shares=%u blocks=%u workspace=%zu", pr.shapes.size(), pr.steps,
-                       pr.split ? 2 : 1, tile, waves_m * waves_n * 64, table_size_[1], table_size_[2], table_size_[3], table_size_[4], workspace_bytes_);
+    describe_ = strfmt("muon matrices=%zu steps=%d parts=%d tile=%u threads=%u stages=%u gram=%u square=%u apply=%u shared=%u,%u,%u shares=%u blocks=%u tickets_at=%zu shared_at=%zu workspace=%zu",
+                       pr.shapes.size(), pr.steps, pr.split ? 2 : 1, tile, threads_, stages, table_size_[1], table_size_[2], table_size_[3], shared[0], shared[1], shared[2],
+                       table_size_[4], table_size_[5], tickets_at_, shared_at_, workspace_bytes_);
 }
 
 Muon::~Muon() {
@@ -428,7 +633,8 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
     Buffers b;
     HE_HIP(hipMalloc((void**)&b.tables, table_bytes_));
     hipError_t e = hipMalloc((void**)&b.workspace, workspace_bytes_);
-    for (int t = 0; t < 5 && e == hipSuccess; t++) e = hipMemcpy(b.tables + table_at_[t], tables_[t].data(), tables_[t].size(), hipMemcpyHostToDevice);
+    if (e == hipSuccess && tickets_) e = hipMemset(b.workspace + tickets_at_, 0, (size_t)tickets_ * 4);
+    for (int t = 0; t < kTables && e == hipSuccess; t++) e = hipMemcpy(b.tables + table_at_[t], tables_[t].data(), tables_[t].size(), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         (void)hipFree(b.tables);
         (void)hipFree(b.workspace);
@@ -439,15 +645,16 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
 }
 
 void Muon::products(char* ws, char* tables, hipStream_t stream) {
-    const uint32_t block[3] = {256, 1, 1}, lower[3] = {table_size_[1], 1, 1}, whole[3] = {table_size_[2], 1, 1};
-    char *mats = tables + table_at_[0], *lower_tiles = tables + table_at_[1], *whole_tiles = tables + table_at_[2];
-    for (int k = 0; k < pr_.steps; k++) {
-        uint32_t turn = (uint32_t)k & 1u;
-        void *sym[] = {&mats, &lower_tiles, &ws, &turn}, *all[] = {&mats, &whole_tiles, &ws, &turn};
-        gram_->launch(lower, block, 0, stream, sym);
-        square_->launch(lower, block, 0, stream, sym);
-        apply_->launch(whole, block, 0, stream, all);
-    }
+    const uint32_t block[3] = {threads_, 1, 1};
+    char *mats = tables + table_at_[0], *shared = ws + shared_at_, *tickets = ws + tickets_at_;
+    for (int k = 0; k < pr_.steps; k++)
+        for (int stage = 1; stage <= 3; stage++) {
+            uint32_t turn = (uint32_t)k & 1u, last = k == pr_.steps - 1;
+            char* tasks = tables + table_at_[stage];
+            const uint32_t grid[3] = {table_size_[stage], 1, 1};
+            void* args[] = {&mats, &tasks, &ws, &shared, &tickets, &turn, &last};
+            (stage == 1 ? gram_ : stage == 2 ? square_ : apply_)->launch(grid, block, 0, stream, args);
+        }
 }
 
 void Muon::orthogonalize(const void* const* in, void* const* out, hipStream_t stream) {
@@ -472,7 +679,7 @@ void Muon::step_or_not(const void* const* in, const float* const* momenta, const
     std::lock_guard<std::mutex> lk(mu_);
     const Buffers b = buffers(stream);
     char *mats = b.tables + table_at_[0], *ws = b.workspace;
-    double* sums = (double*)(ws + workspace_bytes_ - table_size_[3] * sizeof(double));
+    double* sums = (double*)(ws + workspace_bytes_ - table_size_[4] * sizeof(double));
     const uint32_t block[3] = {256, 1, 1};
     auto each_group = [&](auto&& launch) {
         for (size_t first = 0; first < count(); first += kGroup) {
@@ -488,20 +695,20 @@ void Muon::step_or_not(const void* const* in, const float* const* momenta, const
         }
     };
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* parts = b.tables + table_at_[3] + part_begin_[first] * sizeof(MuonTile);
+        char* parts = b.tables + table_at_[4] + part_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {part_begin_[last] - part_begin_[first], 1, 1};
         void* args[] = {&mats, &parts, &sums, &o};
         (how ? norm_step_ : norm_)->launch(grid, block, 0, stream, args);
     });
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* blocks = b.tables + table_at_[4] + block_begin_[first] * sizeof(MuonTile);
+        char* blocks = b.tables + table_at_[5] + block_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {block_begin_[last] - block_begin_[first], 1, 1};
         void* args[] = {&mats, &blocks, &sums, &ws, &o};
         (how ? convert_step_ : convert_)->launch(grid, block, 0, stream, args);
     });
     products(ws, b.tables, stream);
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* blocks = b.tables + table_at_[4] + block_begin_[first] * sizeof(MuonTile);
+        char* blocks = b.tables + table_at_[5] + block_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {block_begin_[last] - block_begin_[first], 1, 1};
         void* args[] = {&mats, &blocks, &ws, &o};
         (how ? finish_step_ : finish_)->launch(grid, block, 0, stream, args, last == count());
@@ -556,7 +763,7 @@ const char* he_muon_describe(he_muon_t muon) { return muon ? muon->impl.describe
 
 int he_muon_table(he_muon_t muon, int which, void* data, size_t capacity, size_t* bytes) {
     return he::guard([&] {
-        HE_REQUIRE(muon && bytes && which >= 0 && which < 5 && (data || capacity == 0), HE_ERR_INVALID, "bad argument");
+        HE_REQUIRE(muon && bytes && which >= 0 && which < he::Muon::kTables && (data || capacity == 0), HE_ERR_INVALID, "bad argument");
         const std::vector<char>& t = muon->impl.table(which);
         *bytes = t.size();
         if (capacity) memcpy(data, t.data(), std::min(capacity, t.size()));

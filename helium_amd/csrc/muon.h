@@ -19,16 +19,22 @@ struct MuonProblem {
     int steps = 5;
 };
 
-// What the kernels know of a matrix; the device holds an array of these. Offsets are bytes in the workspace. The smaller extent
-// is m, the larger n, both padded to whole tiles with zeros (which every product leaves zeros): X is [mp][np], XT its transpose.
+// What the kernels know of a matrix; the device holds an array of these. The smaller extent is m, the larger n, both padded to whole
+// tiles with zeros (which every product leaves zeros): X is [mp][np], XT its transpose. The others are offsets in the workspace.
 struct MuonMatrix {
     uint32_t rows, cols, mp, np;
     uint32_t tall, first_part, parts;  // parts: shares of the sum of squares
     float shape_scale;                 // sqrt(max(1, rows / cols))
-    uint64_t x[2], xt[2][2], a[2], b[2];  // planes: [high, low]; xt twice, in turn
+    uint64_t x, xt[2], a, b, x_low;    // xt twice, in turn; x_low: what f16 drops of X, where operands are of one part
 };
-struct MuonTile {
+// A workgroup's part of the conversions: a share of the sum of squares (i), or the 64 x 64 values at (i, j).
+struct MuonBlock {
     uint32_t matrix, i, j;
+};
+// A workgroup's part of a product: k-tiles k_begin .. k_end - 1 of the tile (i, j), share `share` of `shares`; those of a tile that
+// several work on are parked at `slot` onwards.
+struct MuonTask {
+    uint32_t matrix, i, j, k_begin, k_end, slot, share, shares;
 };
 
 struct MuonStep {
@@ -46,8 +52,9 @@ public:
     const std::string& source() const { return source_; }
     const std::string& describe() const { return describe_; }
     size_t count() const { return pr_.shapes.size(); }
-    // The tables the kernels read, as bytes: 0 matrices, 1 tiles of symmetric products, 2 tiles of whole ones, 3 shares of the
-    // sums of squares, 4 blocks of the conversions.
+    // The tables the kernels read, as bytes: 0 matrices, 1 to 3 tasks of the three products, 4 shares of the sums of squares,
+    // 5 blocks of the conversions.
+    static constexpr int kTables = 6;
     const std::vector<char>& table(int which) const { return tables_[which]; }
     size_t workspace_bytes() const { return workspace_bytes_; }
 
@@ -62,10 +69,11 @@ private:
     void products(char* ws, char* tables, hipStream_t stream);
     MuonProblem pr_;
     std::vector<MuonMatrix> matrices_;
-    std::vector<char> tables_[5];
-    size_t table_at_[5] = {}, table_bytes_ = 0, workspace_bytes_ = 0;
-    std::array<uint32_t, 5> table_size_{};
-    std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 3 and 4
+    std::vector<char> tables_[kTables];
+    size_t table_at_[kTables] = {}, table_bytes_ = 0, workspace_bytes_ = 0, tickets_at_ = 0, shared_at_ = 0;
+    std::array<uint32_t, kTables> table_size_{};
+    uint32_t threads_ = 256, tickets_ = 0;
+    std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 4 and 5
     std::string source_, describe_;
     std::unique_ptr<JitKernel> norm_, convert_, gram_, square_, apply_, finish_, norm_step_, convert_step_, finish_step_;
     std::mutex mu_;

@@ -504,8 +504,8 @@ int he_muon_orthogonalize(he_muon_t muon, const void* const* in, void* const* ou
 int he_muon_step(he_muon_t muon, const void* const* gradients, const float* const* momenta, const float* const* weights,
                  float* const* new_momenta, float* const* new_weights, int count, float learning_rate, float momentum, float weight_decay,
                  int nesterov, he_stream_t stream);
-/* The generated HIP source, how the products are cut, and the tables the kernels read (0 matrices, 1 tiles of the symmetric products,
- * 2 of the whole ones, 3 shares of the sums of squares, 4 blocks of the conversions), for inspection and tests. */
+/* The generated HIP source, how the products are cut, and the tables the kernels read (0 matrices, 1 to 3 the tasks of the three
+ * products of a step, 4 shares of the sums of squares, 5 blocks of the conversions), for inspection and tests. */
 const char* he_muon_source(he_muon_t muon);
 const char* he_muon_describe(he_muon_t muon);
 int he_muon_table(he_muon_t muon, int which, void* data, size_t capacity, size_t* bytes);

@@ -12,8 +12,9 @@ from muon_cases import SHAPES, check, matrix, to_f32, to_storage
 from oracle import muon as oracle
 
 MATRIX = np.dtype([("rows", "u4"), ("cols", "u4"), ("mp", "u4"), ("np", "u4"), ("tall", "u4"), ("first_part", "u4"), ("parts", "u4"),
-                   ("shape_scale", "f4"), ("x", "u8", 2), ("xt", "u8", (2, 2)), ("a", "u8", 2), ("b", "u8", 2)])
-TILE = np.dtype([("matrix", "u4"), ("i", "u4"), ("j", "u4")])
+                   ("shape_scale", "f4"), ("x", "u8"), ("xt", "u8", 2), ("a", "u8"), ("b", "u8"), ("x_low", "u8")])
+TASK = np.dtype([(k, "u4") for k in ("matrix", "i", "j", "k_begin", "k_end", "slot", "share", "shares")])
+BLOCK = np.dtype([("matrix", "u4"), ("i", "u4"), ("j", "u4")])
 
 
 def test_singular_values_go_where_the_polynomial_takes_them():
@@ -65,9 +66,11 @@ static inline double emu_shfl64(double v, int mask) {
 def emulated(shapes, dtype, split, steps, in_storage, step=None):
     """The launches of a call, one after the other. `step`: (momenta, weights, learning rate, mu, decay, nesterov)."""
     muon = ha.Muon(shapes, dtype, precision="f32_f32" if split else "f16_f32", steps=steps)
-    mats, lower, whole, parts, blocks = (np.frombuffer(muon.table(t), MATRIX if t == 0 else TILE) for t in range(5))
-    workspace = int(muon.description.split("workspace=")[1].split()[0])
-    threads = int(muon.description.split("threads=")[1].split()[0])
+    mats, gram, square, apply, parts, blocks = (np.frombuffer(muon.table(t), [MATRIX, TASK, TASK, TASK, BLOCK, BLOCK][t]) for t in range(6))
+    said = dict(s.split("=") for s in muon.description.split()[1:])
+    workspace, threads, tile = int(said["workspace"]), int(said["threads"]), int(said["tile"])
+    slots = max(1, *map(int, said["shared"].split(",")))
+    parked, tickets = np.full(slots * tile * tile, np.nan, np.float32), np.zeros(slots, np.uint32)
     names = [f"in{k}" for k in range(len(shapes))]
     fill = "".join(f"o.in[{k}] = in{k}; " for k in range(len(shapes)))
     params = ", ".join(f"const elem_t* in{k}" for k in range(len(shapes)))
@@ -80,12 +83,12 @@ def emulated(shapes, dtype, split, steps, in_storage, step=None):
     fill_out = "".join(f"o.out[{k}] = out{k}; " for k in range(len(shapes)))
     which = "true" if step else "false"
     wrappers = f"""
-extern "C" void emu_norm(const Matrix* m, const Tile* t, double* s, {params}) {{ Operands o{{}}; {fill} norm_part<{which}>(m, t, s, o); }}
-extern "C" void emu_convert(const Matrix* m, const Tile* t, const double* s, char* ws, {params}) {{ Operands o{{}}; {fill} convert_block<{which}>(m, t, s, ws, o); }}
-extern "C" void emu_finish(const Matrix* m, const Tile* t, const char* ws, {params}, {outs}) {{ Operands o{{}}; {fill} {fill_out} finish_block<{which}>(m, t, ws, o); }}
-extern "C" void emu_gram(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<GRAM>(m, t, ws, *turn); }}
-extern "C" void emu_square(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<SQUARE>(m, t, ws, *turn); }}
-extern "C" void emu_apply(const Matrix* m, const Tile* t, char* ws, const u32* turn) {{ product<APPLY>(m, t, ws, *turn); }}
+extern "C" void emu_norm(const Matrix* m, const Block* t, double* s, {params}) {{ Operands o{{}}; {fill} norm_part<{which}>(m, t, s, o); }}
+extern "C" void emu_convert(const Matrix* m, const Block* t, const double* s, char* ws, {params}) {{ Operands o{{}}; {fill} convert_block<{which}>(m, t, s, ws, o); }}
+extern "C" void emu_finish(const Matrix* m, const Block* t, const char* ws, {params}, {outs}) {{ Operands o{{}}; {fill} {fill_out} finish_block<{which}>(m, t, ws, o); }}
+extern "C" void emu_gram(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<GRAM>(m, t, ws, parked, tickets, *turn, *last); }}
+extern "C" void emu_square(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<SQUARE>(m, t, ws, parked, tickets, *turn, *last); }}
+extern "C" void emu_apply(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<APPLY>(m, t, ws, parked, tickets, *turn, *last); }}
 """
     text = SHFL + muon.source + wrappers
     given = [(a, 0) for a in in_storage]
@@ -100,9 +103,10 @@ extern "C" void emu_apply(const Matrix* m, const Tile* t, char* ws, const u32* t
         given = [(a, 0) for a in in_storage] + [b for m, n, w in zip(momenta, new_momenta, weights) for b in ((m, 0), (n, 0), (w, 0))]
     ws, = run_kernel(text, "emu_convert", len(blocks), 256, [(mats, 0), (blocks, 0), (sums, 0), (np.empty(workspace, np.uint8), 1)] + given)
     for k in range(steps):
-        turn = np.array([k & 1], np.uint32)
-        for entry, tiles in (("emu_gram", lower), ("emu_square", lower), ("emu_apply", whole)):
-            ws, = run_kernel(text, entry, len(tiles), threads, [(mats, 0), (tiles, 0), (ws, 2), (turn, 0)])
+        turn, last = np.array([k & 1], np.uint32), np.array([k == steps - 1], np.uint32)
+        for entry, tasks in (("emu_gram", gram), ("emu_square", square), ("emu_apply", apply)):
+            ws, _, left = run_kernel(text, entry, len(tasks), threads, [(mats, 0), (tasks, 0), (ws, 2), (parked, 1), (tickets, 2), (turn, 0), (last, 0)])
+            assert not left.any(), "tickets not back at zero"
     outs = [np.empty(s, np.float32 if step else in_storage[0].dtype) for s in shapes]
     return run_kernel(text, "emu_finish", len(blocks), 256, [(mats, 0), (blocks, 0), (ws, 0)] + given + [(o, 1) for o in outs]), new_momenta
 
