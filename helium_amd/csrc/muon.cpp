@@ -3,6 +3,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <functional>
+#include <future>
+#include <queue>
 #include <sstream>
 
 namespace he {
@@ -26,8 +29,8 @@ typedef unsigned long long u64;
 typedef _Float16 f16_t;
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef u32 u32x4 __attribute__((ext_vector_type(4)));
 #if BF16
 typedef __bf16 elem_t;
 #elif F16
@@ -41,16 +44,6 @@ typedef float elem_t;
 #endif
 #ifndef WAIT_LOADS
 #define WAIT_LOADS(n) (0x0070 | ((n) & 15) | (((n) >> 4) << 14))   /* vmcnt(n), and lgkmcnt(0): this wave's reads of LDS are done */
-#endif
-#ifndef KERNEL_ATTRS
-#define KERNEL_ATTRS __attribute__((amdgpu_waves_per_eu(2, 2)))
-#endif
-#ifndef HE_WS_STORE
-// Partial results on their way to another workgroup: device-scope accesses go past the L2 of the XCD they come from, so what is
-// written this way and waited for before a ticket is taken is there for whoever sees the ticket.
-#define HE_WS_STORE(p, v) __hip_atomic_store((p), (v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-#define HE_WS_LOAD(p) __hip_atomic_load((p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-#define HE_WS_TICKET(p) __hip_atomic_fetch_add((p), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
 #endif
 struct Matrix {
     u32 rows, cols, mp, np;
@@ -293,22 +286,23 @@ extern "C" __global__ __launch_bounds__(256) void muon_finish_step(const Matrix*
 //   square  B = b A + c A A     P = Q = A, E = A     lower tiles, stored twice
 //   apply   X = a X + B X       P = B, Q = XT, E = X  whole, stored as X and as XT
 const char* kProduct = R"HIP(
-#define BM TILE
-#define BN TILE
 #define WAVES (WAVES_M * WAVES_N)
-#define WTM (BM / WAVES_M)
-#define WTN (BN / WAVES_N)
+#define WTM (TILE / WAVES_M)
+#define WTN (TILE / WAVES_N)
 #define MB (WTM / 32)
 #define NB (WTN / 32)
-#define BK (64 / PARTS)                 /* values of a row in a k-tile: 128 bytes */
-#define KS (BK / 16)                    /* matrix instructions along a k-tile */
-#define STAGE_HALVES ((BM + BN) * 64)
-#define LOADS ((BM + BN) / 8 / WAVES)   /* direct loads of a wave per k-tile: 8 rows of 128 bytes each */
-#define SROWS (WTM < 64 ? WTM : 64)     /* a wave's strip: rows and columns of results that go through LDS at a time */
-#define SCOLS (WTN < 64 ? WTN : 64)
-#define STRIP_PITCH (SCOLS + 1)         /* odd: rows and columns are both read without bank conflicts */
-#define STRIP_FLOATS (WAVES * SROWS * STRIP_PITCH)
-#define LDS_HALVES (STAGES * STAGE_HALVES > 2 * STRIP_FLOATS ? STAGES * STAGE_HALVES : 2 * STRIP_FLOATS)
+#define ROW 64                          /* halves of a row in a k-tile: 128 bytes, 8 chunks */
+#define KS (4 / PARTS)                  /* matrix instructions along a k-tile */
+#define STAGE_HALVES (2 * TILE * ROW)
+#define LOADS (2 * TILE / 8 / WAVES)    /* direct loads of a wave per k-tile: 8 rows each */
+#define READS (PARTS * (MB + NB))       /* fragments of one k-step */
+#define MMAS ((SPLIT ? 3 : 1) * MB * NB)
+#define SM (MB % 2 ? 1 : 2)             /* a wave's strip, in blocks of 32 x 32: what goes through LDS at a time */
+#define SN (NB % 2 ? 1 : 2)
+#define STRIP_FLOATS(sm, sn) ((sm) * 32 * ((sn) * 32 + 1))   /* odd pitch: rows and columns are both read without bank conflicts */
+#define STRIPS_HALVES (2 * WAVES * STRIP_FLOATS(SM, SN))
+#define LDS_HALVES (STAGES * STAGE_HALVES > STRIPS_HALVES ? STAGES * STAGE_HALVES : STRIPS_HALVES)
+#define PARKED (TILE * TILE)            /* floats of a tile that waits to be added up */
 enum { GRAM, SQUARE, APPLY };
 
 __device__ __forceinline__ void strip_sync() {
@@ -317,25 +311,80 @@ __device__ __forceinline__ void strip_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ shared_tiles, u32* __restrict__ tickets, u32 turn, u32 last_step) {
+// The results of 32 RM x 32 RN sums at (row0, col0) of the product. A lane holds rows (e / 4) * 8 + half * 4 + e % 4 of column lane % 32
+// of each 32 x 32 block; through a strip of LDS that belongs to the wave it gets 8 neighbours of a row, adds E, stores them, and
+// puts them back for the transposed copy.
+template <int STAGE, int RM, int RN>
+__device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix& m, char* __restrict__ ws, u32 row0, u32 col0, bool mirrored, u32 turn, float* strip) {
+    constexpr u32 strip_pitch = RN * 32 + 1, row_lanes = RN * 4, col_lanes = RM * 4;   // lanes along a row of the strip, and along a column
+    const u32 lane = threadIdx.x & 63u, half = lane >> 5;
+    const u32 pitch = STAGE == APPLY ? m.np : m.mp;
+    const f16_t* e_rows = (const f16_t*)(ws + (STAGE == SQUARE ? m.a : m.x));
+    f16_t *plain = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.x)), *turned = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.xt[turn ^ 1u]));
+    // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
+    // singular values with it)
+    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.x_low) : nullptr;
+#pragma unroll
+    for (int i = 0; i < RM; i++)
+#pragma unroll
+        for (int j = 0; j < RN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) strip[(i * 32 + (e / 4) * 8 + half * 4 + e % 4) * strip_pitch + j * 32 + (lane & 31u)] = acc[i][j][e];
+    strip_sync();
+#pragma unroll
+    for (u32 s = 0; s < RM * 32 * row_lanes / 64; s++) {
+        const u32 r = s * (64 / row_lanes) + lane / row_lanes, c = lane % row_lanes * 8;
+        float v[8], other[8];
+        if (STAGE != GRAM) get(e_rows, row0 + r, col0 + c, pitch, other, low);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float sum = strip[r * strip_pitch + c + e];
+            v[e] = STAGE == GRAM ? sum * (A_SCALE / (X_SCALE * X_SCALE))
+                 : STAGE == SQUARE ? NS_B * other[e] + (NS_C * B_SCALE / (A_SCALE * A_SCALE)) * sum
+                                   : NS_A * other[e] + (1.0f / B_SCALE) * sum;
+            strip[r * strip_pitch + c + e] = v[e];
+        }
+        put(plain, row0 + r, col0 + c, pitch, v, low);
+    }
+    strip_sync();
+    if (mirrored)
+#pragma unroll
+        for (u32 s = 0; s < RN * 32 * col_lanes / 64; s++) {
+            const u32 c = s * (64 / col_lanes) + lane / col_lanes, r = lane % col_lanes * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = strip[(r + e) * strip_pitch + c];
+            put(turned, col0 + c, row0 + r, m.mp, v, nullptr);
+        }
+    strip_sync();
+}
+
+struct Fragments { f16x8 a[PARTS][MB], b[PARTS][NB]; };
+struct True { constexpr operator bool() const { return true; } };
+struct False { constexpr operator bool() const { return false; } };
+
+template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u32 turn, u32 last_step) {
     __shared__ __attribute__((aligned(16))) f16_t lds[LDS_HALVES];
-    __shared__ u32 last;
     const Task t = tasks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
     const u32 k_len = (STAGE == GRAM ? m.np : m.mp) * PARTS;   // halves of a row
-    const f16_t* p_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b)) + (u64)t.i * BM * k_len;
-    const f16_t* q_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[turn])) + (u64)t.j * BN * k_len;
-    // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows
-    // meet 8 different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes.
+    const u32 p_limit = m.mp, q_limit = STAGE == APPLY ? m.np : m.mp;
+    const f16_t* p_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b));
+    const f16_t* q_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[turn]));
+    // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows meet 8
+    // different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes. (A tile that ends beyond the matrix loads its first rows
+    // there: sums that nothing stores.)
     const u32 lane_off = (lane >> 3) * k_len + (((lane & 7u) ^ (lane >> 3)) << 3);
     auto fetch = [&](u32 kt, u32 slot) {
         f16_t* base = lds + slot * STAGE_HALVES;
 #pragma unroll
         for (int l = 0; l < LOADS; l++) {
             const u32 row = (wave * LOADS + l) * 8;   // of P's rows, then Q's
-            const f16_t* src = (row < BM ? p_rows + (u64)row * k_len : q_rows + (u64)(row - BM) * k_len) + (u64)kt * 64 + lane_off;
-            __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * 64), 16, 0, 0);
+            const bool is_p = row < TILE;
+            const u32 at = is_p ? t.i * TILE + row : t.j * TILE + row - TILE, limit = is_p ? p_limit : q_limit;
+            const f16_t* src = (is_p ? p_rows : q_rows) + (u64)(at < limit ? at : 0u) * k_len + (u64)kt * ROW + lane_off;
+            __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * ROW), 16, 0, 0);
         }
     };
     f32x16 acc[MB][NB];
@@ -346,139 +395,143 @@ template <int STAGE> __device__ __forceinline__ void product(const Matrix* __res
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
     const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane & 7u;
-    u32 slot = 0;
+    Fragments f[2];
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; s++)
-        if (t.k_begin + s < t.k_end) fetch(t.k_begin + s, s);
-    for (u32 kt = t.k_begin; kt < t.k_end; kt++) {
+    for (int part = 0; part < PARTS; part++) {
+#pragma unroll
+        for (int i = 0; i < MB; i++) f[1].a[part][i] = f16x8(f16_t(0.0f));
+#pragma unroll
+        for (int j = 0; j < NB; j++) f[1].b[part][j] = f16x8(f16_t(0.0f));
+    }
+    auto read = [&](Fragments& g, const f16_t* stage, int kk) {
+        const f16_t *p = stage + (wave_m * WTM + frag_row) * ROW, *q = stage + (TILE + wave_n * WTN + frag_row) * ROW;
+#pragma unroll
+        for (int part = 0; part < PARTS; part++) {
+            const u32 chunk = (((kk * 2 + half) * PARTS + part) ^ swz) * 8;
+#pragma unroll
+            for (int i = 0; i < MB; i++) g.a[part][i] = *(const f16x8*)(p + i * 32 * ROW + chunk);
+#pragma unroll
+            for (int j = 0; j < NB; j++) g.b[part][j] = *(const f16x8*)(q + j * 32 * ROW + chunk);
+        }
+    };
+    auto multiply = [&](const Fragments& g) {
+        // high x high, high x low, low x high
+#pragma unroll
+        for (int c = 0; c < (SPLIT ? 3 : 1); c++)
+#pragma unroll
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.a[c == 2][i], g.b[c == 1][j], acc[i][j], 0, 0, 0);
+    };
+    // One k-tile. The loop is rotated by a k-step: the matrix instructions that the last k-tile left over cover the barrier's way, the
+    // first reads of this one and the loads of the one to come; each further step's reads are issued between the instructions of
+    // the step before. The order is asked for, since the compiler by itself reads, waits and multiplies in turn.
+    u32 slot = 0;
+    auto k_tile = [&](u32 kt, auto more) {
         // this wave's loads of the k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'
-        if (kt + STAGES - 2 < t.k_end) __builtin_amdgcn_s_waitcnt(WAIT_LOADS((STAGES - 2) * LOADS));
+        if (more) __builtin_amdgcn_s_waitcnt(WAIT_LOADS((STAGES - 2) * LOADS));
         else __builtin_amdgcn_s_waitcnt(WAIT_LOADS(0));
         // (the bare barrier: __syncthreads() would wait for all loads; no wave still reads the stage that is filled next)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (kt + STAGES - 1 < t.k_end) fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1);
-        const f16_t *p = lds + slot * STAGE_HALVES + (wave_m * WTM + frag_row) * 64, *q = lds + slot * STAGE_HALVES + (BM + wave_n * WTN + frag_row) * 64;
+        const f16_t* stage = lds + slot * STAGE_HALVES;
+        read(f[0], stage, 0);
+        if (more) fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1);
+        multiply(f[1]);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
-        for (int kk = 0; kk < KS; kk++) {
-            f16x8 a[PARTS][MB], b[PARTS][NB];
+        for (int n = 0; n < MMAS; n++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) {
-                const u32 chunk = (((kk * 2 + half) * PARTS + part) ^ swz) * 8;
+            for (int l = n * LOADS / MMAS; l < (n + 1) * LOADS / MMAS; l++)
+                if (more) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
 #pragma unroll
-                for (int i = 0; i < MB; i++) a[part][i] = *(const f16x8*)(p + i * 32 * 64 + chunk);
+        for (int kk = 1; kk < KS; kk++) {
+            read(f[kk & 1], stage, kk);
+            multiply(f[(kk & 1) ^ 1]);
 #pragma unroll
-                for (int j = 0; j < NB; j++) b[part][j] = *(const f16x8*)(q + j * 32 * 64 + chunk);
+            for (int n = 0; n < MMAS; n++) {
+                // (reads behind the first instruction: the wait for its operands is for all reads before it)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (n * 2 < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (n * 2 + 1 < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            // high x high, high x low, low x high
-#pragma unroll
-            for (int c = 0; c < (SPLIT ? 3 : 1); c++)
-#pragma unroll
-                for (int i = 0; i < MB; i++)
-#pragma unroll
-                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[c == 2][i], b[c == 1][j], acc[i][j], 0, 0, 0);
         }
         slot = slot + 1 < STAGES ? slot + 1 : 0;
-    }
+    };
+    const u32 k_count = t.k_end - t.k_begin, ahead = STAGES - 1 < k_count ? STAGES - 1 : k_count;
+    for (u32 s = 0; s < ahead; s++) fetch(t.k_begin + s, s);
+    u32 kt = t.k_begin;
+    for (; kt + ahead < t.k_end; kt++) k_tile(kt, True());
+    for (; kt < t.k_end; kt++) k_tile(kt, False());
+    multiply(f[1]);
 
-    // A tile whose sum several workgroups share: each parks its part, the last to arrive adds them up in their order and goes on.
+    // A share of a tile's sum waits in memory for the launch that adds them up, block by block of 32 x 32, as the lanes hold it.
     if (t.shares > 1) {
-        u64* mine = (u64*)(shared_tiles + (u64)(t.slot + t.share) * (BM * BN)) + wave * (WTM * WTN / 2) + lane;
+        f32x4* to = (f32x4*)(parked + (u64)(t.slot + t.share) * PARKED);
 #pragma unroll
         for (int i = 0; i < MB; i++)
 #pragma unroll
             for (int j = 0; j < NB; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float two[2] = {acc[i][j][2 * e], acc[i][j][2 * e + 1]};
-                    HE_WS_STORE(mine + ((i * NB + j) * 8 + e) * 64, __builtin_bit_cast(u64, two));
+                for (int e = 0; e < 4; e++) {
+                    f32x4 four = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+                    to[((wave_m * MB + i) * (TILE / 32) + wave_n * NB + j) * 256 + e * 64 + lane] = four;
                 }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (threadIdx.x == 0) last = HE_WS_TICKET(tickets + t.slot) + 1 == t.shares;
-        __syncthreads();
-        if (!last) return;
-        if (threadIdx.x == 0) HE_WS_STORE(tickets + t.slot, 0u);   // as the next launch wants it
-#pragma unroll
-        for (int i = 0; i < MB; i++)
-#pragma unroll
-            for (int j = 0; j < NB; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-        for (u32 s = 0; s < t.shares; s++) {
-            const u64* from = (const u64*)(shared_tiles + (u64)(t.slot + s) * (BM * BN)) + wave * (WTM * WTN / 2) + lane;
-#pragma unroll
-            for (int i = 0; i < MB; i++)
-#pragma unroll
-                for (int j = 0; j < NB; j++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        struct Two { float v[2]; } two = __builtin_bit_cast(Two, HE_WS_LOAD(from + ((i * NB + j) * 8 + e) * 64));
-                        acc[i][j][2 * e] += two.v[0];
-                        acc[i][j][2 * e + 1] += two.v[1];
-                    }
-        }
+        return;
     }
     __syncthreads();   // the operand stages become the waves' strips
-
-    // Results: a lane holds rows (e / 4) * 8 + half * 4 + e % 4 of column lane % 32 of each 32 x 32 block. Through a strip in LDS a lane gets
-    // 8 neighbours of a row, adds E, stores them, and puts them back for the transposed copy.
-    const u32 pitch = STAGE == APPLY ? m.np : m.mp;
-    const f16_t* e_rows = (const f16_t*)(ws + (STAGE == SQUARE ? m.a : m.x));
-    f16_t *plain = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.x)), *turned = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.xt[turn ^ 1u]));
-    // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
-    // singular values with it)
-    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.x_low) : nullptr;
-    float* strip = (float*)lds + wave * (SROWS * STRIP_PITCH);
-    const bool mirrored = STAGE == APPLY ? !last_step : t.i != t.j;
-    constexpr u32 row_lanes = SCOLS / 8, col_lanes = SROWS / 8;   // lanes along a row of the strip, and along a column
+    float* strip = (float*)lds + wave * STRIP_FLOATS(SM, SN);
 #pragma unroll
-    for (int i = 0; i < WTM / SROWS; i++)
+    for (int i = 0; i < MB; i += SM)
 #pragma unroll
-        for (int j = 0; j < WTN / SCOLS; j++) {
-            const u32 row0 = t.i * BM + wave_m * WTM + i * SROWS, col0 = t.j * BN + wave_n * WTN + j * SCOLS;
+        for (int j = 0; j < NB; j += SN) {
+            const u32 row0 = t.i * TILE + (wave_m * MB + i) * 32, col0 = t.j * TILE + (wave_n * NB + j) * 32;
+            if (row0 >= p_limit || col0 >= q_limit) continue;
+            f32x16 part[SM][SN];
 #pragma unroll
-            for (int di = 0; di < SROWS / 32; di++)
+            for (int di = 0; di < SM; di++)
 #pragma unroll
-                for (int dj = 0; dj < SCOLS / 32; dj++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        strip[(di * 32 + (e / 4) * 8 + half * 4 + e % 4) * STRIP_PITCH + dj * 32 + frag_row] = acc[i * (SROWS / 32) + di][j * (SCOLS / 32) + dj][e];
-            strip_sync();
-#pragma unroll
-            for (u32 s = 0; s < SROWS * row_lanes / 64; s++) {
-                const u32 r = s * (64 / row_lanes) + lane / row_lanes, c = lane % row_lanes * 8;
-                float v[8], other[8];
-                if (STAGE != GRAM) get(e_rows, row0 + r, col0 + c, pitch, other, low);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float sum = strip[r * STRIP_PITCH + c + e];
-                    v[e] = STAGE == GRAM ? sum * (A_SCALE / (X_SCALE * X_SCALE))
-                         : STAGE == SQUARE ? NS_B * other[e] + (NS_C * B_SCALE / (A_SCALE * A_SCALE)) * sum
-                                           : NS_A * other[e] + (1.0f / B_SCALE) * sum;
-                    strip[r * STRIP_PITCH + c + e] = v[e];
-                }
-                put(plain, row0 + r, col0 + c, pitch, v, low);
-            }
-            strip_sync();
-            if (mirrored)
-#pragma unroll
-                for (u32 s = 0; s < SCOLS * col_lanes / 64; s++) {
-                    const u32 c = s * (64 / col_lanes) + lane / col_lanes, r = lane % col_lanes * 8;
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = strip[(r + e) * STRIP_PITCH + c];
-                    put(turned, col0 + c, row0 + r, m.mp, v, nullptr);
-                }
-            strip_sync();
+                for (int dj = 0; dj < SN; dj++) part[di][dj] = acc[i + di][j + dj];
+            finish<STAGE, SM, SN>(part, m, ws, row0, col0, STAGE == APPLY ? !last_step : t.i != t.j, turn, strip);
         }
 }
 
-#define KERNEL(name, stage) extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ shared_tiles, u32* __restrict__ tickets, u32 turn, u32 last_step) { product<stage>(mats, tasks, ws, shared_tiles, tickets, turn, last_step); }
-KERNEL(muon_gram, GRAM)
-KERNEL(muon_square, SQUARE)
-KERNEL(muon_apply, APPLY)
+// The shares of a tile added up in their order: a wave per 32 x 32 block, four waves in a workgroup. `tiles`: the first share's task of each.
+template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u32 turn, u32 last_step) {
+    __shared__ float strips[4 * STRIP_FLOATS(1, 1)];
+    constexpr u32 blocks = (TILE / 32) * (TILE / 32);
+    const Task t = tiles[blockIdx.x / (blocks / 4)];
+    const Matrix& m = mats[t.matrix];
+    const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x % (blocks / 4) * 4 + wave;
+    const u32 row0 = t.i * TILE + block / (TILE / 32) * 32, col0 = t.j * TILE + block % (TILE / 32) * 32;
+    if (row0 >= m.mp || col0 >= (STAGE == APPLY ? m.np : m.mp)) return;
+    const f32x4* from = (const f32x4*)(parked + (u64)t.slot * PARKED) + block * 256 + lane;
+    f32x16 sum[1][1];
+#pragma unroll
+    for (int e = 0; e < 16; e++) sum[0][0][e] = 0.0f;
+    for (u32 s = 0; s < t.shares; s += 4) {
+        f32x4 got[4][4];
+#pragma unroll
+        for (u32 d = 0; d < 4; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                got[d][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (s + d < t.shares) got[d][e] = from[(u64)(s + d) * (PARKED / 4) + e * 64];
+            }
+#pragma unroll
+        for (u32 d = 0; d < 4; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sum[0][0][e] += got[d][e / 4][e % 4];
+    }
+    finish<STAGE, 1, 1>(sum, m, ws, row0, col0, STAGE == APPLY ? !last_step : t.i != t.j, turn, strips + wave * STRIP_FLOATS(1, 1));
+}
+
+#define KERNELS(name, stage) \
+    extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void muon_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u32 turn, u32 last_step) { product<stage>(mats, tasks, ws, parked, turn, last_step); } \
+    extern "C" __global__ __launch_bounds__(256) void muon_join_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u32 turn, u32 last_step) { join<stage>(mats, tiles, ws, parked, turn, last_step); }
 )HIP";
 
 struct OperandsArg {
@@ -504,38 +557,64 @@ void deal(std::vector<MuonTask>& tasks) {
     tasks.swap(out);
 }
 
-// The tasks of one product of every matrix: bands of four tile rows, column by column; a tile's sum is dealt to several workgroups
-// where there are too few tiles to fill the chip. `slots`: workgroups that it runs at once; `least`: k-tiles a share has at least.
-std::vector<MuonTask> tasks_of(const std::vector<MuonMatrix>& mats, uint32_t tile, bool lower, bool along_n, uint32_t bk, uint32_t slots, uint32_t least,
-                               uint32_t* shared) {
-    uint64_t units = 0, tiles = 0;
-    for (const MuonMatrix& m : mats) {
-        const uint64_t ti = m.mp / tile, count = lower ? ti * (ti + 1) / 2 : ti * (m.np / tile);
-        tiles += count;
-        units += count * ((along_n ? m.np : m.mp) / bk);
-    }
-    const uint64_t target = tiles >= slots ? units : std::max<uint64_t>(least, (units + slots - 1) / slots);
-    std::vector<MuonTask> out;
-    *shared = 0;
+// How a product's tiles are made: the waves of a workgroup, its ring of k-tiles in LDS, and the workgroups that a CU holds. And what
+// the choice between them goes by, microseconds measured on products of 64 to 4096 rows: a task's `base`, and what a k-tile takes
+// in a workgroup that has a CU to itself (`alone`) and on a full chip, for operands of one part and of two.
+struct TileShape {
+    uint32_t tile, waves_m, waves_n, stages, per_cu;
+    const char* attrs;
+    double base, alone[2], full[2];
+};
+const TileShape kTiles[] = {
+    {64, 2, 2, 4, 2, "", 2.5, {0.22, 0.28}, {0.42, 0.50}},
+    {128, 2, 2, 2, 2, "__attribute__((amdgpu_waves_per_eu(2, 2)))", 3.5, {0.65, 0.85}, {1.17, 1.65}},
+    {192, 2, 2, 3, 1, "__attribute__((amdgpu_waves_per_eu(1, 1)))", 5.0, {0.70, 0.85}, {1.13, 2.00}},
+    {256, 2, 4, 2, 1, "__attribute__((amdgpu_waves_per_eu(2, 2)))", 6.0, {1.25, 2.00}, {1.80, 2.85}},
+};
+constexpr uint32_t kCUs = 256;
+
+// How one product of every matrix is cut into tasks: tiles, and where there are too few of them to fill the chip or their sums are
+// long, shares of `target` k-tiles or a little more of each sum, which a second launch adds up.
+struct Cut {
+    std::vector<MuonTask> tasks, joins;  // joins: a task of each tile that is shared
+    uint32_t parked = 0;                 // shares that wait in memory
+    double estimate = 0;                 // microseconds
+};
+Cut cut_product(const std::vector<MuonMatrix>& mats, const TileShape& shape, bool lower, bool along_n, int parts, uint32_t target) {
+    Cut cut;
+    const uint32_t tile = shape.tile, bk = 64 / parts;
+    auto over = [&](uint32_t extent) { return (extent + tile - 1) / tile; };
     for (size_t k = 0; k < mats.size(); k++) {
         const MuonMatrix& m = mats[k];
-        const uint32_t ti = m.mp / tile, tj = lower ? ti : m.np / tile, kt = (along_n ? m.np : m.mp) / bk;
-        const uint32_t shares = (uint32_t)std::max<uint64_t>(1, kt / target);
-        for (uint32_t g = 0; g < ti; g += 4)
+        const uint32_t ti = over(m.mp), tj = lower ? ti : over(m.np), kt = (along_n ? m.np : m.mp) / bk, shares = std::max(1u, kt / target);
+        for (uint32_t g = 0; g < ti; g += 4)  // bands of four tile rows, column by column
             for (uint32_t j = 0; j < tj; j++)
                 for (uint32_t i = g; i < std::min(g + 4, ti); i++) {
                     if (lower && j > i) continue;
                     for (uint32_t s = 0; s < shares; s++)
-                        out.push_back({(uint32_t)k, i, j, (uint32_t)((uint64_t)kt * s / shares), (uint32_t)((uint64_t)kt * (s + 1) / shares), *shared, s, shares});
-                    if (shares > 1) *shared += shares;
+                        cut.tasks.push_back({(uint32_t)k, i, j, (uint32_t)((uint64_t)kt * s / shares), (uint32_t)((uint64_t)kt * (s + 1) / shares), cut.parked, s, shares});
+                    if (shares > 1) {
+                        cut.joins.push_back(cut.tasks.back());
+                        cut.parked += shares;
+                    }
                 }
     }
-    deal(out);
-    return out;
+    deal(cut.tasks);
+    // Every task goes to the workgroup place that is free first; a k-tile takes the longer the fuller the chip is.
+    const size_t slots = (size_t)kCUs * shape.per_cu;
+    const double f = std::min(1.0, (double)cut.tasks.size() / slots), each = shape.alone[parts - 1] + (shape.full[parts - 1] - shape.alone[parts - 1]) * f * f;
+    std::priority_queue<double, std::vector<double>, std::greater<double>> free_at;
+    for (const MuonTask& t : cut.tasks) {
+        const double begin = free_at.size() < slots ? 0.0 : free_at.top();
+        if (free_at.size() == slots) free_at.pop();
+        const double end = begin + shape.base + each * (t.k_end - t.k_begin);
+        free_at.push(end);
+        cut.estimate = std::max(cut.estimate, end);
+    }
+    // (a launch, and the shares read at about 5 TB/s)
+    if (cut.parked) cut.estimate += 2.5 + 4.0 * cut.parked * tile * tile / 5e6;
+    return cut;
 }
-
-int env_int(const char* name, int dflt) { return tuning::get_int(name, dflt); }
-
 template <class T> std::vector<char> bytes_of(const std::vector<T>& v) {
     std::vector<char> out(v.size() * sizeof(T));
     if (!v.empty()) memcpy(out.data(), v.data(), out.size());
@@ -548,9 +627,6 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     HE_REQUIRE(!pr.shapes.empty() && pr.shapes.size() <= 65536, HE_ERR_INVALID, "muon: %zu matrices, 1 to 65536 are taken", pr.shapes.size());
     HE_REQUIRE(pr.dtype == HE_F16 || pr.dtype == HE_BF16 || pr.dtype == HE_F32, HE_ERR_INVALID, "muon does not take dtype %s", dtype_name(pr.dtype));
     HE_REQUIRE(pr.steps >= 1 && pr.steps <= 32, HE_ERR_INVALID, "muon: %d steps, 1 to 32 are taken", pr.steps);
-    const uint32_t tile = (uint32_t)env_int("HELIUM_HIP_MUON_TILE", 128), stages = (uint32_t)env_int("HELIUM_HIP_MUON_STAGES", 2), bk = pr.split ? 32 : 64;
-    const uint32_t waves_m = tile == 64 ? 2 : 2, waves_n = tile == 256 ? 4 : 2;
-    threads_ = waves_m * waves_n * 64;
     uint64_t at = 0, parts = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -565,7 +641,7 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
                    "muon: matrix %zu is %lld x %lld; extents up to 2^20 by 32768 are taken", k, (long long)rows, (long long)cols);
         MuonMatrix m{};
         m.rows = (uint32_t)rows, m.cols = (uint32_t)cols, m.tall = rows > cols;
-        auto padded = [&](int64_t v) { return (uint32_t)((v + tile - 1) / tile * tile); };
+        auto padded = [&](int64_t v) { return (uint32_t)((v + kBlock - 1) / kBlock * kBlock); };
         m.mp = padded(std::min(rows, cols)), m.np = padded(std::max(rows, cols));
         m.shape_scale = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
         const uint64_t bytes = pr.split ? 4 : 2, x = m.mp * bytes * m.np, a = m.mp * bytes * m.mp;
@@ -586,38 +662,76 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     }
     part_begin_.push_back((uint32_t)shares.size());
     block_begin_.push_back((uint32_t)blocks.size());
-    const uint32_t slots = 256 * (tile == 256 ? 1 : 2), least = (uint32_t)env_int("HELIUM_HIP_MUON_LEAST", 8);
-    uint32_t shared[3];
-    const std::vector<MuonTask> gram = tasks_of(matrices_, tile, true, true, bk, slots, least, &shared[0]),
-                                square = tasks_of(matrices_, tile, true, false, bk, slots, least, &shared[1]),
-                                apply = tasks_of(matrices_, tile, false, false, bk, slots, least, &shared[2]);
-    const uint32_t most = std::max({shared[0], shared[1], shared[2]});
-    tickets_ = most;
-    tickets_at_ = take((uint64_t)most * 4);
-    shared_at_ = take((uint64_t)most * tile * tile * 4);
+    // the products, largest extent first: A = X X^T along n, B from A A and X from B X along m
+    const char* names[3] = {"gram", "square", "apply"};
+    uint32_t most = 0;
+    std::string cuts;
+    for (int p = 0; p < 3; p++) {
+        Product& product = products_[p];
+        const int forced = tuning::get_int("HELIUM_HIP_MUON_TILE", -1), only = forced >= 0 ? forced : tuning::get_int((std::string("HELIUM_HIP_MUON_TILE_") + names[p]).c_str(), -1);
+        const TileShape* chosen = nullptr;
+        Cut cut;
+        for (const TileShape& candidate : kTiles)
+            for (uint32_t target : {1u << 30, 64u, 32u, 16u, 8u, 4u}) {
+                if (only >= 0 && candidate.tile != (uint32_t)only) continue;
+                Cut c = cut_product(matrices_, candidate, p < 2, p == 0, pr.split ? 2 : 1, target);
+                if (c.tasks.size() >= (1u << 28) || (uint64_t)c.parked * candidate.tile * candidate.tile >= (1u << 30) || (chosen && c.estimate >= cut.estimate)) continue;
+                cut = std::move(c);
+                chosen = &candidate;
+            }
+        HE_REQUIRE(chosen, HE_ERR_UNSUPPORTED, "muon: the group is too large for one launch");
+        const TileShape& shape = *chosen;
+        const std::vector<MuonTask>&tasks = cut.tasks, &joins = cut.joins;
+        const uint32_t parked = cut.parked;
+        tables_[1 + p] = bytes_of(tasks), tables_[4 + p] = bytes_of(joins);
+        product.threads = shape.waves_m * shape.waves_n * 64;
+        product.grid = (uint32_t)tasks.size();
+        product.join_grid = (uint32_t)joins.size() * (shape.tile / 32) * (shape.tile / 32) / 4;
+        product.text = strfmt("#define TILE %u\n#define WAVES_M %u\n#define WAVES_N %u\n#define STAGES %u\n#ifndef KERNEL_ATTRS\n#define KERNEL_ATTRS %s\n#endif\n", shape.tile,
+                              shape.waves_m, shape.waves_n, shape.stages, shape.attrs);
+        most = std::max(most, parked * shape.tile * shape.tile);
+        cuts += strfmt("\nmuon_%s tile=%u threads=%u stages=%u grid=%u join_grid=%u parked=%u estimate=%.1f", names[p], shape.tile, product.threads, shape.stages, product.grid,
+                       product.join_grid, parked * shape.tile * shape.tile, cut.estimate);
+    }
+    shared_at_ = take((uint64_t)most * 4);
     // (a share's place among the sums is its block's, plus where its launch begins)
     for (size_t k = 0; k < pr.shapes.size(); k++)
         for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) shares[p].j = part_begin_[k / kGroup * kGroup];
     workspace_bytes_ = take(parts * sizeof(double)) + parts * sizeof(double);
-    tables_[0] = bytes_of(matrices_), tables_[1] = bytes_of(gram), tables_[2] = bytes_of(square), tables_[3] = bytes_of(apply);
-    tables_[4] = bytes_of(shares), tables_[5] = bytes_of(blocks);
-    table_size_ = {(uint32_t)matrices_.size(), (uint32_t)gram.size(), (uint32_t)square.size(), (uint32_t)apply.size(), (uint32_t)shares.size(), (uint32_t)blocks.size()};
+    tables_[0] = bytes_of(matrices_), tables_[7] = bytes_of(shares), tables_[8] = bytes_of(blocks);
+    shares_ = (uint32_t)shares.size();
     for (int t = 0; t < kTables; t++) {
         table_at_[t] = table_bytes_;
         table_bytes_ += (tables_[t].size() + 255) / 256 * 256;
     }
     std::ostringstream s;
     s << "#define GROUP " << kGroup << "\n#define PART " << kPart << "ull\n#define STEPS " << pr.steps << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
-      << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define NORM_FLOOR 1e-7\n#define TILE " << tile << "\n#define WAVES_M " << waves_m
-      << "\n#define WAVES_N " << waves_n << "\n#define STAGES " << stages << "\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
-    source_ = s.str() + kCommon + kElements + kProduct;
-    auto make = [&](const char* entry) { return std::make_unique<JitKernel>(source_, entry); };
-    norm_ = make("muon_norm"), convert_ = make("muon_convert"), finish_ = make("muon_finish");
-    norm_step_ = make("muon_norm_step"), convert_step_ = make("muon_convert_step"), finish_step_ = make("muon_finish_step");
-    gram_ = make("muon_gram"), square_ = make("muon_square"), apply_ = make("muon_apply");
-    describe_ = strfmt("muon matrices=%zu steps=%d parts=%d tile=%u threads=%u stages=%u gram=%u square=%u apply=%u shared=%u,%u,%u shares=%u blocks=%u tickets_at=%zu shared_at=%zu workspace=%zu",
-                       pr.shapes.size(), pr.steps, pr.split ? 2 : 1, tile, threads_, stages, table_size_[1], table_size_[2], table_size_[3], shared[0], shared[1], shared[2],
-                       table_size_[4], table_size_[5], tickets_at_, shared_at_, workspace_bytes_);
+      << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define NORM_FLOOR 1e-7\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
+    const std::string head = s.str() + kCommon;
+    std::vector<std::pair<std::unique_ptr<JitKernel>*, std::pair<std::string, std::string>>> kernels;  // where to, text, entry
+    const std::string elements = head + kElements;
+    for (auto& k : {std::make_pair(&norm_, "muon_norm"), std::make_pair(&convert_, "muon_convert"), std::make_pair(&finish_, "muon_finish"), std::make_pair(&norm_step_, "muon_norm_step"),
+                    std::make_pair(&convert_step_, "muon_convert_step"), std::make_pair(&finish_step_, "muon_finish_step")})
+        kernels.push_back({k.first, {elements, k.second}});
+    source_ = elements;
+    for (int p = 0; p < 3; p++) {
+        const std::string name = names[p];
+        Product& product = products_[p];
+        product.text = head + product.text + kProduct + "KERNELS(" + name + ", " + (p == 0 ? "GRAM" : p == 1 ? "SQUARE" : "APPLY") + ")\n";
+        source_ += "\n//// product " + name + "\n" + product.text;
+        kernels.push_back({&product.kernel, {product.text, "muon_" + name}});
+        if (product.join_grid) kernels.push_back({&product.join, {product.text, "muon_join_" + name}});
+    }
+    // (each text is compiled once, all of them side by side)
+    std::map<std::string, std::future<void>> compiled;
+    for (auto& k : kernels) {
+        const std::string& text = k.second.first;
+        if (!compiled.count(text)) compiled[text] = std::async(std::launch::async, [&text] { (void)rtc_compile(text, "muon", {}); });
+    }
+    for (auto& c : compiled) c.second.get();
+    for (auto& k : kernels) k.first->reset(new JitKernel(k.second.first, k.second.second));
+    describe_ = strfmt("muon matrices=%zu steps=%d parts=%d shares=%u blocks=%zu shared_at=%zu workspace=%zu", pr.shapes.size(), pr.steps, pr.split ? 2 : 1, shares_,
+                       blocks.size(), shared_at_, workspace_bytes_) + cuts;
 }
 
 Muon::~Muon() {
@@ -633,7 +747,6 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
     Buffers b;
     HE_HIP(hipMalloc((void**)&b.tables, table_bytes_));
     hipError_t e = hipMalloc((void**)&b.workspace, workspace_bytes_);
-    if (e == hipSuccess && tickets_) e = hipMemset(b.workspace + tickets_at_, 0, (size_t)tickets_ * 4);
     for (int t = 0; t < kTables && e == hipSuccess; t++) e = hipMemcpy(b.tables + table_at_[t], tables_[t].data(), tables_[t].size(), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
         (void)hipFree(b.tables);
@@ -645,15 +758,18 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
 }
 
 void Muon::products(char* ws, char* tables, hipStream_t stream) {
-    const uint32_t block[3] = {threads_, 1, 1};
-    char *mats = tables + table_at_[0], *shared = ws + shared_at_, *tickets = ws + tickets_at_;
+    const uint32_t join_block[3] = {256, 1, 1};
+    char *mats = tables + table_at_[0], *parked = ws + shared_at_;
     for (int k = 0; k < pr_.steps; k++)
-        for (int stage = 1; stage <= 3; stage++) {
+        for (int p = 0; p < 3; p++) {
+            const Product& product = products_[p];
             uint32_t turn = (uint32_t)k & 1u, last = k == pr_.steps - 1;
-            char* tasks = tables + table_at_[stage];
-            const uint32_t grid[3] = {table_size_[stage], 1, 1};
-            void* args[] = {&mats, &tasks, &ws, &shared, &tickets, &turn, &last};
-            (stage == 1 ? gram_ : stage == 2 ? square_ : apply_)->launch(grid, block, 0, stream, args);
+            char *tasks = tables + table_at_[1 + p], *joins = tables + table_at_[4 + p];
+            const uint32_t grid[3] = {product.grid, 1, 1}, block[3] = {product.threads, 1, 1}, join_grid[3] = {product.join_grid, 1, 1};
+            void* args[] = {&mats, &tasks, &ws, &parked, &turn, &last};
+            product.kernel->launch(grid, block, 0, stream, args);
+            void* join_args[] = {&mats, &joins, &ws, &parked, &turn, &last};
+            if (product.join_grid) product.join->launch(join_grid, join_block, 0, stream, join_args);
         }
 }
 
@@ -679,7 +795,7 @@ void Muon::step_or_not(const void* const* in, const float* const* momenta, const
     std::lock_guard<std::mutex> lk(mu_);
     const Buffers b = buffers(stream);
     char *mats = b.tables + table_at_[0], *ws = b.workspace;
-    double* sums = (double*)(ws + workspace_bytes_ - table_size_[4] * sizeof(double));
+    double* sums = (double*)(ws + workspace_bytes_ - shares_ * sizeof(double));
     const uint32_t block[3] = {256, 1, 1};
     auto each_group = [&](auto&& launch) {
         for (size_t first = 0; first < count(); first += kGroup) {
@@ -695,20 +811,20 @@ void Muon::step_or_not(const void* const* in, const float* const* momenta, const
         }
     };
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* parts = b.tables + table_at_[4] + part_begin_[first] * sizeof(MuonBlock);
+        char* parts = b.tables + table_at_[7] + part_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {part_begin_[last] - part_begin_[first], 1, 1};
         void* args[] = {&mats, &parts, &sums, &o};
         (how ? norm_step_ : norm_)->launch(grid, block, 0, stream, args);
     });
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* blocks = b.tables + table_at_[5] + block_begin_[first] * sizeof(MuonBlock);
+        char* blocks = b.tables + table_at_[8] + block_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {block_begin_[last] - block_begin_[first], 1, 1};
         void* args[] = {&mats, &blocks, &sums, &ws, &o};
         (how ? convert_step_ : convert_)->launch(grid, block, 0, stream, args);
     });
     products(ws, b.tables, stream);
     each_group([&](OperandsArg& o, size_t first, size_t last) {
-        char* blocks = b.tables + table_at_[5] + block_begin_[first] * sizeof(MuonBlock);
+        char* blocks = b.tables + table_at_[8] + block_begin_[first] * sizeof(MuonBlock);
         const uint32_t grid[3] = {block_begin_[last] - block_begin_[first], 1, 1};
         void* args[] = {&mats, &blocks, &ws, &o};
         (how ? finish_step_ : finish_)->launch(grid, block, 0, stream, args, last == count());

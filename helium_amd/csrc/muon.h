@@ -52,9 +52,9 @@ public:
     const std::string& source() const { return source_; }
     const std::string& describe() const { return describe_; }
     size_t count() const { return pr_.shapes.size(); }
-    // The tables the kernels read, as bytes: 0 matrices, 1 to 3 tasks of the three products, 4 shares of the sums of squares,
-    // 5 blocks of the conversions.
-    static constexpr int kTables = 6;
+    // The tables the kernels read, as bytes: 0 matrices, 1 to 3 tasks of the three products, 4 to 6 those of their tiles that several
+    // workgroups share, 7 shares of the sums of squares, 8 blocks of the conversions.
+    static constexpr int kTables = 9;
     const std::vector<char>& table(int which) const { return tables_[which]; }
     size_t workspace_bytes() const { return workspace_bytes_; }
 
@@ -70,12 +70,16 @@ private:
     MuonProblem pr_;
     std::vector<MuonMatrix> matrices_;
     std::vector<char> tables_[kTables];
-    size_t table_at_[kTables] = {}, table_bytes_ = 0, workspace_bytes_ = 0, tickets_at_ = 0, shared_at_ = 0;
-    std::array<uint32_t, kTables> table_size_{};
-    uint32_t threads_ = 256, tickets_ = 0;
-    std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 4 and 5
+    size_t table_at_[kTables] = {}, table_bytes_ = 0, workspace_bytes_ = 0, shared_at_ = 0;
+    uint32_t shares_ = 0;
+    struct Product {
+        uint32_t grid = 0, threads = 0, join_grid = 0;
+        std::string text;
+        std::unique_ptr<JitKernel> kernel, join;
+    } products_[3];
+    std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 7 and 8
     std::string source_, describe_;
-    std::unique_ptr<JitKernel> norm_, convert_, gram_, square_, apply_, finish_, norm_step_, convert_step_, finish_step_;
+    std::unique_ptr<JitKernel> norm_, convert_, finish_, norm_step_, convert_step_, finish_step_;
     std::mutex mu_;
     std::map<hipStream_t, Buffers> per_stream_;
 };

@@ -66,11 +66,11 @@ static inline double emu_shfl64(double v, int mask) {
 def emulated(shapes, dtype, split, steps, in_storage, step=None):
     """The launches of a call, one after the other. `step`: (momenta, weights, learning rate, mu, decay, nesterov)."""
     muon = ha.Muon(shapes, dtype, precision="f32_f32" if split else "f16_f32", steps=steps)
-    mats, gram, square, apply, parts, blocks = (np.frombuffer(muon.table(t), [MATRIX, TASK, TASK, TASK, BLOCK, BLOCK][t]) for t in range(6))
-    said = dict(s.split("=") for s in muon.description.split()[1:])
-    workspace, threads, tile = int(said["workspace"]), int(said["threads"]), int(said["tile"])
-    slots = max(1, *map(int, said["shared"].split(",")))
-    parked, tickets = np.full(slots * tile * tile, np.nan, np.float32), np.zeros(slots, np.uint32)
+    mats, tasks, joins = np.frombuffer(muon.table(0), MATRIX), [np.frombuffer(muon.table(t), TASK) for t in (1, 2, 3)], [np.frombuffer(muon.table(t), TASK) for t in (4, 5, 6)]
+    parts, blocks = (np.frombuffer(muon.table(t), BLOCK) for t in (7, 8))
+    said = [dict(s.split("=") for s in line.split()[1:]) for line in muon.description.splitlines()]
+    workspace = int(said[0]["workspace"])
+    elements, *products = muon.source.split("\n//// product ")
     names = [f"in{k}" for k in range(len(shapes))]
     fill = "".join(f"o.in[{k}] = in{k}; " for k in range(len(shapes)))
     params = ", ".join(f"const elem_t* in{k}" for k in range(len(shapes)))
@@ -86,11 +86,8 @@ def emulated(shapes, dtype, split, steps, in_storage, step=None):
 extern "C" void emu_norm(const Matrix* m, const Block* t, double* s, {params}) {{ Operands o{{}}; {fill} norm_part<{which}>(m, t, s, o); }}
 extern "C" void emu_convert(const Matrix* m, const Block* t, const double* s, char* ws, {params}) {{ Operands o{{}}; {fill} convert_block<{which}>(m, t, s, ws, o); }}
 extern "C" void emu_finish(const Matrix* m, const Block* t, const char* ws, {params}, {outs}) {{ Operands o{{}}; {fill} {fill_out} finish_block<{which}>(m, t, ws, o); }}
-extern "C" void emu_gram(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<GRAM>(m, t, ws, parked, tickets, *turn, *last); }}
-extern "C" void emu_square(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<SQUARE>(m, t, ws, parked, tickets, *turn, *last); }}
-extern "C" void emu_apply(const Matrix* m, const Task* t, char* ws, float* parked, u32* tickets, const u32* turn, const u32* last) {{ product<APPLY>(m, t, ws, parked, tickets, *turn, *last); }}
 """
-    text = SHFL + muon.source + wrappers
+    text = SHFL + elements + wrappers
     given = [(a, 0) for a in in_storage]
     sums = np.zeros(len(parts))
     if step:
@@ -104,9 +101,17 @@ extern "C" void emu_apply(const Matrix* m, const Task* t, char* ws, float* parke
     ws, = run_kernel(text, "emu_convert", len(blocks), 256, [(mats, 0), (blocks, 0), (sums, 0), (np.empty(workspace, np.uint8), 1)] + given)
     for k in range(steps):
         turn, last = np.array([k & 1], np.uint32), np.array([k == steps - 1], np.uint32)
-        for entry, tasks in (("emu_gram", gram), ("emu_square", square), ("emu_apply", apply)):
-            ws, _, left = run_kernel(text, entry, len(tasks), threads, [(mats, 0), (tasks, 0), (ws, 2), (parked, 1), (tickets, 2), (turn, 0), (last, 0)])
-            assert not left.any(), "tickets not back at zero"
+        for p, product in enumerate(products):
+            name, body = product.split("\n", 1)
+            cut = {key: int(v) for key, v in said[1 + p].items() if key != "estimate"}
+            body = SHFL + body + f"""
+extern "C" void emu_product(const Matrix* m, const Task* t, char* ws, float* parked, const u32* turn, const u32* last) {{ product<{name.upper()}>(m, t, ws, parked, *turn, *last); }}
+extern "C" void emu_join(const Matrix* m, const Task* t, char* ws, const float* parked, const u32* turn, const u32* last) {{ join<{name.upper()}>(m, t, ws, parked, *turn, *last); }}
+"""
+            parked = np.full(max(cut["parked"], 1), np.nan, np.float32)
+            ws, parked = run_kernel(body, "emu_product", cut["grid"], cut["threads"], [(mats, 0), (tasks[p], 0), (ws, 2), (parked, 2), (turn, 0), (last, 0)])
+            if cut["join_grid"]:
+                ws, = run_kernel(body, "emu_join", cut["join_grid"], 256, [(mats, 0), (joins[p], 0), (ws, 2), (parked, 0), (turn, 0), (last, 0)])
     outs = [np.empty(s, np.float32 if step else in_storage[0].dtype) for s in shapes]
     return run_kernel(text, "emu_finish", len(blocks), 256, [(mats, 0), (blocks, 0), (ws, 0)] + given + [(o, 1) for o in outs]), new_momenta
 
