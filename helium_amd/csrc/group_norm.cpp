@@ -39,6 +39,9 @@ typedef elem_t vec_t __attribute__((ext_vector_type(V)));
 #ifndef HE_FAST_RCP
 #define HE_FAST_RCP(x) __builtin_amdgcn_rcpf(x)
 #endif
+#ifndef HE_EXP2
+#define HE_EXP2(x) __builtin_amdgcn_exp2f(x)
+#endif
 
 // A vector whose channels all lie in one group adds up to one number, one that spans groups to one per channel.
 #define ACC ((D % V) == 0 ? 1 : V)
@@ -56,7 +59,9 @@ __device__ __forceinline__ Place place() {
     Place p;
     p.tx = threadIdx.x % TX;
     p.ty = threadIdx.x / TX;
-    u64 b = blockIdx.x;
+    // Blocks are dealt round-robin to the 8 XCDs, each with an L2 of its own: an XCD takes neighbours, whose slices share cache lines.
+    const u32 xcd = blockIdx.x % 8u;
+    u64 b = xcd * (BLOCKS / 8u) + (xcd < BLOCKS % 8u ? xcd : BLOCKS % 8u) + blockIdx.x / 8u;
     p.slice = (u32)(b % SLICES);
     b /= SLICES;
     p.chunk = (u32)(b % CHUNKS);
@@ -69,8 +74,9 @@ __device__ __forceinline__ Place place() {
 __device__ __forceinline__ u64 origin(const Place& p) {
     return (p.n * PIXELS + (u64)p.chunk * ROWS + p.ty) * C + (u64)p.slice * SC + p.tx * V;
 }
-#define COLUMN(p, q) ((p).tx + (q) * TX < CV)
-#define HELD(p, r, q) ((r) * TY < (p).left && COLUMN(p, q))
+#define COLUMN(p, q) (CV % TX == 0 || (p).tx + (q) * TX < CV)
+// (what holds for every thread is not asked of each)
+#define HELD(p, r, q) ((WHOLE && ((r) + 1) * TY <= PIXELS ? TX * TY == T || (p).ty < TY : (r) * TY < (p).left) && COLUMN(p, q))
 
 __device__ __forceinline__ void load_held(const elem_t* __restrict__ x, const Place& p, vec_t (&held)[RPT][NC]) {
     const u64 o = origin(p);
@@ -107,6 +113,19 @@ template <int N> __device__ __forceinline__ void fold_rows(float (&a)[NC][N], co
     }
     __syncthreads();
 }
+// The sums of fold_rows() per entry, out[e] for all E entries of a row: LANES neighbouring threads add one up.
+template <int E, int LANES> __device__ __forceinline__ void fold_entries(const float* red, float* out) {
+    const u32 l = threadIdx.x % LANES;
+    for (u32 e0 = 0; e0 < E; e0 += T / LANES) {
+        const u32 e = e0 + threadIdx.x / LANES;
+        float s = 0.0f;
+        if (e < E)
+            for (u32 row = l; row < RED_ROWS; row += LANES) s += red[row * E + e];
+        for (int m = LANES / 2; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+        if (e < E && l == 0) out[e] = s;
+    }
+    __syncthreads();
+}
 // The sums of fold_rows() per group: out[g], g < KG. Each group is added up by LPG neighbouring threads.
 __device__ __forceinline__ void fold_groups(const float* red, float* out) {
     const u32 g = threadIdx.x / LPG, l = threadIdx.x % LPG;
@@ -120,11 +139,14 @@ __device__ __forceinline__ void fold_groups(const float* red, float* out) {
 }
 __device__ __forceinline__ u32 group_of(u32 channel) { return channel / D; }   // within the slice
 
+// 1 / (1 + exp(-z)); z2 is -z log2(e)
+#define SIGMOID(z2) HE_FAST_RCP(1.0f + HE_EXP2(z2))
+#define NEG_LOG2E -1.44269504f
 __device__ __forceinline__ float activate(float z) {
 #if ACT == 1
     return z > 0.0f ? z : (z != z ? z : 0.0f);
 #elif ACT == 2
-    return z * HE_FAST_RCP(1.0f + __expf(-z));
+    return z * SIGMOID(z * NEG_LOG2E);
 #else
     return z;
 #endif
@@ -134,23 +156,26 @@ __device__ __forceinline__ float slope_times(float dy, float z) {
 #if ACT == 1
     return z > 0.0f ? dy : (z != z ? z : 0.0f);
 #elif ACT == 2
-    const float s = HE_FAST_RCP(1.0f + __expf(-z));
-    return dy * (s + z * s * (1.0f - s));
+    const float s = SIGMOID(z * NEG_LOG2E);
+    return dy * (s + s * (z - z * s));
 #else
     return dy;
 #endif
 }
+#if STREAM
+#define STORE(p, v) __builtin_nontemporal_store(v, p)
+#else
+#define STORE(p, v) (*(p) = (v))
+#endif
 )HIP";
 
 // Statistics. A workgroup holds its part of a sample in registers, takes the mean of each group in it, then the sum of squared
-// distances from that mean (not E[x^2] - E[x]^2, which loses all digits of a variance that is small beside the mean). `merge`
-// joins the parts of a group: M2 = sum of M2_i + n_i (mean_i - mean)^2.
+// distances from that mean (not E[x^2] - E[x]^2, which loses all digits of a variance that is small beside the mean). Where a
+// workgroup holds all pixels of its groups (WHOLE), it goes on and the tensor is read once. Otherwise `merge` joins the parts of a
+// group, M2 = sum of M2_i + n_i (mean_i - mean)^2, and `apply` reads the tensor again.
 const char* kForward = R"HIP(
-extern "C" __global__ __launch_bounds__(T) void group_norm_stats(const elem_t* __restrict__ x, float* __restrict__ parts) {
-    __shared__ float red[RED_ROWS * CV * ACC], group_mean[KG], group_m2[KG];
-    const Place p = place();
-    vec_t held[RPT][NC];
-    load_held(x, p, held);
+// mean[g] and m2[g] of the workgroup's pixels
+__device__ __forceinline__ void part_statistics(const vec_t (&held)[RPT][NC], const Place& p, float count, float* red, float* mean_of, float* m2_of) {
     float a[NC][ACC];
 #pragma unroll
     for (int q = 0; q < NC; q++)
@@ -163,16 +188,17 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_stats(const elem_t* _
 #pragma unroll
             for (int i = 0; i < V; i++) a[q][i % ACC] += (float)AT(held[r][q], i);
     fold_rows<ACC>(a, p, red);
-    fold_groups(red, group_mean);
-    const u64 first = (u64)p.chunk * ROWS;
-    const float count = (float)(PIXELS - first < ROWS ? PIXELS - first : ROWS) * (float)D, inverse = 1.0f / count;
+    fold_groups(red, mean_of);
+    const float inverse = 1.0f / count;
+    for (u32 g = threadIdx.x; g < KG; g += T) mean_of[g] *= inverse;
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < NC; q++) {
         float mean[ACC];
 #pragma unroll
         for (int i = 0; i < ACC; i++) {
             a[q][i] = 0.0f;
-            mean[i] = COLUMN(p, q) ? group_mean[group_of((p.tx + q * TX) * V + i)] * inverse : 0.0f;
+            mean[i] = COLUMN(p, q) ? mean_of[group_of((p.tx + q * TX) * V + i)] : 0.0f;
         }
 #pragma unroll
         for (int r = 0; r < RPT; r++)
@@ -184,50 +210,12 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_stats(const elem_t* _
                 }
     }
     fold_rows<ACC>(a, p, red);
-    fold_groups(red, group_m2);
-    for (u32 g = threadIdx.x; g < KG; g += T) {
-        float* to = parts + (((p.n * G + p.slice * KG + g) * CHUNKS) + p.chunk) * 2;
-        to[0] = group_mean[g] * inverse;
-        to[1] = group_m2[g];
-    }
+    fold_groups(red, m2_of);
 }
 
-// One wave per (sample, group).
-extern "C" __global__ __launch_bounds__(256) void group_norm_merge(const float* __restrict__ parts, float* __restrict__ stats,
-                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    const u64 of = (u64)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const u32 lane = threadIdx.x & 63u;
-    const bool mine = of < (u64)BATCH * G;
-    const float* from = parts + (mine ? of : 0) * CHUNKS * 2;
-    const float whole = (float)PIXELS * (float)D;
-    float s = 0.0f;
-    for (u32 c = lane; c < CHUNKS; c += 64) {
-        const u64 left = PIXELS - (u64)c * ROWS;
-        s += from[c * 2] * ((float)(left < ROWS ? left : ROWS) * (float)D / whole);
-    }
-    for (int m = 32; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
-    float m2 = 0.0f;
-    for (u32 c = lane; c < CHUNKS; c += 64) {
-        const u64 left = PIXELS - (u64)c * ROWS;
-        const float d = from[c * 2] - s;
-        m2 += from[c * 2 + 1] + d * d * ((float)(left < ROWS ? left : ROWS) * (float)D);
-    }
-    for (int m = 32; m > 0; m /= 2) m2 += __shfl_xor(m2, m, 64);
-    if (mine && lane == 0) {
-        const float rstd = 1.0f / sqrtf(m2 / whole + EPS);
-        stats[of * 2] = s;
-        stats[of * 2 + 1] = rstd;
-        if (mean_out) mean_out[of] = s;
-        if (rstd_out) rstd_out[of] = rstd;
-    }
-}
-
-extern "C" __global__ __launch_bounds__(T) void group_norm_apply(const elem_t* __restrict__ x, const param_t* __restrict__ gamma,
-                                                                 const param_t* __restrict__ beta, const float* __restrict__ stats,
-                                                                 elem_t* __restrict__ y) {
-    const Place p = place();
-    vec_t held[RPT][NC];
-    load_held(x, p, held);
+// act(gamma (x - mean) rstd + beta); mean_of and rstd_of: of the slice's groups, `step` apart
+__device__ __forceinline__ void store_applied(const vec_t (&held)[RPT][NC], const Place& p, const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
+                                              const float* mean_of, const float* rstd_of, u32 step, elem_t* __restrict__ y) {
     const u64 o = origin(p);
 #pragma unroll
     for (int q = 0; q < NC; q++) {
@@ -236,9 +224,8 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_apply(const elem_t* _
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const u32 c = (p.tx + q * TX) * V + i;
-            const float* st = stats + (p.n * G + p.slice * KG + group_of(c)) * 2;
-            mean[i % ACC] = st[0];
-            scale[i] = st[1] * (float)gamma[p.slice * SC + c];
+            mean[i % ACC] = mean_of[group_of(c) * step];
+            scale[i] = rstd_of[group_of(c) * step] * (float)gamma[p.slice * SC + c];
             shift[i] = (float)beta[p.slice * SC + c];
         }
 #pragma unroll
@@ -247,36 +234,292 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_apply(const elem_t* _
                 vec_t out;
 #pragma unroll
                 for (int i = 0; i < V; i++) AT(out, i) = (elem_t)activate(((float)AT(held[r][q], i) - mean[i % ACC]) * scale[i] + shift[i]);
-                *(vec_t*)(y + o + (u64)r * TY * C + q * TX * V) = out;
+                STORE((vec_t*)(y + o + (u64)r * TY * C + q * TX * V), out);
             }
     }
 }
+
+#if WHOLE
+extern "C" __global__ __launch_bounds__(T) void group_norm_forward(const elem_t* __restrict__ x, const param_t* __restrict__ gamma,
+                                                                   const param_t* __restrict__ beta, elem_t* __restrict__ y,
+                                                                   float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    __shared__ float red[RED_ROWS * CV * ACC], mean_of[KG], m2_of[KG];
+    const Place p = place();
+    vec_t held[RPT][NC];
+    load_held(x, p, held);
+    const float count = (float)PIXELS * (float)D;
+    part_statistics(held, p, count, red, mean_of, m2_of);
+    for (u32 g = threadIdx.x; g < KG; g += T) {
+        const float rstd = 1.0f / sqrtf(m2_of[g] / count + EPS);
+        m2_of[g] = rstd;
+        if (mean_out) mean_out[p.n * G + p.slice * KG + g] = mean_of[g];
+        if (rstd_out) rstd_out[p.n * G + p.slice * KG + g] = rstd;
+    }
+    __syncthreads();
+    store_applied(held, p, gamma, beta, mean_of, m2_of, 1, y);
+}
+#else
+extern "C" __global__ __launch_bounds__(T) void group_norm_stats(const elem_t* __restrict__ x, float* __restrict__ parts) {
+    __shared__ float red[RED_ROWS * CV * ACC], mean_of[KG], m2_of[KG];
+    const Place p = place();
+    vec_t held[RPT][NC];
+    load_held(x, p, held);
+    const u64 first = (u64)p.chunk * ROWS;
+    part_statistics(held, p, (float)(PIXELS - first < ROWS ? PIXELS - first : ROWS) * (float)D, red, mean_of, m2_of);
+    for (u32 g = threadIdx.x; g < KG; g += T) {
+        float* to = parts + (((p.n * G + p.slice * KG + g) * CHUNKS) + p.chunk) * 2;
+        to[0] = mean_of[g];
+        to[1] = m2_of[g];
+    }
+}
+
+// The parts c = first, first + step, ... of a group, weighted by their pixels: a thread's share of the mean, and of the sum of squared
+// distances from it.
+#define PIXELS_OF(c) (PIXELS - (u64)(c) * ROWS < ROWS ? PIXELS - (u64)(c) * ROWS : ROWS)
+__device__ __forceinline__ float share_of_mean(const float* __restrict__ parts, u32 first, u32 step) {
+    const float whole = (float)PIXELS * (float)D;
+    float s = 0.0f;
+    for (u32 c = first; c < CHUNKS; c += step) s += parts[c * 2] * ((float)PIXELS_OF(c) * (float)D / whole);
+    return s;
+}
+__device__ __forceinline__ float share_of_m2(const float* __restrict__ parts, u32 first, u32 step, float mean) {
+    float m2 = 0.0f;
+    for (u32 c = first; c < CHUNKS; c += step) {
+        const float d = parts[c * 2] - mean;
+        m2 += parts[c * 2 + 1] + d * d * ((float)PIXELS_OF(c) * (float)D);
+    }
+    return m2;
+}
+__device__ __forceinline__ float rstd_from(float m2) { return 1.0f / sqrtf(m2 / ((float)PIXELS * (float)D) + EPS); }
+
+#if MERGE
+// One workgroup per (sample, group).
+extern "C" __global__ __launch_bounds__(256) void group_norm_merge(const float* __restrict__ parts, float* __restrict__ stats,
+                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    __shared__ float waves[2][4];
+    const u64 of = blockIdx.x;
+    const float* from = parts + of * CHUNKS * 2;
+    float s = share_of_mean(from, threadIdx.x, 256);
+    for (int m = 32; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+    if ((threadIdx.x & 63u) == 0) waves[0][threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = waves[0][0] + waves[0][1] + waves[0][2] + waves[0][3];
+    float m2 = share_of_m2(from, threadIdx.x, 256, s);
+    for (int m = 32; m > 0; m /= 2) m2 += __shfl_xor(m2, m, 64);
+    if ((threadIdx.x & 63u) == 0) waves[1][threadIdx.x >> 6] = m2;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const float rstd = rstd_from(waves[1][0] + waves[1][1] + waves[1][2] + waves[1][3]);
+        stats[of * 2] = s;
+        stats[of * 2 + 1] = rstd;
+        if (mean_out) mean_out[of] = s;
+        if (rstd_out) rstd_out[of] = rstd;
+    }
+}
+#endif
+
+// `from`: the groups' statistics, or (few parts) the parts themselves, which every workgroup then joins for its groups; the first of a
+// sample also writes the statistics.
+extern "C" __global__ __launch_bounds__(T) void group_norm_apply(const elem_t* __restrict__ x, const param_t* __restrict__ gamma,
+                                                                 const param_t* __restrict__ beta, const float* __restrict__ from,
+                                                                 elem_t* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    const Place p = place();
+    vec_t held[RPT][NC];
+    load_held(x, p, held);
+#if MERGE
+    const float* of = from + (p.n * G + p.slice * KG) * 2;
+    store_applied(held, p, gamma, beta, of, of + 1, 2, y);
+#else
+    __shared__ float mean_of[KG], rstd_of[KG];
+    const u32 g = threadIdx.x / LPG, l = threadIdx.x % LPG;
+    const u64 at = p.n * G + p.slice * KG + (g < KG ? g : 0);
+    float s = share_of_mean(from + at * CHUNKS * 2, l, LPG);
+    for (int m = LPG / 2; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+    float m2 = share_of_m2(from + at * CHUNKS * 2, l, LPG, s);
+    for (int m = LPG / 2; m > 0; m /= 2) m2 += __shfl_xor(m2, m, 64);
+    if (g < KG && l == 0) {
+        mean_of[g] = s;
+        rstd_of[g] = rstd_from(m2);
+        if (mean_out && p.chunk == 0) mean_out[at] = s;
+        if (rstd_out && p.chunk == 0) rstd_out[at] = rstd_of[g];
+    }
+    __syncthreads();
+    store_applied(held, p, gamma, beta, mean_of, rstd_of, 1, y);
+#endif
+}
+#endif
 )HIP";
 
 // Gradients. With dz = dy act'(z), a sample's sums over its pixels, A_c = sum dz and B_c = sum dz xh, give everything: dbeta and
 // dgamma are their sums over the samples, and a group's s1 = sum gamma_c A_c / M, s2 = sum gamma_c B_c / M are what
-// dx = rstd (gamma_c dz - s1 - xh s2) takes away.
+// dx = rstd (gamma_c dz - s1 - xh s2) takes away. A workgroup that holds all pixels of its groups (WHOLE) reads x and dy once.
 const char* kBackward = R"HIP(
-struct Column { float mean[V], rstd[V], gamma[V], beta[V]; };
+struct Column { float mean[ACC], rstd[ACC], scale[V], shift[V]; };   // z = (x - mean) scale + shift
 __device__ __forceinline__ void load_column(Column& k, const Place& p, int q, const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
                                             const float* __restrict__ mean, const float* __restrict__ rstd) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const u32 c = (p.tx + q * TX) * V + i;
         const u64 g = p.n * G + p.slice * KG + group_of(c);
-        k.mean[i] = mean[g];
-        k.rstd[i] = rstd[g];
-        k.gamma[i] = (float)gamma[p.slice * SC + c];
-        k.beta[i] = (float)beta[p.slice * SC + c];
+        k.mean[i % ACC] = mean[g];
+        k.rstd[i % ACC] = rstd[g];
+        k.scale[i] = rstd[g] * (float)gamma[p.slice * SC + c];
+        k.shift[i] = (float)beta[p.slice * SC + c];
+    }
+}
+__device__ __forceinline__ float from_mean(const Column& k, int i, float x) { return x - k.mean[i % ACC]; }
+__device__ __forceinline__ float dz_of(const Column& k, int i, float from_mean, float dy) { return slope_times(dy, from_mean * k.scale[i] + k.shift[i]); }
+
+// A channel's sums over the pixels that a thread holds: dz, and dz (x - mean), which times rstd is dz xh.
+__device__ __forceinline__ void add_to_sums(float (&a)[2 * V], int i, float from_mean, float dz) {
+    a[2 * i] += dz;
+    a[2 * i + 1] += dz * from_mean;
+}
+__device__ __forceinline__ void end_sums(float (&a)[2 * V], const Column& k) {
+#pragma unroll
+    for (int i = 0; i < V; i++) a[2 * i + 1] *= k.rstd[i % ACC];
+}
+// dx of one element: scale dz - (rstd s1 + (x - mean) rstd^2 s2)
+struct Minus { float by[ACC], slope[ACC]; };
+__device__ __forceinline__ elem_t dx_of(const Column& k, const Minus& s, int i, float from_mean, float dz) {
+    return (elem_t)(k.scale[i] * dz - (from_mean * s.slope[i % ACC] + s.by[i % ACC]));
+}
+// The groups' s1 and s2 from the channels' sums over all pixels.
+__device__ __forceinline__ void group_sums_of(const float* sums, const param_t* __restrict__ gamma, const Place& p, float* out) {
+    const u32 g = threadIdx.x / LPG, l = threadIdx.x % LPG;
+    float s1 = 0.0f, s2 = 0.0f;
+    if (g < KG)
+        for (u32 c = g * D + l; c < (g + 1) * D; c += LPG) {
+            const float w = (float)gamma[p.slice * SC + c];
+            s1 += w * sums[2 * c];
+            s2 += w * sums[2 * c + 1];
+        }
+    for (int m = LPG / 2; m > 0; m /= 2) {
+        s1 += __shfl_xor(s1, m, 64);
+        s2 += __shfl_xor(s2, m, 64);
+    }
+    const float whole = (float)PIXELS * (float)D;
+    if (g < KG && l == 0) {
+        out[2 * g] = s1 / whole;
+        out[2 * g + 1] = s2 / whole;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void load_minus(Minus& s, const Column& k, const Place& p, int q, const float* group_sums) {
+#pragma unroll
+    for (int i = 0; i < ACC; i++) {
+        const u32 g = group_of((p.tx + q * TX) * V + i);
+        s.by[i] = k.rstd[i] * group_sums[2 * g];
+        s.slope[i] = k.rstd[i] * k.rstd[i] * group_sums[2 * g + 1];
     }
 }
 
+// The samples' sums [batch][2][C] added up: 64 channels to a workgroup, the samples shared by its waves.
+template <int WAVES> __device__ __forceinline__ void parameter_gradients(u64 block, const float* __restrict__ samples, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    __shared__ float part[2][WAVES][64];
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const u64 c = block * 64 + lane;
+    float a = 0.0f, b = 0.0f;
+    if (c < C)
+        for (u64 n = wave; n < BATCH; n += WAVES) {
+            a += samples[(n * 2) * C + c];
+            b += samples[(n * 2 + 1) * C + c];
+        }
+    part[0][wave][lane] = a;
+    part[1][wave][lane] = b;
+    __syncthreads();
+    if (wave == 0 && c < C) {
+        for (u32 w = 1; w < WAVES; w++) {
+            a += part[0][w][lane];
+            b += part[1][w][lane];
+        }
+        dbeta[c] = a;
+        dgamma[c] = b;
+    }
+}
+
+#if WHOLE
+// (silu's slope costs more than the rest: dz is held in f32 then, instead of dy and a second round of slopes)
+#define HOLD_DZ (ACT == 2)
+extern "C" __global__ __launch_bounds__(T) void group_norm_backward(const elem_t* __restrict__ dy, const elem_t* __restrict__ x,
+                                                                    const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
+                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                    float* __restrict__ samples, elem_t* __restrict__ dx) {
+    __shared__ float red[RED_ROWS * CV * V * 2], sums[SC * 2], group_sums[KG * 2];
+    const Place p = place();
+    vec_t hx[RPT][NC], hd[RPT][NC];
+    load_held(x, p, hx);
+    load_held(dy, p, hd);
+    float a[NC][2 * V];
+#if HOLD_DZ
+    float dz[RPT][NC][V];
+#endif
+#pragma unroll
+    for (int q = 0; q < NC; q++) {
+#pragma unroll
+        for (int i = 0; i < 2 * V; i++) a[q][i] = 0.0f;
+        if (p.ty < TY && COLUMN(p, q)) {
+            Column k;
+            load_column(k, p, q, gamma, beta, mean, rstd);
+#pragma unroll
+            for (int r = 0; r < RPT; r++) {
+#if HOLD_DZ
+#pragma unroll
+                for (int i = 0; i < V; i++) dz[r][q][i] = 0.0f;
+#endif
+                if (HELD(p, r, q))
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float c = from_mean(k, i, (float)AT(hx[r][q], i)), d = dz_of(k, i, c, (float)AT(hd[r][q], i));
+                        add_to_sums(a[q], i, c, d);
+#if HOLD_DZ
+                        dz[r][q][i] = d;
+#endif
+                    }
+            }
+            end_sums(a[q], k);
+        }
+    }
+    fold_rows<2 * V>(a, p, red);
+    fold_entries<SC * 2, LPE>(red, sums);
+    for (u32 e = threadIdx.x; e < SC * 2; e += T) samples[(p.n * 2 + (e & 1)) * C + p.slice * SC + (e >> 1)] = sums[e];
+    group_sums_of(sums, gamma, p, group_sums);
+    const u64 o = origin(p);
+#pragma unroll
+    for (int q = 0; q < NC; q++) {
+        if (p.ty >= TY || !COLUMN(p, q)) continue;
+        Column k;
+        load_column(k, p, q, gamma, beta, mean, rstd);
+        Minus s;
+        load_minus(s, k, p, q, group_sums);
+#pragma unroll
+        for (int r = 0; r < RPT; r++)
+            if (HELD(p, r, q)) {
+                vec_t out;
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float c = from_mean(k, i, (float)AT(hx[r][q], i));
+#if HOLD_DZ
+                    AT(out, i) = dx_of(k, s, i, c, dz[r][q][i]);
+#else
+                    AT(out, i) = dx_of(k, s, i, c, dz_of(k, i, c, (float)AT(hd[r][q], i)));
+#endif
+                }
+                STORE((vec_t*)(dx + o + (u64)r * TY * C + q * TX * V), out);
+            }
+    }
+}
+
+extern "C" __global__ __launch_bounds__(256) void group_norm_parameters(const float* __restrict__ samples, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    parameter_gradients<4>(blockIdx.x, samples, dgamma, dbeta);
+}
+#else
 // parts: [batch * CHUNKS][2][C]
 extern "C" __global__ __launch_bounds__(T) void group_norm_sums(const elem_t* __restrict__ dy, const elem_t* __restrict__ x,
                                                                 const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
                                                                 const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                 float* __restrict__ parts) {
-    __shared__ float red[RED_ROWS * CV * V * 2];
+    __shared__ float red[RED_ROWS * CV * V * 2], sums[SC * 2];
     const Place p = place();
     vec_t hx[RPT][NC], hd[RPT][NC];
     load_held(x, p, hx);
@@ -294,113 +537,71 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_sums(const elem_t* __
                 if (HELD(p, r, q))
 #pragma unroll
                     for (int i = 0; i < V; i++) {
-                        const float xh = ((float)AT(hx[r][q], i) - k.mean[i]) * k.rstd[i];
-                        const float dz = slope_times((float)AT(hd[r][q], i), xh * k.gamma[i] + k.beta[i]);
-                        a[q][2 * i] += dz;
-                        a[q][2 * i + 1] += dz * xh;
+                        const float c = from_mean(k, i, (float)AT(hx[r][q], i));
+                        add_to_sums(a[q], i, c, dz_of(k, i, c, (float)AT(hd[r][q], i)));
                     }
+            end_sums(a[q], k);
         }
     }
     fold_rows<2 * V>(a, p, red);
-    for (u32 e = threadIdx.x; e < CV * V * 2; e += T) {
-        float s = 0.0f;
-        for (u32 row = 0; row < RED_ROWS; row++) s += red[row * (CV * V * 2) + e];
-        parts[((p.n * CHUNKS + p.chunk) * 2 + (e & 1)) * C + p.slice * SC + (e >> 1)] = s;
-    }
+    fold_entries<SC * 2, LPE>(red, sums);
+    for (u32 e = threadIdx.x; e < SC * 2; e += T) parts[((p.n * CHUNKS + p.chunk) * 2 + (e & 1)) * C + p.slice * SC + (e >> 1)] = sums[e];
 }
 
-// The chunks of a sample joined: its channels' sums [batch][2][C], and s1, s2 of its groups [batch][G][2]. One wave per group.
-extern "C" __global__ __launch_bounds__(256) void group_norm_fold(const float* __restrict__ parts, const param_t* __restrict__ gamma,
-                                                                  float* __restrict__ samples, float* __restrict__ group_sums) {
-    const u64 of = (u64)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const u32 lane = threadIdx.x & 63u;
-    if (of >= (u64)BATCH * G) return;
-    const u64 n = of / G;
-    const u32 g = (u32)(of % G);
-    float s1 = 0.0f, s2 = 0.0f;
-    for (u32 c = g * D + lane; c < (g + 1) * D; c += 64) {
-        float a = 0.0f, b = 0.0f;
-        for (u32 k = 0; k < CHUNKS; k++) {
-            a += parts[((n * CHUNKS + k) * 2) * C + c];
-            b += parts[((n * CHUNKS + k) * 2 + 1) * C + c];
-        }
-        samples[(n * 2) * C + c] = a;
-        samples[(n * 2 + 1) * C + c] = b;
-        s1 += (float)gamma[c] * a;
-        s2 += (float)gamma[c] * b;
-    }
-    for (int m = 32; m > 0; m /= 2) {
-        s1 += __shfl_xor(s1, m, 64);
-        s2 += __shfl_xor(s2, m, 64);
-    }
-    const float whole = (float)PIXELS * (float)D;
-    if (lane == 0) {
-        group_sums[of * 2] = s1 / whole;
-        group_sums[of * 2 + 1] = s2 / whole;
-    }
-}
-
-// The workgroups behind the tensor's own add up the samples' sums: 64 channels each, a quarter of the samples per wave.
-__device__ __forceinline__ void parameter_gradients(u64 block, const float* __restrict__ samples, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    __shared__ float part[2][T / 64][64];
-    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const u64 c = block * 64 + lane;
-    float a = 0.0f, b = 0.0f;
-    if (c < C)
-        for (u64 n = wave; n < BATCH; n += T / 64) {
-            a += samples[(n * 2) * C + c];
-            b += samples[(n * 2 + 1) * C + c];
-        }
-    part[0][wave][lane] = a;
-    part[1][wave][lane] = b;
+// The chunks of a sample added up: [batch][2][C]. A workgroup takes 32 of a sample's 2 C sums, its 32 rows of threads every 32nd chunk.
+extern "C" __global__ __launch_bounds__(1024) void group_norm_fold(const float* __restrict__ parts, float* __restrict__ samples) {
+    __shared__ float part[32][33];
+    const u64 per = (2 * C + 31) / 32, n = blockIdx.x / per, e = blockIdx.x % per * 32 + (threadIdx.x & 31u);
+    const u32 row = threadIdx.x >> 5, column = threadIdx.x & 31u;
+    float s = 0.0f;
+    if (e < 2 * C)
+        for (u64 k = row; k < CHUNKS; k += 32) s += parts[(n * CHUNKS + k) * (2 * C) + e];
+    part[row][column] = s;
     __syncthreads();
-    if (wave == 0 && c < C) {
-        for (u32 w = 1; w < T / 64; w++) {
-            a += part[0][w][lane];
-            b += part[1][w][lane];
-        }
-        dbeta[c] = a;
-        dgamma[c] = b;
-    }
+    // (transposed: a row's threads now hold one sum's 32 shares)
+    s = part[column][row];
+    for (int m = 16; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+    const u64 mine = blockIdx.x % per * 32 + row;
+    if (column == 0 && mine < 2 * C) samples[n * (2 * C) + mine] = s;
 }
 
+// The workgroups behind the tensor's own add up the samples' sums.
 extern "C" __global__ __launch_bounds__(T) void group_norm_gradient(const elem_t* __restrict__ dy, const elem_t* __restrict__ x,
                                                                     const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                                    const float* __restrict__ samples, const float* __restrict__ group_sums,
-                                                                    elem_t* __restrict__ dx, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    if (blockIdx.x >= BLOCKS) return parameter_gradients(blockIdx.x - BLOCKS, samples, dgamma, dbeta);
+                                                                    const float* __restrict__ samples, elem_t* __restrict__ dx,
+                                                                    float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    if (blockIdx.x >= BLOCKS) return parameter_gradients<T / 64>(blockIdx.x - BLOCKS, samples, dgamma, dbeta);
+    __shared__ float sums[SC * 2], group_sums[KG * 2];
     const Place p = place();
     vec_t hx[RPT][NC], hd[RPT][NC];
     load_held(x, p, hx);
     load_held(dy, p, hd);
+    for (u32 e = threadIdx.x; e < SC * 2; e += T) sums[e] = samples[(p.n * 2 + (e & 1)) * C + p.slice * SC + (e >> 1)];
+    __syncthreads();
+    group_sums_of(sums, gamma, p, group_sums);
     const u64 o = origin(p);
 #pragma unroll
     for (int q = 0; q < NC; q++) {
         if (p.ty >= TY || !COLUMN(p, q)) continue;
         Column k;
         load_column(k, p, q, gamma, beta, mean, rstd);
-        float s1[V], s2[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const u64 g = p.n * G + p.slice * KG + group_of((p.tx + q * TX) * V + i);
-            s1[i] = group_sums[g * 2];
-            s2[i] = group_sums[g * 2 + 1];
-        }
+        Minus s;
+        load_minus(s, k, p, q, group_sums);
 #pragma unroll
         for (int r = 0; r < RPT; r++)
             if (HELD(p, r, q)) {
                 vec_t out;
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const float xh = ((float)AT(hx[r][q], i) - k.mean[i]) * k.rstd[i];
-                    const float dz = slope_times((float)AT(hd[r][q], i), xh * k.gamma[i] + k.beta[i]);
-                    AT(out, i) = (elem_t)(k.rstd[i] * (k.gamma[i] * dz - s1[i] - xh * s2[i]));
+                    const float c = from_mean(k, i, (float)AT(hx[r][q], i));
+                    AT(out, i) = dx_of(k, s, i, c, dz_of(k, i, c, (float)AT(hd[r][q], i)));
                 }
-                *(vec_t*)(dx + o + (u64)r * TY * C + q * TX * V) = out;
+                STORE((vec_t*)(dx + o + (u64)r * TY * C + q * TX * V), out);
             }
     }
 }
+#endif
 )HIP";
 
 int pow2_floor(int64_t x) {
@@ -419,14 +620,15 @@ std::string definitions(const GroupNormProblem& pr, const GroupNormTiling& t) {
       << "\n#define CHUNKS " << t.chunks << "\n#define BLOCKS " << t.grid << "ull\n#define LPG "
       << std::min(64, pow2_floor(t.threads / t.slice_groups)) << "\n#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 "
       << (pr.dtype == HE_F16) << "\n#define PARAM_SAME " << (pr.param_dtype == pr.dtype) << "\n#define ACT " << pr.activation
-      << "\n#define EPS " << strfmt("%.9gf", (double)pr.epsilon) << "\n";
+      << "\n#define EPS " << strfmt("%.9gf", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge 
+      << "\n#define LPE " << std::min<int64_t>(64, pow2_floor(std::max<int64_t>(1, t.threads / (2 * t.slice)))) << "\n";
     return s.str();
 }
 
 }  // namespace
 
 std::string GroupNormTiling::describe() const {
-    return strfmt("vec=%d threads=%d slice=%lld(%d groups) tx=%lld ty=%lld columns=%d rows_per_thread=%d chunks=%lld grid=%llu", vec, threads,
+    return strfmt("%s vec=%d threads=%d slice=%lld(%d groups) tx=%lld ty=%lld columns=%d rows_per_thread=%d chunks=%lld grid=%llu", whole ? "whole" : "parts", vec, threads,
                   (long long)slice, slice_groups, (long long)tx, (long long)ty, columns, rows_per_thread, (long long)chunks, (unsigned long long)grid);
 }
 
@@ -436,7 +638,44 @@ GroupNormTiling plan_group_norm(const GroupNormProblem& pr, bool backward) {
     const int64_t d = pr.channels / pr.groups;
     t.vec = 16 / esz;
     while (pr.channels % t.vec) t.vec /= 2;
+    // registers that one vector of a pixel takes: x; going back also dy, or what silu makes of it in f32
+    const int raw = std::max(1, t.vec * esz / 4);
+    const auto vector_regs = [&](bool whole) { return raw + (!backward ? 0 : whole && pr.activation == HE_ACT_SILU ? t.vec : raw); };
+    t.stream = (uint64_t)pr.batch * pr.pixels * pr.channels * esz >= (4u << 20) && tuning::get_int("HELIUM_HIP_NORM_STREAM", 1);
+
+    // Whole groups of a sample to a workgroup, if its registers hold them and that is estimated to take less than two ways through
+    // memory: of slices the one that costs least, then as few threads as keep a thread's data in 32 registers. Microseconds, from
+    // measurements of 0.1 to 270 MB: 5.5 MB are moved in one where a pixel's part of a slice is at least 64 bytes (32 bytes:
+    // a third, 16: an eighth of that), one workgroup moves 45 KB, and a thousand workgroups take 1.5 to begin and end.
+    const int forced_k = tuning::get_int("HELIUM_HIP_NORM_SLICE", 0), forced_t = tuning::get_int("HELIUM_HIP_NORM_THREADS", 0);
+    const double bytes = (double)pr.batch * pr.pixels * pr.channels * esz, moved = backward ? 3 : 2;
+    double best = backward ? 12 + 5 * bytes / 5.5e6 : 9 + 3 * bytes / 5.5e6;
+    if (forced_k || forced_t) best = 1e30;
+    for (int64_t k = 1; k <= pr.groups && !tuning::get_int("HELIUM_HIP_NORM_PARTS", 0); k++) {
+        if (pr.groups % k || k * d % t.vec || (forced_k && k != forced_k)) continue;
+        const int64_t tx = k * d / t.vec;
+        int threads = 0;
+        for (int candidate : {256, 512, 1024}) {
+            if (k > candidate || tx > candidate || (forced_t && candidate != forced_t)) continue;
+            const int64_t regs = (pr.pixels + candidate / tx - 1) / (candidate / tx) * vector_regs(true);
+            if (regs > (candidate == 1024 ? 56 : 64)) continue;
+            threads = candidate;
+            if (regs <= 32) break;
+        }
+        if (!threads) continue;
+        const double segment = (double)k * d * esz, eff = k == pr.groups || segment >= 64 ? 1.0 : std::pow(segment / 64, 1.5);
+        const double cost = (backward ? 8 : 5) + 1.5e-3 * pr.batch * (pr.groups / k) + std::max(moved * bytes / (5.5e6 * eff * (backward ? 0.65 : 1.0)), moved * segment * pr.pixels / 45e3);
+        if (cost >= best) continue;
+        best = cost;
+        t.whole = true;
+        t.threads = threads, t.slice_groups = (int)k, t.slice = k * d, t.tx = tx, t.ty = threads / tx, t.columns = 1;
+        t.rows_per_thread = (int)((pr.pixels + t.ty - 1) / t.ty), t.chunks = 1;
+        t.grid = (uint64_t)pr.batch * (pr.groups / k);
+    }
+    if (t.whole) return t;
+
     // The narrowest slice of whole groups and whole vectors that is at least 256 bytes of a pixel.
+    t.threads = 256;
     for (int64_t k = 1; k <= pr.groups; k++) {
         if (pr.groups % k || k * d % t.vec || k > t.threads) continue;
         t.slice_groups = (int)k;
@@ -449,12 +688,12 @@ GroupNormTiling plan_group_norm(const GroupNormProblem& pr, bool backward) {
     t.ty = t.threads / t.tx;
     t.columns = (int)((cv + t.tx - 1) / t.tx);
     // 64 registers of data per thread, fewer where that leaves compute units idle
-    const int64_t vector_regs = std::max(1, t.vec * esz / 4) * (backward ? 2 : 1);
-    int64_t rpt = std::max<int64_t>(1, 64 / (vector_regs * t.columns));
+    int64_t rpt = std::max<int64_t>(1, 64 / (vector_regs(false) * t.columns));
     const int64_t slices = pr.groups / t.slice_groups;
     while (rpt > 1 && (t.ty * (rpt / 2) >= pr.pixels || (uint64_t)(pr.batch * slices) * ((pr.pixels + t.ty * rpt - 1) / (t.ty * rpt)) < 1024)) rpt /= 2;
     t.rows_per_thread = (int)rpt;
     t.chunks = (pr.pixels + t.rows() - 1) / t.rows();
+    t.merge = t.chunks > 32;
     t.grid = (uint64_t)pr.batch * slices * t.chunks;
     return t;
 }
@@ -477,19 +716,26 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
     bwd_ = plan_group_norm(pr, true);
     HE_REQUIRE(std::max(fwd_.grid, bwd_.grid) < (1ull << 31) - 16384, HE_ERR_UNSUPPORTED, "group norm: the tensor is too large for one launch");
     const std::string forward = definitions(pr, fwd_) + kCommon + kForward, backward = definitions(pr, bwd_) + kCommon + kBackward;
-    auto make = [](const std::string& text, const char* entry) {
-        return std::async(std::launch::async, [&text, entry] { return std::make_unique<JitKernel>(text, entry); });
-    };
-    auto f = make(forward, "group_norm_stats"), b = make(backward, "group_norm_sums");
-    stats_ = f.get();
-    sums_ = b.get();
-    // (the other entries of the same texts: compiled already)
-    merge_.reset(new JitKernel(forward, "group_norm_merge"));
-    apply_.reset(new JitKernel(forward, "group_norm_apply"));
-    fold_.reset(new JitKernel(backward, "group_norm_fold"));
-    gradient_.reset(new JitKernel(backward, "group_norm_gradient"));
+    auto compiled = std::async(std::launch::async, [&] { (void)rtc_compile(backward, "group_norm", {}); });
+    auto make = [](const std::string& text, const char* entry) { return std::make_unique<JitKernel>(text, entry); };
+    if (fwd_.whole) {
+        whole_forward_ = make(forward, "group_norm_forward");
+    } else {
+        stats_ = make(forward, "group_norm_stats");
+        if (fwd_.merge) merge_ = make(forward, "group_norm_merge");
+        apply_ = make(forward, "group_norm_apply");
+    }
+    compiled.get();
+    if (bwd_.whole) {
+        whole_backward_ = make(backward, "group_norm_backward");
+        parameters_ = make(backward, "group_norm_parameters");
+    } else {
+        sums_ = make(backward, "group_norm_sums");
+        fold_ = make(backward, "group_norm_fold");
+        gradient_ = make(backward, "group_norm_gradient");
+    }
     const uint64_t rows = (uint64_t)pr.batch * pr.groups, sums = (uint64_t)pr.batch * 2 * pr.channels;
-    scratch_floats_ = std::max(rows * 2 * (fwd_.chunks + 1), sums * (bwd_.chunks + 1) + rows * 2);
+    scratch_floats_ = std::max(rows * 2 * (fwd_.chunks + 1), sums * (bwd_.chunks + 1));
     source_ = forward + "\n" + backward;
     describe_ = "group_norm forward: " + fwd_.describe() + "\ngroup_norm backward: " + bwd_.describe();
 }
@@ -509,17 +755,22 @@ void GroupNorm::check(std::initializer_list<const void*> tensors, std::initializ
 void GroupNorm::forward(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, hipStream_t stream) {
     if (pr_.batch == 0) return;
     check({x, y}, {gamma, beta}, {mean, rstd});
+    const uint32_t grid[3] = {(uint32_t)fwd_.grid, 1, 1}, block[3] = {(uint32_t)fwd_.threads, 1, 1};
+    if (fwd_.whole) {
+        void* args[] = {&x, &gamma, &beta, &y, &mean, &rstd};
+        whole_forward_->launch(grid, block, 0, stream, args, true);
+        return;
+    }
     const uint64_t rows = (uint64_t)pr_.batch * pr_.groups;
     std::lock_guard<std::mutex> lk(mu_);
     float* parts = scratch_.get(scratch_floats_, 0, stream).floats;
     float* stats = parts + rows * fwd_.chunks * 2;
-    const uint32_t grid[3] = {(uint32_t)fwd_.grid, 1, 1}, block[3] = {(uint32_t)fwd_.threads, 1, 1};
-    const uint32_t merge_grid[3] = {(uint32_t)((rows + 3) / 4), 1, 1}, merge_block[3] = {256, 1, 1};
+    const uint32_t merge_grid[3] = {(uint32_t)rows, 1, 1}, merge_block[3] = {256, 1, 1};
     void* a[] = {&x, &parts};
     stats_->launch(grid, block, 0, stream, a);
     void* b[] = {&parts, &stats, &mean, &rstd};
-    merge_->launch(merge_grid, merge_block, 0, stream, b);
-    void* c[] = {&x, &gamma, &beta, &stats, &y};
+    if (fwd_.merge) merge_->launch(merge_grid, merge_block, 0, stream, b);
+    void* c[] = {&x, &gamma, &beta, fwd_.merge ? &stats : &parts, &y, &mean, &rstd};
     apply_->launch(grid, block, 0, stream, c, true);
 }
 
@@ -530,23 +781,30 @@ void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const
         check({dy, x, dx}, {gamma, beta}, {mean, rstd, dgamma, dbeta});
         HE_REQUIRE(mean && rstd, HE_ERR_INVALID, "group norm: the backward pass needs the statistics of the forward pass");
     }
-    const uint64_t rows = (uint64_t)pr_.batch * pr_.groups, sums = (uint64_t)pr_.batch * 2 * pr_.channels;
+    const uint64_t sums = (uint64_t)pr_.batch * 2 * pr_.channels;
     std::lock_guard<std::mutex> lk(mu_);
-    float* parts = scratch_.get(scratch_floats_, 0, stream).floats;
-    float *samples = parts + sums * bwd_.chunks, *group_sums = samples + sums;
-    const uint32_t block[3] = {(uint32_t)bwd_.threads, 1, 1};
+    float *samples = scratch_.get(scratch_floats_, 0, stream).floats, *parts = samples + sums;
+    const uint32_t channel_blocks = (uint32_t)((pr_.channels + 63) / 64), small[3] = {256, 1, 1};
+    const uint32_t grid[3] = {(uint32_t)bwd_.grid, 1, 1}, block[3] = {(uint32_t)bwd_.threads, 1, 1};
+    if (bwd_.whole) {
+        const uint32_t last_grid[3] = {channel_blocks, 1, 1};
+        void* a[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &samples, &dx};
+        if (pr_.batch) whole_backward_->launch(grid, block, 0, stream, a);
+        void* b[] = {&samples, &dgamma, &dbeta};
+        parameters_->launch(last_grid, small, 0, stream, b, true);
+        return;
+    }
     if (pr_.batch) {
-        const uint32_t grid[3] = {(uint32_t)bwd_.grid, 1, 1};
-        const uint32_t fold_grid[3] = {(uint32_t)((rows + 3) / 4), 1, 1}, fold_block[3] = {256, 1, 1};
+        const uint32_t fold_grid[3] = {(uint32_t)(pr_.batch * ((2 * pr_.channels + 31) / 32)), 1, 1}, fold_block[3] = {1024, 1, 1};
         void* a[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &parts};
         sums_->launch(grid, block, 0, stream, a);
-        void* b[] = {&parts, &gamma, &samples, &group_sums};
+        void* b[] = {&parts, &samples};
         fold_->launch(fold_grid, fold_block, 0, stream, b);
     }
     // (without samples only the parameters' gradients are left, all zero)
-    const uint32_t grid[3] = {(uint32_t)(bwd_.grid + (pr_.channels + 63) / 64), 1, 1};
-    void* c[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &samples, &group_sums, &dx, &dgamma, &dbeta};
-    gradient_->launch(grid, block, 0, stream, c, true);
+    const uint32_t last_grid[3] = {(uint32_t)bwd_.grid + channel_blocks, 1, 1};
+    void* c[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &samples, &dx, &dgamma, &dbeta};
+    gradient_->launch(last_grid, block, 0, stream, c, true);
 }
 
 }  // namespace he

@@ -21,6 +21,9 @@ struct GroupNormProblem {
 // How one pass over the tensor is cut: a workgroup takes `rows` pixels of `slice` channels (whole groups) of one sample and
 // holds them in registers; `tx` threads stand side by side along the channels, `threads / tx` pixels below each other.
 struct GroupNormTiling {
+    bool whole = false;   // a workgroup holds all pixels of its groups
+    bool merge = false;   // statistics of so many parts that a launch of their own joins them
+    bool stream = false;  // results bypass the caches on their way to memory
     int vec = 1;          // elements per access
     int threads = 256;
     int slice_groups = 1; // groups per workgroup
@@ -50,7 +53,7 @@ private:
     GroupNormProblem pr_;
     GroupNormTiling fwd_, bwd_;
     std::string source_, describe_;
-    std::unique_ptr<JitKernel> stats_, merge_, apply_, sums_, fold_, gradient_;
+    std::unique_ptr<JitKernel> whole_forward_, stats_, merge_, apply_, whole_backward_, parameters_, sums_, fold_, gradient_;
     std::mutex mu_;  // a call's launches follow each other on their stream: they share the stream's scratch
     uint64_t scratch_floats_ = 0;
     ReduceScratch scratch_;

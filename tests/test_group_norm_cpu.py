@@ -37,36 +37,42 @@ def test_the_oracles_gradients_are_those_of_its_forward_pass(activation):
 def launch(norm, backward):
     """Grid, threads, parts of a sample and text of the forward or the backward pass."""
     line = norm.description.splitlines()[backward]
-    return [int(re.search(k + r"=(\d+)", line).group(1)) for k in ("grid", "threads", "chunks")] + ["#define BATCH" + norm.source.split("#define BATCH")[1 + backward]]
+    return [int(re.search(k + r"=(\d+)", line).group(1)) for k in ("grid", "threads", "chunks")] + ["#define HE_EXP2(x) exp2f(x)\n#define BATCH" + norm.source.split("#define BATCH")[1 + backward]]
 
 
 def forward_emulated(norm, shape, host):
     n, p, c, groups = shape
     grid, threads, chunks, text = launch(norm, False)
     y, stat = np.empty((n, p, c), host["x"].dtype), np.empty((n, groups), np.float32)
+    if norm.description.startswith("group_norm forward: whole"):
+        return run_kernel(text, "group_norm_forward", grid, threads, [(host[k], 0) for k in ("x", "gamma", "beta")] + [(y, 1), (stat, 1), (stat, 1)])
     parts, = run_kernel(text, "group_norm_stats", grid, threads, [(host["x"], 0), (np.empty((n, groups, chunks, 2), np.float32), 1)])
-    stats, mean, rstd = run_kernel(text, "group_norm_merge", (n * groups + 3) // 4, 256,
-                                   [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)])
-    y, = run_kernel(text, "group_norm_apply", grid, threads, [(host["x"], 0), (host["gamma"], 0), (host["beta"], 0), (stats, 0), (y, 1)])
-    return y, mean, rstd
+    mean, rstd = stat, stat
+    if chunks > 32:
+        parts, mean, rstd = run_kernel(text, "group_norm_merge", n * groups, 256, [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)])
+    return run_kernel(text, "group_norm_apply", grid, threads, [(host["x"], 0), (host["gamma"], 0), (host["beta"], 0), (parts, 0), (y, 1), (mean, 2), (rstd, 2)])
 
 
 def backward_emulated(norm, shape, host, mean, rstd):
     n, p, c, groups = shape
     grid, threads, chunks, text = launch(norm, True)
     given = [(host[k], 0) for k in ("dy", "x", "gamma", "beta")] + [(mean, 0), (rstd, 0)]
+    dx, dparam, sums = np.empty((n, p, c), host["x"].dtype), np.empty(c, np.float32), np.empty((n, 2, c), np.float32)
+    if norm.description.splitlines()[1].startswith("group_norm backward: whole"):
+        samples, dx = run_kernel(text, "group_norm_backward", grid, threads, given + [(sums, 1), (dx, 1)])
+        return [dx] + run_kernel(text, "group_norm_parameters", (c + 63) // 64, 256, [(samples, 0), (dparam, 1), (dparam, 1)])
     parts, = run_kernel(text, "group_norm_sums", grid, threads, given + [(np.empty((n * chunks, 2, c), np.float32), 1)])
-    samples, sums = run_kernel(text, "group_norm_fold", (n * groups + 3) // 4, 256,
-                               [(parts, 0), (host["gamma"], 0), (np.empty((n, 2, c), np.float32), 1), (np.empty((n, groups, 2), np.float32), 1)])
-    return run_kernel(text, "group_norm_gradient", grid + (c + 63) // 64, threads,
-                      given + [(samples, 0), (sums, 0), (np.empty((n, p, c), host["x"].dtype), 1), (np.empty(c, np.float32), 1), (np.empty(c, np.float32), 1)])
+    samples, = run_kernel(text, "group_norm_fold", n * ((2 * c + 31) // 32), 1024, [(parts, 0), (sums, 1)])
+    return run_kernel(text, "group_norm_gradient", grid + (c + 63) // 64, threads, given + [(samples, 0), (dx, 1), (dparam, 1), (dparam, 1)])
 
 
 CASES = [(shape, ("f32", "bf16", "f16")[k % 3], ("none", "relu", "silu")[(k // 2) % 3]) for k, shape in enumerate(SHAPES)]
 
 
+@pytest.mark.parametrize("parts", ["0", "1"])
 @pytest.mark.parametrize("shape,dtype,activation", CASES)
-def test_the_kernels_match_the_oracle(shape, dtype, activation):
+def test_the_kernels_match_the_oracle(monkeypatch, shape, dtype, activation, parts):
+    monkeypatch.setenv("HELIUM_HIP_NORM_PARTS", parts)   # 1: through memory also where a workgroup could hold its groups
     param_dtype = dtype if shape[1] % 2 else "f32"
     norm = ha.GroupNorm(*shape, dtype, param_dtype=param_dtype, activation=activation, epsilon=EPSILON)
     host, v, mean, rstd = inputs(shape, dtype, param_dtype, activation, seed=shape[1])
