@@ -42,6 +42,11 @@ typedef float elem_t;
 #define LDS_AS __attribute__((address_space(3)))
 #define GLOBAL_AS __attribute__((address_space(1)))
 #endif
+#ifndef FREXP_EXP
+#define FREXP_EXP(x) __builtin_amdgcn_frexp_exp(x)
+#define LDEXP_F64(x, n) __builtin_amdgcn_ldexp(x, n)
+#define LDEXP_F32(x, n) __builtin_amdgcn_ldexpf(x, n)
+#endif
 #ifndef WAIT_LOADS
 #define WAIT_LOADS(n) (0x0070 | ((n) & 15) | (((n) >> 4) << 14))   /* vmcnt(n), and lgkmcnt(0): this wave's reads of LDS are done */
 #endif
@@ -203,7 +208,10 @@ template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix*
         if (lane == 0) total = s;
     }
     __syncthreads();
-    const double scale = (double)X_SCALE / (sqrt(total) + (double)NORM_FLOOR);
+    // (the factor as a mantissa and a power of two: a norm beyond 2^126 leaves no f32 of its reciprocal)
+    const double factor = (double)X_SCALE / (sqrt(total) + (double)NORM_FLOOR);
+    const int power = FREXP_EXP(factor);
+    const float mantissa = (float)LDEXP_F64(factor, -power);
     f16_t *natural = (f16_t*)(ws + (m.tall ? m.xt[0] : m.x)), *turned = (f16_t*)(ws + (m.tall ? m.x : m.xt[0])), *low = (f16_t*)(ws + m.x_low);
     const u32 c = t.j * 64 + (lane & 7u) * 8;
 #pragma unroll
@@ -213,7 +221,7 @@ template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix*
         updates_of<STEP>(o, k, r, c, m.rows, m.cols, v);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[e] = (float)((double)v[e] * scale);
+            v[e] = LDEXP_F32(v[e] * mantissa, power);
             tile[i][(lane & 7u) * 8 + e] = v[e];
         }
         put(natural, r, c, cols_p, v, SPLIT || m.tall ? nullptr : low);
@@ -545,16 +553,30 @@ struct OperandsArg {
     int32_t nesterov;
 };
 
-// Tasks in the order of their blocks: blocks are dealt round-robin to the 8 XCDs, each with an L2 of its own, so XCD x gets the
-// x-th eighth of a sequence in which neighbours share rows and columns.
+// Tasks in the order of their blocks. The longest sums begin first, so that the chip empties evenly. Of each length, the 8 XCDs, to
+// which blocks are dealt in turn and each of which has an L2 of its own, get an eighth of a sequence in which neighbours share rows
+// and columns.
 void deal(std::vector<MuonTask>& tasks) {
-    const size_t n = tasks.size(), whole = n / 8, over = n % 8;
-    std::vector<MuonTask> out(n);
-    for (size_t b = 0; b < n; b++) {
-        const size_t x = b % 8;
-        out[b] = tasks[x * whole + std::min(x, over) + b / 8];
+    auto length = [](const MuonTask& t) { return t.k_end - t.k_begin; };
+    std::stable_sort(tasks.begin(), tasks.end(), [&](const MuonTask& a, const MuonTask& b) { return length(a) > length(b); });
+    std::vector<MuonTask> queue[8];
+    size_t turn = 0;  // who gets one more where a length's tasks do not divide by 8
+    for (size_t begin = 0, end; begin < tasks.size(); begin = end) {
+        for (end = begin; end < tasks.size() && length(tasks[end]) == length(tasks[begin]);) end++;
+        const size_t n = end - begin;
+        size_t at = begin;
+        for (size_t x = 0; x < 8; x++) {
+            const size_t count = n / 8 + ((x + 8 - turn) % 8 < n % 8);
+            queue[x].insert(queue[x].end(), tasks.begin() + at, tasks.begin() + at + count);
+            at += count;
+        }
+        turn = (turn + n) % 8;
     }
-    tasks.swap(out);
+    // (whoever has the extra tasks comes first in every round of 8)
+    size_t b = 0;
+    for (size_t round = 0; b < tasks.size(); round++)
+        for (size_t x = 0; x < 8; x++)
+            if (round < queue[x].size()) tasks[b++] = queue[x][round];
 }
 
 // How a product's tiles are made: the waves of a workgroup, its ring of k-tiles in LDS, and the workgroups that a CU holds. And what

@@ -60,6 +60,10 @@ static inline double emu_shfl64(double v, int mask) {
     return r;
 }
 #define SHFL_XOR_F64(v, m) emu_shfl64(v, m)
+static inline int emu_frexp_exp(double x) { int e; (void)frexp(x, &e); return e; }
+#define FREXP_EXP(x) emu_frexp_exp(x)
+#define LDEXP_F64(x, n) ldexp(x, n)
+#define LDEXP_F32(x, n) ldexpf(x, n)
 """
 
 
