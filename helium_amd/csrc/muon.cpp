@@ -13,7 +13,6 @@ namespace he {
 namespace {
 
 constexpr int kGroup = 32;       // matrices whose operands one launch takes by value
-constexpr uint32_t kPart = 8192; // elements of one share of a sum of squares
 constexpr uint32_t kBlock = 64;  // rows and columns of one block of the conversions
 
 // Newton-Schulz iteration on f16 matrix cores. With X scaled to a Frobenius norm of at most 1, no singular value ever leaves
@@ -197,17 +196,16 @@ template <bool STEP> __device__ __forceinline__ void norm_part(const Matrix* __r
 // row, 8 values each.
 template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const double* __restrict__ sums, char* __restrict__ ws, const Operands& o) {
     __shared__ float tile[64][65];
-    __shared__ double total;
+    __shared__ double totals[4];
     const Block t = blocks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
     const u32 k = t.matrix - o.first, rows_p = m.tall ? m.np : m.mp, cols_p = m.tall ? m.mp : m.np, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    if (wave == 0) {
-        double s = 0.0;
-        for (u32 p = lane; p < m.parts; p += 64) s += sums[m.first_part + p];
-        for (int d = 32; d > 0; d /= 2) s += SHFL_XOR_F64(s, d);
-        if (lane == 0) total = s;
-    }
+    double s = 0.0;
+    for (u32 p = threadIdx.x; p < m.parts; p += 256) s += sums[m.first_part + p];
+    for (int d = 32; d > 0; d /= 2) s += SHFL_XOR_F64(s, d);
+    if (lane == 0) totals[wave] = s;
     __syncthreads();
+    const double total = totals[0] + totals[1] + totals[2] + totals[3];
     // (the factor as a mantissa and a power of two: a norm beyond 2^126 leaves no f32 of its reciprocal)
     const double factor = (double)X_SCALE / (sqrt(total) + (double)NORM_FLOOR);
     const int power = FREXP_EXP(factor);
@@ -655,7 +653,12 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    std::vector<MuonBlock> shares, blocks;
+    // Shares of the sums of squares: about a thousand, so that they fill the chip and a matrix has few of them to add up.
+    uint64_t values = 0;
+    for (auto& s : pr.shapes) values += (uint64_t)std::max<int64_t>(s[0], 0) * std::max<int64_t>(s[1], 0);
+    uint64_t part = 2048;
+    while (part < 65536 && part * 1024 < values) part *= 2;
+    std::vector<MuonBlock> portions, blocks;
     for (size_t k = 0; k < pr.shapes.size(); k++) {
         const int64_t rows = pr.shapes[k][0], cols = pr.shapes[k][1];
         HE_REQUIRE(rows >= 1 && cols >= 1, HE_ERR_INVALID, "muon: matrix %zu is %lld x %lld", k, (long long)rows, (long long)cols);
@@ -671,18 +674,18 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         if (!pr.split) m.x_low = take(x);
         const uint64_t size = (uint64_t)rows * cols;
         m.first_part = (uint32_t)parts;
-        m.parts = (uint32_t)((size + kPart - 1) / kPart);
+        m.parts = (uint32_t)((size + part - 1) / part);
         parts += m.parts;
-        part_begin_.push_back((uint32_t)shares.size());
+        part_begin_.push_back((uint32_t)portions.size());
         block_begin_.push_back((uint32_t)blocks.size());
-        for (uint32_t p = 0; p < m.parts; p++) shares.push_back({(uint32_t)k, p, 0});
+        for (uint32_t p = 0; p < m.parts; p++) portions.push_back({(uint32_t)k, p, 0});
         const uint32_t br = (m.tall ? m.np : m.mp) / kBlock, bc = (m.tall ? m.mp : m.np) / kBlock;
         for (uint32_t i = 0; i < br; i++)
             for (uint32_t j = 0; j < bc; j++) blocks.push_back({(uint32_t)k, i, j});
         matrices_.push_back(m);
-        HE_REQUIRE(blocks.size() < (1u << 30) && shares.size() < (1u << 30), HE_ERR_UNSUPPORTED, "muon: too many elements for one group");
+        HE_REQUIRE(blocks.size() < (1u << 30) && portions.size() < (1u << 30), HE_ERR_UNSUPPORTED, "muon: too many elements for one group");
     }
-    part_begin_.push_back((uint32_t)shares.size());
+    part_begin_.push_back((uint32_t)portions.size());
     block_begin_.push_back((uint32_t)blocks.size());
     // the products, largest extent first: A = X X^T along n, B from A A and X from B X along m
     const char* names[3] = {"gram", "square", "apply"};
@@ -718,16 +721,16 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     shared_at_ = take((uint64_t)most * 4);
     // (a share's place among the sums is its block's, plus where its launch begins)
     for (size_t k = 0; k < pr.shapes.size(); k++)
-        for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) shares[p].j = part_begin_[k / kGroup * kGroup];
+        for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) portions[p].j = part_begin_[k / kGroup * kGroup];
     workspace_bytes_ = take(parts * sizeof(double)) + parts * sizeof(double);
-    tables_[0] = bytes_of(matrices_), tables_[7] = bytes_of(shares), tables_[8] = bytes_of(blocks);
-    shares_ = (uint32_t)shares.size();
+    tables_[0] = bytes_of(matrices_), tables_[7] = bytes_of(portions), tables_[8] = bytes_of(blocks);
+    shares_ = (uint32_t)portions.size();
     for (int t = 0; t < kTables; t++) {
         table_at_[t] = table_bytes_;
         table_bytes_ += (tables_[t].size() + 255) / 256 * 256;
     }
     std::ostringstream s;
-    s << "#define GROUP " << kGroup << "\n#define PART " << kPart << "ull\n#define STEPS " << pr.steps << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
+    s << "#define GROUP " << kGroup << "\n#define PART " << part << "ull\n#define STEPS " << pr.steps << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
       << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define NORM_FLOOR 1e-7\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
     const std::string head = s.str() + kCommon;
     std::vector<std::pair<std::unique_ptr<JitKernel>*, std::pair<std::string, std::string>>> kernels;  // where to, text, entry
