@@ -17,10 +17,16 @@ constexpr uint32_t kBlock = 64;  // rows and columns of one block of the convers
 
 // Newton-Schulz iteration on f16 matrix cores. With X scaled to a Frobenius norm of at most 1, no singular value ever leaves
 // [0, 1.21]: the step's polynomial a s + b s^3 + c s^5 maps [0, 1] there and [1, 1.21] into [0.68, 0.96]. So every entry has a known
-// bound, and fixed powers of two keep f16 operands in range: X 2^12 (at most 4956 of 65504), A 2^13 (1.47 2^13), B 2^13 (|b s + c s^2|
-// stays below 2.81). A value's f16 rounding has 11 bits; its remainder in a second f16 gives 22, and three of the four products of
-// such pairs (the fourth is 2^-22 of the result) run at three times f16's cost, where f32 matrix instructions take sixteen times.
-// Measured against 64 bits: errors as of f32 products, 1e-6 to 1e-5.
+// bound, and fixed powers of two keep f16 operands in range (kScale). A value's f16 rounding has 11 bits; its remainder in a second f16
+// gives 22, and three of the four products of such pairs (the fourth is 2^-22 of the result) run at three times f16's cost, where f32
+// matrix instructions take sixteen times. Measured against 64 bits: errors as of f32 products, 1e-6 to 6e-6.
+//
+// Several steps at once. All matrices of an iteration commute, so its steps can be taken on the m x m side: with A = X X^T and
+// Q_k = a I + b A_k + c A_k A_k, A_(k+1) = Q_k A_k Q_k, and X = Q_(r-1) ... Q_0 X after r steps - one product with X on either end
+// instead of two per step, for 3 m x m products (half of them by symmetry) per step between. It costs digits: an error of A, which is
+// relative to the largest singular value, meets the smallest squared. After three steps in two f16 parts the results are still as of f32
+// (2e-6 to 5e-6, singular values over three decades 5e-6; five at once: 1e-4), so steps go in runs of three at most, and one by one
+// where operands have one part.
 const char* kCommon = R"HIP(
 typedef unsigned short u16;
 typedef unsigned int u32;
@@ -53,9 +59,13 @@ struct Matrix {
     u32 rows, cols, mp, np;
     u32 tall, first_part, parts;
     float shape_scale;
-    u64 x, xt[2], a, b, x_low;
+    u64 at[BUFFERS];
 };
+enum { X, XT, XT2, A, B, C, Q, Q2, X_LOW };   // places of a matrix's buffers in `at`
 struct Block { u32 matrix, i, j; };
+// R = c1 E1 + c2 E2 + cs P Q^T + ci I; operands, results and the transposed results by their places.
+struct Product { u32 p, q, e1, e2, out, turned; float c1, c2, cs, ci; };
+struct Products { Product of[2]; };
 struct Task { u32 matrix, i, j, k_begin, k_end, slot, share, shares; };
 struct Operands {
     const elem_t* in[GROUP];
@@ -68,11 +78,6 @@ struct Operands {
     int nesterov;
 };
 #define X_SCALE 4096.0f
-#define A_SCALE 8192.0f
-#define B_SCALE 8192.0f
-#define NS_A 3.4445f
-#define NS_B -4.7750f
-#define NS_C 2.0315f
 
 // Matrices of the workspace are rows of chunks of 8 values: with PARTS == 2 the chunk's high parts, then its low ones, so that a row's
 // 128 bytes are 32 values in two parts or 64 in one and are moved alike.
@@ -210,7 +215,7 @@ template <bool STEP> __device__ __forceinline__ void convert_block(const Matrix*
     const double factor = (double)X_SCALE / (sqrt(total) + (double)NORM_FLOOR);
     const int power = FREXP_EXP(factor);
     const float mantissa = (float)LDEXP_F64(factor, -power);
-    f16_t *natural = (f16_t*)(ws + (m.tall ? m.xt[0] : m.x)), *turned = (f16_t*)(ws + (m.tall ? m.x : m.xt[0])), *low = (f16_t*)(ws + m.x_low);
+    f16_t *natural = (f16_t*)(ws + m.at[m.tall ? XT : X]), *turned = (f16_t*)(ws + m.at[m.tall ? X : XT]), *low = (f16_t*)(ws + m.at[X_LOW]);
     const u32 c = t.j * 64 + (lane & 7u) * 8;
 #pragma unroll
     for (u32 pass = 0; pass < 2; pass++) {
@@ -241,7 +246,7 @@ template <bool STEP> __device__ __forceinline__ void finish_block(const Matrix* 
     const Block t = blocks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
     const u32 k = t.matrix - o.first, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = t.j * 64 + (lane & 7u) * 8;
-    const f16_t *from = (const f16_t*)(ws + m.x), *low = SPLIT ? nullptr : (const f16_t*)(ws + m.x_low);
+    const f16_t *from = (const f16_t*)(ws + m.at[X]), *low = SPLIT ? nullptr : (const f16_t*)(ws + m.at[X_LOW]);
     if (m.tall) {
 #pragma unroll
         for (u32 pass = 0; pass < 2; pass++) {
@@ -286,11 +291,11 @@ extern "C" __global__ __launch_bounds__(256) void muon_finish(const Matrix* __re
 extern "C" __global__ __launch_bounds__(256) void muon_finish_step(const Matrix* __restrict__ mats, const Block* __restrict__ blocks, const char* __restrict__ ws, Operands o) { finish_block<true>(mats, blocks, ws, o); }
 )HIP";
 
-// One kernel for the three products of a step, each of the form R = alpha P Q^T + beta E with P, Q row-major and contiguous along the
-// sum (X and its transpose are both kept for that; A and B are symmetric):
-//   gram    A = X X^T           P = Q = X            lower tiles, stored twice
-//   square  B = b A + c A A     P = Q = A, E = A     lower tiles, stored twice
-//   apply   X = a X + B X       P = B, Q = XT, E = X  whole, stored as X and as XT
+// One text for the three kinds of products, all of the form R = c1 E1 + c2 E2 + cs P Q^T + ci I with P, Q row-major and contiguous along
+// the sum (X and its transpose are both kept for that; the others are symmetric):
+//   gram    A = X X^T                      m x m along n; lower tiles, stored twice
+//   inner   B = b A + c A A and the like   m x m along m; lower tiles, stored twice; up to two products of a launch
+//   apply   X = a X + B X or Q X           m x n along m; stored as X and as XT
 const char* kProduct = R"HIP(
 #define WAVES (WAVES_M * WAVES_N)
 #define WTM (TILE / WAVES_M)
@@ -309,7 +314,7 @@ const char* kProduct = R"HIP(
 #define STRIPS_HALVES (2 * WAVES * STRIP_FLOATS(SM, SN))
 #define LDS_HALVES (STAGES * STAGE_HALVES > STRIPS_HALVES ? STAGES * STAGE_HALVES : STRIPS_HALVES)
 #define PARKED (TILE * TILE)            /* floats of a tile that waits to be added up */
-enum { GRAM, SQUARE, APPLY };
+enum { GRAM, INNER, APPLY };
 
 __device__ __forceinline__ void strip_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -321,15 +326,15 @@ __device__ __forceinline__ void strip_sync() {
 // of each 32 x 32 block; through a strip of LDS that belongs to the wave it gets 8 neighbours of a row, adds E, stores them, and
 // puts them back for the transposed copy.
 template <int STAGE, int RM, int RN>
-__device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix& m, char* __restrict__ ws, u32 row0, u32 col0, bool mirrored, u32 turn, float* strip) {
+__device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix& m, const Product& pr, char* __restrict__ ws, u32 row0, u32 col0, bool mirrored, float* strip) {
     constexpr u32 strip_pitch = RN * 32 + 1, row_lanes = RN * 4, col_lanes = RM * 4;   // lanes along a row of the strip, and along a column
     const u32 lane = threadIdx.x & 63u, half = lane >> 5;
     const u32 pitch = STAGE == APPLY ? m.np : m.mp;
-    const f16_t* e_rows = (const f16_t*)(ws + (STAGE == SQUARE ? m.a : m.x));
-    f16_t *plain = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.x)), *turned = (f16_t*)(ws + (STAGE == GRAM ? m.a : STAGE == SQUARE ? m.b : m.xt[turn ^ 1u]));
+    const f16_t *e1_rows = (const f16_t*)(ws + m.at[pr.e1]), *e2_rows = (const f16_t*)(ws + m.at[pr.e2]);
+    f16_t *plain = (f16_t*)(ws + m.at[pr.out]), *turned = (f16_t*)(ws + m.at[STAGE == APPLY ? pr.turned : pr.out]);
     // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
     // singular values with it)
-    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.x_low) : nullptr;
+    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.at[X_LOW]) : nullptr;
 #pragma unroll
     for (int i = 0; i < RM; i++)
 #pragma unroll
@@ -340,14 +345,16 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix
 #pragma unroll
     for (u32 s = 0; s < RM * 32 * row_lanes / 64; s++) {
         const u32 r = s * (64 / row_lanes) + lane / row_lanes, c = lane % row_lanes * 8;
-        float v[8], other[8];
-        if (STAGE != GRAM) get(e_rows, row0 + r, col0 + c, pitch, other, low);
+        float v[8], e1[8], e2[8];
+        const bool has_e1 = STAGE != GRAM && pr.c1 != 0.0f, has_e2 = STAGE == INNER && pr.c2 != 0.0f;
+        if (has_e1) get(e1_rows, row0 + r, col0 + c, pitch, e1, low);
+        if (has_e2) get(e2_rows, row0 + r, col0 + c, pitch, e2, nullptr);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float sum = strip[r * strip_pitch + c + e];
-            v[e] = STAGE == GRAM ? sum * (A_SCALE / (X_SCALE * X_SCALE))
-                 : STAGE == SQUARE ? NS_B * other[e] + (NS_C * B_SCALE / (A_SCALE * A_SCALE)) * sum
-                                   : NS_A * other[e] + (1.0f / B_SCALE) * sum;
+            v[e] = pr.cs * strip[r * strip_pitch + c + e];
+            if (has_e1) v[e] += pr.c1 * e1[e];
+            if (has_e2) v[e] += pr.c2 * e2[e];
+            if (STAGE == INNER && row0 + r == col0 + c + e) v[e] += pr.ci;
             strip[r * strip_pitch + c + e] = v[e];
         }
         put(plain, row0 + r, col0 + c, pitch, v, low);
@@ -369,15 +376,16 @@ struct Fragments { f16x8 a[PARTS][MB], b[PARTS][NB]; };
 struct True { constexpr operator bool() const { return true; } };
 struct False { constexpr operator bool() const { return false; } };
 
-template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u32 turn, u32 last_step) {
+template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u64 parked_pitch, const Products& all) {
     __shared__ __attribute__((aligned(16))) f16_t lds[LDS_HALVES];
     const Task t = tasks[blockIdx.x];
     const Matrix& m = mats[t.matrix];
+    const Product& pr = all.of[STAGE == INNER ? blockIdx.y : 0];
+    if (STAGE == INNER) parked += blockIdx.y * parked_pitch;
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
     const u32 k_len = (STAGE == GRAM ? m.np : m.mp) * PARTS;   // halves of a row
     const u32 p_limit = m.mp, q_limit = STAGE == APPLY ? m.np : m.mp;
-    const f16_t* p_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.b));
-    const f16_t* q_rows = (const f16_t*)(ws + (STAGE == GRAM ? m.x : STAGE == SQUARE ? m.a : m.xt[turn]));
+    const f16_t *p_rows = (const f16_t*)(ws + m.at[pr.p]), *q_rows = (const f16_t*)(ws + m.at[pr.q]);
     // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows meet 8
     // different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes. (A tile that ends beyond the matrix loads its first rows
     // there: sums that nothing stores.)
@@ -501,16 +509,18 @@ template <int STAGE> __device__ __forceinline__ void product(const Matrix* __res
             for (int di = 0; di < SM; di++)
 #pragma unroll
                 for (int dj = 0; dj < SN; dj++) part[di][dj] = acc[i + di][j + dj];
-            finish<STAGE, SM, SN>(part, m, ws, row0, col0, STAGE == APPLY ? !last_step : t.i != t.j, turn, strip);
+            finish<STAGE, SM, SN>(part, m, pr, ws, row0, col0, STAGE == APPLY ? pr.turned != X : t.i != t.j, strip);
         }
 }
 
 // The shares of a tile added up in their order: a wave per 32 x 32 block, four waves in a workgroup. `tiles`: the first share's task of each.
-template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u32 turn, u32 last_step) {
+template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u64 parked_pitch, const Products& all) {
     __shared__ float strips[4 * STRIP_FLOATS(1, 1)];
     constexpr u32 blocks = (TILE / 32) * (TILE / 32);
     const Task t = tiles[blockIdx.x / (blocks / 4)];
     const Matrix& m = mats[t.matrix];
+    const Product& pr = all.of[STAGE == INNER ? blockIdx.y : 0];
+    if (STAGE == INNER) parked += blockIdx.y * parked_pitch;
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x % (blocks / 4) * 4 + wave;
     const u32 row0 = t.i * TILE + block / (TILE / 32) * 32, col0 = t.j * TILE + block % (TILE / 32) * 32;
     if (row0 >= m.mp || col0 >= (STAGE == APPLY ? m.np : m.mp)) return;
@@ -532,13 +542,23 @@ template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restri
 #pragma unroll
             for (int e = 0; e < 16; e++) sum[0][0][e] += got[d][e / 4][e % 4];
     }
-    finish<STAGE, 1, 1>(sum, m, ws, row0, col0, STAGE == APPLY ? !last_step : t.i != t.j, turn, strips + wave * STRIP_FLOATS(1, 1));
+    finish<STAGE, 1, 1>(sum, m, pr, ws, row0, col0, STAGE == APPLY ? pr.turned != X : t.i != t.j, strips + wave * STRIP_FLOATS(1, 1));
 }
 
 #define KERNELS(name, stage) \
-    extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void muon_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u32 turn, u32 last_step) { product<stage>(mats, tasks, ws, parked, turn, last_step); } \
-    extern "C" __global__ __launch_bounds__(256) void muon_join_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u32 turn, u32 last_step) { join<stage>(mats, tiles, ws, parked, turn, last_step); }
+    extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void muon_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u64 parked_pitch, Products all) { product<stage>(mats, tasks, ws, parked, parked_pitch, all); } \
+    extern "C" __global__ __launch_bounds__(256) void muon_join_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u64 parked_pitch, Products all) { join<stage>(mats, tiles, ws, parked, parked_pitch, all); }
 )HIP";
+
+struct ProductArg {
+    uint32_t p, q, e1, e2, out, turned;
+    float c1, c2, cs, ci;
+};
+struct ProductsArg {
+    ProductArg of[2];
+};
+constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
+enum { X, XT, XT2, A, B, C, Q, Q2, X_LOW };
 
 struct OperandsArg {
     const void* in[kGroup];
@@ -670,8 +690,11 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         m.mp = padded(std::min(rows, cols)), m.np = padded(std::max(rows, cols));
         m.shape_scale = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
         const uint64_t bytes = pr.split ? 4 : 2, x = m.mp * bytes * m.np, a = m.mp * bytes * m.mp;
-        m.x = take(x), m.xt[0] = take(x), m.xt[1] = take(x), m.a = take(a), m.b = take(a);
-        if (!pr.split) m.x_low = take(x);
+        for (int k : {X, XT, XT2}) m.at[k] = take(x);
+        for (int k : {A, B}) m.at[k] = take(a);
+        if (pr.split)
+            for (int k : {C, Q, Q2}) m.at[k] = take(a);
+        else m.at[X_LOW] = take(x);
         const uint64_t size = (uint64_t)rows * cols;
         m.first_part = (uint32_t)parts;
         m.parts = (uint32_t)((size + part - 1) / part);
@@ -687,12 +710,12 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     }
     part_begin_.push_back((uint32_t)portions.size());
     block_begin_.push_back((uint32_t)blocks.size());
-    // the products, largest extent first: A = X X^T along n, B from A A and X from B X along m
-    const char* names[3] = {"gram", "square", "apply"};
+    // the kinds of products: A = X X^T along n, those of m x m matrices along m, and X from B X along m
+    const char* names[3] = {"gram", "inner", "apply"};
     uint32_t most = 0;
     std::string cuts;
     for (int p = 0; p < 3; p++) {
-        Product& product = products_[p];
+        ProductKind& product = products_[p];
         const int forced = tuning::get_int("HELIUM_HIP_MUON_TILE", -1), only = forced >= 0 ? forced : tuning::get_int((std::string("HELIUM_HIP_MUON_TILE_") + names[p]).c_str(), -1);
         const TileShape* chosen = nullptr;
         Cut cut;
@@ -714,11 +737,14 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         product.join_grid = (uint32_t)joins.size() * (shape.tile / 32) * (shape.tile / 32) / 4;
         product.text = strfmt("#define TILE %u\n#define WAVES_M %u\n#define WAVES_N %u\n#define STAGES %u\n#ifndef KERNEL_ATTRS\n#define KERNEL_ATTRS %s\n#endif\n", shape.tile,
                               shape.waves_m, shape.waves_n, shape.stages, shape.attrs);
-        most = std::max(most, parked * shape.tile * shape.tile);
+        product.parked = parked * shape.tile * shape.tile;
+        product.estimate = cut.estimate;
+        most = std::max(most, product.parked * (p == 1 ? 2 : 1));
         cuts += strfmt("\nmuon_%s tile=%u threads=%u stages=%u grid=%u join_grid=%u parked=%u estimate=%.1f", names[p], shape.tile, product.threads, shape.stages, product.grid,
                        product.join_grid, parked * shape.tile * shape.tile, cut.estimate);
     }
     shared_at_ = take((uint64_t)most * 4);
+    plan_launches();
     // (a share's place among the sums is its block's, plus where its launch begins)
     for (size_t k = 0; k < pr.shapes.size(); k++)
         for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) portions[p].j = part_begin_[k / kGroup * kGroup];
@@ -730,7 +756,7 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         table_bytes_ += (tables_[t].size() + 255) / 256 * 256;
     }
     std::ostringstream s;
-    s << "#define GROUP " << kGroup << "\n#define PART " << part << "ull\n#define STEPS " << pr.steps << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
+    s << "#define GROUP " << kGroup << "\n#define PART " << part << "ull\n#define BUFFERS " << MuonMatrix::kBuffers << "\n#define SPLIT " << (int)pr.split << "\n#define BF16 "
       << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define NORM_FLOOR 1e-7\n#ifndef SHFL_XOR_F64\n#define SHFL_XOR_F64(v, m) __shfl_xor(v, m, 64)\n#endif\n";
     const std::string head = s.str() + kCommon;
     std::vector<std::pair<std::unique_ptr<JitKernel>*, std::pair<std::string, std::string>>> kernels;  // where to, text, entry
@@ -741,8 +767,8 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     source_ = elements;
     for (int p = 0; p < 3; p++) {
         const std::string name = names[p];
-        Product& product = products_[p];
-        product.text = head + product.text + kProduct + "KERNELS(" + name + ", " + (p == 0 ? "GRAM" : p == 1 ? "SQUARE" : "APPLY") + ")\n";
+        ProductKind& product = products_[p];
+        product.text = head + product.text + kProduct + "KERNELS(" + name + ", " + (p == 0 ? "GRAM" : p == 1 ? "INNER" : "APPLY") + ")\n";
         source_ += "\n//// product " + name + "\n" + product.text;
         kernels.push_back({&product.kernel, {product.text, "muon_" + name}});
         if (product.join_grid) kernels.push_back({&product.join, {product.text, "muon_join_" + name}});
@@ -756,7 +782,7 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     for (auto& c : compiled) c.second.get();
     for (auto& k : kernels) k.first->reset(new JitKernel(k.second.first, k.second.second));
     describe_ = strfmt("muon matrices=%zu steps=%d parts=%d shares=%u blocks=%zu shared_at=%zu workspace=%zu", pr.shapes.size(), pr.steps, pr.split ? 2 : 1, shares_,
-                       blocks.size(), shared_at_, workspace_bytes_) + cuts;
+                       blocks.size(), shared_at_, workspace_bytes_) + cuts + launches_text_;
 }
 
 Muon::~Muon() {
@@ -782,20 +808,85 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
     return b;
 }
 
+// What is launched between the conversions: runs of steps, each of them on the m x m side but for its ends.
+void Muon::plan_launches() {
+    std::vector<int> runs(pr_.steps, 1);
+    // Runs of three at most and as even as can be, the longest first, if that is estimated to save a tenth: always where n is well beyond
+    // m, never where they are equal (a classifier's 22 filters, mostly 1 to 9: 569 -> 379 us; 1000 x 512 and 777 x 1203: 221 -> 245).
+    if (pr_.split && !tuning::get_int("HELIUM_HIP_MUON_ONE_BY_ONE", 0)) {
+        const int count = (pr_.steps + 2) / 3;
+        std::vector<int> longer(count, pr_.steps / count);
+        for (int k = 0; k < pr_.steps % count; k++) longer[k]++;
+        auto cost = [&](const std::vector<int>& of) {
+            double total = 0;
+            for (int r : of) total += products_[0].estimate + products_[2].estimate + products_[1].estimate * (r == 1 ? 1 : r == 2 ? 5 : 9);
+            return total;
+        };
+        if (cost(longer) < 0.9 * cost(runs) || tuning::get_int("HELIUM_HIP_MUON_RUNS", 0)) runs = longer;
+    }
+    // scales of what is in the buffers: of X, of A, B and C, and of Q after so many steps (its values are at most a, a^2, a^3)
+    const double sx = 4096, sa = 8192, sq[4] = {0, 8192, 4096, 1024};
+    auto add = [&](int kind, const std::vector<ProductArg>& products) {
+        Launch l{kind, (uint32_t)products.size(), {}};
+        const char* names[3] = {"gram", "inner", "apply"};
+        for (size_t k = 0; k < products.size(); k++) {
+            const ProductArg& a = products[k];
+            memcpy(l.products + k * sizeof(ProductArg), &a, sizeof(a));
+            launches_text_ += strfmt("\nlaunch %s of=%zu p=%u q=%u e1=%u e2=%u out=%u turned=%u c1=%.9g c2=%.9g cs=%.9g ci=%.9g", names[kind], k, a.p, a.q, a.e1, a.e2,
+                                     a.out, a.turned, (double)a.c1, (double)a.c2, (double)a.cs, (double)a.ci);
+        }
+        launches_.push_back(l);
+    };
+    static_assert(sizeof(ProductsArg) <= sizeof(Launch::products), "");
+    auto product = [](uint32_t p, uint32_t q, uint32_t out, uint32_t e1, double c1, double cs, uint32_t e2 = 0, double c2 = 0, double ci = 0, uint32_t turned = X) {
+        return ProductArg{p, q, e1, e2, out, turned, (float)c1, (float)c2, (float)cs, (float)ci};
+    };
+    launches_text_ = "\nruns";
+    for (size_t k = 0; k < runs.size(); k++) launches_text_ += strfmt("%c%d", k ? ',' : ' ', runs[k]);
+    uint32_t from = XT, to = XT2;
+    size_t done = 0;
+    for (int r : runs) {
+        add(0, {product(X, X, A, 0, 0, sa / (sx * sx))});
+        uint32_t q = Q, q_new = Q2;  // of two steps and more; after the first one Q is a I + B, and B is in q
+        std::vector<ProductArg> also;  // (waits for a launch to share)
+        for (int j = 0; j < r; j++) {
+            const uint32_t b = r > 1 && j == 0 ? q : (uint32_t)B;
+            add(1, {product(A, A, b, A, kB, kC * sa / (sa * sa))});
+            if (j > 0) {
+                // Q = (a I + B) Q
+                if (j == 1) also = {product(b, q, q_new, q, kA * sq[2] / sa, sq[2] / (sa * sa), b, kA * sq[2] / sa, kA * kA * sq[2])};
+                else also = {product(b, q, q_new, q, kA * sq[j + 1] / sq[j], sq[j + 1] / (sa * sq[j]))};
+                std::swap(q, q_new);
+            }
+            if (j + 1 < r) {
+                also.insert(also.begin(), product(b, A, C, A, kA, sa / (sa * sa)));  // C = (a I + B) A
+                add(1, also);
+                also.clear();
+                add(1, {product(C, b, A, C, kA, sa / (sa * sa))});  // A = C (a I + B)
+            }
+        }
+        if (!also.empty()) add(1, also);
+        done += r;
+        const bool last = done == (size_t)pr_.steps;
+        if (r == 1) add(2, {product(B, from, X, X, kA, 1 / sa, 0, 0, 0, last ? (uint32_t)X : to)});
+        else add(2, {product(q, from, X, X, 0, 1 / sq[r], 0, 0, 0, last ? (uint32_t)X : to)});
+        std::swap(from, to);
+    }
+}
+
 void Muon::products(char* ws, char* tables, hipStream_t stream) {
     const uint32_t join_block[3] = {256, 1, 1};
     char *mats = tables + table_at_[0], *parked = ws + shared_at_;
-    for (int k = 0; k < pr_.steps; k++)
-        for (int p = 0; p < 3; p++) {
-            const Product& product = products_[p];
-            uint32_t turn = (uint32_t)k & 1u, last = k == pr_.steps - 1;
-            char *tasks = tables + table_at_[1 + p], *joins = tables + table_at_[4 + p];
-            const uint32_t grid[3] = {product.grid, 1, 1}, block[3] = {product.threads, 1, 1}, join_grid[3] = {product.join_grid, 1, 1};
-            void* args[] = {&mats, &tasks, &ws, &parked, &turn, &last};
-            product.kernel->launch(grid, block, 0, stream, args);
-            void* join_args[] = {&mats, &joins, &ws, &parked, &turn, &last};
-            if (product.join_grid) product.join->launch(join_grid, join_block, 0, stream, join_args);
-        }
+    for (Launch& l : launches_) {
+        const ProductKind& kind = products_[l.kind];
+        char *tasks = tables + table_at_[1 + l.kind], *joins = tables + table_at_[4 + l.kind];
+        const uint32_t grid[3] = {kind.grid, l.count, 1}, block[3] = {kind.threads, 1, 1}, join_grid[3] = {kind.join_grid, l.count, 1};
+        uint64_t parked_pitch = kind.parked;
+        void* args[] = {&mats, &tasks, &ws, &parked, &parked_pitch, l.products};
+        kind.kernel->launch(grid, block, 0, stream, args);
+        void* join_args[] = {&mats, &joins, &ws, &parked, &parked_pitch, l.products};
+        if (kind.join_grid) kind.join->launch(join_grid, join_block, 0, stream, join_args);
+    }
 }
 
 void Muon::orthogonalize(const void* const* in, void* const* out, hipStream_t stream) {

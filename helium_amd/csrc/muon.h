@@ -20,12 +20,13 @@ struct MuonProblem {
 };
 
 // What the kernels know of a matrix; the device holds an array of these. The smaller extent is m, the larger n, both padded to whole
-// tiles with zeros (which every product leaves zeros): X is [mp][np], XT its transpose. The others are offsets in the workspace.
+// blocks of 64 with zeros (which every product leaves zeros): X is [mp][np], XT its transpose. `at`: where its buffers lie in the workspace.
 struct MuonMatrix {
     uint32_t rows, cols, mp, np;
     uint32_t tall, first_part, parts;  // parts: shares of the sum of squares
     float shape_scale;                 // sqrt(max(1, rows / cols))
-    uint64_t x, xt[2], a, b, x_low;    // xt twice, in turn; x_low: what f16 drops of X, where operands are of one part
+    static constexpr int kBuffers = 9;
+    uint64_t at[kBuffers];  // X, its transpose (twice, in turn), A, B, C, Q (twice), and what f16 drops of X where operands are of one part
 };
 // A workgroup's part of the conversions: a share of the sum of squares (i), or the 64 x 64 values at (i, j).
 struct MuonBlock {
@@ -72,11 +73,20 @@ private:
     std::vector<char> tables_[kTables];
     size_t table_at_[kTables] = {}, table_bytes_ = 0, workspace_bytes_ = 0, shared_at_ = 0;
     uint32_t shares_ = 0;
-    struct Product {
-        uint32_t grid = 0, threads = 0, join_grid = 0;
+    struct ProductKind {
+        uint32_t grid = 0, threads = 0, join_grid = 0, parked = 0;
+        double estimate = 0;
         std::string text;
         std::unique_ptr<JitKernel> kernel, join;
     } products_[3];
+    struct Launch {
+        int kind;
+        uint32_t count;                      // products
+        alignas(8) unsigned char products[80];  // as the kernel takes them
+    };
+    std::vector<Launch> launches_;
+    std::string launches_text_;
+    void plan_launches();
     std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 7 and 8
     std::string source_, describe_;
     std::unique_ptr<JitKernel> norm_, convert_, finish_, norm_step_, convert_step_, finish_step_;

@@ -44,19 +44,34 @@ def _product(p, q):
     return p[0] @ q[0].T + (p[0] @ q[1].T + p[1] @ q[0].T)
 
 
-def modelled(u, split, steps=5):
-    """orthogonalize() with operands of one or two f16 parts and f32 sums."""
+def modelled(u, split, steps=5, runs=None):
+    """orthogonalize() with operands of one or two f16 parts and f32 sums. `runs`: how many steps at a time are taken on the
+    smaller side (A = X X^T, A <- Q A Q with Q = a I + b A + c A A, X <- the product of the Q's times X); one by one unless given."""
     a, b, c = (np.float32(v) for v in COEFFICIENTS)
-    sx, sa = np.float32(4096), np.float32(8192)
+    sx, sa, sq = np.float32(4096), np.float32(8192), [None, np.float32(8192), np.float32(4096), np.float32(1024)]
     count = 2 if split else 1
     x = np.asarray(u, np.float64)
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
     x = (x / (np.sqrt((x * x).sum()) + NORM_FLOOR)).astype(np.float32)
-    for _ in range(steps):
+    turned = lambda p: [np.ascontiguousarray(v.T) for v in p[:2]]  # noqa: E731
+    symmetric = lambda v: np.tril(v) + np.tril(v, -1).T  # noqa: E731
+    assert sum(runs or [1] * steps) == steps
+    for run in runs or [1] * steps:
         xp = _parts(x, sx, count)
-        ap = _parts(_product(xp, xp) / (sx * sx), sa, count)
-        bp = _parts(b * (ap[0] + ap[1]) / sa + c * _product(ap, ap) / (sa * sa), sa, count)
-        x = a * xp[2] + _product(bp, [np.ascontiguousarray(v.T) for v in xp[:2]]) / (sa * sx)
+        ap = _parts(symmetric(_product(xp, xp) / (sx * sx)), sa, count)
+        for j in range(run):
+            bp = _parts(symmetric(b * ap[2] + c * _product(ap, ap) / (sa * sa)), sa, count)
+            if j == 0:
+                qp = bp
+            elif j == 1:
+                q = symmetric(a * a * np.eye(len(x), dtype=np.float32) + a * qp[2] + a * bp[2] + _product(bp, qp) / (sa * sa))
+                qp = _parts(q, sq[2], count)
+            else:
+                qp = _parts(symmetric(a * qp[2] + _product(bp, qp) / (sa * sq[j])), sq[j + 1], count)
+            if j + 1 < run:
+                cp = _parts(symmetric(a * ap[2] + _product(bp, ap) / (sa * sa)), sa, count)
+                ap = _parts(symmetric(a * cp[2] + _product(cp, bp) / (sa * sa)), sa, count)
+        x = a * xp[2] + _product(bp, turned(xp)) / (sa * sx) if run == 1 else _product(qp, turned(xp)) / (sq[run] * sx)
     x = _parts(x, sx, 2)[2]
     return x.T if tall else x

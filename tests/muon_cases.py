@@ -14,6 +14,10 @@ from oracle import muon as oracle
 SHAPES = [(1, 1), (1, 7), (9, 1), (3, 5), (8, 8), (31, 33), (64, 64), (65, 40), (130, 20), (40, 200), (128, 128), (129, 257)]
 
 
+def runs_of(muon):
+    return [int(r) for r in muon.description.split("\nruns ")[1].split("\n")[0].split(",")]
+
+
 def matrix(shape, kind, seed):
     rng = np.random.default_rng(seed)
     r, c = shape
@@ -28,10 +32,10 @@ def matrix(shape, kind, seed):
     return rng.standard_normal(shape)
 
 
-def check(got, u, dtype, split, steps=5):
-    """`got` f32, `u` the matrix as the kernel saw it."""
+def check(got, u, dtype, split, steps=5, runs=None):
+    """`got` f32, `u` the matrix as the kernel saw it, `runs` how its steps were taken."""
     want = oracle.orthogonalize(u, steps)
-    off = np.linalg.norm(oracle.modelled(u, split, steps) - want)
+    off = np.linalg.norm(oracle.modelled(u, split, steps, runs) - want)
     size = np.linalg.norm(want)
     allowed = 4 * off + 1e-6 * size + HALF_STEP[dtype] * size + TINY[dtype] * np.sqrt(want.size)
     far = np.linalg.norm(got - want)

@@ -8,11 +8,12 @@ import pytest
 import helium_amd as ha
 from cpu_emul import run_kernel
 from helium_amd import _ffi
-from muon_cases import SHAPES, check, matrix, to_f32, to_storage
+from muon_cases import SHAPES, check, matrix, runs_of, to_f32, to_storage
 from oracle import muon as oracle
 
 MATRIX = np.dtype([("rows", "u4"), ("cols", "u4"), ("mp", "u4"), ("np", "u4"), ("tall", "u4"), ("first_part", "u4"), ("parts", "u4"),
-                   ("shape_scale", "f4"), ("x", "u8"), ("xt", "u8", 2), ("a", "u8"), ("b", "u8"), ("x_low", "u8")])
+                   ("shape_scale", "f4"), ("at", "u8", 9)])
+PRODUCT = np.dtype([(k, "u4") for k in ("p", "q", "e1", "e2", "out", "turned")] + [(k, "f4") for k in ("c1", "c2", "cs", "ci")])
 TASK = np.dtype([(k, "u4") for k in ("matrix", "i", "j", "k_begin", "k_end", "slot", "share", "shares")])
 BLOCK = np.dtype([("matrix", "u4"), ("i", "u4"), ("j", "u4")])
 
@@ -42,11 +43,28 @@ def test_five_steps_bring_the_documented_range_near_one():
 
 
 @pytest.mark.parametrize("kind", ["normal", "low_rank", "one_entry", "zero"])
-@pytest.mark.parametrize("split", [True, False])
-def test_the_documented_arithmetic_is_within_the_tests_own_tolerance(kind, split):
+@pytest.mark.parametrize("split,runs", [(True, None), (False, None), (True, [3, 2])])
+def test_the_documented_arithmetic_is_within_the_tests_own_tolerance(kind, split, runs):
     for k, shape in enumerate(SHAPES):
         u = matrix(shape, kind, 1 + k).astype(np.float32)
-        check(oracle.modelled(u, split), u, "f32", split)
+        check(oracle.modelled(u, split, 5, runs), u, "f32", split, 5, runs)
+
+
+def test_several_steps_at_once_cost_few_digits():
+    """Singular values over three decades, where an error of X X^T weighs most: in 64 bits the two forms are one."""
+    rng = np.random.default_rng(2)
+    u, _, vt = np.linalg.svd(rng.standard_normal((96, 400)), full_matrices=False)
+    u = (u * np.logspace(0, -3, 96)) @ vt
+    want = oracle.orthogonalize(u)
+    far = {str(r): np.linalg.norm(oracle.modelled(u, True, 5, r) - want) / np.linalg.norm(want) for r in (None, [3, 2])}
+    assert far["None"] < 1e-5 and far["[3, 2]"] < 1e-5, far
+
+
+def test_how_steps_are_taken_goes_by_shape_and_precision():
+    runs = lambda *a, **k: runs_of(ha.Muon(*a, **k))  # noqa: E731
+    assert runs([(512, 512)], "f32") == [1] * 5
+    assert runs([(512, 4608)], "f32") == [3, 2] and runs([(4608, 512)], "f32", steps=4) == [2, 2] and runs([(512, 4608)], "f32", steps=7) == [3, 2, 2]
+    assert runs([(512, 4608)], "bf16", precision="f16_f32") == [1] * 5
 
 
 SHFL = r"""
@@ -72,7 +90,7 @@ def emulated(shapes, dtype, split, steps, in_storage, step=None):
     muon = ha.Muon(shapes, dtype, precision="f32_f32" if split else "f16_f32", steps=steps)
     mats, tasks, joins = np.frombuffer(muon.table(0), MATRIX), [np.frombuffer(muon.table(t), TASK) for t in (1, 2, 3)], [np.frombuffer(muon.table(t), TASK) for t in (4, 5, 6)]
     parts, blocks = (np.frombuffer(muon.table(t), BLOCK) for t in (7, 8))
-    said = [dict(s.split("=") for s in line.split()[1:]) for line in muon.description.splitlines()]
+    said = [dict(s.split("=") for s in line.split()[1:]) for line in muon.description.splitlines() if line.startswith("muon")]
     workspace = int(said[0]["workspace"])
     elements, *products = muon.source.split("\n//// product ")
     names = [f"in{k}" for k in range(len(shapes))]
@@ -103,30 +121,41 @@ extern "C" void emu_finish(const Matrix* m, const Block* t, const char* ws, {par
     if step:  # from here on the new momenta are inputs
         given = [(a, 0) for a in in_storage] + [b for m, n, w in zip(momenta, new_momenta, weights) for b in ((m, 0), (n, 0), (w, 0))]
     ws, = run_kernel(text, "emu_convert", len(blocks), 256, [(mats, 0), (blocks, 0), (sums, 0), (np.empty(workspace, np.uint8), 1)] + given)
-    for k in range(steps):
-        turn, last = np.array([k & 1], np.uint32), np.array([k == steps - 1], np.uint32)
-        for p, product in enumerate(products):
-            name, body = product.split("\n", 1)
-            cut = {key: int(v) for key, v in said[1 + p].items() if key != "estimate"}
-            body = SHFL + body + f"""
-extern "C" void emu_product(const Matrix* m, const Task* t, char* ws, float* parked, const u32* turn, const u32* last) {{ product<{name.upper()}>(m, t, ws, parked, *turn, *last); }}
-extern "C" void emu_join(const Matrix* m, const Task* t, char* ws, const float* parked, const u32* turn, const u32* last) {{ join<{name.upper()}>(m, t, ws, parked, *turn, *last); }}
+    kinds, launches = {}, []
+    for p, product in enumerate(products):
+        name, body = product.split("\n", 1)
+        kinds[name] = {key: int(v) for key, v in said[1 + p].items() if key != "estimate"}, tasks[p], joins[p], SHFL + body + f"""
+extern "C" void emu_product(const Matrix* m, const Task* t, char* ws, float* parked, const u64* pitch, const Products* all) {{ product<{name.upper()}>(m, t, ws, parked, *pitch, *all); }}
+extern "C" void emu_join(const Matrix* m, const Task* t, char* ws, const float* parked, const u64* pitch, const Products* all) {{ join<{name.upper()}>(m, t, ws, parked, *pitch, *all); }}
 """
-            parked = np.full(max(cut["parked"], 1), np.nan, np.float32)
-            ws, parked = run_kernel(body, "emu_product", cut["grid"], cut["threads"], [(mats, 0), (tasks[p], 0), (ws, 2), (parked, 2), (turn, 0), (last, 0)])
-            if cut["join_grid"]:
-                ws, = run_kernel(body, "emu_join", cut["join_grid"], 256, [(mats, 0), (joins[p], 0), (ws, 2), (parked, 0), (turn, 0), (last, 0)])
+    for line in muon.description.split("\nlaunch ")[1:]:
+        name, *fields = line.split()
+        fields = dict(f.split("=") for f in fields)
+        if fields["of"] == "0":
+            launches.append((name, np.zeros(2, PRODUCT), [0]))
+        _, given_products, count = launches[-1]
+        count[0] += 1
+        for key in PRODUCT.names:
+            given_products[int(fields["of"])][key] = float(fields[key])
+    for name, all_products, (count,) in launches:
+        cut, tasks_of, joins_of, body = kinds[name]
+        pitch, parked = np.array([cut["parked"]], np.uint64), np.full(max(cut["parked"], 1) * 2, np.nan, np.float32)
+        ws, parked = run_kernel(body, "emu_product", cut["grid"], cut["threads"], [(mats, 0), (tasks_of, 0), (ws, 2), (parked, 2), (pitch, 0), (all_products, 0)], grid_y=count)
+        if cut["join_grid"]:
+            ws, = run_kernel(body, "emu_join", cut["join_grid"], 256, [(mats, 0), (joins_of, 0), (ws, 2), (parked, 0), (pitch, 0), (all_products, 0)], grid_y=count)
     outs = [np.empty(s, np.float32 if step else in_storage[0].dtype) for s in shapes]
     return run_kernel(text, "emu_finish", len(blocks), 256, [(mats, 0), (blocks, 0), (ws, 0)] + given + [(o, 1) for o in outs]), new_momenta
 
 
-@pytest.mark.parametrize("dtype,split,steps", [("f32", True, 2), ("bf16", False, 2), ("f16", False, 1), ("f32", False, 3)])
-def test_the_kernels_match_the_oracle(dtype, split, steps):
-    shapes = [(5, 9), (70, 33), (1, 1), (40, 150)]
+@pytest.mark.parametrize("dtype,split,steps,runs", [("f32", True, 1, "0"), ("f32", True, 3, "1"), ("f32", True, 5, "1"), ("f32", True, 2, "0"), ("bf16", False, 2, "0"), ("f16", False, 1, "0")])
+def test_the_kernels_match_the_oracle(monkeypatch, dtype, split, steps, runs):
+    monkeypatch.setenv("HELIUM_HIP_MUON_RUNS", runs)          # several steps at once, whatever they are estimated to take
+    monkeypatch.setenv("HELIUM_HIP_MUON_ONE_BY_ONE", "1" if runs == "0" else "0")
+    shapes = [(70, 90), (1, 1)] if steps > 2 else [(5, 9), (70, 33), (1, 1), (40, 150)]
     stored = [to_storage(matrix(s, "normal", 3), dtype) for s in shapes]
     got, _ = emulated(shapes, dtype, split, steps, stored)
     for g, s in zip(got, stored):
-        check(to_f32(g, dtype), to_f32(s, dtype), dtype, split, steps)
+        check(to_f32(g, dtype), to_f32(s, dtype), dtype, split, steps, {"0": None, "1": {3: [3], 5: [3, 2]}.get(steps)}[runs])
 
 
 @pytest.mark.parametrize("nesterov", [0, 1])

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import helium_amd as ha
-from muon_cases import SHAPES, check, matrix, to_f32, to_storage
+from muon_cases import SHAPES, check, matrix, runs_of, to_f32, to_storage
 from oracle import muon as oracle
 from test_group_norm_gpu import address, back, device
 
@@ -38,6 +38,22 @@ def test_larger_matrices_by_themselves(gpu, shape, dtype, precision):
     stored = [to_storage(matrix(shape, "normal", 2), dtype)]
     got, = orthogonalized([shape], stored, dtype, precision)
     check(to_f32(got, dtype), to_f32(stored[0], dtype), dtype, precision == "f32_f32")
+
+
+@pytest.mark.parametrize("runs", ["one by one", "several"])
+@pytest.mark.parametrize("tile", [64, 128, 192, 256])
+def test_every_cut_of_the_products(gpu, monkeypatch, tile, runs):
+    """Tiles and forms that the sizes here would not be given: matrices that end inside a tile, shared sums, all in one group."""
+    monkeypatch.setenv("HELIUM_HIP_MUON_TILE", str(tile))
+    monkeypatch.setenv("HELIUM_HIP_MUON_RUNS" if runs == "several" else "HELIUM_HIP_MUON_ONE_BY_ONE", "1")
+    shapes = [(200, 700), (64, 64), (500, 260), (3, 5), (130, 1), (400, 400)]
+    stored = [to_storage(matrix(s, "normal", 14), "f32") for s in shapes]
+    for precision in ("f32_f32", "f16_f32"):
+        muon = ha.Muon(shapes, "f32", precision=precision)
+        assert f"tile={tile} " in muon.description
+        assert runs_of(muon) == ([3, 2] if runs == "several" and precision == "f32_f32" else [1] * 5)
+        for g, s in zip(orthogonalized(shapes, stored, "f32", None, muon=muon), stored):
+            check(g, s, "f32", precision == "f32_f32", 5, runs_of(muon))
 
 
 @pytest.mark.parametrize("steps", [1, 2, 3, 4])
