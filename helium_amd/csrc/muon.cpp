@@ -64,8 +64,13 @@ struct Matrix {
 enum { X, XT, XT2, A, B, C, Q, Q2, X_LOW };   // places of a matrix's buffers in `at`
 struct Block { u32 matrix, i, j; };
 // R = c1 E1 + c2 E2 + cs P Q^T + ci I; operands, results and the transposed results by their places.
-struct Product { u32 p, q, e1, e2, out, turned; float c1, c2, cs, ci; };
-struct Products { Product of[2]; };
+// R = c1 E1 + c2 E2 + cs P Q^T + ci I of one matrix: operands and results by their offsets in the workspace. parked_at: of the product's
+// shares, in floats. (All that a workgroup has to look up lies together, one look behind its task.)
+struct Product {
+    u32 mp, np;
+    float c1, c2, cs, ci;
+    u64 p, q, e1, e2, out, turned, low, parked_at;
+};
 struct Task { u32 matrix, i, j, k_begin, k_end, slot, share, shares; };
 struct Operands {
     const elem_t* in[GROUP];
@@ -322,19 +327,26 @@ __device__ __forceinline__ void strip_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// Where results come together and go. Looked up ahead of the sums: at their end each look would be waited for.
+struct Ends { const f16_t *e1, *e2; f16_t *plain, *turned, *low; };
+template <int STAGE> __device__ __forceinline__ Ends ends_of(const Product& m, char* __restrict__ ws) {
+    Ends n;
+    n.e1 = (const f16_t*)(ws + m.e1), n.e2 = (const f16_t*)(ws + m.e2);
+    n.plain = (f16_t*)(ws + m.out), n.turned = (f16_t*)(ws + m.turned);
+    // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
+    // singular values with it)
+    n.low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.low) : nullptr;
+    return n;
+}
+
 // The results of 32 RM x 32 RN sums at (row0, col0) of the product. A lane holds rows (e / 4) * 8 + half * 4 + e % 4 of column lane % 32
 // of each 32 x 32 block; through a strip of LDS that belongs to the wave it gets 8 neighbours of a row, adds E, stores them, and
 // puts them back for the transposed copy.
 template <int STAGE, int RM, int RN>
-__device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix& m, const Product& pr, char* __restrict__ ws, u32 row0, u32 col0, bool mirrored, float* strip) {
+__device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Ends& ends, const Product& m, u32 row0, u32 col0, bool mirrored, float* strip) {
     constexpr u32 strip_pitch = RN * 32 + 1, row_lanes = RN * 4, col_lanes = RM * 4;   // lanes along a row of the strip, and along a column
     const u32 lane = threadIdx.x & 63u, half = lane >> 5;
     const u32 pitch = STAGE == APPLY ? m.np : m.mp;
-    const f16_t *e1_rows = (const f16_t*)(ws + m.at[pr.e1]), *e2_rows = (const f16_t*)(ws + m.at[pr.e2]);
-    f16_t *plain = (f16_t*)(ws + m.at[pr.out]), *turned = (f16_t*)(ws + m.at[STAGE == APPLY ? pr.turned : pr.out]);
-    // (of X the low part counts in either precision: what f16 drops of a X in each step would stay dropped, and the small
-    // singular values with it)
-    f16_t* low = STAGE == APPLY && !SPLIT ? (f16_t*)(ws + m.at[X_LOW]) : nullptr;
 #pragma unroll
     for (int i = 0; i < RM; i++)
 #pragma unroll
@@ -346,18 +358,18 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix
     for (u32 s = 0; s < RM * 32 * row_lanes / 64; s++) {
         const u32 r = s * (64 / row_lanes) + lane / row_lanes, c = lane % row_lanes * 8;
         float v[8], e1[8], e2[8];
-        const bool has_e1 = STAGE != GRAM && pr.c1 != 0.0f, has_e2 = STAGE == INNER && pr.c2 != 0.0f;
-        if (has_e1) get(e1_rows, row0 + r, col0 + c, pitch, e1, low);
-        if (has_e2) get(e2_rows, row0 + r, col0 + c, pitch, e2, nullptr);
+        const bool has_e1 = STAGE != GRAM && m.c1 != 0.0f, has_e2 = STAGE == INNER && m.c2 != 0.0f;
+        if (has_e1) get(ends.e1, row0 + r, col0 + c, pitch, e1, ends.low);
+        if (has_e2) get(ends.e2, row0 + r, col0 + c, pitch, e2, nullptr);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            v[e] = pr.cs * strip[r * strip_pitch + c + e];
-            if (has_e1) v[e] += pr.c1 * e1[e];
-            if (has_e2) v[e] += pr.c2 * e2[e];
-            if (STAGE == INNER && row0 + r == col0 + c + e) v[e] += pr.ci;
+            v[e] = m.cs * strip[r * strip_pitch + c + e];
+            if (has_e1) v[e] += m.c1 * e1[e];
+            if (has_e2) v[e] += m.c2 * e2[e];
+            if (STAGE == INNER && row0 + r == col0 + c + e) v[e] += m.ci;
             strip[r * strip_pitch + c + e] = v[e];
         }
-        put(plain, row0 + r, col0 + c, pitch, v, low);
+        put(ends.plain, row0 + r, col0 + c, pitch, v, ends.low);
     }
     strip_sync();
     if (mirrored)
@@ -367,7 +379,7 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[RM][RN], const Matrix
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = strip[(r + e) * strip_pitch + c];
-            put(turned, col0 + c, row0 + r, m.mp, v, nullptr);
+            put(ends.turned, col0 + c, row0 + r, m.mp, v, nullptr);
         }
     strip_sync();
 }
@@ -376,16 +388,16 @@ struct Fragments { f16x8 a[PARTS][MB], b[PARTS][NB]; };
 struct True { constexpr operator bool() const { return true; } };
 struct False { constexpr operator bool() const { return false; } };
 
-template <int STAGE> __device__ __forceinline__ void product(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u64 parked_pitch, const Products& all) {
+template <int STAGE> __device__ __forceinline__ void product(const Product* __restrict__ products, u32 matrices, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked) {
     __shared__ __attribute__((aligned(16))) f16_t lds[LDS_HALVES];
     const Task t = tasks[blockIdx.x];
-    const Matrix& m = mats[t.matrix];
-    const Product& pr = all.of[STAGE == INNER ? blockIdx.y : 0];
-    if (STAGE == INNER) parked += blockIdx.y * parked_pitch;
+    const Product m = products[(STAGE == INNER ? blockIdx.y * matrices : 0u) + t.matrix];
+    if (STAGE == INNER) parked += m.parked_at;
+    const Ends ends = ends_of<STAGE>(m, ws);
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
     const u32 k_len = (STAGE == GRAM ? m.np : m.mp) * PARTS;   // halves of a row
     const u32 p_limit = m.mp, q_limit = STAGE == APPLY ? m.np : m.mp;
-    const f16_t *p_rows = (const f16_t*)(ws + m.at[pr.p]), *q_rows = (const f16_t*)(ws + m.at[pr.q]);
+    const f16_t *p_rows = (const f16_t*)(ws + m.p), *q_rows = (const f16_t*)(ws + m.q);
     // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows meet 8
     // different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes. (A tile that ends beyond the matrix loads its first rows
     // there: sums that nothing stores.)
@@ -509,18 +521,18 @@ template <int STAGE> __device__ __forceinline__ void product(const Matrix* __res
             for (int di = 0; di < SM; di++)
 #pragma unroll
                 for (int dj = 0; dj < SN; dj++) part[di][dj] = acc[i + di][j + dj];
-            finish<STAGE, SM, SN>(part, m, pr, ws, row0, col0, STAGE == APPLY ? pr.turned != X : t.i != t.j, strip);
+            finish<STAGE, SM, SN>(part, ends, m, row0, col0, STAGE == APPLY ? m.turned != m.out : t.i != t.j, strip);
         }
 }
 
 // The shares of a tile added up in their order: a wave per 32 x 32 block, four waves in a workgroup. `tiles`: the first share's task of each.
-template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u64 parked_pitch, const Products& all) {
+template <int STAGE> __device__ __forceinline__ void join(const Product* __restrict__ products, u32 matrices, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked) {
     __shared__ float strips[4 * STRIP_FLOATS(1, 1)];
     constexpr u32 blocks = (TILE / 32) * (TILE / 32);
     const Task t = tiles[blockIdx.x / (blocks / 4)];
-    const Matrix& m = mats[t.matrix];
-    const Product& pr = all.of[STAGE == INNER ? blockIdx.y : 0];
-    if (STAGE == INNER) parked += blockIdx.y * parked_pitch;
+    const Product m = products[(STAGE == INNER ? blockIdx.y * matrices : 0u) + t.matrix];
+    if (STAGE == INNER) parked += m.parked_at;
+    const Ends ends = ends_of<STAGE>(m, ws);
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = blockIdx.x % (blocks / 4) * 4 + wave;
     const u32 row0 = t.i * TILE + block / (TILE / 32) * 32, col0 = t.j * TILE + block % (TILE / 32) * 32;
     if (row0 >= m.mp || col0 >= (STAGE == APPLY ? m.np : m.mp)) return;
@@ -542,21 +554,14 @@ template <int STAGE> __device__ __forceinline__ void join(const Matrix* __restri
 #pragma unroll
             for (int e = 0; e < 16; e++) sum[0][0][e] += got[d][e / 4][e % 4];
     }
-    finish<STAGE, 1, 1>(sum, m, pr, ws, row0, col0, STAGE == APPLY ? pr.turned != X : t.i != t.j, strips + wave * STRIP_FLOATS(1, 1));
+    finish<STAGE, 1, 1>(sum, ends, m, row0, col0, STAGE == APPLY ? m.turned != m.out : t.i != t.j, strips + wave * STRIP_FLOATS(1, 1));
 }
 
 #define KERNELS(name, stage) \
-    extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void muon_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked, u64 parked_pitch, Products all) { product<stage>(mats, tasks, ws, parked, parked_pitch, all); } \
-    extern "C" __global__ __launch_bounds__(256) void muon_join_##name(const Matrix* __restrict__ mats, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked, u64 parked_pitch, Products all) { join<stage>(mats, tiles, ws, parked, parked_pitch, all); }
+    extern "C" __global__ __launch_bounds__(WAVES * 64) KERNEL_ATTRS void muon_##name(const Product* __restrict__ products, u32 matrices, const Task* __restrict__ tasks, char* __restrict__ ws, float* __restrict__ parked) { product<stage>(products, matrices, tasks, ws, parked); } \
+    extern "C" __global__ __launch_bounds__(256) void muon_join_##name(const Product* __restrict__ products, u32 matrices, const Task* __restrict__ tiles, char* __restrict__ ws, const float* __restrict__ parked) { join<stage>(products, matrices, tiles, ws, parked); }
 )HIP";
 
-struct ProductArg {
-    uint32_t p, q, e1, e2, out, turned;
-    float c1, c2, cs, ci;
-};
-struct ProductsArg {
-    ProductArg of[2];
-};
 constexpr double kA = 3.4445, kB = -4.7750, kC = 2.0315;
 enum { X, XT, XT2, A, B, C, Q, Q2, X_LOW };
 
@@ -826,20 +831,27 @@ void Muon::plan_launches() {
     }
     // scales of what is in the buffers: of X, of A, B and C, and of Q after so many steps (its values are at most a, a^2, a^3)
     const double sx = 4096, sa = 8192, sq[4] = {0, 8192, 4096, 1024};
-    auto add = [&](int kind, const std::vector<ProductArg>& products) {
-        Launch l{kind, (uint32_t)products.size(), {}};
+    // (what a launch computes lies in a table on the device: a kernel's own parameters come from host memory, and longer ones took
+    // the 20 small launches of a 64 x 576 matrix 79 -> 96 us)
+    std::vector<MuonProduct> table;
+    struct Formula {
+        uint32_t p, q, out, e1, e2, turned;  // places in MuonMatrix::at
+        double c1, c2, cs, ci;
+    };
+    auto add = [&](int kind, const std::vector<Formula>& products) {
+        launches_.push_back({kind, (uint32_t)products.size(), table.size() * sizeof(MuonProduct)});
         const char* names[3] = {"gram", "inner", "apply"};
         for (size_t k = 0; k < products.size(); k++) {
-            const ProductArg& a = products[k];
-            memcpy(l.products + k * sizeof(ProductArg), &a, sizeof(a));
-            launches_text_ += strfmt("\nlaunch %s of=%zu p=%u q=%u e1=%u e2=%u out=%u turned=%u c1=%.9g c2=%.9g cs=%.9g ci=%.9g", names[kind], k, a.p, a.q, a.e1, a.e2,
-                                     a.out, a.turned, (double)a.c1, (double)a.c2, (double)a.cs, (double)a.ci);
+            const Formula& f = products[k];
+            for (const MuonMatrix& m : matrices_)
+                table.push_back({m.mp, m.np, (float)f.c1, (float)f.c2, (float)f.cs, (float)f.ci, m.at[f.p], m.at[f.q], m.at[f.e1], m.at[f.e2], m.at[f.out], m.at[f.turned],
+                                 m.at[X_LOW], k * products_[kind].parked});
+            launches_text_ += strfmt("\nlaunch %s of=%zu c1=%.9g c2=%.9g cs=%.9g ci=%.9g", names[kind], k, f.c1, f.c2, f.cs, f.ci);
         }
-        launches_.push_back(l);
     };
-    static_assert(sizeof(ProductsArg) <= sizeof(Launch::products), "");
-    auto product = [](uint32_t p, uint32_t q, uint32_t out, uint32_t e1, double c1, double cs, uint32_t e2 = 0, double c2 = 0, double ci = 0, uint32_t turned = X) {
-        return ProductArg{p, q, e1, e2, out, turned, (float)c1, (float)c2, (float)cs, (float)ci};
+    // (a result that is not stored transposed as well, or in its own place as symmetric ones are, is given its own place)
+    auto product = [](uint32_t p, uint32_t q, uint32_t out, uint32_t e1, double c1, double cs, uint32_t e2 = X, double c2 = 0, double ci = 0, uint32_t turned = X) {
+        return Formula{p, q, out, e1, e2, turned == X ? out : turned, c1, c2, cs, ci};
     };
     launches_text_ = "\nruns";
     for (size_t k = 0; k < runs.size(); k++) launches_text_ += strfmt("%c%d", k ? ',' : ' ', runs[k]);
@@ -848,7 +860,7 @@ void Muon::plan_launches() {
     for (int r : runs) {
         add(0, {product(X, X, A, 0, 0, sa / (sx * sx))});
         uint32_t q = Q, q_new = Q2;  // of two steps and more; after the first one Q is a I + B, and B is in q
-        std::vector<ProductArg> also;  // (waits for a launch to share)
+        std::vector<Formula> also;  // (waits for a launch to share)
         for (int j = 0; j < r; j++) {
             const uint32_t b = r > 1 && j == 0 ? q : (uint32_t)B;
             add(1, {product(A, A, b, A, kB, kC * sa / (sa * sa))});
@@ -872,19 +884,21 @@ void Muon::plan_launches() {
         else add(2, {product(q, from, X, X, 0, 1 / sq[r], 0, 0, 0, last ? (uint32_t)X : to)});
         std::swap(from, to);
     }
+    tables_[9] = bytes_of(table);
 }
 
 void Muon::products(char* ws, char* tables, hipStream_t stream) {
     const uint32_t join_block[3] = {256, 1, 1};
-    char *mats = tables + table_at_[0], *parked = ws + shared_at_;
-    for (Launch& l : launches_) {
+    char* parked = ws + shared_at_;
+    uint32_t matrices = (uint32_t)matrices_.size();
+    for (const Launch& l : launches_) {
         const ProductKind& kind = products_[l.kind];
         char *tasks = tables + table_at_[1 + l.kind], *joins = tables + table_at_[4 + l.kind];
         const uint32_t grid[3] = {kind.grid, l.count, 1}, block[3] = {kind.threads, 1, 1}, join_grid[3] = {kind.join_grid, l.count, 1};
-        uint64_t parked_pitch = kind.parked;
-        void* args[] = {&mats, &tasks, &ws, &parked, &parked_pitch, l.products};
+        char* what = tables + table_at_[9] + l.products_at;
+        void* args[] = {&what, &matrices, &tasks, &ws, &parked};
         kind.kernel->launch(grid, block, 0, stream, args);
-        void* join_args[] = {&mats, &joins, &ws, &parked, &parked_pitch, l.products};
+        void* join_args[] = {&what, &matrices, &joins, &ws, &parked};
         if (kind.join_grid) kind.join->launch(join_grid, join_block, 0, stream, join_args);
     }
 }

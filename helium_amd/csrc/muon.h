@@ -38,6 +38,14 @@ struct MuonTask {
     uint32_t matrix, i, j, k_begin, k_end, slot, share, shares;
 };
 
+// R = c1 E1 + c2 E2 + cs P Q^T + ci I of one matrix: operands and results by their offsets in the workspace; parked_at: where the
+// product's shares wait, in floats.
+struct MuonProduct {
+    uint32_t mp, np;
+    float c1, c2, cs, ci;
+    uint64_t p, q, e1, e2, out, turned, low, parked_at;
+};
+
 struct MuonStep {
     float learning_rate, momentum, weight_decay;
     int32_t nesterov;
@@ -54,8 +62,9 @@ public:
     const std::string& describe() const { return describe_; }
     size_t count() const { return pr_.shapes.size(); }
     // The tables the kernels read, as bytes: 0 matrices, 1 to 3 tasks of the three products, 4 to 6 those of their tiles that several
-    // workgroups share, 7 shares of the sums of squares, 8 blocks of the conversions.
-    static constexpr int kTables = 9;
+    // workgroups share, 7 shares of the sums of squares, 8 blocks of the conversions, 9 what the launches compute
+    // (a MuonProduct per matrix and product).
+    static constexpr int kTables = 10;
     const std::vector<char>& table(int which) const { return tables_[which]; }
     size_t workspace_bytes() const { return workspace_bytes_; }
 
@@ -81,8 +90,8 @@ private:
     } products_[3];
     struct Launch {
         int kind;
-        uint32_t count;                      // products
-        alignas(8) unsigned char products[80];  // as the kernel takes them
+        uint32_t count;      // products
+        size_t products_at;  // in table 9
     };
     std::vector<Launch> launches_;
     std::string launches_text_;

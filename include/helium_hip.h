@@ -506,7 +506,7 @@ int he_muon_step(he_muon_t muon, const void* const* gradients, const float* cons
                  int nesterov, he_stream_t stream);
 /* The generated HIP source, how the products are cut, and the tables the kernels read (0 matrices, 1 to 3 the tasks of the three
  * products of a step, 4 to 6 those of their tiles that several workgroups share, 7 shares of the sums of squares, 8 blocks of the
- * conversions), for inspection and tests. */
+ * conversions, 9 what each launch computes of each matrix), for inspection and tests. */
 const char* he_muon_source(he_muon_t muon);
 const char* he_muon_describe(he_muon_t muon);
 int he_muon_table(he_muon_t muon, int which, void* data, size_t capacity, size_t* bytes);

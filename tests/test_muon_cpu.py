@@ -13,7 +13,8 @@ from oracle import muon as oracle
 
 MATRIX = np.dtype([("rows", "u4"), ("cols", "u4"), ("mp", "u4"), ("np", "u4"), ("tall", "u4"), ("first_part", "u4"), ("parts", "u4"),
                    ("shape_scale", "f4"), ("at", "u8", 9)])
-PRODUCT = np.dtype([(k, "u4") for k in ("p", "q", "e1", "e2", "out", "turned")] + [(k, "f4") for k in ("c1", "c2", "cs", "ci")])
+PRODUCT = np.dtype([(k, "u4") for k in ("mp", "np")] + [(k, "f4") for k in ("c1", "c2", "cs", "ci")]
+                   + [(k, "u8") for k in ("p", "q", "e1", "e2", "out", "turned", "low", "parked_at")])
 TASK = np.dtype([(k, "u4") for k in ("matrix", "i", "j", "k_begin", "k_end", "slot", "share", "shares")])
 BLOCK = np.dtype([("matrix", "u4"), ("i", "u4"), ("j", "u4")])
 
@@ -121,28 +122,24 @@ extern "C" void emu_finish(const Matrix* m, const Block* t, const char* ws, {par
     if step:  # from here on the new momenta are inputs
         given = [(a, 0) for a in in_storage] + [b for m, n, w in zip(momenta, new_momenta, weights) for b in ((m, 0), (n, 0), (w, 0))]
     ws, = run_kernel(text, "emu_convert", len(blocks), 256, [(mats, 0), (blocks, 0), (sums, 0), (np.empty(workspace, np.uint8), 1)] + given)
-    kinds, launches = {}, []
+    kinds = {}
     for p, product in enumerate(products):
         name, body = product.split("\n", 1)
         kinds[name] = {key: int(v) for key, v in said[1 + p].items() if key != "estimate"}, tasks[p], joins[p], SHFL + body + f"""
-extern "C" void emu_product(const Matrix* m, const Task* t, char* ws, float* parked, const u64* pitch, const Products* all) {{ product<{name.upper()}>(m, t, ws, parked, *pitch, *all); }}
-extern "C" void emu_join(const Matrix* m, const Task* t, char* ws, const float* parked, const u64* pitch, const Products* all) {{ join<{name.upper()}>(m, t, ws, parked, *pitch, *all); }}
+extern "C" void emu_product(const Product* what, const u32* matrices, const Task* t, char* ws, float* parked) {{ product<{name.upper()}>(what, *matrices, t, ws, parked); }}
+extern "C" void emu_join(const Product* what, const u32* matrices, const Task* t, char* ws, const float* parked) {{ join<{name.upper()}>(what, *matrices, t, ws, parked); }}
 """
-    for line in muon.description.split("\nlaunch ")[1:]:
-        name, *fields = line.split()
-        fields = dict(f.split("=") for f in fields)
-        if fields["of"] == "0":
-            launches.append((name, np.zeros(2, PRODUCT), [0]))
-        _, given_products, count = launches[-1]
-        count[0] += 1
-        for key in PRODUCT.names:
-            given_products[int(fields["of"])][key] = float(fields[key])
-    for name, all_products, (count,) in launches:
+    what, matrices = np.frombuffer(muon.table(9), PRODUCT).reshape(-1, len(shapes)), np.array([len(shapes)], np.uint32)
+    lines = [line.split()[:2] for line in muon.description.split("\nlaunch ")[1:]]
+    for k, (name, of) in enumerate(lines):
+        if of != "of=0":
+            continue
+        count = 2 if k + 1 < len(lines) and lines[k + 1][1] == "of=1" else 1
         cut, tasks_of, joins_of, body = kinds[name]
-        pitch, parked = np.array([cut["parked"]], np.uint64), np.full(max(cut["parked"], 1) * 2, np.nan, np.float32)
-        ws, parked = run_kernel(body, "emu_product", cut["grid"], cut["threads"], [(mats, 0), (tasks_of, 0), (ws, 2), (parked, 2), (pitch, 0), (all_products, 0)], grid_y=count)
+        parked = np.full(max(cut["parked"], 1) * 2, np.nan, np.float32)
+        ws, parked = run_kernel(body, "emu_product", cut["grid"], cut["threads"], [(what[k:k + count], 0), (matrices, 0), (tasks_of, 0), (ws, 2), (parked, 2)], grid_y=count)
         if cut["join_grid"]:
-            ws, = run_kernel(body, "emu_join", cut["join_grid"], 256, [(mats, 0), (joins_of, 0), (ws, 2), (parked, 0), (pitch, 0), (all_products, 0)], grid_y=count)
+            ws, = run_kernel(body, "emu_join", cut["join_grid"], 256, [(what[k:k + count], 0), (matrices, 0), (joins_of, 0), (ws, 2), (parked, 0)], grid_y=count)
     outs = [np.empty(s, np.float32 if step else in_storage[0].dtype) for s in shapes]
     return run_kernel(text, "emu_finish", len(blocks), 256, [(mats, 0), (blocks, 0), (ws, 0)] + given + [(o, 1) for o in outs]), new_momenta
 
