@@ -63,7 +63,6 @@ struct Matrix {
 };
 enum { X, XT, XT2, A, B, C, Q, Q2, X_LOW };   // places of a matrix's buffers in `at`
 struct Block { u32 matrix, i, j; };
-// R = c1 E1 + c2 E2 + cs P Q^T + ci I; operands, results and the transposed results by their places.
 // R = c1 E1 + c2 E2 + cs P Q^T + ci I of one matrix: operands and results by their offsets in the workspace. parked_at: of the product's
 // shares, in floats. (All that a workgroup has to look up lies together, one look behind its task.)
 struct Product {
