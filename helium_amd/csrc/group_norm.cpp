@@ -293,26 +293,29 @@ __device__ __forceinline__ float share_of_m2(const float* __restrict__ parts, u3
 __device__ __forceinline__ float rstd_from(float m2) { return 1.0f / sqrtf(m2 / ((float)PIXELS * (float)D) + EPS); }
 
 #if MERGE
-// One workgroup per (sample, group).
-extern "C" __global__ __launch_bounds__(256) void group_norm_merge(const float* __restrict__ parts, float* __restrict__ stats,
-                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    __shared__ float waves[2][4];
+// The parts of a (sample, group) by one workgroup, which has a thread to each of up to 1024: the parts were written on other XCDs and
+// every look at them is a long one.
+__device__ __forceinline__ float over_mergers(float s, float* waves) {
+    for (int m = 32; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+    if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0f;
+#pragma unroll
+    for (u32 w = 0; w < MERGERS / 64; w++) s += waves[w];
+    return s;
+}
+extern "C" __global__ __launch_bounds__(MERGERS) void group_norm_merge(const float* __restrict__ parts, float* __restrict__ stats,
+                                                                      float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    __shared__ float waves[2][MERGERS / 64];
     const u64 of = blockIdx.x;
     const float* from = parts + of * CHUNKS * 2;
-    float s = share_of_mean(from, threadIdx.x, 256);
-    for (int m = 32; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
-    if ((threadIdx.x & 63u) == 0) waves[0][threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = waves[0][0] + waves[0][1] + waves[0][2] + waves[0][3];
-    float m2 = share_of_m2(from, threadIdx.x, 256, s);
-    for (int m = 32; m > 0; m /= 2) m2 += __shfl_xor(m2, m, 64);
-    if ((threadIdx.x & 63u) == 0) waves[1][threadIdx.x >> 6] = m2;
-    __syncthreads();
+    const float mean = over_mergers(share_of_mean(from, threadIdx.x, MERGERS), waves[0]);
+    const float m2 = over_mergers(share_of_m2(from, threadIdx.x, MERGERS, mean), waves[1]);
     if (threadIdx.x == 0) {
-        const float rstd = rstd_from(waves[1][0] + waves[1][1] + waves[1][2] + waves[1][3]);
-        stats[of * 2] = s;
+        const float rstd = rstd_from(m2);
+        stats[of * 2] = mean;
         stats[of * 2 + 1] = rstd;
-        if (mean_out) mean_out[of] = s;
+        if (mean_out) mean_out[of] = mean;
         if (rstd_out) rstd_out[of] = rstd;
     }
 }
@@ -620,7 +623,7 @@ std::string definitions(const GroupNormProblem& pr, const GroupNormTiling& t) {
       << "\n#define CHUNKS " << t.chunks << "\n#define BLOCKS " << t.grid << "ull\n#define LPG "
       << std::min(64, pow2_floor(t.threads / t.slice_groups)) << "\n#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 "
       << (pr.dtype == HE_F16) << "\n#define PARAM_SAME " << (pr.param_dtype == pr.dtype) << "\n#define ACT " << pr.activation
-      << "\n#define EPS " << strfmt("%.9gf", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge 
+      << "\n#define EPS " << strfmt("%.9gf", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge << "\n#define MERGERS " << t.mergers()
       << "\n#define LPE " << std::min<int64_t>(64, pow2_floor(std::max<int64_t>(1, t.threads / (2 * t.slice)))) << "\n";
     return s.str();
 }
@@ -714,7 +717,8 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
     HE_REQUIRE(pr.pixels <= (int64_t)1 << 40 && pr.batch <= (int64_t)1 << 31, HE_ERR_UNSUPPORTED, "group norm: extents too large");
     fwd_ = plan_group_norm(pr, false);
     bwd_ = plan_group_norm(pr, true);
-    HE_REQUIRE(std::max(fwd_.grid, bwd_.grid) < (1ull << 31) - 16384, HE_ERR_UNSUPPORTED, "group norm: the tensor is too large for one launch");
+    const uint64_t fold_grid = (uint64_t)pr.batch * ((2 * pr.channels + 31) / 32), merge_grid = fwd_.merge ? (uint64_t)pr.batch * pr.groups : 0;
+    HE_REQUIRE(std::max({fwd_.grid, bwd_.grid, fold_grid, merge_grid}) < (1ull << 31) - 16384, HE_ERR_UNSUPPORTED, "group norm: the tensor is too large for one launch");
     const std::string forward = definitions(pr, fwd_) + kCommon + kForward, backward = definitions(pr, bwd_) + kCommon + kBackward;
     auto compiled = std::async(std::launch::async, [&] { (void)rtc_compile(backward, "group_norm", {}); });
     auto make = [](const std::string& text, const char* entry) { return std::make_unique<JitKernel>(text, entry); };
@@ -765,7 +769,7 @@ void GroupNorm::forward(const void* x, const void* gamma, const void* beta, void
     std::lock_guard<std::mutex> lk(mu_);
     float* parts = scratch_.get(scratch_floats_, 0, stream).floats;
     float* stats = parts + rows * fwd_.chunks * 2;
-    const uint32_t merge_grid[3] = {(uint32_t)rows, 1, 1}, merge_block[3] = {256, 1, 1};
+    const uint32_t merge_grid[3] = {(uint32_t)rows, 1, 1}, merge_block[3] = {(uint32_t)fwd_.mergers(), 1, 1};
     void* a[] = {&x, &parts};
     stats_->launch(grid, block, 0, stream, a);
     void* b[] = {&parts, &stats, &mean, &rstd};

@@ -23,6 +23,11 @@ struct GroupNormProblem {
 struct GroupNormTiling {
     bool whole = false;   // a workgroup holds all pixels of its groups
     bool merge = false;   // statistics of so many parts that a launch of their own joins them
+    int mergers() const {  // threads of its workgroups
+        int n = 64;
+        while (n < 1024 && n < chunks) n *= 2;
+        return n;
+    }
     bool stream = false;  // results bypass the caches on their way to memory
     int vec = 1;          // elements per access
     int threads = 256;

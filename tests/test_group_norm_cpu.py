@@ -49,7 +49,7 @@ def forward_emulated(norm, shape, host):
     parts, = run_kernel(text, "group_norm_stats", grid, threads, [(host["x"], 0), (np.empty((n, groups, chunks, 2), np.float32), 1)])
     mean, rstd = stat, stat
     if chunks > 32:
-        parts, mean, rstd = run_kernel(text, "group_norm_merge", n * groups, 256, [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)])
+        parts, mean, rstd = run_kernel(text, "group_norm_merge", n * groups, int(re.search(r"#define MERGERS (\d+)", text).group(1)), [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)])
     return run_kernel(text, "group_norm_apply", grid, threads, [(host["x"], 0), (host["gamma"], 0), (host["beta"], 0), (parts, 0), (y, 1), (mean, 2), (rstd, 2)])
 
 
@@ -80,6 +80,12 @@ def test_the_kernels_match_the_oracle(monkeypatch, shape, dtype, activation, par
     check_forward(shape, dtype, activation, v, to_f32(y, dtype), got_mean, got_rstd)
     dx, dgamma, dbeta = backward_emulated(norm, shape, host, mean, rstd)
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
+def test_more_blocks_than_a_launch_has_are_refused():
+    """2^32 workgroups of the second launch, though the tensor's own launch would have fewer than 2^31."""
+    with pytest.raises(ha.HeliumError, match="too large for one launch"):
+        ha.GroupNorm(1 << 30, 1, 64, 1, "bf16")
 
 
 @pytest.mark.parametrize("kwargs,says", [
