@@ -309,7 +309,7 @@ const char* kProduct = R"HIP(
 #define ROW 64                          /* halves of a row in a k-tile: 128 bytes, 8 chunks */
 #define KS (4 / PARTS)                  /* matrix instructions along a k-tile */
 #define STAGE_HALVES (2 * TILE * ROW)
-#define LOADS (2 * TILE / 8 / WAVES)    /* direct loads of a wave per k-tile: 8 rows each */
+#define LOADS (2 * TILE / 8 / WAVES)    /* direct loads of a wave per k-tile: 8 rows each; an even number */
 #define READS (PARTS * (MB + NB))       /* fragments of one k-step */
 #define MMAS ((SPLIT ? 3 : 1) * MB * NB)
 #define SM (MB % 2 ? 1 : 2)             /* a wave's strip, in blocks of 32 x 32: what goes through LDS at a time */
@@ -397,10 +397,10 @@ template <int STAGE> __device__ __forceinline__ void product(const Product* __re
     const u32 k_len = (STAGE == GRAM ? m.np : m.mp) * PARTS;   // halves of a row
     const u32 p_limit = m.mp, q_limit = STAGE == APPLY ? m.np : m.mp;
     const f16_t *p_rows = (const f16_t*)(ws + m.p), *q_rows = (const f16_t*)(ws + m.q);
-    // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads of 8 neighbouring rows meet 8
-    // different bank groups, the chunk (l % 8) ^ (l / 8) of its 128 bytes. (A tile that ends beyond the matrix loads its first rows
-    // there: sums that nothing stores.)
-    const u32 lane_off = (lane >> 3) * k_len + (((lane & 7u) ^ (lane >> 3)) << 3);
+    // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads meet different banks, the chunk
+    // (l % 8) ^ (row / 2 % 8) of its 128 bytes: two rows fill the 64 banks, so rows two apart must differ. (A tile that ends beyond the
+    // matrix loads its first rows there: sums that nothing stores.)
+    const u32 lane_row = (lane >> 3) * k_len, lane_off[2] = {lane_row + (((lane & 7u) ^ (lane >> 4)) << 3), lane_row + (((lane & 7u) ^ (4u + (lane >> 4))) << 3)};
     auto fetch = [&](u32 kt, u32 slot) {
         f16_t* base = lds + slot * STAGE_HALVES;
 #pragma unroll
@@ -408,7 +408,7 @@ template <int STAGE> __device__ __forceinline__ void product(const Product* __re
             const u32 row = (wave * LOADS + l) * 8;   // of P's rows, then Q's
             const bool is_p = row < TILE;
             const u32 at = is_p ? t.i * TILE + row : t.j * TILE + row - TILE, limit = is_p ? p_limit : q_limit;
-            const f16_t* src = (is_p ? p_rows : q_rows) + (u64)(at < limit ? at : 0u) * k_len + (u64)kt * ROW + lane_off;
+            const f16_t* src = (is_p ? p_rows : q_rows) + (u64)(at < limit ? at : 0u) * k_len + (u64)kt * ROW + lane_off[l & 1];
             __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * ROW), 16, 0, 0);
         }
     };
@@ -419,7 +419,7 @@ template <int STAGE> __device__ __forceinline__ void product(const Product* __re
         for (int j = 0; j < NB; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-    const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane & 7u;
+    const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane >> 1 & 7u;
     Fragments f[2];
 #pragma unroll
     for (int part = 0; part < PARTS; part++) {
