@@ -562,13 +562,21 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_sums(const elem_t* __
 }
 
 // The chunks of a sample added up: [batch][2][C]. A workgroup takes 32 of a sample's 2 C sums, its 32 rows of threads every 32nd chunk.
+// Bound by the latency of reading what other XCDs wrote: four chunks at a time instead of one take the whole backward pass of 2 x 262144 x 128
+// from 146 to 136 us.
 extern "C" __global__ __launch_bounds__(1024) void group_norm_fold(const float* __restrict__ parts, float* __restrict__ samples) {
     __shared__ float part[32][33];
     const u64 per = (2 * C + 31) / 32, n = blockIdx.x / per, e = blockIdx.x % per * 32 + (threadIdx.x & 31u);
     const u32 row = threadIdx.x >> 5, column = threadIdx.x & 31u;
     float s = 0.0f;
     if (e < 2 * C)
-        for (u64 k = row; k < CHUNKS; k += 32) s += parts[(n * CHUNKS + k) * (2 * C) + e];
+        for (u64 k = row; k < CHUNKS; k += 128) {
+            float of[4];   // (four on their way at a time)
+#pragma unroll
+            for (u32 d = 0; d < 4; d++) of[d] = k + d * 32 < CHUNKS ? parts[(n * CHUNKS + k + d * 32) * (2 * C) + e] : 0.0f;
+#pragma unroll
+            for (u32 d = 0; d < 4; d++) s += of[d];
+        }
     part[row][column] = s;
     __syncthreads();
     // (transposed: a row's threads now hold one sum's 32 shares)
@@ -700,10 +708,11 @@ GroupNormTiling plan_group_norm(const GroupNormProblem& pr, bool backward) {
     t.tx = std::min<int64_t>(cv, t.threads);
     t.ty = t.threads / t.tx;
     t.columns = (int)((cv + t.tx - 1) / t.tx);
-    // 64 registers of data per thread, half or less of that where that leaves compute units idle
+    // 64 registers of data per thread, half or less of that where that leaves compute units idle (forward below 1024 workgroups;
+    // backward, whose parts are many sums that `fold` reads, below 512: 1 x 65536 x 64 bf16 19.3 -> 16.9 us, 8 x 4096 x 320 31.5 -> 30.2)
     int64_t rpt = std::max<int64_t>(1, 64 / (vector_regs(false) * t.columns));
     const int64_t slices = pr.groups / t.slice_groups;
-    while (rpt > 1 && (t.ty * (rpt / 2) >= pr.pixels || (uint64_t)(pr.batch * slices) * ((pr.pixels + t.ty * rpt - 1) / (t.ty * rpt)) < 1024)) rpt /= 2;
+    while (rpt > 1 && (t.ty * (rpt / 2) >= pr.pixels || (uint64_t)(pr.batch * slices) * ((pr.pixels + t.ty * rpt - 1) / (t.ty * rpt)) < (backward ? 512u : 1024u))) rpt /= 2;
     // (forward, a full chip does better with 48 registers of data: 2 x 262144 x 128 bf16 71 -> 68 us, 64 x 3136 x 256 54 -> 52, 32 x 784 x 512
     // f32 28.0 -> 27.4; backward 96 -> 98-103 for 32 or 96 instead of 64)
     if (!backward && rpt * vector_regs(false) * t.columns == 64) rpt = rpt * 3 / 4;
