@@ -19,13 +19,14 @@ constexpr uint32_t kBlock = 64;  // rows and columns of one block of the convers
 // [0, 1.21]: the step's polynomial a s + b s^3 + c s^5 maps [0, 1] there and [1, 1.21] into [0.68, 0.96]. So every entry has a known
 // bound, and fixed powers of two keep f16 operands in range (kScale). A value's f16 rounding has 11 bits; its remainder in a second f16
 // gives 22, and three of the four products of such pairs (the fourth is 2^-22 of the result) run at three times f16's cost, where f32
-// matrix instructions take sixteen times. Measured against 64 bits: errors as of f32 products, 1e-6 to 6e-6.
+// matrix instructions take sixteen times. Measured against 64 bits: errors as of f32 products, 1e-6 to 2.5e-6.
 //
 // Several steps at once. All matrices of an iteration commute, so its steps can be taken on the m x m side: with A = X X^T and
 // Q_k = a I + b A_k + c A_k A_k, A_(k+1) = Q_k A_k Q_k, and X = Q_(r-1) ... Q_0 X after r steps - one product with X on either end
 // instead of two per step, for 3 m x m products (half of them by symmetry) per step between. It costs digits: an error of A, which is
-// relative to the largest singular value, meets the smallest squared. After three steps in two f16 parts the results are still as of f32
-// (2e-6 to 5e-6, singular values over three decades 5e-6; five at once: 1e-4), so steps go in runs of three at most, and one by one
+// relative to the largest singular value, meets the smallest squared. After three steps in two f16 parts errors are up to three times
+// those of f32 products (2e-6 to 7e-6 against 1e-6 to 3e-6; singular values over three decades 6e-6 against 4e-6, a few directions 35 times as strong as
+// the rest 2.0e-5 against 1.1e-5; five at once: 1e-4), so steps go in runs of three at most, and one by one
 // where operands have one part.
 const char* kCommon = R"HIP(
 typedef unsigned short u16;
