@@ -641,7 +641,7 @@ std::string definitions(const GroupNormProblem& pr, const GroupNormTiling& t) {
       << "\n#define CHUNKS " << t.chunks << "\n#define BLOCKS " << t.grid << "ull\n#define LPG "
       << std::min(64, pow2_floor(t.threads / t.slice_groups)) << "\n#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 "
       << (pr.dtype == HE_F16) << "\n#define PARAM_SAME " << (pr.param_dtype == pr.dtype) << "\n#define ACT " << pr.activation
-      << "\n#define EPS " << strfmt("%.9gf", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge << "\n#define MERGERS " << t.mergers()
+      << "\n#define EPS " << strfmt("%.9ef", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge << "\n#define MERGERS " << t.mergers()
       << "\n#define LPE " << std::min<int64_t>(64, pow2_floor(std::max<int64_t>(1, t.threads / (2 * t.slice)))) << "\n";
     return s.str();
 }

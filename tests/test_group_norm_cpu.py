@@ -82,6 +82,23 @@ def test_the_kernels_match_the_oracle(monkeypatch, shape, dtype, activation, par
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
 
 
+@pytest.mark.parametrize("parts", ["0", "1"])
+@pytest.mark.parametrize("epsilon", [0.0, 1.0, 2.0 ** -149])
+def test_every_accepted_epsilon_compiles(monkeypatch, epsilon, parts):
+    """Whole numbers among them, and the smallest value there is."""
+    monkeypatch.setenv("HELIUM_HIP_NORM_PARTS", parts)
+    shape = (2, 37, 32, 4)
+    norm = ha.GroupNorm(*shape, "f32", epsilon=epsilon)
+    host, v, _, _ = inputs(shape, "f32", "f32", "none", seed=12)
+    y, mean, rstd = forward_emulated(norm, shape, host)
+    want, wmean, wrstd = oracle.forward(v["x"], v["gamma"], v["beta"], 4, "none", epsilon)
+    # (sums of 296 values of about 2.5: 1024 roundings of 2^-24 each are more than their error, relative to |mean| + std and to the variance)
+    assert np.abs(mean - wmean).max() < 1024 * 2.0 ** -24 * 10 and np.abs(rstd / wrstd - 1).max() < 2 * 1024 * 2.0 ** -24
+    assert np.abs(y - want).max() < 4 * 1024 * 2.0 ** -24 * np.abs(want).max() * 10
+    dx, dgamma, dbeta = backward_emulated(norm, shape, host, wmean.astype(np.float32), wrstd.astype(np.float32))
+    assert np.isfinite(dx).all() and np.isfinite(dgamma).all() and np.isfinite(dbeta).all()
+
+
 def test_more_blocks_than_a_launch_has_are_refused():
     """2^32 workgroups of the second launch, though the tensor's own launch would have fewer than 2^31."""
     with pytest.raises(ha.HeliumError, match="too large for one launch"):
