@@ -113,8 +113,12 @@ template <int N> __device__ __forceinline__ void fold_rows(float (&a)[NC][N], co
     }
     __syncthreads();
 }
-// The sums of fold_rows() per entry, out[e] for all E entries of a row: LANES neighbouring threads add one up.
+// The sums of fold_rows() per entry, out[e] for all E entries of a row: LANES neighbouring threads add one up. Where there is one row
+// it is the sums already, and `out` is `red`: a pixel of 16384 channels leaves 128 KB of them, and a workgroup has 160 KB of LDS.
+#define ONE_ROW (RED_ROWS == 1)
+#define SUMS_APART (ONE_ROW ? 1 : SC * 2)
 template <int E, int LANES> __device__ __forceinline__ void fold_entries(const float* red, float* out) {
+    if (ONE_ROW) return;
     const u32 l = threadIdx.x % LANES;
     for (u32 e0 = 0; e0 < E; e0 += T / LANES) {
         const u32 e = e0 + threadIdx.x / LANES;
@@ -458,7 +462,8 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_backward(const elem_t
                                                                     const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                     float* __restrict__ samples, elem_t* __restrict__ dx) {
-    __shared__ float red[RED_ROWS * CV * V * 2], sums[SC * 2], group_sums[KG * 2];
+    __shared__ float red[RED_ROWS * CV * V * 2], sums_apart[SUMS_APART], group_sums[KG * 2];
+    float* sums = ONE_ROW ? red : sums_apart;
     const Place p = place();
     vec_t hx[RPT][NC], hd[RPT][NC];
     load_held(x, p, hx);
@@ -532,7 +537,8 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_sums(const elem_t* __
                                                                 const param_t* __restrict__ gamma, const param_t* __restrict__ beta,
                                                                 const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                 float* __restrict__ parts) {
-    __shared__ float red[RED_ROWS * CV * V * 2], sums[SC * 2];
+    __shared__ float red[RED_ROWS * CV * V * 2], sums_apart[SUMS_APART];
+    float* sums = ONE_ROW ? red : sums_apart;
     const Place p = place();
     vec_t hx[RPT][NC], hd[RPT][NC];
     load_held(x, p, hx);
@@ -734,7 +740,7 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
                dtype_name(pr.param_dtype));
     HE_REQUIRE(pr.activation >= HE_ACT_NONE && pr.activation <= HE_ACT_SILU, HE_ERR_INVALID, "group norm: unknown activation %d", pr.activation);
     HE_REQUIRE(std::isfinite(pr.epsilon) && pr.epsilon >= 0, HE_ERR_INVALID, "group norm: epsilon %g", (double)pr.epsilon);
-    // (kernels count channels, and vectors of LDS, in 32 bits)
+    // (a group's channels stay together: two sums of each of 16384 are 128 KB of a workgroup's 160 KB of LDS)
     HE_REQUIRE(pr.channels <= 16384, HE_ERR_UNSUPPORTED, "group norm: %lld channels, at most 16384 are taken", (long long)pr.channels);
     HE_REQUIRE(pr.pixels <= (int64_t)1 << 40 && pr.batch <= (int64_t)1 << 31, HE_ERR_UNSUPPORTED, "group norm: extents too large");
     fwd_ = plan_group_norm(pr, false);

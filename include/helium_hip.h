@@ -461,7 +461,7 @@ int he_pool_release(void* ptr, const he_block* block, uint64_t scope);
 typedef struct he_group_norm_s* he_group_norm_t;
 enum { HE_ACT_NONE = 0, HE_ACT_RELU = 1, HE_ACT_SILU = 2 };
 
-/* x is [batch, pixels, channels] (NHWC), row-major and packed; `groups` divides the channels. Over the pixels * (channels / groups)
+/* x is [batch, pixels, channels] (NHWC), row-major and packed; `groups` divides the channels, at most 16384. Over the pixels * (channels / groups)
  * values of a sample's group: xh = (x - mean) * rstd, rstd = 1 / sqrt(variance + epsilon), z = gamma[c] * xh + beta[c], y = act(z):
  * z, max(z, 0) or z * sigmoid(z). dtype: HE_F32, HE_BF16 or HE_F16, of x, y and their gradients; param_dtype: of gamma and beta,
  * HE_F32 or dtype. Arithmetic and sums are f32, y is rounded once. batch may be 0 (then a call writes nothing, but for the

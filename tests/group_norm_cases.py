@@ -31,6 +31,10 @@ SHAPES = [
     (2, 2049, 24, 6),     # the last of them with one pixel
 ]
 
+# wide groups, that no workgroup holds a pixel of with one vector to a thread
+WIDE = [((1, 10, 10244, 1), "f32"), ((1, 3, 12288, 1), "f16"), ((2, 2, 16384, 1), "bf16"),
+        ((1, 5, 16380, 4), "bf16"), ((1, 2, 16001, 1), "f32")]
+
 
 def to_storage(x, dtype):
     x = np.asarray(x, np.float32)

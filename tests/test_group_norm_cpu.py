@@ -8,7 +8,7 @@ import pytest
 
 import helium_amd as ha
 from cpu_emul import run_kernel
-from group_norm_cases import EPSILON, SHAPES, check_backward, check_forward, inputs, to_f32
+from group_norm_cases import EPSILON, SHAPES, WIDE, check_backward, check_forward, inputs, to_f32
 from helium_amd import _ffi
 from oracle import group_norm as oracle
 
@@ -80,6 +80,17 @@ def test_the_kernels_match_the_oracle(monkeypatch, shape, dtype, activation, par
     check_forward(shape, dtype, activation, v, to_f32(y, dtype), got_mean, got_rstd)
     dx, dgamma, dbeta = backward_emulated(norm, shape, host, mean, rstd)
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
+@pytest.mark.parametrize("shape,dtype", WIDE)
+def test_groups_of_more_channels_than_a_workgroup_has_threads(shape, dtype):
+    """Up to the widest slice there is, also of single elements: sums of every channel, in the 160 KB of a workgroup's LDS."""
+    norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
+    host, v, mean, rstd = inputs(shape, dtype, "f32", "silu", seed=13)
+    y, got_mean, got_rstd = forward_emulated(norm, shape, host)
+    check_forward(shape, dtype, "silu", v, to_f32(y, dtype), got_mean, got_rstd)
+    dx, dgamma, dbeta = backward_emulated(norm, shape, host, mean, rstd)
+    check_backward(shape, dtype, "silu", v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
 
 
 @pytest.mark.parametrize("parts", ["0", "1"])

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import helium_amd as ha
-from group_norm_cases import EPSILON, SHAPES, check_backward, check_forward, inputs, to_f32, to_storage
+from group_norm_cases import EPSILON, SHAPES, WIDE, check_backward, check_forward, inputs, to_f32, to_storage
 from oracle import group_norm as oracle
 
 pytestmark = pytest.mark.gpu
@@ -77,6 +77,16 @@ def test_forward_and_backward_match_the_oracle(gpu, shape, dtype, activation):
     check_forward(shape, dtype, activation, v, to_f32(y, dtype), got_mean, got_rstd)
     dx, dgamma, dbeta = run_backward(norm, shape, host, mean, rstd)
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
+@pytest.mark.parametrize("shape,dtype", WIDE)
+def test_wide_groups_match_the_oracle(gpu, shape, dtype):
+    norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
+    host, v, mean, rstd = inputs(shape, dtype, "f32", "silu", seed=13)
+    y, got_mean, got_rstd = run_forward(norm, shape, host)
+    check_forward(shape, dtype, "silu", v, to_f32(y, dtype), got_mean, got_rstd)
+    dx, dgamma, dbeta = run_backward(norm, shape, host, mean, rstd)
+    check_backward(shape, dtype, "silu", v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
 
 
 @pytest.mark.parametrize("shape", [(2, 49, 32, 8), (1, 20000, 48, 4)])
