@@ -721,7 +721,7 @@ GroupNormTiling plan_group_norm(const GroupNormProblem& pr, bool backward) {
     while (rpt > 1 && (t.ty * (rpt / 2) >= pr.pixels || (uint64_t)(pr.batch * slices) * ((pr.pixels + t.ty * rpt - 1) / (t.ty * rpt)) < (backward ? 512u : 1024u))) rpt /= 2;
     // (forward, a full chip does better with 48 registers of data: 2 x 262144 x 128 bf16 71 -> 68 us, 64 x 3136 x 256 54 -> 52, 32 x 784 x 512
     // f32 28.0 -> 27.4; backward 96 -> 98-103 for 32 or 96 instead of 64)
-    if (!backward && rpt * vector_regs(false) * t.columns == 64) rpt = rpt * 3 / 4;
+    if (!backward && rpt % 4 == 0 && rpt * vector_regs(false) * t.columns == 64) rpt = rpt / 4 * 3;
     t.rows_per_thread = (int)rpt;
     t.chunks = (pr.pixels + t.rows() - 1) / t.rows();
     t.merge = t.chunks > 32;

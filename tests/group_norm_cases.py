@@ -34,6 +34,8 @@ SHAPES = [
 # wide groups, that no workgroup holds a pixel of with one vector to a thread
 WIDE = [((1, 10, 10244, 1), "f32"), ((1, 3, 12288, 1), "f16"), ((2, 2, 16384, 1), "bf16"),
         ((1, 5, 16380, 4), "bf16"), ((1, 2, 16001, 1), "f32")]
+# the widest of them: one vector of each column is all that a thread holds
+WIDEST = [((1, 10, 16384, 1), "f32"), ((4, 64, 15368, 1), "f32"), ((1, 10, 16383, 1), "f32"), ((1, 10, 16129, 1), "bf16")]
 
 
 def to_storage(x, dtype):

@@ -8,7 +8,7 @@ import pytest
 
 import helium_amd as ha
 from cpu_emul import run_kernel
-from group_norm_cases import EPSILON, SHAPES, WIDE, check_backward, check_forward, inputs, to_f32
+from group_norm_cases import EPSILON, SHAPES, WIDE, WIDEST, check_backward, check_forward, inputs, to_f32
 from helium_amd import _ffi
 from oracle import group_norm as oracle
 
@@ -91,6 +91,25 @@ def test_groups_of_more_channels_than_a_workgroup_has_threads(shape, dtype):
     check_forward(shape, dtype, "silu", v, to_f32(y, dtype), got_mean, got_rstd)
     dx, dgamma, dbeta = backward_emulated(norm, shape, host, mean, rstd)
     check_backward(shape, dtype, "silu", v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
+@pytest.mark.parametrize("shape,dtype", WIDEST)
+def test_a_thread_has_at_least_one_pixel(shape, dtype):
+    norm = ha.GroupNorm(*shape, dtype, epsilon=EPSILON)
+    assert all(int(n) >= 1 for n in re.findall(r"rows_per_thread=(\d+)", norm.description)), norm.description
+    if shape[1] > 10:
+        return  # (its 256 blocks take minutes under emulation)
+    host, v, mean, rstd = inputs(shape, dtype, "f32", "none", seed=14)
+    y, got_mean, got_rstd = forward_emulated(norm, shape, host)
+    check_forward(shape, dtype, "none", v, to_f32(y, dtype), got_mean, got_rstd)
+
+
+def test_forward_parts_hold_48_registers_or_all_64():
+    """Three quarters of the rows where they divide, never a half."""
+    rows = lambda *shape: int(re.search(r"rows_per_thread=(\d+)", ha.GroupNorm(*shape, "bf16").description).group(1))  # noqa: E731
+    assert rows(2, 262144, 128, 32) == 12       # 16 vectors of 4 registers
+    assert rows(64, 1000, 16384, 8) == 12       # one column of 2048 channels
+    assert rows(64, 1000, 16384, 1) == 2        # eight columns: two rows, 64 registers
 
 
 @pytest.mark.parametrize("parts", ["0", "1"])

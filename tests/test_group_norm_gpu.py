@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import helium_amd as ha
-from group_norm_cases import EPSILON, SHAPES, WIDE, check_backward, check_forward, inputs, to_f32, to_storage
+from group_norm_cases import EPSILON, SHAPES, WIDE, WIDEST, check_backward, check_forward, inputs, to_f32, to_storage
 from oracle import group_norm as oracle
 
 pytestmark = pytest.mark.gpu
@@ -79,7 +79,7 @@ def test_forward_and_backward_match_the_oracle(gpu, shape, dtype, activation):
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
 
 
-@pytest.mark.parametrize("shape,dtype", WIDE)
+@pytest.mark.parametrize("shape,dtype", WIDE + WIDEST)
 def test_wide_groups_match_the_oracle(gpu, shape, dtype):
     norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
     host, v, mean, rstd = inputs(shape, dtype, "f32", "silu", seed=13)
