@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <future>
+#include <numeric>
 #include <sstream>
 
 namespace he {
@@ -431,16 +432,32 @@ __device__ __forceinline__ void load_minus(Minus& s, const Column& k, const Plac
     }
 }
 
-// The samples' sums [batch][2][C] added up: 64 channels to a workgroup, the samples shared by its waves.
+// The samples' sums [batch][2][C] added up for the parameters, in an order that is fixed and with no chain of more than a few hundred
+// additions. Up to 1024 samples: 64 channels to a workgroup, the samples shared by its waves. More of them are first added up 256 to a row, until
+// 1024 rows or fewer are left (FINAL, FINAL_AT floats behind the samples): a workgroup takes 64 of the 2 C sums of 256 rows.
+extern "C" __global__ __launch_bounds__(256) void group_norm_level(const float* __restrict__ from, float* __restrict__ to, u64 count) {
+    __shared__ float part[4][64];
+    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const u64 columns = (2 * C + 63) / 64, row = blockIdx.x / columns, e = blockIdx.x % columns * 64 + lane;
+    const u64 end = row * 256 + 256 < count ? row * 256 + 256 : count;
+    float s = 0.0f;
+    if (e < 2 * C)
+#pragma unroll 8
+        for (u64 n = row * 256 + wave; n < end; n += 4) s += from[n * (2 * C) + e];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && e < 2 * C) to[row * (2 * C) + e] = s + part[1][lane] + part[2][lane] + part[3][lane];
+}
 template <int WAVES> __device__ __forceinline__ void parameter_gradients(u64 block, const float* __restrict__ samples, float* __restrict__ dgamma, float* __restrict__ dbeta) {
     __shared__ float part[2][WAVES][64];
+    const float* rows = samples + FINAL_AT;
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const u64 c = block * 64 + lane;
     float a = 0.0f, b = 0.0f;
     if (c < C)
-        for (u64 n = wave; n < BATCH; n += WAVES) {
-            a += samples[(n * 2) * C + c];
-            b += samples[(n * 2 + 1) * C + c];
+        for (u64 n = wave; n < FINAL; n += WAVES) {
+            a += rows[(n * 2) * C + c];
+            b += rows[(n * 2 + 1) * C + c];
         }
     part[0][wave][lane] = a;
     part[1][wave][lane] = b;
@@ -637,10 +654,20 @@ int pow2_floor(int64_t x) {
     return p;
 }
 
+// Rows of sums that the parameters' gradients come from: the samples', then fewer and fewer, one behind the other.
+std::vector<uint64_t> sum_levels(const GroupNormProblem& pr) {
+    std::vector<uint64_t> rows{(uint64_t)pr.batch};
+    while (rows.back() > 1024) rows.push_back((rows.back() + 255) / 256);
+    return rows;
+}
+uint64_t all_rows(const std::vector<uint64_t>& levels) { return std::accumulate(levels.begin(), levels.end(), (uint64_t)0); }
+
 std::string definitions(const GroupNormProblem& pr, const GroupNormTiling& t) {
     const int64_t d = pr.channels / pr.groups;
+    const std::vector<uint64_t> levels = sum_levels(pr);
     std::ostringstream s;
-    s << "#define BATCH " << pr.batch << "ull\n#define PIXELS " << pr.pixels << "ull\n#define C " << pr.channels << "\n#define G " << pr.groups
+    s << "#define BATCH " << pr.batch << "ull\n#define FINAL " << levels.back() << "ull\n#define FINAL_AT " << (all_rows(levels) - levels.back()) * 2 * pr.channels
+      << "ull\n#define PIXELS " << pr.pixels << "ull\n#define C " << pr.channels << "\n#define G " << pr.groups
       << "\n#define D " << d << "\n#define V " << t.vec << "\n#define T " << t.threads << "\n#define KG " << t.slice_groups << "\n#define SC "
       << t.slice << "\n#define SLICES " << pr.groups / t.slice_groups << "\n#define CV " << t.slice / t.vec << "\n#define TX " << t.tx
       << "\n#define TY " << t.ty << "\n#define NC " << t.columns << "\n#define RPT " << t.rows_per_thread << "\n#define ROWS " << t.rows()
@@ -749,6 +776,7 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
     HE_REQUIRE(std::max({fwd_.grid, bwd_.grid, fold_grid, merge_grid}) < (1ull << 31) - 16384, HE_ERR_UNSUPPORTED, "group norm: the tensor is too large for one launch");
     const std::string forward = definitions(pr, fwd_) + kCommon + kForward, backward = definitions(pr, bwd_) + kCommon + kBackward;
     auto compiled = std::async(std::launch::async, [&] { (void)rtc_compile(backward, "group_norm", {}); });
+    levels_ = sum_levels(pr);
     auto make = [](const std::string& text, const char* entry) { return std::make_unique<JitKernel>(text, entry); };
     if (fwd_.whole) {
         whole_forward_ = make(forward, "group_norm_forward");
@@ -758,6 +786,7 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
         apply_ = make(forward, "group_norm_apply");
     }
     compiled.get();
+    if (levels_.size() > 1) level_ = make(backward, "group_norm_level");
     if (bwd_.whole) {
         whole_backward_ = make(backward, "group_norm_backward");
         parameters_ = make(backward, "group_norm_parameters");
@@ -766,10 +795,11 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
         fold_ = make(backward, "group_norm_fold");
         gradient_ = make(backward, "group_norm_gradient");
     }
-    const uint64_t rows = (uint64_t)pr.batch * pr.groups, sums = (uint64_t)pr.batch * 2 * pr.channels;
-    scratch_floats_ = std::max(rows * 2 * (fwd_.chunks + 1), sums * (bwd_.chunks + 1));
+    const uint64_t rows = (uint64_t)pr.batch * pr.groups, sums = 2 * (uint64_t)pr.channels;
+    scratch_floats_ = std::max(rows * 2 * (fwd_.chunks + 1), sums * (all_rows(levels_) + pr.batch * bwd_.chunks));
     source_ = forward + "\n" + backward;
-    describe_ = "group_norm forward: " + fwd_.describe() + "\ngroup_norm backward: " + bwd_.describe();
+    describe_ = "group_norm forward: " + fwd_.describe() + "\ngroup_norm backward: " + bwd_.describe() + " samples=";
+    for (size_t k = 0; k < levels_.size(); k++) describe_ += (k ? "," : "") + std::to_string(levels_[k]);
 }
 
 GroupNorm::~GroupNorm() { scratch_.release(); }
@@ -806,6 +836,19 @@ void GroupNorm::forward(const void* x, const void* gamma, const void* beta, void
     apply_->launch(grid, block, 0, stream, c, true);
 }
 
+void GroupNorm::add_levels(float* samples, hipStream_t stream) {
+    const uint64_t sums = 2 * (uint64_t)pr_.channels, columns = (sums + 63) / 64;
+    const uint32_t block[3] = {256, 1, 1};
+    for (size_t k = 1; k < levels_.size(); k++) {
+        uint64_t count = levels_[k - 1];
+        float* to = samples + count * sums;
+        const uint32_t grid[3] = {(uint32_t)(levels_[k] * columns), 1, 1};
+        void* args[] = {&samples, &to, &count};
+        level_->launch(grid, block, 0, stream, args);
+        samples = to;
+    }
+}
+
 void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean, const float* rstd, void* dx,
                          float* dgamma, float* dbeta, hipStream_t stream) {
     HE_REQUIRE(dgamma && dbeta, HE_ERR_INVALID, "group norm: the parameters' gradients are null");
@@ -813,15 +856,16 @@ void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const
         check({dy, x, dx}, {gamma, beta}, {mean, rstd, dgamma, dbeta});
         HE_REQUIRE(mean && rstd, HE_ERR_INVALID, "group norm: the backward pass needs the statistics of the forward pass");
     }
-    const uint64_t sums = (uint64_t)pr_.batch * 2 * pr_.channels;
+    const uint64_t sums = 2 * (uint64_t)pr_.channels;
     std::lock_guard<std::mutex> lk(mu_);
-    float *samples = scratch_.get(scratch_floats_, 0, stream).floats, *parts = samples + sums;
+    float *samples = scratch_.get(scratch_floats_, 0, stream).floats, *parts = samples + sums * all_rows(levels_);
     const uint32_t channel_blocks = (uint32_t)((pr_.channels + 63) / 64), small[3] = {256, 1, 1};
     const uint32_t grid[3] = {(uint32_t)bwd_.grid, 1, 1}, block[3] = {(uint32_t)bwd_.threads, 1, 1};
     if (bwd_.whole) {
         const uint32_t last_grid[3] = {channel_blocks, 1, 1};
         void* a[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &samples, &dx};
         if (pr_.batch) whole_backward_->launch(grid, block, 0, stream, a);
+        add_levels(samples, stream);
         void* b[] = {&samples, &dgamma, &dbeta};
         parameters_->launch(last_grid, small, 0, stream, b, true);
         return;
@@ -832,6 +876,7 @@ void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const
         sums_->launch(grid, block, 0, stream, a);
         void* b[] = {&parts, &samples};
         fold_->launch(fold_grid, fold_block, 0, stream, b);
+        add_levels(samples, stream);
     }
     // (without samples only the parameters' gradients are left, all zero)
     const uint32_t last_grid[3] = {(uint32_t)bwd_.grid + channel_blocks, 1, 1};

@@ -55,10 +55,12 @@ public:
 
 private:
     void check(std::initializer_list<const void*> tensors, std::initializer_list<const void*> params, std::initializer_list<const void*> stats) const;
+    void add_levels(float* samples, hipStream_t stream);
     GroupNormProblem pr_;
+    std::vector<uint64_t> levels_;
     GroupNormTiling fwd_, bwd_;
     std::string source_, describe_;
-    std::unique_ptr<JitKernel> whole_forward_, stats_, merge_, apply_, whole_backward_, parameters_, sums_, fold_, gradient_;
+    std::unique_ptr<JitKernel> whole_forward_, stats_, merge_, apply_, whole_backward_, parameters_, sums_, fold_, level_, gradient_;
     std::mutex mu_;  // a call's launches follow each other on their stream: they share the stream's scratch
     uint64_t scratch_floats_ = 0;
     ReduceScratch scratch_;

@@ -112,6 +112,32 @@ def test_forward_parts_hold_48_registers_or_all_64():
     assert rows(64, 1000, 16384, 1) == 2        # eight columns: two rows, 64 registers
 
 
+LEVEL = """
+extern "C" void emu_level(const float* from, float* to, const u64* count) { group_norm_level(from, to, *count); }
+"""
+
+
+@pytest.mark.parametrize("batch,channels,levels", [(1024, 5, [1024]), (1025, 40, [1025, 5]), (300000, 3, [300000, 1172, 5])])
+def test_sums_over_many_samples_are_no_long_chains(batch, channels, levels):
+    """Every sum a tenth: added up one after the other in f32 each rounding leans to the same side, and 75000 of them lose four digits."""
+    norm = ha.GroupNorm(batch, 1, channels, 1, "f32")
+    text = launch(norm, True)[3]
+    assert [int(n) for n in norm.description.split("samples=")[1].split(",")] == levels
+    sums = np.full((batch, 2, channels), 0.1, np.float32) * np.array([[1], [-2]], np.float32)
+    rows = [sums]
+    for count in levels[1:]:
+        rows += run_kernel(text + LEVEL, "emu_level", count * ((2 * channels + 63) // 64), 256,
+                           [(rows[-1], 0), (np.empty((count, 2, channels), np.float32), 1), (np.array([len(rows[-1])], np.uint64), 0)])
+    together = np.concatenate([r.reshape(-1) for r in rows])
+    text += """
+extern "C" void emu_parameters(const float* samples, float* dgamma, float* dbeta) { parameter_gradients<4>(blockIdx.x, samples, dgamma, dbeta); }
+"""
+    dgamma, dbeta = run_kernel(text, "emu_parameters", (channels + 63) // 64, 256, [(together, 0)] + [(np.empty(channels, np.float32), 1)] * 2)
+    # chains of at most 256 + 64 + 64 additions and the few that join them, each off by 2^-24 of the sum
+    for got, each in ((dbeta, np.float32(0.1)), (dgamma, np.float32(-0.2))):
+        assert np.abs(got / (batch * np.float64(each)) - 1).max() < 400 * 2.0 ** -24, got
+
+
 @pytest.mark.parametrize("parts", ["0", "1"])
 @pytest.mark.parametrize("epsilon", [0.0, 1.0, 2.0 ** -149])
 def test_every_accepted_epsilon_compiles(monkeypatch, epsilon, parts):

@@ -79,6 +79,18 @@ def test_forward_and_backward_match_the_oracle(gpu, shape, dtype, activation):
     check_backward(shape, dtype, activation, v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
 
 
+@pytest.mark.parametrize("parts", ["0", "1"])
+@pytest.mark.parametrize("shape,dtype", [((5000, 1, 64, 8), "bf16"), ((1025, 3, 40, 5), "f16"), ((300000, 1, 8, 2), "f32")])
+def test_many_samples_of_few_pixels_match_the_oracle(gpu, monkeypatch, shape, dtype, parts):
+    monkeypatch.setenv("HELIUM_HIP_NORM_PARTS", parts)
+    norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
+    host, v, mean, rstd = inputs(shape, dtype, "f32", "silu", seed=15)
+    y, got_mean, got_rstd = run_forward(norm, shape, host)
+    check_forward(shape, dtype, "silu", v, to_f32(y, dtype), got_mean, got_rstd)
+    dx, dgamma, dbeta = run_backward(norm, shape, host, mean, rstd)
+    check_backward(shape, dtype, "silu", v, mean, rstd, to_f32(dx, dtype), dgamma, dbeta)
+
+
 @pytest.mark.parametrize("shape,dtype", WIDE + WIDEST)
 def test_wide_groups_match_the_oracle(gpu, shape, dtype):
     norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
