@@ -317,16 +317,19 @@ __device__ __forceinline__ float over_mergers(float s, float* waves) {
 extern "C" __global__ __launch_bounds__(MERGERS) void group_norm_merge(const float* __restrict__ parts, float* __restrict__ stats,
                                                                       float* __restrict__ mean_out, float* __restrict__ rstd_out) {
     __shared__ float waves[2][MERGERS / 64];
-    const u64 of = blockIdx.x;
-    const float* from = parts + of * CHUNKS * 2;
-    const float mean = over_mergers(share_of_mean(from, threadIdx.x, MERGERS), waves[0]);
-    const float m2 = over_mergers(share_of_m2(from, threadIdx.x, MERGERS, mean), waves[1]);
-    if (threadIdx.x == 0) {
-        const float rstd = rstd_from(m2);
-        stats[of * 2] = mean;
-        stats[of * 2 + 1] = rstd;
-        if (mean_out) mean_out[of] = mean;
-        if (rstd_out) rstd_out[of] = rstd;
+    for (u64 of = blockIdx.x; of < BATCH * G; of += MERGE_BLOCKS) {
+        const float* from = parts + of * CHUNKS * 2;
+        const float mean = over_mergers(share_of_mean(from, threadIdx.x, MERGERS), waves[0]);
+        const float m2 = over_mergers(share_of_m2(from, threadIdx.x, MERGERS, mean), waves[1]);
+        if (threadIdx.x == 0) {
+            const float rstd = rstd_from(m2);
+            stats[of * 2] = mean;
+            stats[of * 2 + 1] = rstd;
+            if (mean_out) mean_out[of] = mean;
+            if (rstd_out) rstd_out[of] = rstd;
+        }
+        // (the next group's sums take the places of this one's)
+        if (BATCH * G > MERGE_BLOCKS) __syncthreads();
     }
 }
 #endif
@@ -584,29 +587,33 @@ extern "C" __global__ __launch_bounds__(T) void group_norm_sums(const elem_t* __
     for (u32 e = threadIdx.x; e < SC * 2; e += T) parts[((p.n * CHUNKS + p.chunk) * 2 + (e & 1)) * C + p.slice * SC + (e >> 1)] = sums[e];
 }
 
-// The chunks of a sample added up: [batch][2][C]. A workgroup takes 32 of a sample's 2 C sums, its 32 rows of threads every 32nd chunk.
+// The chunks of a sample added up (one chunk is its sample's sums already, and none is launched): [batch][2][C]. A workgroup takes 32 of a sample's 2 C sums, its 32 rows of threads every 32nd chunk.
 // Bound by the latency of reading what other XCDs wrote: four chunks at a time instead of one take the whole backward pass of 2 x 262144 x 128
 // from 146 to 136 us.
 extern "C" __global__ __launch_bounds__(1024) void group_norm_fold(const float* __restrict__ parts, float* __restrict__ samples) {
     __shared__ float part[32][33];
-    const u64 per = (2 * C + 31) / 32, n = blockIdx.x / per, e = blockIdx.x % per * 32 + (threadIdx.x & 31u);
+    const u64 per = (2 * C + 31) / 32;
     const u32 row = threadIdx.x >> 5, column = threadIdx.x & 31u;
-    float s = 0.0f;
-    if (e < 2 * C)
-        for (u64 k = row; k < CHUNKS; k += 128) {
-            float of[4];   // (four on their way at a time)
+    for (u64 b = blockIdx.x; b < BATCH * per; b += FOLD_BLOCKS) {
+        const u64 n = b / per, e = b % per * 32 + column;
+        float s = 0.0f;
+        if (e < 2 * C)
+            for (u64 k = row; k < CHUNKS; k += 128) {
+                float of[4];   // (four on their way at a time)
 #pragma unroll
-            for (u32 d = 0; d < 4; d++) of[d] = k + d * 32 < CHUNKS ? parts[(n * CHUNKS + k + d * 32) * (2 * C) + e] : 0.0f;
+                for (u32 d = 0; d < 4; d++) of[d] = k + d * 32 < CHUNKS ? parts[(n * CHUNKS + k + d * 32) * (2 * C) + e] : 0.0f;
 #pragma unroll
-            for (u32 d = 0; d < 4; d++) s += of[d];
-        }
-    part[row][column] = s;
-    __syncthreads();
-    // (transposed: a row's threads now hold one sum's 32 shares)
-    s = part[column][row];
-    for (int m = 16; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
-    const u64 mine = blockIdx.x % per * 32 + row;
-    if (column == 0 && mine < 2 * C) samples[n * (2 * C) + mine] = s;
+                for (u32 d = 0; d < 4; d++) s += of[d];
+            }
+        part[row][column] = s;
+        __syncthreads();
+        // (transposed: a row's threads now hold one sum's 32 shares)
+        s = part[column][row];
+        for (int m = 16; m > 0; m /= 2) s += __shfl_xor(s, m, 64);
+        const u64 mine = b % per * 32 + row;
+        if (column == 0 && mine < 2 * C) samples[n * (2 * C) + mine] = s;
+        if (BATCH * per > FOLD_BLOCKS) __syncthreads();
+    }
 }
 
 // The workgroups behind the tensor's own add up the samples' sums.
@@ -654,6 +661,12 @@ int pow2_floor(int64_t x) {
     return p;
 }
 
+// A launch has fewer than 2^32 threads. The tensor's own launches are refused beyond that; of the small ones between them, whose workgroups
+// of up to 1024 threads come to it sooner, a workgroup then does the work of several.
+constexpr uint64_t kThreads = 1ull << 32;
+uint32_t fold_blocks(const GroupNormProblem& pr) { return (uint32_t)std::min<uint64_t>((uint64_t)pr.batch * ((2 * pr.channels + 31) / 32), (kThreads - 1) / 1024); }
+uint32_t merge_blocks(const GroupNormProblem& pr, const GroupNormTiling& t) { return (uint32_t)std::min<uint64_t>((uint64_t)pr.batch * pr.groups, (kThreads - 1) / t.mergers()); }
+
 // Rows of sums that the parameters' gradients come from: the samples', then fewer and fewer, one behind the other.
 std::vector<uint64_t> sum_levels(const GroupNormProblem& pr) {
     std::vector<uint64_t> rows{(uint64_t)pr.batch};
@@ -675,6 +688,7 @@ std::string definitions(const GroupNormProblem& pr, const GroupNormTiling& t) {
       << std::min(64, pow2_floor(t.threads / t.slice_groups)) << "\n#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 "
       << (pr.dtype == HE_F16) << "\n#define PARAM_SAME " << (pr.param_dtype == pr.dtype) << "\n#define ACT " << pr.activation
       << "\n#define EPS " << strfmt("%.9ef", (double)pr.epsilon) << "\n#define WHOLE " << (int)t.whole << "\n#define STREAM " << (int)t.stream << "\n#define MERGE " << (int)t.merge << "\n#define MERGERS " << t.mergers()
+      << "\n#define MERGE_BLOCKS " << merge_blocks(pr, t) << "ull\n#define FOLD_BLOCKS " << fold_blocks(pr) << "ull"
       << "\n#define LPE " << std::min<int64_t>(64, pow2_floor(std::max<int64_t>(1, t.threads / (2 * t.slice)))) << "\n";
     return s.str();
 }
@@ -769,14 +783,16 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
     HE_REQUIRE(std::isfinite(pr.epsilon) && pr.epsilon >= 0, HE_ERR_INVALID, "group norm: epsilon %g", (double)pr.epsilon);
     // (a group's channels stay together: two sums of each of 16384 are 128 KB of a workgroup's 160 KB of LDS)
     HE_REQUIRE(pr.channels <= 16384, HE_ERR_UNSUPPORTED, "group norm: %lld channels, at most 16384 are taken", (long long)pr.channels);
-    HE_REQUIRE(pr.pixels <= (int64_t)1 << 40 && pr.batch <= (int64_t)1 << 31, HE_ERR_UNSUPPORTED, "group norm: extents too large");
+    // (2^46 elements are beyond any memory, and leave products of counts their 64 bits)
+    HE_REQUIRE((double)pr.batch * (double)pr.pixels * (double)pr.channels <= (double)(1ull << 46), HE_ERR_UNSUPPORTED, "group norm: extents too large");
     fwd_ = plan_group_norm(pr, false);
     bwd_ = plan_group_norm(pr, true);
-    const uint64_t fold_grid = (uint64_t)pr.batch * ((2 * pr.channels + 31) / 32), merge_grid = fwd_.merge ? (uint64_t)pr.batch * pr.groups : 0;
-    HE_REQUIRE(std::max({fwd_.grid, bwd_.grid, fold_grid, merge_grid}) < (1ull << 31) - 16384, HE_ERR_UNSUPPORTED, "group norm: the tensor is too large for one launch");
+    levels_ = sum_levels(pr);
+    const uint64_t channel_blocks = (pr.channels + 63) / 64, level_blocks = levels_.size() > 1 ? levels_[1] * ((2 * pr.channels + 63) / 64) : 0;
+    HE_REQUIRE(fwd_.grid < kThreads / fwd_.threads && bwd_.grid + channel_blocks < kThreads / bwd_.threads && level_blocks < kThreads / 256, HE_ERR_UNSUPPORTED,
+               "group norm: the tensor is too large for one launch");
     const std::string forward = definitions(pr, fwd_) + kCommon + kForward, backward = definitions(pr, bwd_) + kCommon + kBackward;
     auto compiled = std::async(std::launch::async, [&] { (void)rtc_compile(backward, "group_norm", {}); });
-    levels_ = sum_levels(pr);
     auto make = [](const std::string& text, const char* entry) { return std::make_unique<JitKernel>(text, entry); };
     if (fwd_.whole) {
         whole_forward_ = make(forward, "group_norm_forward");
@@ -792,7 +808,7 @@ GroupNorm::GroupNorm(const GroupNormProblem& pr) : pr_(pr) {
         parameters_ = make(backward, "group_norm_parameters");
     } else {
         sums_ = make(backward, "group_norm_sums");
-        fold_ = make(backward, "group_norm_fold");
+        if (bwd_.chunks > 1) fold_ = make(backward, "group_norm_fold");
         gradient_ = make(backward, "group_norm_gradient");
     }
     const uint64_t rows = (uint64_t)pr.batch * pr.groups, sums = 2 * (uint64_t)pr.channels;
@@ -827,7 +843,7 @@ void GroupNorm::forward(const void* x, const void* gamma, const void* beta, void
     std::lock_guard<std::mutex> lk(mu_);
     float* parts = scratch_.get(scratch_floats_, 0, stream).floats;
     float* stats = parts + rows * fwd_.chunks * 2;
-    const uint32_t merge_grid[3] = {(uint32_t)rows, 1, 1}, merge_block[3] = {(uint32_t)fwd_.mergers(), 1, 1};
+    const uint32_t merge_grid[3] = {merge_blocks(pr_, fwd_), 1, 1}, merge_block[3] = {(uint32_t)fwd_.mergers(), 1, 1};
     void* a[] = {&x, &parts};
     stats_->launch(grid, block, 0, stream, a);
     void* b[] = {&parts, &stats, &mean, &rstd};
@@ -858,7 +874,7 @@ void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const
     }
     const uint64_t sums = 2 * (uint64_t)pr_.channels;
     std::lock_guard<std::mutex> lk(mu_);
-    float *samples = scratch_.get(scratch_floats_, 0, stream).floats, *parts = samples + sums * all_rows(levels_);
+    float *samples = scratch_.get(scratch_floats_, 0, stream).floats, *parts = fold_ ? samples + sums * all_rows(levels_) : samples;
     const uint32_t channel_blocks = (uint32_t)((pr_.channels + 63) / 64), small[3] = {256, 1, 1};
     const uint32_t grid[3] = {(uint32_t)bwd_.grid, 1, 1}, block[3] = {(uint32_t)bwd_.threads, 1, 1};
     if (bwd_.whole) {
@@ -871,11 +887,11 @@ void GroupNorm::backward(const void* dy, const void* x, const void* gamma, const
         return;
     }
     if (pr_.batch) {
-        const uint32_t fold_grid[3] = {(uint32_t)(pr_.batch * ((2 * pr_.channels + 31) / 32)), 1, 1}, fold_block[3] = {1024, 1, 1};
+        const uint32_t fold_grid[3] = {fold_blocks(pr_), 1, 1}, fold_block[3] = {1024, 1, 1};
         void* a[] = {&dy, &x, &gamma, &beta, &mean, &rstd, &parts};
         sums_->launch(grid, block, 0, stream, a);
         void* b[] = {&parts, &samples};
-        fold_->launch(fold_grid, fold_block, 0, stream, b);
+        if (fold_) fold_->launch(fold_grid, fold_block, 0, stream, b);
         add_levels(samples, stream);
     }
     // (without samples only the parameters' gradients are left, all zero)

@@ -155,6 +155,54 @@ def test_every_accepted_epsilon_compiles(monkeypatch, epsilon, parts):
     assert np.isfinite(dx).all() and np.isfinite(dgamma).all() and np.isfinite(dbeta).all()
 
 
+def launches(norm):
+    """Workgroups and threads of every launch but the levels'."""
+    forward, backward = ({k: int(v) for k, v in re.findall(r"#define (MERGE_BLOCKS|MERGERS|FOLD_BLOCKS|BLOCKS|T) (\d+)", "#define BATCH" + t)}
+                         for t in norm.source.split("#define BATCH")[1:])
+    return [(forward["BLOCKS"], forward["T"]), (backward["BLOCKS"] + (norm.channels + 63) // 64, backward["T"]),
+            (forward["MERGE_BLOCKS"], forward["MERGERS"]), (backward["FOLD_BLOCKS"], 1024)]
+
+
+@pytest.mark.parametrize("shape,dtype", [((1 << 20, 1, 64, 1), "bf16"), ((1 << 22, 1, 2, 1), "f32"), ((1 << 14, 6400, 256, 256), "f32"), ((1 << 10, 1 << 10, 16384, 1), "f32")])
+def test_every_launch_has_fewer_threads_than_two_to_the_32(shape, dtype):
+    """Where the small launches between the tensor's own would have 2^32 and more: a thread block of 1024 to 32 sums, or to a group."""
+    norm = ha.GroupNorm(*shape, dtype)
+    for blocks, threads in launches(norm):
+        assert blocks * threads < 1 << 32, norm.description
+
+
+def test_tensors_of_more_blocks_than_a_launch_has_are_refused_at_creation():
+    assert launches(ha.GroupNorm((1 << 24) - 2, 1, 64, 1, "bf16"))[1] == ((1 << 24) - 1, 256)   # (with the workgroup of the parameters)
+    for batch in ((1 << 24) - 1, 1 << 24):
+        with pytest.raises(ha.HeliumError, match="too large for one launch"):
+            ha.GroupNorm(batch, 1, 64, 1, "bf16")
+    for extents in ((1 << 62, 1 << 2), (1 << 31, 1 << 40), (1, 1 << 62)):   # (whose products wrap)
+        with pytest.raises(ha.HeliumError, match="extents too large"):
+            ha.GroupNorm(*extents, 64, 1, "bf16")
+
+
+def test_few_workgroups_merge_and_fold_as_many_do(monkeypatch):
+    """The launches whose workgroups may have to take several groups or sums in turn, made to."""
+    shape = (3, 9000, 40, 4)
+    norm = ha.GroupNorm(*shape, "f32")
+    host, v, mean, rstd = inputs(shape, "f32", "f32", "none", seed=16)
+    n, p, c, groups = shape
+    grid, threads, chunks, text = launch(norm, False)
+    assert chunks > 32
+    mergers = int(re.search(r"#define MERGERS (\d+)", text).group(1))
+    parts, = run_kernel(text, "group_norm_stats", grid, threads, [(host["x"], 0), (np.empty((n, groups, chunks, 2), np.float32), 1)])
+    stat = np.empty((n, groups), np.float32)
+    merged = [run_kernel(re.sub(r"#define MERGE_BLOCKS \d+", f"#define MERGE_BLOCKS {blocks}", text), "group_norm_merge", blocks, mergers,
+                         [(parts, 0), (np.empty((n, groups, 2), np.float32), 1), (stat, 1), (stat, 1)]) for blocks in (n * groups, 5)]
+    assert all(np.array_equal(a, b) for a, b in zip(*merged)) and np.allclose(merged[0][1], mean, atol=1e-4)
+    chunks, text = launch(norm, True)[2:]
+    sums = np.random.default_rng(17).standard_normal((n, chunks, 2, c)).astype(np.float32)
+    folded = [run_kernel(re.sub(r"#define FOLD_BLOCKS \d+", f"#define FOLD_BLOCKS {blocks}", text), "group_norm_fold", blocks, 1024,
+                         [(sums, 0), (np.empty((n, 2, c), np.float32), 1)])[0] for blocks in (n * 3, 2)]
+    # (chains of chunks / 32 and five more additions)
+    assert np.array_equal(*folded) and (np.abs(folded[0] - sums.astype(np.float64).sum(axis=1)) <= (chunks / 32 + 6) * 2.0 ** -24 * np.abs(sums).sum(axis=1)).all()
+
+
 def test_more_blocks_than_a_launch_has_are_refused():
     """2^32 workgroups of the second launch, though the tensor's own launch would have fewer than 2^31."""
     with pytest.raises(ha.HeliumError, match="too large for one launch"):

@@ -80,7 +80,7 @@ def test_forward_and_backward_match_the_oracle(gpu, shape, dtype, activation):
 
 
 @pytest.mark.parametrize("parts", ["0", "1"])
-@pytest.mark.parametrize("shape,dtype", [((5000, 1, 64, 8), "bf16"), ((1025, 3, 40, 5), "f16"), ((300000, 1, 8, 2), "f32")])
+@pytest.mark.parametrize("shape,dtype", [((5000, 1, 64, 8), "bf16"), ((1025, 3, 40, 5), "f16"), ((300000, 1, 8, 2), "f32"), ((1 << 22, 1, 2, 1), "f32")])
 def test_many_samples_of_few_pixels_match_the_oracle(gpu, monkeypatch, shape, dtype, parts):
     monkeypatch.setenv("HELIUM_HIP_NORM_PARTS", parts)
     norm = ha.GroupNorm(*shape, dtype, activation="silu", epsilon=EPSILON)
