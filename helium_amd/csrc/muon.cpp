@@ -5,7 +5,6 @@
 #include <cstring>
 #include <functional>
 #include <future>
-#include <queue>
 #include <sstream>
 
 namespace he {
@@ -14,6 +13,8 @@ namespace {
 
 constexpr int kGroup = 32;       // matrices whose operands one launch takes by value
 constexpr uint32_t kBlock = 64;  // rows and columns of one block of the conversions
+// A launch has fewer than 2^32 threads. So a group has fewer than 2^24 blocks: 2^36 values, whose workspace would be more than 500 GB.
+constexpr uint64_t kThreads = 1ull << 32, kMostBlocks = kThreads / 256 - 1;
 
 // Newton-Schulz iteration on f16 matrix cores. With X scaled to a Frobenius norm of at most 1, no singular value ever leaves
 // [0, 1.21]: the step's polynomial a s + b s^3 + c s^5 maps [0, 1] there and [1, 1.21] into [0.68, 0.96]. So every entry has a known
@@ -622,6 +623,7 @@ struct TileShape {
     uint32_t tile, waves_m, waves_n, stages, per_cu;
     const char* attrs;
     double base, alone[2], full[2];
+    uint32_t threads() const { return waves_m * waves_n * 64; }
 };
 const TileShape kTiles[] = {
     {64, 2, 2, 4, 2, "", 2.5, {0.22, 0.28}, {0.42, 0.50}},
@@ -633,44 +635,79 @@ constexpr uint32_t kCUs = 256;
 
 // How one product of every matrix is cut into tasks: tiles, and where there are too few of them to fill the chip or their sums are
 // long, shares of `target` k-tiles or a little more of each sum, which a second launch adds up.
+struct Tiles {
+    uint32_t ti, tj, kt, shares;  // tile rows and columns, k-tiles of a sum and how many tasks share it
+    Tiles(const MuonMatrix& m, uint32_t tile, bool lower, bool along_n, int parts, uint32_t target) {
+        ti = (m.mp + tile - 1) / tile, tj = lower ? ti : (m.np + tile - 1) / tile;
+        kt = (along_n ? m.np : m.mp) / (64 / parts), shares = std::max(1u, kt / target);
+    }
+};
+// What a cut comes to, from counts alone: a large group has candidates of a thousand million tasks.
+struct CutSize {
+    uint64_t tasks = 0, parked = 0;  // parked: shares that wait in memory
+    double estimate = 0;             // microseconds
+};
+CutSize size_cut(const std::vector<MuonMatrix>& mats, const TileShape& shape, bool lower, bool along_n, int parts, uint32_t target) {
+    CutSize size;
+    std::map<uint32_t, uint64_t, std::greater<uint32_t>> lengths;  // how many tasks have so many k-tiles, the longest first
+    for (const MuonMatrix& m : mats) {
+        const Tiles t(m, shape.tile, lower, along_n, parts, target);
+        const uint64_t tiles = lower ? (uint64_t)t.ti * (t.ti + 1) / 2 : (uint64_t)t.ti * t.tj, longer = t.kt % t.shares;
+        size.tasks += tiles * t.shares;
+        if (t.shares > 1) size.parked += tiles * t.shares;
+        if (longer) lengths[t.kt / t.shares + 1] += tiles * longer;
+        lengths[t.kt / t.shares] += tiles * (t.shares - longer);
+    }
+    // Every task goes to the workgroup place that is free first; a k-tile takes the longer the fuller the chip is. `free_at`: how many
+    // places are free from when on. Places that become free within one task's time of each other take turns, a task each.
+    const uint64_t slots = (uint64_t)kCUs * shape.per_cu;
+    const double f = std::min(1.0, (double)size.tasks / slots), each = shape.alone[parts - 1] + (shape.full[parts - 1] - shape.alone[parts - 1]) * f * f;
+    std::map<double, uint64_t> free_at{{0.0, slots}};
+    for (auto [length, count] : lengths) {
+        const double time = shape.base + each * length;
+        while (count) {
+            const auto first = free_at.begin();
+            if (count >= slots && free_at.rbegin()->first - first->first <= time) {
+                const uint64_t rounds = count / slots;
+                std::map<double, uint64_t> later;
+                for (auto& [at, places] : free_at) later[at + rounds * time] += places;
+                free_at = std::move(later);
+                count -= rounds * slots;
+                continue;
+            }
+            const uint64_t taken = std::min(count, first->second);
+            free_at[first->first + time] += taken;
+            if (taken == first->second) free_at.erase(first);
+            else first->second -= taken;
+            count -= taken;
+        }
+    }
+    size.estimate = free_at.rbegin()->first;
+    // (a launch, and the shares read at about 5 TB/s)
+    if (size.parked) size.estimate += 2.5 + 4.0 * size.parked * shape.tile * shape.tile / 5e6;
+    return size;
+}
 struct Cut {
     std::vector<MuonTask> tasks, joins;  // joins: a task of each tile that is shared
-    uint32_t parked = 0;                 // shares that wait in memory
-    double estimate = 0;                 // microseconds
 };
 Cut cut_product(const std::vector<MuonMatrix>& mats, const TileShape& shape, bool lower, bool along_n, int parts, uint32_t target) {
     Cut cut;
-    const uint32_t tile = shape.tile, bk = 64 / parts;
-    auto over = [&](uint32_t extent) { return (extent + tile - 1) / tile; };
+    uint32_t parked = 0;
     for (size_t k = 0; k < mats.size(); k++) {
-        const MuonMatrix& m = mats[k];
-        const uint32_t ti = over(m.mp), tj = lower ? ti : over(m.np), kt = (along_n ? m.np : m.mp) / bk, shares = std::max(1u, kt / target);
-        for (uint32_t g = 0; g < ti; g += 4)  // bands of four tile rows, column by column
-            for (uint32_t j = 0; j < tj; j++)
-                for (uint32_t i = g; i < std::min(g + 4, ti); i++) {
+        const Tiles t(mats[k], shape.tile, lower, along_n, parts, target);
+        for (uint32_t g = 0; g < t.ti; g += 4)  // bands of four tile rows, column by column
+            for (uint32_t j = 0; j < t.tj; j++)
+                for (uint32_t i = g; i < std::min(g + 4, t.ti); i++) {
                     if (lower && j > i) continue;
-                    for (uint32_t s = 0; s < shares; s++)
-                        cut.tasks.push_back({(uint32_t)k, i, j, (uint32_t)((uint64_t)kt * s / shares), (uint32_t)((uint64_t)kt * (s + 1) / shares), cut.parked, s, shares});
-                    if (shares > 1) {
+                    for (uint32_t s = 0; s < t.shares; s++)
+                        cut.tasks.push_back({(uint32_t)k, i, j, (uint32_t)((uint64_t)t.kt * s / t.shares), (uint32_t)((uint64_t)t.kt * (s + 1) / t.shares), parked, s, t.shares});
+                    if (t.shares > 1) {
                         cut.joins.push_back(cut.tasks.back());
-                        cut.parked += shares;
+                        parked += t.shares;
                     }
                 }
     }
     deal(cut.tasks);
-    // Every task goes to the workgroup place that is free first; a k-tile takes the longer the fuller the chip is.
-    const size_t slots = (size_t)kCUs * shape.per_cu;
-    const double f = std::min(1.0, (double)cut.tasks.size() / slots), each = shape.alone[parts - 1] + (shape.full[parts - 1] - shape.alone[parts - 1]) * f * f;
-    std::priority_queue<double, std::vector<double>, std::greater<double>> free_at;
-    for (const MuonTask& t : cut.tasks) {
-        const double begin = free_at.size() < slots ? 0.0 : free_at.top();
-        if (free_at.size() == slots) free_at.pop();
-        const double end = begin + shape.base + each * (t.k_end - t.k_begin);
-        free_at.push(end);
-        cut.estimate = std::max(cut.estimate, end);
-    }
-    // (a launch, and the shares read at about 5 TB/s)
-    if (cut.parked) cut.estimate += 2.5 + 4.0 * cut.parked * tile * tile / 5e6;
     return cut;
 }
 template <class T> std::vector<char> bytes_of(const std::vector<T>& v) {
@@ -719,12 +756,12 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         parts += m.parts;
         part_begin_.push_back((uint32_t)portions.size());
         block_begin_.push_back((uint32_t)blocks.size());
+        HE_REQUIRE(blocks.size() + (uint64_t)(m.mp / kBlock) * (m.np / kBlock) <= kMostBlocks, HE_ERR_UNSUPPORTED, "muon: too many elements for one group");
         for (uint32_t p = 0; p < m.parts; p++) portions.push_back({(uint32_t)k, p, 0});
         const uint32_t br = (m.tall ? m.np : m.mp) / kBlock, bc = (m.tall ? m.mp : m.np) / kBlock;
         for (uint32_t i = 0; i < br; i++)
             for (uint32_t j = 0; j < bc; j++) blocks.push_back({(uint32_t)k, i, j});
         matrices_.push_back(m);
-        HE_REQUIRE(blocks.size() < (1u << 30) && portions.size() < (1u << 30), HE_ERR_UNSUPPORTED, "muon: too many elements for one group");
     }
     part_begin_.push_back((uint32_t)portions.size());
     block_begin_.push_back((uint32_t)blocks.size());
@@ -736,30 +773,34 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         ProductKind& product = products_[p];
         const int forced = tuning::get_int("HELIUM_HIP_MUON_TILE", -1), only = forced >= 0 ? forced : tuning::get_int((std::string("HELIUM_HIP_MUON_TILE_") + names[p]).c_str(), -1);
         const TileShape* chosen = nullptr;
-        Cut cut;
+        CutSize size;
+        uint32_t chosen_target = 0;
         for (const TileShape& candidate : kTiles)
             for (uint32_t target : {1u << 30, 64u, 32u, 16u, 8u, 4u}) {
                 if (only >= 0 && candidate.tile != (uint32_t)only) continue;
-                Cut c = cut_product(matrices_, candidate, p < 2, p == 0, pr.split ? 2 : 1, target);
-                if (c.tasks.size() >= (1u << 28) || (uint64_t)c.parked * candidate.tile * candidate.tile >= (1u << 30) || (chosen && c.estimate >= cut.estimate)) continue;
-                cut = std::move(c);
+                const CutSize c = size_cut(matrices_, candidate, p < 2, p == 0, pr.split ? 2 : 1, target);
+                // (4 GB of shares are the most that is made; tiles of 64 that nobody shares are no more than the blocks, so one candidate is always left)
+                if (c.tasks * candidate.threads() >= kThreads || c.parked * candidate.tile * candidate.tile >= (1u << 30) || (chosen && c.estimate >= size.estimate)) continue;
+                size = c;
                 chosen = &candidate;
+                chosen_target = target;
             }
-        HE_REQUIRE(chosen, HE_ERR_UNSUPPORTED, "muon: the group is too large for one launch");
+        HE_REQUIRE(chosen, HE_ERR_INVALID, "muon: there are no tiles of %d", only);
         const TileShape& shape = *chosen;
+        const Cut cut = cut_product(matrices_, shape, p < 2, p == 0, pr.split ? 2 : 1, chosen_target);
         const std::vector<MuonTask>&tasks = cut.tasks, &joins = cut.joins;
-        const uint32_t parked = cut.parked;
+        const uint32_t parked = (uint32_t)size.parked;
         tables_[1 + p] = bytes_of(tasks), tables_[4 + p] = bytes_of(joins);
-        product.threads = shape.waves_m * shape.waves_n * 64;
+        product.threads = shape.threads();
         product.grid = (uint32_t)tasks.size();
         product.join_grid = (uint32_t)joins.size() * (shape.tile / 32) * (shape.tile / 32) / 4;
         product.text = strfmt("#define TILE %u\n#define WAVES_M %u\n#define WAVES_N %u\n#define STAGES %u\n#ifndef KERNEL_ATTRS\n#define KERNEL_ATTRS %s\n#endif\n", shape.tile,
                               shape.waves_m, shape.waves_n, shape.stages, shape.attrs);
         product.parked = parked * shape.tile * shape.tile;
-        product.estimate = cut.estimate;
+        product.estimate = size.estimate;
         most = std::max(most, product.parked * (p == 1 ? 2 : 1));
         cuts += strfmt("\nmuon_%s tile=%u threads=%u stages=%u grid=%u join_grid=%u parked=%u estimate=%.1f", names[p], shape.tile, product.threads, shape.stages, product.grid,
-                       product.join_grid, parked * shape.tile * shape.tile, cut.estimate);
+                       product.join_grid, parked * shape.tile * shape.tile, size.estimate);
     }
     shared_at_ = take((uint64_t)most * 4);
     plan_launches();

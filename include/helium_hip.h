@@ -488,8 +488,9 @@ int he_group_norm_destroy(he_group_norm_t norm);
  * ================================================================================================== */
 typedef struct he_muon_s* he_muon_t;
 
-/* A group of `count` matrices of any extents, shapes[2 k] x shapes[2 k + 1], row-major and packed; a call treats all of them with one
- * launch per stage. dtype: HE_F32, HE_BF16 or HE_F16, of the matrices that come in. The orthogonalised form of U: X = U / (|U| + 1e-7)
+/* A group of `count` matrices, at most 65536, shapes[2 k] x shapes[2 k + 1], row-major and packed; a call treats all of them with one
+ * launch per stage. Extents are up to 2^20 by 32768, either way round, and fewer than 2^36 values in all (each extent rounded up to a multiple
+ * of 64). dtype: HE_F32, HE_BF16 or HE_F16, of the matrices that come in. The orthogonalised form of U: X = U / (|U| + 1e-7)
  * (Frobenius norm, transposed where there are more rows than columns), then `steps` times S = X X^T, X = a X + (b S + c S S) X with
  * (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value to about 1 (0.7 to 1.2 in five steps where it was at least
  * 1/100 of the norm; 0 stays 0). precision: HE_PREC_F32_F32 (one to three times the error of f32 products) or HE_PREC_F16_F32 (f16 operands,

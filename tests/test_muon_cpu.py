@@ -1,6 +1,8 @@
 """Orthogonalised updates without a GPU: the oracle's properties, the kernels under emulation (host AddressSanitizer checks every
 access) against the oracle, and what the entry points refuse."""
 import ctypes
+import heapq
+import time
 
 import numpy as np
 import pytest
@@ -167,6 +169,53 @@ def test_the_kernels_step_matches_the_oracles(nesterov):
         assert np.abs(nm - want_m).max() < 4 * 2.0 ** -24 * np.abs(want_m).max()
         # the orthogonalised part is good to some 1e-6 of values up to 1.2, times 0.1 sqrt(rows / columns)
         assert np.abs(nw - want_w).max() < 1e-5
+
+
+@pytest.mark.parametrize("precision", ["f32_f32", "f16_f32"])
+@pytest.mark.parametrize("shapes", [[(4096, 4096)] * 128 + [(4096, 11008)] * 96, [(32768, 262144)], [(8, 8)] * 65536, [(1 << 20, 32768)]])
+def test_large_groups_are_cut_in_seconds(shapes, precision):
+    """What the choice of tiles goes by is counted, not made: candidates of these groups have up to a thousand million tasks."""
+    began = time.monotonic()
+    muon = ha.Muon(shapes, "bf16", precision=precision)
+    assert time.monotonic() - began < 20   # (most of a second or two is the compiler's; made and dealt, the first group took 50 seconds)
+    for line in muon.description.splitlines()[1:4]:
+        said = dict(s.split("=") for s in line.split()[1:])
+        assert int(said["grid"]) * int(said["threads"]) < 1 << 32 and int(said["join_grid"]) * 256 < 1 << 32
+
+
+def test_groups_of_more_blocks_than_a_launch_has_are_refused_before_anything_is_made():
+    began = time.monotonic()
+    for shapes in ([(1 << 20, 32768)] * 2, [(4096, 4096)] * 65536):
+        with pytest.raises(ha.HeliumError, match="too many elements"):
+            ha.Muon(shapes, "f32")
+    assert time.monotonic() - began < 10
+
+
+def lengths_by_simulation(lengths, slots, base, each):
+    """When the last of these tasks ends, each given to the place that is free first, the longest ones first."""
+    free = [0.0] * slots
+    for n in sorted(lengths, reverse=True):
+        heapq.heappush(free, heapq.heappop(free) + base + each * n)
+    return max(free)
+
+
+@pytest.mark.parametrize("shapes", [[(64, 576)], [(1000, 512), (777, 1203)], [(4096, 1024), (1024, 4096)], [(700, 3000)] * 9, [(128, 128)] * 2000])
+def test_a_cuts_estimate_is_that_of_its_own_tasks(monkeypatch, shapes):
+    """The estimate comes from counts of tasks of each length; here the tasks that were made are dealt out one by one."""
+    tiles = {64: (2, 2.5, 0.28, 0.50), 128: (2, 3.5, 0.85, 1.65), 192: (1, 5.0, 0.85, 2.00), 256: (1, 6.0, 2.00, 2.85)}
+    for tile, (per_cu, base, alone, full) in tiles.items():
+        monkeypatch.setenv("HELIUM_HIP_MUON_TILE", str(tile))
+        muon = ha.Muon(shapes, "f32")
+        for p, line in enumerate(muon.description.splitlines()[1:4]):
+            said = dict(s.split("=") for s in line.split()[1:])
+            tasks = np.frombuffer(muon.table(1 + p), TASK)
+            assert len(tasks) == int(said["grid"])
+            slots = 256 * per_cu
+            f = min(1.0, len(tasks) / slots)
+            want = lengths_by_simulation([int(t["k_end"]) - int(t["k_begin"]) for t in tasks], slots, base, alone + (full - alone) * f * f)
+            if int(said["parked"]):
+                want += 2.5 + 4.0 * int(said["parked"]) / 5e6
+            assert abs(float(said["estimate"]) - want) < 0.051 + 1e-9 * want, (tile, line, want)   # (printed with one digit)
 
 
 @pytest.mark.parametrize("shapes,dtype,precision,steps,says", [
