@@ -744,12 +744,6 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         auto padded = [&](int64_t v) { return (uint32_t)((v + kBlock - 1) / kBlock * kBlock); };
         m.mp = padded(std::min(rows, cols)), m.np = padded(std::max(rows, cols));
         m.shape_scale = (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
-        const uint64_t bytes = pr.split ? 4 : 2, x = m.mp * bytes * m.np, a = m.mp * bytes * m.mp;
-        for (int k : {X, XT, XT2}) m.at[k] = take(x);
-        for (int k : {A, B}) m.at[k] = take(a);
-        if (pr.split)
-            for (int k : {C, Q, Q2}) m.at[k] = take(a);
-        else m.at[X_LOW] = take(x);
         const uint64_t size = (uint64_t)rows * cols;
         m.first_part = (uint32_t)parts;
         m.parts = (uint32_t)((size + part - 1) / part);
@@ -802,8 +796,20 @@ Muon::Muon(const MuonProblem& pr) : pr_(pr) {
         cuts += strfmt("\nmuon_%s tile=%u threads=%u stages=%u grid=%u join_grid=%u parked=%u estimate=%.1f", names[p], shape.tile, product.threads, shape.stages, product.grid,
                        product.join_grid, parked * shape.tile * shape.tile, size.estimate);
     }
+    // What the launches read and write, and no more: X's transpose a second time if there is a run after the first, C and the Q's if a
+    // run has several steps.
+    const std::vector<int> runs = choose_runs();
+    const bool several = *std::max_element(runs.begin(), runs.end()) > 1;
+    for (MuonMatrix& m : matrices_) {
+        const uint64_t bytes = pr.split ? 4 : 2, x = m.mp * bytes * m.np, a = m.mp * bytes * m.mp;
+        for (int k : {X, XT, A, B}) m.at[k] = take(k == X || k == XT ? x : a);
+        if (runs.size() > 1) m.at[XT2] = take(x);
+        if (several)
+            for (int k : {C, Q, Q2}) m.at[k] = take(a);
+        if (!pr.split) m.at[X_LOW] = take(x);
+    }
     shared_at_ = take((uint64_t)most * 4);
-    plan_launches();
+    plan_launches(runs);
     // (a share's place among the sums is its block's, plus where its launch begins)
     for (size_t k = 0; k < pr.shapes.size(); k++)
         for (uint32_t p = part_begin_[k]; p < part_begin_[k + 1]; p++) portions[p].j = part_begin_[k / kGroup * kGroup];
@@ -867,8 +873,8 @@ Muon::Buffers Muon::buffers(hipStream_t stream) {
     return b;
 }
 
-// What is launched between the conversions: runs of steps, each of them on the m x m side but for its ends.
-void Muon::plan_launches() {
+// How many steps at a time are taken on the m x m side.
+std::vector<int> Muon::choose_runs() const {
     std::vector<int> runs(pr_.steps, 1);
     // Runs of three at most and as even as can be, the longest first, if that is estimated to save a tenth: always where n is well beyond
     // m, never where they are equal (a classifier's 22 filters, mostly 1 to 9: 569 -> 379 us; 1000 x 512 and 777 x 1203: 221 -> 245).
@@ -883,6 +889,11 @@ void Muon::plan_launches() {
         };
         if (cost(longer) < 0.9 * cost(runs) || tuning::get_int("HELIUM_HIP_MUON_RUNS", 0)) runs = longer;
     }
+    return runs;
+}
+
+// What is launched between the conversions: runs of steps, each of them on the m x m side but for its ends.
+void Muon::plan_launches(const std::vector<int>& runs) {
     // scales of what is in the buffers: of X, of A, B and C, and of Q after so many steps (its values are at most a, a^2, a^3)
     const double sx = 4096, sa = 8192, sq[4] = {0, 8192, 4096, 1024};
     // (what a launch computes lies in a table on the device: a kernel's own parameters come from host memory, and longer ones took

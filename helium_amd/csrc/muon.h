@@ -95,7 +95,8 @@ private:
     };
     std::vector<Launch> launches_;
     std::string launches_text_;
-    void plan_launches();
+    std::vector<int> choose_runs() const;
+    void plan_launches(const std::vector<int>& runs);
     std::vector<uint32_t> part_begin_, block_begin_;  // per matrix: first entry of tables 7 and 8
     std::string source_, describe_;
     std::unique_ptr<JitKernel> norm_, convert_, finish_, norm_step_, convert_step_, finish_step_;

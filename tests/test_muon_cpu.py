@@ -183,6 +183,21 @@ def test_large_groups_are_cut_in_seconds(shapes, precision):
         assert int(said["grid"]) * int(said["threads"]) < 1 << 32 and int(said["join_grid"]) * 256 < 1 << 32
 
 
+@pytest.mark.parametrize("shapes,precision,steps,values", [
+    ([(4096, 4096)], "f32_f32", 5, 5 * 4096 ** 2),                  # one step at a time: X, X^T twice, A and B
+    ([(4096, 4096)], "f32_f32", 1, 4 * 4096 ** 2),
+    ([(512, 4608)], "f32_f32", 5, 3 * 512 * 4608 + 5 * 512 ** 2),   # runs of three and two: C and two Q's too
+    ([(4600, 500)], "f32_f32", 3, 2 * 512 * 4608 + 5 * 512 ** 2),   # one run of three
+    ([(512, 4608)], "f16_f32", 5, 4 * 512 * 4608 + 2 * 512 ** 2),   # X's low part
+])
+def test_the_workspace_holds_what_the_launches_use(shapes, precision, steps, values):
+    muon = ha.Muon(shapes, "bf16", precision=precision, steps=steps)
+    lines = [dict(s.split("=") for s in line.split()[1:]) for line in muon.description.splitlines()[:4]]
+    parked = max(int(line["parked"]) * (2 if p == 1 else 1) for p, line in enumerate(lines[1:]))
+    matrices = values * (4 if precision == "f32_f32" else 2)
+    assert 0 <= int(lines[0]["workspace"]) - matrices - 4 * parked - 8 * int(lines[0]["shares"]) < 16 * 256   # (each buffer begins at 256 bytes)
+
+
 def test_groups_of_more_blocks_than_a_launch_has_are_refused_before_anything_is_made():
     began = time.monotonic()
     for shapes in ([(1 << 20, 32768)] * 2, [(4096, 4096)] * 65536):
