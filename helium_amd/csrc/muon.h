@@ -15,7 +15,7 @@ namespace he {
 struct MuonProblem {
     std::vector<std::array<int64_t, 2>> shapes;  // rows, columns
     int dtype = HE_F32;                          // of the matrices that come in (and of orthogonalised ones that go out)
-    bool split = true;                           // f32_f32: f16 operands in two parts; otherwise in one
+    bool split = true;                           // f32_f32, and f16 matrices: f16 operands in two parts; otherwise in one
     int steps = 5;
 };
 

@@ -494,7 +494,8 @@ typedef struct he_muon_s* he_muon_t;
  * (Frobenius norm, transposed where there are more rows than columns), then `steps` times S = X X^T, X = a X + (b S + c S S) X with
  * (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value to about 1 (0.7 to 1.2 in five steps where it was at least
  * 1/100 of the norm; 0 stays 0). precision: HE_PREC_F32_F32 (one to three times the error of f32 products) or HE_PREC_F16_F32 (f16 operands,
- * f32 sums; results good to about 3 digits, for gradients in 16 bits). Compiles the kernels; needs no device. */
+ * f32 sums; results good to about 3 digits, for gradients in bf16; f16 results hold more than that, and f16 matrices are treated as at
+ * HE_PREC_F32_F32). Compiles the kernels; needs no device. */
 int he_muon_create(he_muon_t* muon, const int64_t* shapes, int count, int dtype, int precision, int steps);
 /* out[k] (of `dtype`) is the orthogonalised in[k]; it may be in[k]. Lists of `count` device addresses in host memory, aligned to 16
  * bytes. The first call on a stream allocates workspace for it, later ones allocate nothing; calls on several streams may overlap. */

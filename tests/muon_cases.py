@@ -45,3 +45,12 @@ def check(got, u, dtype, split, steps=5, runs=None):
     each = each if np.count_nonzero(want) > 64 else np.maximum(each, allowed)
     wrong = np.abs(got - want) > each
     assert not wrong.any(), (int(wrong.sum()), np.argwhere(wrong)[0], got[wrong][0], want[wrong][0])
+
+
+def check_rounded_once(got, u, dtype, steps=5):
+    """`got` is the exact result as well as its type holds it: each value off by half a step of the type, and by what five steps with
+    f32 products are off (below 1e-5 of the result's norm) on top."""
+    want = oracle.orthogonalize(u, steps)
+    size = np.linalg.norm(want)
+    far = np.linalg.norm(got - want)
+    assert far <= (HALF_STEP[dtype] + 1e-5) * size + TINY[dtype] * np.sqrt(want.size), (far / size, HALF_STEP[dtype])

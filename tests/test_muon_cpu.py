@@ -10,7 +10,7 @@ import pytest
 import helium_amd as ha
 from cpu_emul import run_kernel
 from helium_amd import _ffi
-from muon_cases import SHAPES, check, matrix, runs_of, to_f32, to_storage
+from muon_cases import SHAPES, check, check_rounded_once, matrix, runs_of, to_f32, to_storage
 from oracle import muon as oracle
 
 MATRIX = np.dtype([("rows", "u4"), ("cols", "u4"), ("mp", "u4"), ("np", "u4"), ("tall", "u4"), ("first_part", "u4"), ("parts", "u4"),
@@ -155,6 +155,16 @@ def test_the_kernels_match_the_oracle(monkeypatch, dtype, split, steps, runs):
     got, _ = emulated(shapes, dtype, split, steps, stored)
     for g, s in zip(got, stored):
         check(to_f32(g, dtype), to_f32(s, dtype), dtype, split, steps, {"0": None, "1": {3: [3], 5: [3, 2]}.get(steps)}[runs])
+
+
+def test_f16_results_have_the_digits_of_their_type(monkeypatch):
+    """Also at f16_f32: five steps with operands of 11 bits would leave a result of 11 bits with eight of them."""
+    monkeypatch.setenv("HELIUM_HIP_MUON_ONE_BY_ONE", "1")
+    shapes = [(40, 70)]
+    stored = [to_storage(matrix(s, "normal", 21), "f16") for s in shapes]
+    got, _ = emulated(shapes, "f16", False, 5, stored)
+    for g, s in zip(got, stored):
+        check_rounded_once(to_f32(g, "f16"), to_f32(s, "f16"), "f16")
 
 
 @pytest.mark.parametrize("nesterov", [0, 1])

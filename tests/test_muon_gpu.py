@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import helium_amd as ha
-from muon_cases import SHAPES, check, matrix, runs_of, to_f32, to_storage
+from muon_cases import SHAPES, check, check_rounded_once, matrix, runs_of, to_f32, to_storage
 from oracle import muon as oracle
 from test_group_norm_gpu import address, back, device
 
@@ -38,6 +38,14 @@ def test_larger_matrices_by_themselves(gpu, shape, dtype, precision):
     stored = [to_storage(matrix(shape, "normal", 2), dtype)]
     got, = orthogonalized([shape], stored, dtype, precision)
     check(to_f32(got, dtype), to_f32(stored[0], dtype), dtype, precision == "f32_f32")
+
+
+@pytest.mark.parametrize("precision", ["f32_f32", "f16_f32"])
+@pytest.mark.parametrize("shape", LARGER + [(64, 576)])
+def test_f16_results_have_the_digits_of_their_type(gpu, shape, precision):
+    stored = [to_storage(matrix(shape, "normal", 22), "f16")]
+    got, = orthogonalized([shape], stored, "f16", precision)
+    check_rounded_once(to_f32(got, "f16"), to_f32(stored[0], "f16"), "f16")
 
 
 @pytest.mark.parametrize("runs", ["one by one", "several"])
