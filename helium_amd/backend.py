@@ -41,6 +41,7 @@ OPT_REMATERIALIZE = 2
 OPT_CANCEL_TRANSPOSES = 3
 OPT_HOIST_BROADCASTS = 4
 OPT_STREAM_FAN_OUT = 5  # 0 one stream, 1 where it pays (default), 2 every step with several instructions
+OPT_MUON_SEVERAL_STEPS = 6  # of Muon objects made from then on: 0 one Newton-Schulz step at a time, 1 several where it pays (default)
 
 
 def set_option(option, value):

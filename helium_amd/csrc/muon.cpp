@@ -1,6 +1,7 @@
 #include "muon.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <functional>
@@ -18,16 +19,16 @@ constexpr uint64_t kThreads = 1ull << 32, kMostBlocks = kThreads / 256 - 1;
 
 // Newton-Schulz iteration on f16 matrix cores. With X scaled to a Frobenius norm of at most 1, no singular value ever leaves
 // [0, 1.21]: the step's polynomial a s + b s^3 + c s^5 maps [0, 1] there and [1, 1.21] into [0.68, 0.96]. So every entry has a known
-// bound, and fixed powers of two keep f16 operands in range (kScale). A value's f16 rounding has 11 bits; its remainder in a second f16
+// bound, and fixed powers of two keep f16 operands in range (X_SCALE, and the scales in plan_launches()). A value's f16 rounding has 11 bits; its remainder in a second f16
 // gives 22, and three of the four products of such pairs (the fourth is 2^-22 of the result) run at three times f16's cost, where f32
-// matrix instructions take sixteen times. Measured against 64 bits: errors as of f32 products, 1e-6 to 2.5e-6.
+// matrix instructions take sixteen times. Errors are 0.7 to 1.6 times those of f32 products (1e-6 to 4e-6 of the result's norm).
 //
 // Several steps at once. All matrices of an iteration commute, so its steps can be taken on the m x m side: with A = X X^T and
 // Q_k = a I + b A_k + c A_k A_k, A_(k+1) = Q_k A_k Q_k, and X = Q_(r-1) ... Q_0 X after r steps - one product with X on either end
 // instead of two per step, for 3 m x m products (half of them by symmetry) per step between. It costs digits: an error of A, which is
-// relative to the largest singular value, meets the smallest squared. After three steps in two f16 parts errors are up to three times
-// those of f32 products (2e-6 to 7e-6 against 1e-6 to 3e-6; singular values over three decades 6e-6 against 4e-6, a few directions 35 times as strong as
-// the rest 2.0e-5 against 1.1e-5; five at once: 1e-4), so steps go in runs of three at most, and one by one
+// relative to the largest singular value, meets the smallest squared. After runs of three and two errors are 0.8 to 2.5 times those of f32
+// products, and up to 8 times (7e-6 of the norm against 9e-7) on 20 x 60 with a few directions 35 times as strong as the rest; five at once: 1e-4.
+// So steps go in runs of three at most, one by one where the caller says so (HE_OPT_MUON_SEVERAL_STEPS) and
 // where operands have one part.
 const char* kCommon = R"HIP(
 typedef unsigned short u16;
@@ -716,7 +717,11 @@ template <class T> std::vector<char> bytes_of(const std::vector<T>& v) {
     return out;
 }
 
+std::atomic<bool> g_several_steps{true};
+
 }  // namespace
+
+void set_muon_several_steps(bool may) { g_several_steps = may; }
 
 Muon::Muon(const MuonProblem& pr) : pr_(pr) {
     HE_REQUIRE(!pr.shapes.empty() && pr.shapes.size() <= 65536, HE_ERR_INVALID, "muon: %zu matrices, 1 to 65536 are taken", pr.shapes.size());
@@ -878,7 +883,7 @@ std::vector<int> Muon::choose_runs() const {
     std::vector<int> runs(pr_.steps, 1);
     // Runs of three at most and as even as can be, the longest first, if that is estimated to save a tenth: always where n is well beyond
     // m, never where they are equal (a classifier's 22 filters, mostly 1 to 9: 569 -> 379 us; 1000 x 512 and 777 x 1203: 221 -> 245).
-    if (pr_.split && !tuning::get_int("HELIUM_HIP_MUON_ONE_BY_ONE", 0)) {
+    if (pr_.split && g_several_steps.load() && !tuning::get_int("HELIUM_HIP_MUON_ONE_BY_ONE", 0)) {
         const int count = (pr_.steps + 2) / 3;
         std::vector<int> longer(count, pr_.steps / count);
         for (int k = 0; k < pr_.steps % count; k++) longer[k]++;

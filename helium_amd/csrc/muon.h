@@ -51,6 +51,9 @@ struct MuonStep {
     int32_t nesterov;
 };
 
+// Whether several steps may be taken at a time (HE_OPT_MUON_SEVERAL_STEPS).
+void set_muon_several_steps(bool may);
+
 class Muon {
 public:
     explicit Muon(const MuonProblem& pr);

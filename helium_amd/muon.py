@@ -29,7 +29,7 @@ class Muon:
 
     Construction generates and compiles the kernels and needs no GPU. Operands are lists of DeviceBuffers, Tensors or raw device addresses,
     one per matrix: gradients (and orthogonalised matrices) of type `dtype`, momenta and weights f32. precision "f32_f32" gives
-    one to three times the error of f32 products, "f16_f32" about three digits at a third of the time (f16 matrices, whose results hold more,
+    the error of f32 products, or some times that where it takes several steps at once (backend.OPT_MUON_SEVERAL_STEPS), "f16_f32" about three digits at a third of the time (f16 matrices, whose results hold more,
     are treated as at "f32_f32").
     """
 

@@ -411,9 +411,11 @@ int he_fgraph_subdivide(he_fgraph_t graph, uint64_t* nodes, int32_t* portions, i
  * (helium/src/cuda.rs:190-221). 1: only steps whose instructions are too small to fill the device and numerous enough to
  * outweigh the joins (each costs the host 15-20 us here), those of up to 1 MB that share launches counted as one; all
  * others run on the first stream in plan order. 0: one stream. Takes effect from the next he_execute_graph; results do
- * not depend on it. */
+ * not depend on it.
+ * HE_OPT_MUON_SEVERAL_STEPS (default 1): not of graphs: whether he_muon_create at HE_PREC_F32_F32 may take several steps at a time (below).
+ * 0: one by one. Takes effect from the next he_muon_create. */
 enum { HE_OPT_FUSE_MATMUL_EPILOGUE = 0, HE_OPT_FOLD_SWAP_INTO_REDUCE = 1, HE_OPT_REMATERIALIZE = 2, HE_OPT_CANCEL_TRANSPOSES = 3,
-       HE_OPT_HOIST_BROADCASTS = 4, HE_OPT_STREAM_FAN_OUT = 5 };
+       HE_OPT_HOIST_BROADCASTS = 4, HE_OPT_STREAM_FAN_OUT = 5, HE_OPT_MUON_SEVERAL_STEPS = 6 };
 int he_backend_set_option(int option, int64_t value);
 
 /* Counters of the last he_execute_graph on this thread: [0] steps run, [1] instructions, [2] streams used,
@@ -493,9 +495,12 @@ typedef struct he_muon_s* he_muon_t;
  * of 64). dtype: HE_F32, HE_BF16 or HE_F16, of the matrices that come in. The orthogonalised form of U: X = U / (|U| + 1e-7)
  * (Frobenius norm, transposed where there are more rows than columns), then `steps` times S = X X^T, X = a X + (b S + c S S) X with
  * (a, b, c) = (3.4445, -4.7750, 2.0315), which takes every singular value to about 1 (0.7 to 1.2 in five steps where it was at least
- * 1/100 of the norm; 0 stays 0). precision: HE_PREC_F32_F32 (one to three times the error of f32 products) or HE_PREC_F16_F32 (f16 operands,
- * f32 sums; results good to about 3 digits, for gradients in bf16; f16 results hold more than that, and f16 matrices are treated as at
- * HE_PREC_F32_F32). Compiles the kernels; needs no device. */
+ * 1/100 of the norm; 0 stays 0). precision: HE_PREC_F32_F32: operands of 22 bits and f32 sums, as far off as f32 products are (0.7 to
+ * 1.6 times). Where the group's extents make it faster (the smaller ones well below the larger), up to three steps at a time are taken on the
+ * smaller side: commonly 0.8 to 2.5 times as far off as f32 products, up to 8 times (7e-6 of a result's norm) on small matrices of a few strong
+ * directions. HE_OPT_MUON_SEVERAL_STEPS = 0 forgoes that; he_muon_describe says which it is ("runs"). HE_PREC_F16_F32: operands of 11
+ * bits and f32 sums, results good to about 3 digits, for gradients in bf16; f16 results hold more than that, and f16 matrices are treated as
+ * at HE_PREC_F32_F32. What a matrix's result is to the last bit goes by the whole group. Compiles the kernels; needs no device. */
 int he_muon_create(he_muon_t* muon, const int64_t* shapes, int count, int dtype, int precision, int steps);
 /* out[k] (of `dtype`) is the orthogonalised in[k]; it may be in[k]. Lists of `count` device addresses in host memory, aligned to 16
  * bytes. The first call on a stream allocates workspace for it, later ones allocate nothing; calls on several streams may overlap. */

@@ -54,3 +54,25 @@ def check_rounded_once(got, u, dtype, steps=5):
     size = np.linalg.norm(want)
     far = np.linalg.norm(got - want)
     assert far <= (HALF_STEP[dtype] + 1e-5) * size + TINY[dtype] * np.sqrt(want.size), (far / size, HALF_STEP[dtype])
+
+
+def f32_products(u, steps=5):
+    """The definition in f32, products and all: what an implementation without matrix cores of 16 bits gives."""
+    a, b, c = (np.float32(v) for v in oracle.COEFFICIENTS)
+    tall = u.shape[0] > u.shape[1]
+    x = np.ascontiguousarray(u.T if tall else u, np.float32)
+    x = x / np.float32(np.sqrt((x.astype(np.float64) ** 2).sum()) + oracle.NORM_FLOOR)
+    for _ in range(steps):
+        s = x @ x.T
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.T if tall else x
+
+
+def spectra(shape, seed):
+    """Matrices whose errors are magnified in different ways."""
+    rng = np.random.default_rng(seed)
+    r, c = shape
+    noise, few = rng.standard_normal(shape), 0.35 * rng.standard_normal((r, 8)) @ rng.standard_normal((8, c))
+    u, _, vt = np.linalg.svd(rng.standard_normal(shape), full_matrices=False)
+    weak = np.where(np.arange(r)[:, None] % 2, noise, 1e-3 * noise)
+    return {"noise": noise, "few directions": noise + few, "few strong directions": noise + 4 * few, "decades": (u * np.logspace(0, -3, min(shape))) @ vt, "weak rows": weak}

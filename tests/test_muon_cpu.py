@@ -9,7 +9,7 @@ import pytest
 
 import helium_amd as ha
 from cpu_emul import run_kernel
-from helium_amd import _ffi
+from helium_amd import _ffi, backend
 from muon_cases import SHAPES, check, check_rounded_once, matrix, runs_of, to_f32, to_storage
 from oracle import muon as oracle
 
@@ -68,6 +68,15 @@ def test_how_steps_are_taken_goes_by_shape_and_precision():
     assert runs([(512, 512)], "f32") == [1] * 5
     assert runs([(512, 4608)], "f32") == [3, 2] and runs([(4608, 512)], "f32", steps=4) == [2, 2] and runs([(512, 4608)], "f32", steps=7) == [3, 2, 2]
     assert runs([(512, 4608)], "bf16", precision="f16_f32") == [1] * 5
+
+
+def test_a_caller_can_have_steps_one_by_one():
+    try:
+        backend.set_option(backend.OPT_MUON_SEVERAL_STEPS, 0)
+        assert runs_of(ha.Muon([(512, 4608)], "f32")) == [1] * 5
+    finally:
+        backend.set_option(backend.OPT_MUON_SEVERAL_STEPS, 1)
+    assert runs_of(ha.Muon([(512, 4608)], "f32")) == [3, 2]
 
 
 SHFL = r"""

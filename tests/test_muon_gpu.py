@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 import helium_amd as ha
-from muon_cases import SHAPES, check, check_rounded_once, matrix, runs_of, to_f32, to_storage
+from helium_amd import backend
+from muon_cases import SHAPES, check, check_rounded_once, f32_products, matrix, runs_of, spectra, to_f32, to_storage
 from oracle import muon as oracle
 from test_group_norm_gpu import address, back, device
 
@@ -46,6 +47,25 @@ def test_f16_results_have_the_digits_of_their_type(gpu, shape, precision):
     stored = [to_storage(matrix(shape, "normal", 22), "f16")]
     got, = orthogonalized([shape], stored, "f16", precision)
     check_rounded_once(to_f32(got, "f16"), to_f32(stored[0], "f16"), "f16")
+
+
+@pytest.mark.parametrize("several,times", [(0, 3), (1, 12)])
+@pytest.mark.parametrize("shape", [(20, 60), (64, 576), (128, 128), (256, 2304), (512, 512), (1000, 300)])
+def test_f32_results_are_as_far_off_as_f32_products_are(gpu, monkeypatch, shape, several, times):
+    """What is documented (0.7 to 1.6 times, and up to 8 with several steps at once; both with half of it and more to spare: the orders of the sums differ)."""
+    if several:
+        monkeypatch.setenv("HELIUM_HIP_MUON_RUNS", "1")   # whatever they are estimated to take
+    try:
+        backend.set_option(backend.OPT_MUON_SEVERAL_STEPS, several)
+        muon = ha.Muon([shape], "f32")
+    finally:
+        backend.set_option(backend.OPT_MUON_SEVERAL_STEPS, 1)
+    assert runs_of(muon) == ([3, 2] if several else [1] * 5)
+    for name, u in spectra(shape, 23).items():
+        u = u.astype(np.float32)
+        want = oracle.orthogonalize(u)
+        far, off = (np.linalg.norm(v - want) for v in (orthogonalized([shape], [u], "f32", None, muon=muon)[0], f32_products(u)))
+        assert far <= times * off, (name, far / off)
 
 
 @pytest.mark.parametrize("runs", ["one by one", "several"])
