@@ -69,7 +69,6 @@ public:
     // (a MuonProduct per matrix and product).
     static constexpr int kTables = 10;
     const std::vector<char>& table(int which) const { return tables_[which]; }
-    size_t workspace_bytes() const { return workspace_bytes_; }
 
 private:
     struct Buffers {
