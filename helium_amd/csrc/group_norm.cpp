@@ -180,8 +180,8 @@ __device__ __forceinline__ float slope_times(float dy, float z) {
 // M2 = sum of M2_i + n_i (mean_i - mean)^2 (by `apply` itself, or by `merge` where they are more than 32), and the tensor is read again.
 // Sums are f32: a thread its own values, then trees.
 //
-// Bound by memory. WHOLE, 64 x 3136 x 256 bf16 in 32 groups: 47 us, 4.3 TB/s for one read and one write; a workgroup of 1024 threads
-// fills a CU's registers and loads, sums and stores in turn. In parts 52 us. In parts, 2 x 262144 x 128 bf16: statistics 22 us (6.1
+// Bound by memory. WHOLE, 64 x 3136 x 256 bf16 in 32 groups: 47 us for one read and one write, 5.1 TB/s of what crosses the L2s' far
+// side: in 105 MB, out 139 MB for 103 MB of results (a workgroup's 64 bytes of a pixel are half a cache line). In parts 52 us. In parts, 2 x 262144 x 128 bf16: statistics 22 us (6.1
 // TB/s), merge 5, apply 41 (6.5 TB/s). 1 x 49 x 512: one launch of 3.7 us.
 const char* kForward = R"HIP(
 // mean[g] and m2[g] of the workgroup's pixels
