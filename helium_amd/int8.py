@@ -1,0 +1,51 @@
+"""Quantised matrices over the C ABI: rows of 8-bit whole numbers with an f32 scale each."""
+import ctypes as C
+
+from . import _ffi
+from ._ffi import check, lib
+from .device import _h
+from .group_norm import _at
+
+_ffi._sig("he_quantized_pitch", C.c_int64, restype=C.c_int64)
+_ffi._sig("he_quantize_rows_create", C.POINTER(C.c_void_p), C.c_int64, C.c_int)
+_ffi._sig("he_quantize_rows_destroy", C.c_void_p)
+_ffi._sig("he_quantize_rows", C.c_void_p, C.c_int64, *[C.c_void_p] * 4)
+_ffi._sig("he_quantize_rows_source", C.c_void_p, restype=C.c_char_p)
+_ffi._sig("he_quantize_rows_describe", C.c_void_p, restype=C.c_char_p)
+
+
+def pitch(columns):
+    """Bytes of a quantised matrix' row: its columns, and zeros up to a multiple of 16."""
+    return lib.he_quantized_pitch(columns)
+
+
+class QuantizeRows:
+    """q = round(127 x / A), scale = A / 127 with A a row's largest |x|, for rows of `columns` values of type `dtype`."""
+
+    def __init__(self, columns, dtype):
+        self.columns = int(columns)
+        self.handle = C.c_void_p()
+        check(lib.he_quantize_rows_create(C.byref(self.handle), self.columns, _ffi.DTYPES[dtype]))
+
+    @property
+    def source(self):
+        return lib.he_quantize_rows_source(self.handle).decode()
+
+    @property
+    def description(self):
+        return lib.he_quantize_rows_describe(self.handle).decode()
+
+    def quantize(self, rows, x, q, scales, stream=None):
+        """x [rows, columns] -> q, rows of pitch(columns) bytes, and scales [rows]."""
+        check(lib.he_quantize_rows(self.handle, rows, _at(x), _at(q), _at(scales), _h(stream)))
+
+    def close(self):
+        if self.handle:
+            lib.he_quantize_rows_destroy(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

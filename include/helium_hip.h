@@ -519,6 +519,52 @@ const char* he_muon_describe(he_muon_t muon);
 int he_muon_table(he_muon_t muon, int which, void* data, size_t capacity, size_t* bytes);
 int he_muon_destroy(he_muon_t muon);
 
+/* ==================================================================================================
+ * 10. Root-mean-square norm over rows, with the residual's addition: what normalises the tokens of a residual stream as group norm does
+ *     the pixels of an image. Into its operand's type, with a gradient, or into 8 bits, for section 11. No counterpart in the reference.
+ * ================================================================================================== */
+typedef struct he_rms_norm_s* he_rms_norm_t;
+
+/* Rows of `columns` values (at most 32768), row-major and packed; how many there are is each call's. h = x + residual, rounded to the
+ * residual's type, or x itself without one; rstd = 1 / sqrt(mean of h^2 + epsilon); y = h * rstd * gamma[c]. dtype: HE_F32, HE_BF16 or
+ * HE_F16, of x, y and their gradients; residual_dtype: HE_F32 or dtype, or -1: there is no residual; param_dtype: of gamma, HE_F32 or
+ * dtype. Arithmetic and sums are f32 (squares of values beyond 1e19 overflow). to_i8: y is quantised as section 11 has it, a row's scale
+ * being the largest |y| / 127; q may differ from the correctly rounded one by 1 where y / scale is next to the middle of two whole numbers.
+ * Compiles the kernels; needs no device. */
+int he_rms_norm_create(he_rms_norm_t* norm, int64_t columns, int dtype, int residual_dtype, int param_dtype, int to_i8, float epsilon);
+/* new_residual receives h (NULL, as residual, where there is none) and may be residual; y may be x where their types are the same. rstd [rows] is what the
+ * backward pass reads, NULL where there is none; scales [rows] with to_i8 only. Tensors are aligned to 16 bytes, or to the
+ * largest power of two that divides a row's bytes where that is less; quantised rows to 16. rows may be 0. */
+int he_rms_norm_forward(he_rms_norm_t norm, int64_t rows, const void* x, const void* gamma, const void* residual, void* new_residual, void* y,
+                        float* rstd, float* scales, he_stream_t stream);
+/* dy: of y; h, rstd: as the forward pass had them; dh: what reaches h from its other readers, NULL for nothing. The gradient of h, which is
+ * that of x and of the residual, goes to dx (dtype) and dresidual (residual_dtype), of which one may be NULL; dx may be dy, or h where their types are the same,
+ * and dresidual may be dh or h. dgamma [columns] is f32, summed over the rows in a fixed order, zero without rows. Not with to_i8. The first call
+ * on a stream allocates scratch for it, later ones allocate nothing; calls on several streams may overlap. Captured graphs that may run at the
+ * same time are captured on streams of their own, or from handles of their own. */
+int he_rms_norm_backward(he_rms_norm_t norm, int64_t rows, const void* dy, const void* h, const void* gamma, const float* rstd, const void* dh,
+                         void* dx, void* dresidual, float* dgamma, he_stream_t stream);
+const char* he_rms_norm_source(he_rms_norm_t norm);
+const char* he_rms_norm_describe(he_rms_norm_t norm);
+int he_rms_norm_destroy(he_rms_norm_t norm);
+
+/* ==================================================================================================
+ * 11. Products in 8-bit integers with a scale for each row of either operand. No counterpart in the reference, whose products
+ *     (helium-ir/src/opgraph/op/precision.rs) end at 8-bit floats.
+ * ================================================================================================== */
+/* A quantised matrix: rows of he_quantized_pitch(columns) bytes (columns rounded up to a multiple of 16), whole numbers from -127 to 127 and zeros
+ * behind the columns, aligned to 16 bytes; and an f32 scale per row: the value is scale * q. */
+int64_t he_quantized_pitch(int64_t columns);
+
+typedef struct he_quantize_rows_s* he_quantize_rows_t;
+/* scale = A / 127 with A the largest |x| of the row, q = the whole number nearest to 127 x / A, ties to even. A row of zeros has scale 0; one that is
+ * not finite throughout has scale NaN and zeros (products with it are NaN). dtype: of x, HE_F32, HE_BF16 or HE_F16; at most 32768 columns. */
+int he_quantize_rows_create(he_quantize_rows_t* quantize, int64_t columns, int dtype);
+int he_quantize_rows(he_quantize_rows_t quantize, int64_t rows, const void* x, void* q, float* scales, he_stream_t stream);
+const char* he_quantize_rows_source(he_quantize_rows_t quantize);
+const char* he_quantize_rows_describe(he_quantize_rows_t quantize);
+int he_quantize_rows_destroy(he_quantize_rows_t quantize);
+
 #ifdef __cplusplus
 }
 #endif
