@@ -1,4 +1,4 @@
-"""Quantised matrices over the C ABI: rows of 8-bit whole numbers with an f32 scale each."""
+"""Quantised matrices, rows of 8-bit whole numbers with an f32 scale each, and their products, over the C ABI."""
 import ctypes as C
 
 from . import _ffi
@@ -12,6 +12,11 @@ _ffi._sig("he_quantize_rows_destroy", C.c_void_p)
 _ffi._sig("he_quantize_rows", C.c_void_p, C.c_int64, *[C.c_void_p] * 4)
 _ffi._sig("he_quantize_rows_source", C.c_void_p, restype=C.c_char_p)
 _ffi._sig("he_quantize_rows_describe", C.c_void_p, restype=C.c_char_p)
+_ffi._sig("he_int8_matmul_create", C.POINTER(C.c_void_p), C.c_int64, C.c_int64, C.c_int)
+_ffi._sig("he_int8_matmul_destroy", C.c_void_p)
+_ffi._sig("he_int8_matmul", C.c_void_p, C.c_int64, *[C.c_void_p] * 7)
+_ffi._sig("he_int8_matmul_source", C.c_void_p, restype=C.c_char_p)
+_ffi._sig("he_int8_matmul_describe", C.c_void_p, C.c_int64, C.c_char_p, C.c_size_t)
 
 
 def pitch(columns):
@@ -42,6 +47,44 @@ class QuantizeRows:
     def close(self):
         if self.handle:
             lib.he_quantize_rows_destroy(self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Int8Matmul:
+    """y = x weights^T of quantised matrices: tokens of `inputs` values, a row of weights for each of `channels`, results of type `dtype`.
+
+    A quantised matrix has rows of pitch(columns) bytes, whole numbers from -127 to 127 and zeros behind the columns, and an f32 scale for
+    each: QuantizeRows makes them of weights and activations, RmsNorm(output="i8") of a normalised residual stream.
+    """
+
+    def __init__(self, inputs, channels, dtype):
+        self.inputs, self.channels = int(inputs), int(channels)
+        self.handle = C.c_void_p()
+        check(lib.he_int8_matmul_create(C.byref(self.handle), self.inputs, self.channels, _ffi.DTYPES[dtype]))
+
+    @property
+    def source(self):
+        return lib.he_int8_matmul_source(self.handle).decode()
+
+    def describe(self, tokens):
+        """How a call with so many tokens is cut."""
+        text = C.create_string_buffer(256)
+        check(lib.he_int8_matmul_describe(self.handle, tokens, text, len(text)))
+        return text.value.decode()
+
+    def multiply(self, tokens, x, x_scales, weights, weight_scales, y, bias=None, stream=None):
+        """y[t][n] = x_scales[t] weight_scales[n] (x[t] . weights[n]) + bias[n]"""
+        check(lib.he_int8_matmul(self.handle, tokens, _at(x), _at(x_scales), _at(weights), _at(weight_scales), _at(bias), _at(y), _h(stream)))
+
+    def close(self):
+        if self.handle:
+            lib.he_int8_matmul_destroy(self.handle)
             self.handle = C.c_void_p()
 
     def __del__(self):

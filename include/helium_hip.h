@@ -565,6 +565,22 @@ const char* he_quantize_rows_source(he_quantize_rows_t quantize);
 const char* he_quantize_rows_describe(he_quantize_rows_t quantize);
 int he_quantize_rows_destroy(he_quantize_rows_t quantize);
 
+typedef struct he_int8_matmul_s* he_int8_matmul_t;
+/* y[t][n] = x_scales[t] * weight_scales[n] * (sum over k of x[t][k] weights[n][k]) + bias[n]: x and weights are quantised matrices of `inputs`
+ * columns (fewer than 2^17), weights with a row for each of `channels` (at most 2^24); how many tokens there are is each call's. Sums are exact, in
+ * 32-bit whole numbers; y is row-major and packed, of dtype (HE_F32, HE_BF16 or HE_F16), rounded once from f32. Compiles the kernels; needs no
+ * device. */
+int he_int8_matmul_create(he_int8_matmul_t* matmul, int64_t inputs, int64_t channels, int dtype);
+/* x and weights are aligned to 16 bytes, everything else to its own type; bias may be NULL; y shares no memory with the operands. At most 2^24
+ * tokens; there may be none. The first call on a stream that shares out its sums allocates scratch for it, later ones allocate nothing; calls on several
+ * streams may overlap. Captured graphs that may run at the same time are captured on streams of their own, or from handles of their own. */
+int he_int8_matmul(he_int8_matmul_t matmul, int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales,
+                   const float* bias, void* y, he_stream_t stream);
+/* The generated HIP source of all shapes, and how a call with so many tokens is cut (at most `capacity` bytes of text). */
+const char* he_int8_matmul_source(he_int8_matmul_t matmul);
+int he_int8_matmul_describe(he_int8_matmul_t matmul, int64_t tokens, char* text, size_t capacity);
+int he_int8_matmul_destroy(he_int8_matmul_t matmul);
+
 #ifdef __cplusplus
 }
 #endif

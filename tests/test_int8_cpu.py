@@ -1,0 +1,138 @@
+"""Products in 8-bit integers without a GPU: the generated kernels under the CPU emulation, how calls are cut, and what is refused."""
+import ctypes
+import re
+
+import numpy as np
+import pytest
+
+import helium_amd as ha
+from cpu_emul import run_kernel
+from group_norm_cases import to_f32
+from helium_amd import _ffi
+from int8_cases import SMALL, check, inputs
+from oracle import int8 as oracle
+
+# the matrix instructions: lane l holds 16 neighbouring k of row l % 32 (or 16); c[i] is row (i / 4) * 8 + (l / 32) * 4 + i % 4 of
+# column l % 32, or row (l / 16) * 4 + i of column l % 16
+SHIM = r"""
+typedef int emu_i32x4 __attribute__((ext_vector_type(4)));
+typedef int emu_i32x16 __attribute__((ext_vector_type(16)));
+static signed char g_i8a[1024][16], g_i8b[1024][16];
+template <int SIDE, class C> static inline C emu_i8(emu_i32x4 a, emu_i32x4 b, C c) {
+    unsigned tid = threadIdx.x, base = tid & ~63u, lane = tid & 63u;
+    memcpy(g_i8a[tid], &a, 16);
+    memcpy(g_i8b[tid], &b, 16);
+    WAVE_BAR();
+    for (int i = 0; i < SIDE * SIDE / 64; i++) {
+        unsigned row = SIDE == 32 ? (i / 4) * 8 + (lane / 32) * 4 + i % 4 : (lane / 16) * 4 + i, col = lane % SIDE;
+        for (int g = 0; g < 64 / SIDE; g++)
+            for (int k = 0; k < 16; k++) c[i] += g_i8a[base + row + SIDE * g][k] * g_i8b[base + col + SIDE * g][k];
+    }
+    WAVE_BAR();
+    return c;
+}
+#define MFMA_32(a, b, c) emu_i8<32>(a, b, c)
+#define MFMA_16(a, b, c) emu_i8<16>(a, b, c)
+"""
+
+FIELDS = ("x", "x_scales", "weights", "weight_scales")
+
+
+def emulated(op, host, dtype, shape, shares):
+    """What the kernels of one of the shapes make of a call."""
+    tokens, channels, columns = len(host["x"]), len(host["weights"]), host["x"].shape[1]
+    said = dict(re.findall(r"(\w+)=(\w+)", op.describe(tokens)))
+    assert int(said["shape"]) == shape
+    stream, threads, grid = "blocks_n" in said, int(said["threads"]), int(said["grid"])
+    text = SHIM + op.source.split("//// shape\n")[1 + shape]
+    call = f"Call c{{x, w, xs, ws, {'bias' if host['bias'] is not None else 'nullptr'}, y, {tokens}, {channels}, {columns}}};"
+    params = "const u8* x, const float* xs, const u8* w, const float* ws, const float* bias, out_t* y"
+    kernel = "int8_stream(c)" if stream else f"int8_product(c, {grid}, {said['shares']}, parked)"
+    text += f"\nextern \"C\" void emu({params}, i32x4* parked) {{ {call} {kernel}; }}\n"
+    if not stream and shares > 1:
+        text += f"extern \"C\" void emu_join({params}, const i32x4* parked) {{ {call} int8_join(c, {grid}, {said['shares']}, parked); }}\n"
+    given = [(host[k], 0) for k in FIELDS] + [(host["bias"] if host["bias"] is not None else np.zeros(1, np.float32), 0)]
+    y = np.empty((tokens, channels), np.float32 if dtype == "f32" else np.uint16)
+    parked = np.zeros(grid * int(said["shares"]) * np.prod([int(n) for n in said.get("tile", "1x1").split("x")]) if shares > 1 else 1, np.int32)
+    y, parked = run_kernel(text, "emu", grid, threads, given + [(y, 1), (parked, 2)], grid_y=int(said["shares"]))
+    if int(said["shares"]) > 1:
+        y, = run_kernel(text, "emu_join", grid, threads, given + [(y, 1), (parked, 0)])
+    return y
+
+
+def shapes():
+    """The number of shapes, from the source of one product."""
+    return ha.Int8Matmul(16, 16, "f32").source.count("//// shape\n")
+
+
+# tiles of every third size, streams of every one (k-th size, shape)
+PAIRS = [(k, shape) for shape in range(6) for k in range(len(SMALL)) if shape > 2 or (shape + k) % 3 == 0]
+
+
+@pytest.mark.parametrize("k,shape", PAIRS)
+def test_the_kernels_match_the_oracle(monkeypatch, k, shape):
+    tokens, columns, channels = SMALL[k]
+    dtype, shares = ("f32", "bf16", "f16")[k % 3], 1 + (k % 2) * (shape in (1, 2))
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
+    host = inputs(tokens, columns, channels, bias=k % 2, seed=k)
+    y = emulated(ha.Int8Matmul(columns, channels, dtype), host, dtype, shape, shares)
+    check(host, dtype, to_f32(y, dtype))
+
+
+@pytest.mark.parametrize("shape,tokens,columns,channels,shares", [(2, 70, 700, 130, 1), (2, 70, 1400, 70, 3), (1, 130, 400, 130, 1)])
+def test_several_tiles_and_rounds_of_the_ring(monkeypatch, shape, tokens, columns, channels, shares):
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
+    host = inputs(tokens, columns, channels, bias=True, seed=9)
+    y = emulated(ha.Int8Matmul(columns, channels, "f16"), host, "f16", shape, shares)
+    check(host, "f16", to_f32(y, "f16"))
+
+
+def test_the_oracles_product_is_exact():
+    host = inputs(2, 40, 3, True, 1)
+    want = [[sum(int(a) * int(b) for a, b in zip(x, w)) for w in host["weights"]] for x in host["x"]]
+    want = np.array(want) * host["x_scales"].astype(np.float64)[:, None] * host["weight_scales"].astype(np.float64) + host["bias"]
+    assert np.allclose(oracle.product(*[host[k] for k in FIELDS], host["bias"]), want, rtol=1e-14)
+
+
+def test_every_shape_has_a_launch_for_every_call():
+    assert shapes() == 6
+    for inputs_, channels in ((1, 1), (4096, 4096), (131071, 17), (512, 1 << 20)):
+        op = ha.Int8Matmul(inputs_, channels, "bf16")
+        for tokens in (1, 15, 16, 17, 64, 65, 200, 1000, 5000):
+            said = dict(re.findall(r"(\w+)=(\w+)", op.describe(tokens)))
+            assert int(said["grid"]) >= 1 and int(said["shares"]) >= 1
+            assert int(said["shares"]) == 1 or (int(said["grid"]) * int(said["shares"]) <= 512 and int(said["shares"]) <= -(-inputs_ // 128))
+
+
+@pytest.mark.parametrize("kwargs,says", [
+    (dict(inputs=0), "0 inputs"),
+    (dict(channels=-1), "-1 channels"),
+    (dict(inputs=1 << 17), "131071 are taken"),
+    (dict(channels=(1 << 24) + 1), "2.24 are taken"),
+    (dict(dtype="u32"), "dtype u32"),
+])
+def test_what_cannot_be_multiplied_is_refused(kwargs, says):
+    with pytest.raises(ha.HeliumError, match=says):
+        ha.Int8Matmul(**{**dict(inputs=64, channels=64, dtype="f32"), **kwargs})
+
+
+def test_operands_are_checked_before_any_launch():
+    op, good = ha.Int8Matmul(64, 32, "bf16"), 4096
+    fine = dict(tokens=2, x=good, x_scales=good, weights=good, weight_scales=good, y=good)
+    for given, says in ((dict(x=None), "tokens are null"), (dict(x=good + 8), "tokens are null or not aligned to 16"), (dict(weights=good + 4), "weights are null or not aligned to 16"),
+                        (dict(x_scales=None), "tokens' scales"), (dict(weight_scales=good + 2), "weights' scales"), (dict(y=good + 1), "result is null or not aligned to 2"),
+                        (dict(bias=good + 2), "bias is not aligned"), (dict(tokens=-1), "-1 tokens"), (dict(tokens=1 << 25), "at most 2.24")):
+        with pytest.raises(ha.HeliumError, match=says):
+            op.multiply(**{**fine, **given})
+    with pytest.raises(ha.HeliumError, match="too many for one launch"):
+        ha.Int8Matmul(64, 1 << 24, "bf16").multiply(**dict(fine, tokens=1 << 24))
+    op.multiply(0, None, None, None, None, None)
+    h = ctypes.c_void_p()
+    assert _ffi.lib.he_int8_matmul_create(None, 64, 64, _ffi.F32) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_int8_matmul(None, 1, *[None] * 7) == _ffi.ERR_INVALID
+    assert _ffi.lib.he_int8_matmul_describe(h, 1, None, 0) == _ffi.ERR_INVALID
+    with pytest.raises(ha.HeliumError):
+        op.describe(0)
+    assert _ffi.lib.he_int8_matmul_destroy(None) == _ffi.OK

@@ -66,8 +66,8 @@ def test_quantized_rows_are_the_oracles(gpu, shape, dtype):
     rows, columns = shape
     x = borders(rows, columns, dtype, columns)
     want, want_scales = oracle_int8.quantize(to_f32(x, dtype))
-    q, scales = empty((rows, pitch(columns)), np.int8), empty((rows,), np.float32)
-    ha.QuantizeRows(columns, dtype).quantize(rows, Array(x).at, q.at, scales.at)
+    d, q, scales = Array(x), empty((rows, pitch(columns)), np.int8), empty((rows,), np.float32)
+    ha.QuantizeRows(columns, dtype).quantize(rows, d.at, q.at, scales.at)
     got = q.back()
     assert np.array_equal(got[:, :columns], want) and not got[:, columns:].any()
     assert np.array_equal(scales.back(), want_scales, equal_nan=True)
@@ -91,7 +91,7 @@ def test_results_may_take_an_operands_place(gpu, shape, dtype):
     norm.backward(rows, d["dy"].at, d["h"].at, d["gamma"].at, d["rstd"].at, None, dgamma.at, dh=d["dh"].at, dresidual=d["dh"].at)
     assert np.array_equal(d["dh"].back(), apart[1]) and np.array_equal(dgamma.back(), apart[2])
     # nothing but this norm reads h
-    norm.backward(rows, Array(host["dy"]).at, d["h"].at, d["gamma"].at, d["rstd"].at, d["dy"].at, dgamma.at)
+    norm.backward(rows, d["dy"].at, d["h"].at, d["gamma"].at, d["rstd"].at, d["dy"].at, dgamma.at)
     alone = dict(v)
     del alone["dh"]
     check_backward(dtype, dtype, alone, to_f32(d["dy"].back(), dtype), None, dgamma.back(), -(-rows // 256))
