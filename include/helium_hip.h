@@ -581,6 +581,30 @@ const char* he_int8_matmul_source(he_int8_matmul_t matmul);
 int he_int8_matmul_describe(he_int8_matmul_t matmul, int64_t tokens, char* text, size_t capacity);
 int he_int8_matmul_destroy(he_int8_matmul_t matmul);
 
+/* ==================================================================================================
+ * 12. The norm of all gradients of a model together, and clipping: what a training step does between its gradients and the optimizer's
+ *     step (section 9, or Sgd, helium/src/optimizer/sgd.rs). No counterpart in the reference.
+ * ================================================================================================== */
+typedef struct he_gradient_clip_s* he_gradient_clip_t;
+/* `count` tensors (at most 65536) of sizes[k] values (0 or more) and type dtypes[k] (HE_F32, HE_BF16 or HE_F16), packed. Compiles the kernels;
+ * needs no device. */
+int he_gradient_clip_create(he_gradient_clip_t* clip, const int64_t* sizes, const int* dtypes, int count);
+/* norm[0] = sqrt(sum of the squares of all values), added up in 64 bits in a fixed order. A list of `count` device addresses in host memory,
+ * each aligned to its own type; that of a tensor without values may be NULL. The first call on a stream allocates workspace for it, later ones allocate
+ * nothing; calls on several streams may overlap. Captured graphs that may run at the same time are captured on streams of their own, or from
+ * handles of their own. */
+int he_gradient_norm(he_gradient_clip_t clip, const void* const* gradients, int count, float* norm, he_stream_t stream);
+/* out[k] = gradients[k] * min(1, most / (norm + 1e-6)), rounded once to its type, and the norm (before clipping) in norm[0], which may be NULL. out[k] may be
+ * gradients[k]; otherwise it shares no memory with any of them. most is 0 or more, infinity for no clipping. A norm that is NaN makes every result NaN, an infinite one
+ * zeros (NaN where a value is infinite): norm[0] tells. */
+int he_gradient_clip(he_gradient_clip_t clip, const void* const* gradients, void* const* out, int count, float most, float* norm,
+                     he_stream_t stream);
+/* The generated HIP source, how the tensors are cut, and the table the kernels read, for inspection and tests. */
+const char* he_gradient_clip_source(he_gradient_clip_t clip);
+const char* he_gradient_clip_describe(he_gradient_clip_t clip);
+int he_gradient_clip_table(he_gradient_clip_t clip, void* data, size_t capacity, size_t* bytes);
+int he_gradient_clip_destroy(he_gradient_clip_t clip);
+
 #ifdef __cplusplus
 }
 #endif
