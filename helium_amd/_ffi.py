@@ -3,6 +3,7 @@
 There is no fallback: if the library is missing, importing this module raises. The signatures below restate
 include/helium_hip.h; tests/test_abi.py checks that every function the header declares is exported.
 """
+import array
 import ctypes as C
 import os
 
@@ -52,6 +53,21 @@ def _sig(name, *argtypes, restype=C.c_int):
     fn.argtypes = list(argtypes)
     fn.restype = restype
     return fn
+
+
+def address(buffer):
+    """A raw address as it is, that of a DeviceBuffer or Tensor; None stays null."""
+    return buffer if type(buffer) is int or buffer is None else getattr(buffer, "ptr", buffer)
+
+
+def addresses(buffers):
+    """A list of device addresses for the C ABI, and its length (element by element through ctypes, 65 tensors took 20 us)."""
+    at = array.array("Q", [b if type(b) is int else _plain(address(b)) for b in buffers])
+    return (C.c_void_p * max(len(at), 1)).from_buffer(at or array.array("Q", [0])), len(at)
+
+
+def _plain(pointer):
+    return pointer if type(pointer) is int else 0 if pointer is None else pointer.value or 0
 
 
 # ---- device shim ---------------------------------------------------------------------------------------

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <future>
+#include <map>
 #include <sstream>
 
 #include "rms_norm.h"
@@ -14,7 +15,8 @@ namespace {
 // ---- device text ---------------------------------------------------------------------------------------------------
 // y[t][n] = (sum over k of x[t][k] w[n][k]) x_scale[t] w_scale[n] + bias[n]. The sums are whole numbers in 32 bits and exact (fewer than 2^17
 // products of at most 2^14), so that no cut of a sum changes a result. The definitions ahead of the text hold the type of the result (BF16, F16)
-// and the shape: of tiles TN, TM, WAVES_N, WAVES_M, STAGES; of streams BN, BM, WAVES.
+// and the shape: of tiles TN, TM, WAVES_N, WAVES_M, STAGES, AHEAD; of streams BN, BM, WAVES,
+// STEPS (of 64 bytes of k, on their way at a time, twice).
 //
 // Weights are the instruction's rows and tokens its columns: a lane then has four neighbouring channels of one token at a time.
 const char* kCommon = R"HIP(
@@ -48,9 +50,31 @@ struct Call {
     const float *x_scales, *w_scales, *bias;
     out_t* y;
     u32 tokens, channels, pitch;   // pitch: bytes of an operand's row
+    u32 blocks, shares;            // of one share; a share's sums wait in `parked`, rows of `parked_pitch` channels, for the launch that adds them up
+    u32 parked_pitch;
+    int* parked;
 };
+__device__ __forceinline__ i32x4* parked_at(const Call& c, u32 share, u32 m, u32 n) {
+    return (i32x4*)(c.parked + ((u64)share * c.tokens + m) * c.parked_pitch + n);
+}
 // One rounding of the sum to f32, one of each product, one of the bias' addition, and that to the result's type.
 __device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale) { return (float)sum * x_scale * w_scale; }
+typedef out_t out4_any __attribute__((ext_vector_type(4), aligned(sizeof(out_t))));
+__device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 sum) {
+    const float x_scale = c.x_scales[m];
+    out_t* to = c.y + (u64)m * c.channels + n;
+    out4_any out;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const u32 of = n + k < c.channels ? n + k : c.channels - 1;
+        out[k] = (out_t)(scaled(sum[k], x_scale, c.w_scales[of]) + (c.bias ? c.bias[of] : 0.0f));
+    }
+    if (n + 4 <= c.channels) *(out4_any*)to = out;
+    else
+#pragma unroll
+        for (u32 k = 0; k < 4; k++)
+            if (n + k < c.channels) to[k] = out[k];
+}
 )HIP";
 
 // Tiles. Rows of 128 bytes of k go from memory straight into a ring of STAGES k-tiles in LDS and from there, 16 bytes to a lane, into the
@@ -75,8 +99,8 @@ const char* kTile = R"HIP(
 __device__ __attribute__((aligned(16))) const u32 nothing[4] = {0, 0, 0, 0};   // what lies behind a row's end
 
 struct Fragments { i32x4 w[NB], x[MB]; };
-struct True { constexpr operator bool() const { return true; } };
-struct False { constexpr operator bool() const { return false; } };
+struct True { static constexpr int value = 1; constexpr operator bool() const { return true; } };
+struct False { static constexpr int value = 0; constexpr operator bool() const { return false; } };
 
 // What a wave stores of its sums: 32 tokens at a time through its strip, so that whole vectors of channels go out.
 __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Call& c, u32 n0, u32 m0, const float* w_scales, const float* bias, out_t* strip) {
@@ -128,24 +152,24 @@ __device__ __forceinline__ void load_channels(const Call& c, u32 n0, float* w_sc
 }
 // Which tile a block makes. Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: an XCD takes neighbours, in groups of
 // four rows of tiles, whose weights and tokens they share.
-__device__ __forceinline__ void place(const Call& c, u32 blocks, u32& tn, u32& tm) {
+__device__ __forceinline__ void place(const Call& c, u32& tn, u32& tm) {
     const u32 tiles_n = (c.channels + TN - 1) / TN, tiles_m = (c.tokens + TM - 1) / TM, xcd = blockIdx.x % 8u;
-    const u32 t = xcd * (blocks / 8u) + (xcd < blocks % 8u ? xcd : blocks % 8u) + blockIdx.x / 8u;
+    const u32 t = xcd * (c.blocks / 8u) + (xcd < c.blocks % 8u ? xcd : c.blocks % 8u) + blockIdx.x / 8u;
     const u32 group = t / (4 * tiles_n), in = t % (4 * tiles_n), high = tiles_m - group * 4 < 4 ? tiles_m - group * 4 : 4;
     tm = group * 4 + in % high;
     tn = in / high;
 }
 
-extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS void int8_product(Call c, u32 blocks, u32 shares, i32x4* __restrict__ parked) {
+extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS void int8_product(Call c) {
     __shared__ __attribute__((aligned(16))) u8 lds[LDS_BYTES];
     __shared__ __attribute__((aligned(16))) float w_scales[TN], bias[TN];
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_n = wave / WAVES_M, wave_m = wave % WAVES_M;
     u32 tn, tm;
-    place(c, blocks, tn, tm);
+    place(c, tn, tm);
     const u32 n0 = tn * TN, m0 = tm * TM;
     const u8 *w_rows = c.w + (u64)n0 * c.pitch, *x_rows = c.x + (u64)m0 * c.pitch;
     const u32 k_tiles = (c.pitch + ROW - 1) / ROW, chunks = c.pitch / 16;
-    const u32 k_begin = (u32)((u64)k_tiles * blockIdx.y / shares), k_end = (u32)((u64)k_tiles * (blockIdx.y + 1) / shares);
+    const u32 k_begin = (u32)((u64)k_tiles * blockIdx.y / c.shares), k_end = (u32)((u64)k_tiles * (blockIdx.y + 1) / c.shares);
     // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads meet different banks, the chunk
     // (l % 8) ^ (row / 2 % 8) of its 128 bytes: two rows fill the 64 banks, so rows two apart must differ. (A tile that ends beyond an
     // operand loads its last row there: sums that nothing stores.)
@@ -175,11 +199,6 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
     const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane >> 1 & 7u;
-    Fragments f[2];
-#pragma unroll
-    for (int i = 0; i < NB; i++) f[1].w[i] = i32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < MB; j++) f[1].x[j] = i32x4{0, 0, 0, 0};
     auto read = [&](Fragments& g, const u8* stage, int kk) {
         const u8 *w = stage + (wave_n * WTN + frag_row) * ROW, *x = stage + (TN + wave_m * WTM + frag_row) * ROW;
         const u32 at = ((kk * 2 + half) ^ swz) * 16;
@@ -194,22 +213,39 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 #pragma unroll
             for (int j = 0; j < MB; j++) acc[i][j] = MFMA_32(g.w[i], g.x[j], acc[i][j]);
     };
-    // One k-tile. The loop is rotated by a k-step: the matrix instructions that the last k-tile left over cover the barrier's way, the
-    // first reads of this one and the loads of the one to come; each further step's reads are issued between the instructions of
-    // the step before. The order is asked for, since the compiler by itself reads, waits and multiplies in turn.
     u32 slot = 0;
-    auto k_tile = [&](u32 kt, auto more) {
-        // this wave's loads of the k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'
+    // This wave's loads of a k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'. No wave still reads the
+    // stage that is filled next. (The bare barrier: __syncthreads() would wait for all loads.)
+    auto meet = [&](auto more) {
         if (more) __builtin_amdgcn_s_waitcnt(WAIT_LOADS((STAGES - 2) * LOADS));
         else __builtin_amdgcn_s_waitcnt(WAIT_LOADS(0));
-        // (the bare barrier: __syncthreads() would wait for all loads; no wave still reads the stage that is filled next)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto fetch_ahead = [&](u32 kt) { fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1); };
+    const u32 k_count = k_end - k_begin, ahead = STAGES - 1 < k_count ? STAGES - 1 : k_count;
+    load_channels(c, n0, w_scales, bias);
+    for (u32 s = 0; s < ahead; s++) fetch(k_begin + s, s);
+    u32 kt = k_begin;
+    Fragments f[2][AHEAD];
+#pragma unroll
+    for (int s = 0; s < AHEAD; s++) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) f[1][s].w[i] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < MB; j++) f[1][s].x[j] = i32x4{0, 0, 0, 0};
+    }
+#if AHEAD == 1
+    // The loop is rotated by a k-step: the matrix instructions that the last k-tile left over cover the barrier's way, the
+    // first reads of this one and the loads of the one to come; each further step's reads are issued between the instructions of
+    // the step before. The order is asked for, since the compiler by itself reads, waits and multiplies in turn.
+    auto k_tile = [&](u32 kt, auto more) {
+        meet(more);
         const u8* stage = lds + slot * STAGE_BYTES;
-        read(f[0], stage, 0);
-        if (more) fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1);
-        multiply(f[1]);
+        read(f[0][0], stage, 0);
+        if (more) fetch_ahead(kt);
+        multiply(f[1][0]);
         __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
         for (int n = 0; n < MMAS; n++) {
@@ -220,8 +256,8 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
         }
 #pragma unroll
         for (int kk = 1; kk < 4; kk++) {
-            read(f[kk & 1], stage, kk);
-            multiply(f[(kk & 1) ^ 1]);
+            read(f[kk & 1][0], stage, kk);
+            multiply(f[(kk & 1) ^ 1][0]);
 #pragma unroll
             for (int n = 0; n < MMAS; n++) {
                 // (reads behind the first instruction: the wait for its operands is for all reads before it)
@@ -232,76 +268,73 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
         }
         slot = slot + 1 < STAGES ? slot + 1 : 0;
     };
-    const u32 k_count = k_end - k_begin, ahead = STAGES - 1 < k_count ? STAGES - 1 : k_count;
-    load_channels(c, n0, w_scales, bias);
-    for (u32 s = 0; s < ahead; s++) fetch(k_begin + s, s);
-    u32 kt = k_begin;
     for (; kt + ahead < k_end; kt++) k_tile(kt, True());
     for (; kt < k_end; kt++) k_tile(kt, False());
-    multiply(f[1]);
+    multiply(f[1][0]);
+#else
+    // A wave of a small tile has few matrix instructions to a k-step, fewer than an LDS read takes to come: the loop is rotated by a whole
+    // k-tile, whose instructions cover the barrier and all reads of the next one.
+    auto k_tile = [&](u32 kt, auto more, auto odd) {
+        constexpr int now = decltype(odd)::value;
+        meet(more);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) read(f[now][kk], lds + slot * STAGE_BYTES, kk);
+        if (more) fetch_ahead(kt);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) multiply(f[now ^ 1][kk]);
+        slot = slot + 1 < STAGES ? slot + 1 : 0;
+        // (all reads and loads first)
+        __builtin_amdgcn_sched_group_barrier(0x100, 4 * READS, 0);
+        if (more) __builtin_amdgcn_sched_group_barrier(0x020, LOADS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 4 * MMAS, 0);
+    };
+    auto either = [&](u32 kt, auto more) {
+        if ((kt - k_begin) & 1) k_tile(kt, more, True());
+        else k_tile(kt, more, False());
+    };
+    for (; kt + ahead + 1 < k_end; kt += 2) {
+        k_tile(kt, True(), False());
+        k_tile(kt + 1, True(), True());
+    }
+    for (; kt + ahead < k_end; kt++) either(kt, True());
+    for (; kt < k_end; kt++) either(kt, False());
+    if (k_count & 1)
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) multiply(f[0][kk]);
+    else
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) multiply(f[1][kk]);
+#endif
 
-    // A share of a tile's sum waits in memory for the launch that adds them up, block by block of 32 x 32, as the lanes hold it.
-    if (SHARED && shares > 1) {
-        i32x4* to = parked + ((u64)(tm * ((c.channels + TN - 1) / TN) + tn) * shares + blockIdx.y) * (TN * TM / 4);
+    if (c.shares > 1) {
 #pragma unroll
-        for (int i = 0; i < NB; i++)
+        for (int j = 0; j < MB; j++) {
+            const u32 m = m0 + wave_m * WTM + j * 32 + frag_row;
 #pragma unroll
-            for (int j = 0; j < MB; j++)
+            for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const i32x4 four = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-                    to[((wave * NB + i) * MB + j) * 256 + e * 64 + lane] = four;
+                    const u32 n = n0 + wave_n * WTN + i * 32 + e * 8 + half * 4;
+                    if (m < c.tokens && n < c.parked_pitch) *parked_at(c, blockIdx.y, m, n) = i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
                 }
+        }
         return;
     }
     __syncthreads();   // the operand stages become the waves' strips
     store_sums(acc, c, n0 + wave_n * WTN, m0 + wave_m * WTM, w_scales + wave_n * WTN, bias + wave_n * WTN, (out_t*)lds + wave * STRIP_VALUES);
 }
 
-#if SHARED
-// The shares of a tile added up. A workgroup takes a tile as `int8_product` does.
-extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) void int8_join(Call c, u32 blocks, u32 shares, const i32x4* __restrict__ parked) {
-    __shared__ __attribute__((aligned(16))) out_t strips[STRIP_VALUES * WAVES_N * WAVES_M];
-    __shared__ __attribute__((aligned(16))) float w_scales[TN], bias[TN];
-    const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wave_n = wave / WAVES_M, wave_m = wave % WAVES_M;
-    const u32 tiles_n = (c.channels + TN - 1) / TN, n0 = blockIdx.x % tiles_n * TN, m0 = blockIdx.x / tiles_n * TM;
-    load_channels(c, n0, w_scales, bias);
-    i32x16 acc[NB][MB];
-#pragma unroll
-    for (int i = 0; i < NB; i++)
-#pragma unroll
-        for (int j = 0; j < MB; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-    for (u32 s = 0; s < shares; s++) {
-        const i32x4* from = parked + ((u64)blockIdx.x * shares + s) * (TN * TM / 4);
-#pragma unroll
-        for (int i = 0; i < NB; i++)
-#pragma unroll
-            for (int j = 0; j < MB; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const i32x4 four = from[((wave * NB + i) * MB + j) * 256 + e * 64 + lane];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) acc[i][j][4 * e + k] += four[k];
-                }
-    }
-    __syncthreads();
-    store_sums(acc, c, n0 + wave_n * WTN, m0 + wave_m * WTM, w_scales + wave_n * WTN, bias + wave_n * WTN, strips + wave * STRIP_VALUES);
-}
-#endif
 )HIP";
 
 // Streams. Reading the weights once is nearly all there is to do for few tokens, so they go straight into registers, as many loads on their way as
 // there is room for; the tokens come out of the L2. The matrix instructions (16 x 16 x 64) are far from being a bound.
 const char* kStream = R"HIP(
-#define STEPS 4   // of 64 bytes of k, on their way at a time
 extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     __shared__ __attribute__((aligned(16))) int sums[WAVES][BM * 16][BN * 16 + 4];
     const u32 lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tiles_n = (c.channels + BN * 16 - 1) / (BN * 16);
     const u32 n0 = blockIdx.x % tiles_n * (BN * 16), m0 = blockIdx.x / tiles_n * (BM * 16);
-    const u32 chunks = c.pitch / 16, steps = (c.pitch + 63) / 64;
-    const u32 begin = (u32)((u64)steps * wave / WAVES), end = (u32)((u64)steps * (wave + 1) / WAVES);
+    // (the waves take turns along k, STEPS steps each: together they read long pieces of a row)
+    const u32 chunks = c.pitch / 16, groups = (c.pitch + 64 * STEPS - 1) / (64 * STEPS), part = blockIdx.y * WAVES + wave, parts = c.shares * WAVES;
     const u8 *w[BN], *x[BM];
 #pragma unroll
     for (int i = 0; i < BN; i++) {
@@ -318,104 +351,192 @@ extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     for (int i = 0; i < BN; i++)
 #pragma unroll
         for (int j = 0; j < BM; j++) acc[i][j] = i32x4{0, 0, 0, 0};
-    for (u32 s = begin; s < end; s += STEPS) {
-        i32x4 fw[STEPS][BN], fx[STEPS][BM];
+    struct Operands { i32x4 w[STEPS][BN], x[STEPS][BM]; } f[2];
+    auto load = [&](Operands& o, u32 group) {
 #pragma unroll
         for (int d = 0; d < STEPS; d++) {
-            const u32 chunk = (s + d) * 4 + (lane >> 4);
-            const bool there = s + d < end && chunk < chunks;
+            const u32 chunk = (group * STEPS + d) * 4 + (lane >> 4);
+            const bool there = chunk < chunks;
 #pragma unroll
             for (int i = 0; i < BN; i++) {
-                fw[d][i] = i32x4{0, 0, 0, 0};
-                if (there) fw[d][i] = *(const i32x4*)(w[i] + chunk * 16);
+                o.w[d][i] = i32x4{0, 0, 0, 0};
+                if (there) o.w[d][i] = *(const i32x4*)(w[i] + chunk * 16);
             }
 #pragma unroll
             for (int j = 0; j < BM; j++) {
-                fx[d][j] = i32x4{0, 0, 0, 0};
-                if (there) fx[d][j] = *(const i32x4*)(x[j] + chunk * 16);
+                o.x[d][j] = i32x4{0, 0, 0, 0};
+                if (there) o.x[d][j] = *(const i32x4*)(x[j] + chunk * 16);
             }
         }
+    };
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
         for (int d = 0; d < STEPS; d++)
 #pragma unroll
             for (int i = 0; i < BN; i++)
 #pragma unroll
-                for (int j = 0; j < BM; j++) acc[i][j] = MFMA_16(fw[d][i], fx[d][j], acc[i][j]);
+                for (int j = 0; j < BM; j++) acc[i][j] = MFMA_16(o.w[d][i], o.x[d][j], acc[i][j]);
+    };
+    // (two groups on their way; what is behind the rows' end is zeros)
+    load(f[0], part);
+    for (u32 g = part; g < groups; g += 2 * parts) {
+        load(f[1], g + parts);
+        multiply(f[0]);
+        load(f[0], g + 2 * parts);
+        multiply(f[1]);
     }
 #pragma unroll
     for (int i = 0; i < BN; i++)
 #pragma unroll
         for (int j = 0; j < BM; j++) *(i32x4*)&sums[wave][j * 16 + (lane & 15u)][i * 16 + (lane >> 4) * 4] = acc[i][j];
     __syncthreads();
-    for (u32 e = threadIdx.x; e < BM * 16 * BN * 16; e += WAVES * 64) {
-        const u32 j = e / (BN * 16), i = e % (BN * 16), m = m0 + j, n = n0 + i;
+    // (four channels to a thread)
+    for (u32 e = threadIdx.x; e < BM * 16 * BN * 4; e += WAVES * 64) {
+        const u32 j = e / (BN * 4), i = e % (BN * 4) * 4, m = m0 + j, n = n0 + i;
         if (m >= c.tokens || n >= c.channels) continue;
-        int sum = 0;
+        i32x4 sum = *(const i32x4*)&sums[0][j][i];
 #pragma unroll
-        for (int v = 0; v < WAVES; v++) sum += sums[v][j][i];
-        c.y[(u64)m * c.channels + n] = (out_t)(scaled(sum, c.x_scales[m], c.w_scales[n]) + (c.bias ? c.bias[n] : 0.0f));
+        for (int v = 1; v < WAVES; v++) sum += *(const i32x4*)&sums[v][j][i];
+        if (c.shares > 1) *parked_at(c, blockIdx.y, m, n) = sum;
+        else store_four(c, m, n, sum);
     }
+}
+)HIP";
+
+// The shares of a call's sums added up: four channels of a token to a thread.
+const char* kJoin = R"HIP(
+extern "C" __global__ __launch_bounds__(256) void int8_join(Call c) {
+    const u32 fours = (c.channels + 3) / 4;
+    const u64 at = (u64)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (u64)c.tokens * fours) return;
+    const u32 m = (u32)(at / fours), n = (u32)(at % fours) * 4;
+    i32x4 sum = *parked_at(c, 0, m, n);
+#pragma unroll 4
+    for (u32 s = 1; s < c.shares; s++) sum += *parked_at(c, s, m, n);
+    store_four(c, m, n, sum);
 }
 )HIP";
 
 constexpr uint64_t kThreads = 1ull << 32;  // a launch has fewer
 constexpr uint64_t kCUs = 256;
-// Workgroups that park a share of a sum, at most: the scratch has room for so many of the largest tile that is shared out.
-constexpr uint64_t kMostParked = 2 * kCUs;
+constexpr uint64_t kMostParked = 1 << 22;  // sums of all shares together, for which the scratch has room
 
+// What the choice goes by (cut_of below), from products of 1 to 8192 tokens: microseconds of a call, of a k-tile in a workgroup that has a CU to itself and
+// on full CUs, and of beginning and ending a workgroup there. The small tiles, whose waves
+// have few matrix instructions to a k-step, read a whole k-tile ahead: 1024 x 4096 x 4096 28.1 -> 25.9 us with 64 x 128 (128 x 128 24.6), 512 tokens
+// 22.6 -> 17.9, 2048 x 1024 x 1024 7.4 -> 6.8. Of 256 x 256 four waves along the channels read less from LDS than two: 66.4 -> 64.
 const Int8Shape kShapes[] = {
-    {false, 256, 256, 2, 4, 2, 1, 0, 0, 0},
-    {false, 128, 128, 2, 2, 2, 2, 0, 0, 0},
-    {false, 64, 64, 2, 2, 4, 2, 0, 0, 0},
-    {true, 0, 0, 0, 0, 0, 1, 1, 1, 8},
-    {true, 0, 0, 0, 0, 0, 1, 1, 2, 8},
-    {true, 0, 0, 0, 0, 0, 1, 2, 4, 8},
+    {256, 256, 4, 2, 2, 1, 1, 9.0, 1.24, 1.76, 6.5},
+    {128, 128, 2, 4, 4, 1, 4, 5.2, 0.46, 0.61, 3.3},
+    {64, 128, 2, 2, 3, 2, 4, 3.6, 0.42, 0.60, 3.2},
+    {64, 64, 2, 2, 3, 3, 4, 3.5, 0.33, 0.43, 2.0},
+    {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 1, 8, 4},
+    {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 2, 8, 4},
+    {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 3, 8, 2},
+    {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 4, 16, 1},
+    {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 2, 4, 16, 1},
 };
 constexpr int kCount = sizeof(kShapes) / sizeof(kShapes[0]);
 
-std::string definitions(const Int8Problem& pr, const Int8Shape& t) {
+std::string definitions(int dtype, const Int8Shape* t) {
     std::ostringstream s;
-    s << "#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16);
-    if (t.stream) s << "\n#define BN " << t.blocks_n << "\n#define BM " << t.blocks_m << "\n#define WAVES " << t.waves << "\n";
-    else
-        s << "\n#define TN " << t.tile_n << "\n#define TM " << t.tile_m << "\n#define WAVES_N " << t.waves_n << "\n#define WAVES_M " << t.waves_m
-          << "\n#define STAGES " << t.stages << "\n#define SHARED " << t.can_share() << "\n#ifndef KERNEL_ATTRS\n#define KERNEL_ATTRS __attribute__((amdgpu_waves_per_eu(" << t.waves_n * t.waves_m * t.per_cu / 4 << ", "
-          << t.waves_n * t.waves_m * t.per_cu / 4 << ")))\n#endif\n";
+    s << "#define BF16 " << (dtype == HE_BF16) << "\n#define F16 " << (dtype == HE_F16) << "\n";
+    if (t && t->stream()) s << "#define BN " << t->blocks_n << "\n#define BM " << t->blocks_m << "\n#define WAVES " << t->waves << "\n#define STEPS " << t->steps << "\n";
+    else if (t)
+        s << "#define TN " << t->tile_n << "\n#define TM " << t->tile_m << "\n#define WAVES_N " << t->waves_n << "\n#define WAVES_M " << t->waves_m
+          << "\n#define STAGES " << t->stages << "\n#define AHEAD " << t->ahead << "\n#ifndef KERNEL_ATTRS\n#define KERNEL_ATTRS __attribute__((amdgpu_waves_per_eu("
+          << t->waves_n * t->waves_m * t->per_cu / 4 << ", " << t->waves_n * t->waves_m * t->per_cu / 4 << ")))\n#endif\n";
     return s.str();
 }
 
 uint64_t cut(int64_t extent, int by) { return ((uint64_t)extent + by - 1) / by; }
+int64_t parked_pitch(const Int8Problem& pr) { return (int64_t)cut(pr.channels, 4) * 4; }
+
+// How long a call would take, in microseconds. Streams: a CU reads 36 KB in one, of weights and tokens alike, the weights come out of memory at 6 TB/s at
+// best, and a workgroup that follows another on its CU takes a while to begin and end. Shares cost a second launch.
+Int8Cut cut_of(const Int8Problem& pr, int64_t tokens, int shape, uint32_t shares) {
+    const Int8Shape& t = kShapes[shape];
+    Int8Cut c;
+    c.shape = shape, c.shares = shares, c.blocks = cut(pr.channels, t.channels()) * cut(tokens, t.tokens());
+    const double pitch = (double)quantized_pitch(pr.inputs), blocks = (double)c.blocks * shares;
+    c.estimate = shares > 1 ? 2.2 + (double)shares * tokens * pr.channels * 4 / 3e6 : 0;
+    if (t.stream()) {
+        const double sums = t.blocks_n * t.blocks_m, rows = 16.0 * t.blocks_n + std::min<double>(16.0 * t.blocks_m, (double)tokens);
+        // (sums of four blocks and more fill a CU's LDS with one workgroup)
+        const double rounds = sums >= 4 && blocks < 4 * kCUs ? std::ceil(blocks / kCUs) : std::max(1.0, blocks / kCUs);
+        c.estimate += 2.5 + 0.08 * sums + std::max(rounds * rows * pitch / shares / 36e3, pr.channels * pitch / 6e6) + (rounds - 1) * (0.2 + 0.02 * t.waves * sums);
+        return c;
+    }
+    const double k_tiles = std::ceil(pitch / 128 / shares), slots = (double)kCUs * t.per_cu, rounds = blocks < 4 * slots ? std::ceil(blocks / slots) : blocks / slots;
+    const bool alone = t.per_cu > 1 ? blocks <= kCUs : blocks <= kCUs / 2;
+    c.estimate += t.base + (alone ? k_tiles * t.alone : rounds * (k_tiles * t.full + t.round) - (t.per_cu > 1 ? 0 : t.round));
+    return c;
+}
 
 struct CallArg {
     const void *x, *w;
     const float *x_scales, *w_scales, *bias;
     void* y;
-    uint32_t tokens, channels, pitch;
+    uint32_t tokens, channels, pitch, blocks, shares, parked_pitch;
+    int32_t* parked;
 };
 
 }  // namespace
 
-std::string Int8Cut::describe(const Int8Problem& pr) const {
+struct Int8Kernels {
+    std::string source;
+    std::unique_ptr<JitKernel> product[kCount], join;
+
+    explicit Int8Kernels(int dtype) {
+        std::vector<std::string> texts(kCount);
+        const std::string joining = definitions(dtype, nullptr) + kCommon + kJoin;
+        std::vector<std::future<void>> compiled;
+        for (int k = 0; k < kCount; k++) {
+            texts[k] = definitions(dtype, &kShapes[k]) + kCommon + (kShapes[k].stream() ? kStream : kTile);
+            compiled.push_back(std::async(std::launch::async, [&texts, k] { (void)rtc_compile(texts[k], "int8_product", {}); }));
+            source += "//// shape\n" + texts[k];
+        }
+        for (auto& f : compiled) f.get();
+        for (int k = 0; k < kCount; k++) product[k] = std::make_unique<JitKernel>(texts[k], kShapes[k].stream() ? "int8_stream" : "int8_product");
+        join = std::make_unique<JitKernel>(joining, "int8_join");
+        source += "//// shape\n" + joining;
+    }
+
+    static std::shared_ptr<Int8Kernels> of(int dtype) {
+        static std::mutex mu;
+        static std::map<int, std::weak_ptr<Int8Kernels>> made;
+        std::lock_guard<std::mutex> lk(mu);
+        std::shared_ptr<Int8Kernels> k = made[dtype].lock();
+        if (!k) made[dtype] = k = std::make_shared<Int8Kernels>(dtype);
+        return k;
+    }
+};
+
+std::string Int8Cut::describe() const {
     const Int8Shape& t = kShapes[shape];
-    if (t.stream) return strfmt("int8 stream shape=%d blocks_n=%d blocks_m=%d waves=%d threads=%d grid=%llu shares=1", shape, t.blocks_n, t.blocks_m, t.waves, t.threads(), (unsigned long long)blocks);
-    return strfmt("int8 tiles shape=%d tile=%dx%d waves=%dx%d stages=%d threads=%d grid=%llu shares=%u", shape, t.tile_n, t.tile_m, t.waves_n, t.waves_m, t.stages, t.threads(),
-                  (unsigned long long)blocks, shares);
+    const std::string how = t.stream() ? strfmt("int8 stream shape=%d blocks_n=%d blocks_m=%d waves=%d", shape, t.blocks_n, t.blocks_m, t.waves)
+                                       : strfmt("int8 tiles shape=%d tile=%dx%d waves=%dx%d stages=%d", shape, t.tile_n, t.tile_m, t.waves_n, t.waves_m, t.stages);
+    return how + strfmt(" threads=%d grid=%llu shares=%u estimate=%.1f", t.threads(), (unsigned long long)blocks, shares, estimate);
 }
 
+// Of all shapes and numbers of shares the one with the least estimate. A share is at least four k-tiles long, or what a stream's waves need to have four
+// steps of it each.
 Int8Cut plan_int8(const Int8Problem& pr, int64_t tokens) {
-    Int8Cut c;
-    const uint64_t big = cut(pr.channels, 256) * cut(tokens, 256), middle = cut(pr.channels, 128) * cut(tokens, 128);
-    c.shape = tokens <= 16 ? 3 : tokens <= 32 ? 4 : tokens <= 64 ? 5 : big >= 200 ? 0 : middle >= 256 ? 1 : 2;
-    if (const int forced = tuning::get_int("HELIUM_HIP_INT8_SHAPE", 0)) c.shape = std::min(forced, kCount) - 1;
-    const Int8Shape& t = kShapes[c.shape];
-    c.blocks = cut(pr.channels, t.channels()) * cut(tokens, t.tokens());
-    const uint64_t k_tiles = cut(quantized_pitch(pr.inputs), 128);
-    if (const int forced = tuning::get_int("HELIUM_HIP_INT8_SHARES", 0)) {
-        c.shares = (uint32_t)std::min<uint64_t>(forced, k_tiles);
+    const int forced = tuning::get_int("HELIUM_HIP_INT8_SHAPE", 0), forced_shares = tuning::get_int("HELIUM_HIP_INT8_SHARES", 0);
+    Int8Cut best = cut_of(pr, tokens, forced ? std::min(forced, kCount) - 1 : 0, 1);
+    if (forced_shares) best.estimate = 1e30;
+    for (int k = 0; k < kCount; k++) {
+        const Int8Shape& t = kShapes[k];
+        if (forced ? k != std::min(forced, kCount) - 1 : t.stream() && t.blocks_m != (int)std::min<uint64_t>(4, cut(tokens, 16))) continue;
+        const uint64_t least = t.stream() ? (uint64_t)t.waves * 256 : 512;  // bytes of k
+        for (uint32_t shares = 1; shares <= 16; shares *= 2) {
+            if (shares > 1 && ((uint64_t)shares * tokens * parked_pitch(pr) > kMostParked || (uint64_t)quantized_pitch(pr.inputs) < least * shares)) break;
+            if (forced_shares && shares != (uint32_t)forced_shares) continue;
+            const Int8Cut c = cut_of(pr, tokens, k, shares);
+            if (c.estimate < best.estimate) best = c;
+        }
     }
-    if (!t.can_share()) c.shares = 1;
-    while (c.shares > 1 && c.blocks * c.shares > kMostParked) c.shares--;
-    return c;
+    return best;
 }
 
 Int8Matmul::Int8Matmul(const Int8Problem& pr) : pr_(pr) {
@@ -424,24 +545,12 @@ Int8Matmul::Int8Matmul(const Int8Problem& pr) : pr_(pr) {
     HE_REQUIRE(pr.inputs < (1 << 17) && pr.channels <= (1 << 24), HE_ERR_UNSUPPORTED, "int8 product: %lld inputs (131071 are taken), %lld channels (2^24 are taken)",
                (long long)pr.inputs, (long long)pr.channels);
     HE_REQUIRE(pr.dtype == HE_F16 || pr.dtype == HE_BF16 || pr.dtype == HE_F32, HE_ERR_INVALID, "int8 product does not give dtype %s", dtype_name(pr.dtype));
-    std::vector<std::string> texts(kCount);
-    std::vector<std::future<void>> compiled;
-    for (int k = 0; k < kCount; k++) {
-        const Int8Shape& t = kShapes[k];
-        texts[k] = definitions(pr, t) + kCommon + (t.stream ? kStream : kTile);
-        compiled.push_back(std::async(std::launch::async, [&texts, k] { (void)rtc_compile(texts[k], "int8_product", {}); }));
-        source_ += "//// shape\n" + texts[k];
-    }
-    for (auto& f : compiled) f.get();
-    for (int k = 0; k < kCount; k++) {
-        Kernels made;
-        made.product = std::make_unique<JitKernel>(texts[k], kShapes[k].stream ? "int8_stream" : "int8_product");
-        if (kShapes[k].can_share()) made.join = std::make_unique<JitKernel>(texts[k], "int8_join");
-        kernels_.push_back(std::move(made));
-    }
+    kernels_ = Int8Kernels::of(pr.dtype);
 }
 
 Int8Matmul::~Int8Matmul() { scratch_.release(); }
+
+const std::string& Int8Matmul::source() const { return kernels_->source; }
 
 void Int8Matmul::multiply(int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales, const float* bias, void* y,
                           hipStream_t stream) {
@@ -461,21 +570,19 @@ void Int8Matmul::multiply(int64_t tokens, const void* x, const float* x_scales, 
     const Int8Shape& t = kShapes[c.shape];
     HE_REQUIRE(c.blocks < kThreads / t.threads(), HE_ERR_UNSUPPORTED, "int8 product: %lld tokens of %lld channels are too many for one launch", (long long)tokens,
                (long long)pr_.channels);
-    CallArg call{x, weights, x_scales, weight_scales, bias, y, (uint32_t)tokens, (uint32_t)pr_.channels, (uint32_t)quantized_pitch(pr_.inputs)};
-    uint32_t blocks = (uint32_t)c.blocks, shares = c.shares;
-    const uint32_t grid[3] = {blocks, shares, 1}, block[3] = {(uint32_t)t.threads(), 1, 1}, join_grid[3] = {blocks, 1, 1};
-    Kernels& k = kernels_[c.shape];
-    if (shares == 1) {
-        void* parked = nullptr;
-        void* args[] = {&call, &blocks, &shares, &parked};
-        k.product->launch(grid, block, 0, stream, args, true);
+    CallArg call{x, weights, x_scales, weight_scales, bias, y, (uint32_t)tokens, (uint32_t)pr_.channels, (uint32_t)quantized_pitch(pr_.inputs), (uint32_t)c.blocks, c.shares,
+                 (uint32_t)parked_pitch(pr_), nullptr};
+    const uint32_t grid[3] = {(uint32_t)c.blocks, c.shares, 1}, block[3] = {(uint32_t)t.threads(), 1, 1};
+    void* args[] = {&call};
+    if (c.shares == 1) {
+        kernels_->product[c.shape]->launch(grid, block, 0, stream, args, true);
         return;
     }
+    const uint32_t join_grid[3] = {(uint32_t)cut(tokens * (int64_t)cut(pr_.channels, 4), 256), 1, 1}, join_block[3] = {256, 1, 1};
     std::lock_guard<std::mutex> lk(mu_);
-    float* parked = scratch_.get(kMostParked * Int8Shape::kSharedTile, 0, stream).floats;
-    void* args[] = {&call, &blocks, &shares, &parked};
-    k.product->launch(grid, block, 0, stream, args);
-    k.join->launch(join_grid, block, 0, stream, args, true);
+    call.parked = (int32_t*)scratch_.get(kMostParked, 0, stream).floats;
+    kernels_->product[c.shape]->launch(grid, block, 0, stream, args);
+    kernels_->join->launch(join_grid, join_block, 0, stream, args, true);
 }
 
 }  // namespace he

@@ -12,7 +12,7 @@ namespace {
 // ---- device text ---------------------------------------------------------------------------------------------------
 // One text for all kernels; the definitions ahead of it hold the problem and the tiling:
 //   C (columns), V, NV, L (lanes of a row), T (threads), BF16 / F16, STREAM_SAME (h has x's type, otherwise f32), PARAM_SAME, RESIDUAL,
-//   TO_I8, NORM, PITCH, EPS, X_ALIGN, H_ALIGN, Y_ALIGN (what rows are aligned to, in bytes), STREAM_OUT
+//   TO_I8, PITCH, EPS, X_ALIGN, H_ALIGN (what vectors are aligned to, in bytes)
 //
 // A row of C values is cut into vectors of V; where V does not divide C the last of them begins at C - V and shares values with the one
 // before it (both make the same results of those; sums leave them out once).
@@ -97,41 +97,40 @@ template <bool SUM, bool MOST> __device__ __forceinline__ void over_row(float& s
     }
 #endif
 }
-#if STREAM_OUT
 #define STORE(p, v) __builtin_nontemporal_store(v, p)
-#else
-#define STORE(p, v) (*(p) = (v))
-#endif
+)HIP";
+
+// 8 bits. Adding 1.5 * 2^23 to a value within +-2^22 rounds it to a whole number, which the sum's last bits are (1.5 * 2^52 in 64 bits).
+// A row that is not finite throughout has no scale: NaN, and zeros.
+const char* kBytes = R"HIP(
+#define WHOLE_BITS(t) bits_of((t) + 12582912.0f)
+struct Steps { float up, size; bool finite; };   // values times `up`, a power of two, have `size` for their largest: 127 / size and its remainder are in range
+__device__ __forceinline__ Steps steps_of(u32 most) {
+    const float size = of_bits(most), up = size < 0x1p-64f ? 0x1p64f : size > 0x1p64f ? 0x1p-64f : 1.0f;
+    return {up, size * up, most < 0x7f800000u};
+}
+__device__ __forceinline__ void store_bytes(u8* row, u32 c, const u32 (&whole)[V], bool finite) {
+    byte_v out;
+#pragma unroll
+    for (int i = 0; i < V; i++) AT(out, i) = (u8)(finite ? whole[i] : 0u);
+    *(byte_v*)(row + c) = out;
+}
+__device__ __forceinline__ void store_padding(u8* row, const Lane& p) {
+    for (u32 c = C + p.l; c < PITCH; c += L) row[c] = 0;
+}
 )HIP";
 
 // A row is read once and held in registers; its sum of squares (and the largest |h gamma|) are joined over its lanes, and the results
 // are written. In 8 bits: with p = h gamma and P = max |p|, q = rint(127 p / P) needs no 1 / rms, which goes into the scale,
 // rstd P / 127, alone.
-//
-// Rows that are only quantised: q = rint(127 x / A), exactly, ties to even (x = A / 2 is one). The f32 quotient is a whole number off at
-// most next to a border, and there the remainder decides: 254 x - 2 q A has no rounding in f32 where x has 11 bits, in f64 where it has 24.
 const char* kForward = R"HIP(
-__device__ __forceinline__ u32 whole(float x, float most, float inverse) {
-    float r = rintf(x * inverse);
-#if !NORM
-#if BF16 || F16
-    const float off = __builtin_fmaf(-2.0f * r, most, 254.0f * x), half = most;
-#else
-    const double off = __builtin_fma(-2.0 * (double)r, (double)most, 254.0 * (double)x), half = most;
-#endif
-    const bool odd = (int)r & 1;
-    if (off > half || (off == half && odd)) r += 1.0f;
-    else if (off < -half || (off == -half && odd)) r -= 1.0f;
-#endif
-    return (u32)(int)r & 255u;
-}
 extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const elem_t* x, const param_t* __restrict__ gamma, const stream_t* residual,
                                                              stream_t* new_residual, void* y, float* __restrict__ rstd_out, float* __restrict__ scales) {
     __shared__ float red[WAVES][2];
     const Lane p = lane();
     const u64 row = (u64)blockIdx.x * ROWS + p.slot;
     const bool there = row < rows;
-    float h[NV][V], sum = 0.0f;
+    float h[NV][V], weight[NV][V], sum = 0.0f;
     u32 most = 0;
     elem_v hx[NV];
 #if RESIDUAL
@@ -140,6 +139,8 @@ extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const ele
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (there && HAS(p, k)) {
+#pragma unroll
+            for (int i = 0; i < V; i++) weight[k][i] = (float)gamma[start(p, k) + i];
             hx[k] = *(const elem_v*)(x + row * C + start(p, k));
 #if RESIDUAL
             hr[k] = *(const stream_v*)(residual + row * C + start(p, k));
@@ -164,61 +165,131 @@ extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const ele
 #endif
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                if (NORM && counts(p, k, i)) sum += h[k][i] * h[k][i];
+                if (counts(p, k, i)) sum += h[k][i] * h[k][i];
 #if TO_I8
-                if (NORM) h[k][i] *= (float)gamma[start(p, k) + i];
+                h[k][i] *= weight[k][i];
                 const u32 size = bits_of(h[k][i]) & 0x7fffffffu;
                 most = size > most ? size : most;
 #endif
             }
         }
     }
-    over_row<NORM, TO_I8>(sum, most, red);
-    float rstd = 1.0f;
-#if NORM
-    rstd = 1.0f / sqrtf(sum / (float)C + EPS);
+    over_row<true, TO_I8>(sum, most, red);
+#if RESIDUAL
+    // (not before all lanes have what they read: a ragged row's last two vectors overlap, and the new residual may lie in the old one's place)
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (there && HAS(p, k)) STORE((stream_v*)(new_residual + row * C + start(p, k)), hr[k]);
+#endif
+    const float rstd = 1.0f / sqrtf(sum / (float)C + EPS);
     if (rstd_out && there && p.l == 0) rstd_out[row] = rstd;
-#endif
 #if TO_I8
-    // A row that is not finite throughout has no scale: NaN, and zeros.
-    const bool finite = most < 0x7f800000u && rstd < __builtin_inff();
-    // (a power of two keeps 127 / size and 254 x in range)
-    const float size = of_bits(most), up = size < 0x1p-64f ? 0x1p64f : size > 0x1p64f ? 0x1p-64f : 1.0f;
-    const float inverse = finite && size > 0.0f ? 127.0f / (size * up) : 0.0f;
-    if (there && p.l == 0) scales[row] = finite ? rstd * size / 127.0f : __builtin_nanf("");
-#endif
+    const Steps s = steps_of(most);
+    const bool finite = s.finite && rstd < __builtin_inff();
+    const float inverse = s.size > 0.0f ? 127.0f / s.size : 0.0f;
+    if (there && p.l == 0) scales[row] = finite ? rstd * of_bits(most) / 127.0f : __builtin_nanf("");
+    if (s.up != 1.0f)
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int i = 0; i < V; i++) h[k][i] *= s.up;
+    u8* to = (u8*)y + row * PITCH;
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (there && HAS(p, k)) {
+            u32 whole[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) whole[i] = bits_of(__builtin_fmaf(h[k][i], inverse, 12582912.0f));
+            store_bytes(to, start(p, k), whole, finite);
+        }
+    if (there) store_padding(to, p);
+#else
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (there && HAS(p, k)) {
             const u32 c = start(p, k);
-#if RESIDUAL
-            STORE((stream_v*)(new_residual + row * C + c), hr[k]);
-#endif
-#if TO_I8
-            byte_v out;
-#pragma unroll
-            for (int i = 0; i < V; i++) AT(out, i) = finite ? (u8)whole(h[k][i] * up, size * up, inverse) : (u8)0;
-            *(byte_v*)((u8*)y + row * PITCH + c) = out;
-#else
             elem_v out;
 #pragma unroll
-            for (int i = 0; i < V; i++) AT(out, i) = (elem_t)(h[k][i] * rstd * (float)gamma[c + i]);
+            for (int i = 0; i < V; i++) AT(out, i) = (elem_t)(h[k][i] * rstd * weight[k][i]);
             STORE((elem_v*)((elem_t*)y + row * C + c), out);
-#endif
         }
-#if TO_I8
-    for (u32 c = C + p.l; c < PITCH; c += L)
-        if (there) ((u8*)y)[row * PITCH + c] = 0;
 #endif
+}
+)HIP";
+
+// q = rint(127 x / A), exactly, ties to even. 127 / A is taken in two parts, and x times both is added up with one rounding: a quotient in the
+// middle of two whole numbers (x = A / 2 has one) is a value of the type, and so comes out as itself. Any other one is further from the middle
+// than it is off: x = a 2^i and A = b 2^j with whole a and b give a distance of at least 1 / (2 a) of x / A, where the error is 2^-16 of that
+// in f32 (a has 8 or 11 bits) and 2^-45 in f64 (24 bits).
+const char* kQuantize = R"HIP(
+#if BF16 || F16
+typedef float wide_t;
+#define ROUNDED(t) WHOLE_BITS(t)
+#else
+typedef double wide_t;
+#define ROUNDED(t) (u32)__builtin_bit_cast(u64, (t) + 6755399441055744.0)
+#endif
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+#if (BF16 || F16) && V > 1
+typedef u16 u16_v __attribute__((ext_vector_type(V)));
+#endif
+extern "C" __global__ __launch_bounds__(T) void rows_quantize(u64 rows, const elem_t* __restrict__ x, u8* __restrict__ y, float* __restrict__ scales) {
+    __shared__ float red[WAVES][2];
+    const Lane p = lane();
+    const u64 row = (u64)blockIdx.x * ROWS + p.slot;
+    const bool there = row < rows;
+    elem_v hx[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        hx[k] = elem_v((elem_t)0.0f);
+        if (there && HAS(p, k)) hx[k] = *(const elem_v*)(x + row * C + start(p, k));
+    }
+    u32 most = 0;
+#if (BF16 || F16) && V > 1
+    // (magnitudes in their own bits, two at a time)
+    u16_v largest = u16_v((u16)0);
+#pragma unroll
+    for (int k = 0; k < NV; k++) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16_v, hx[k]) & u16_v((u16)0x7fff));
+#pragma unroll
+    for (int i = 0; i < V; i++) most = largest[i] > most ? largest[i] : most;
+    most = bits_of((float)__builtin_bit_cast(elem_t, (u16)most)) & 0x7fffffffu;
+#else
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const u32 size = bits_of((float)AT(hx[k], i)) & 0x7fffffffu;
+            most = size > most ? size : most;
+        }
+#endif
+    float none = 0.0f;
+    over_row<false, true>(none, most, red);
+    const Steps s = steps_of(most);
+    const wide_t size = s.size, inverse = size > 0 ? (wide_t)127 / size : (wide_t)0, rest = size > 0 ? fused(-size, inverse, (wide_t)127) / size : (wide_t)0;
+    if (there && p.l == 0) scales[row] = s.finite ? of_bits(most) / 127.0f : __builtin_nanf("");
+    u8* to = y + row * PITCH;
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (there && HAS(p, k)) {
+            u32 whole[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const wide_t v = (float)AT(hx[k], i) * s.up;
+                whole[i] = ROUNDED(fused(v, inverse, v * rest));
+            }
+            store_bytes(to, start(p, k), whole, s.finite);
+        }
+    if (there) store_padding(to, p);
 }
 )HIP";
 
 // With xh = h rstd and flow = dy gamma: dh' = dh + rstd (flow - xh mean(flow xh)), dgamma = sum over the rows of dy xh. A workgroup goes through rows
 // `gridDim.x` apart and keeps its share of dgamma in registers; `rows_fold` adds up the workgroups' shares. The order is fixed.
 const char* kBackward = R"HIP(
-extern "C" __global__ __launch_bounds__(T) void rows_backward(u64 rows, u32 blocks, const elem_t* dy, const stream_t* h, const param_t* __restrict__ gamma,
-                                                              const float* __restrict__ rstd_of, const stream_t* dh, elem_t* dx, stream_t* dresidual,
-                                                              float* __restrict__ parts) {
+template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 blocks, const elem_t* dy, const stream_t* h, const param_t* __restrict__ gamma,
+                                                             const float* __restrict__ rstd_of, const stream_t* dh, elem_t* dx, stream_t* dresidual,
+                                                             float* __restrict__ parts) {
     __shared__ float red[2][WAVES][2];
     __shared__ float joined[ROWS > 1 ? C : 1];
     const Lane p = lane();
@@ -227,21 +298,40 @@ extern "C" __global__ __launch_bounds__(T) void rows_backward(u64 rows, u32 bloc
     for (int k = 0; k < NV; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) share[k][i] = 0.0f;
+    // A row's operands are asked for while the row before is worked on, where a thread has the registers (1024 threads have 128 each). The loads are
+    // the same for every thread and row, from the last one's place where there is none: loads under a condition would be waited for at once.
+    struct Row { elem_v dy[NV]; stream_v h[NV], dh[NV]; float rstd; } next;
+    auto load = [&](Row& r, u64 row) {
+        row = row < rows ? row : rows - 1;
+        r.rstd = rstd_of[row];
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const u32 c = (p.l + k * L) * V;
+            const u64 at = row * C + (c + V > C ? C - V : c);
+            r.dy[k] = *(const elem_v*)(dy + at);
+            r.h[k] = *(const stream_v*)(h + at);
+            if (MORE) r.dh[k] = *(const stream_v*)(dh + at);
+        }
+    };
+    // (gamma stays as well: a load between a row's and the next row's would be waited for with both)
+    #if T < 1024
+    float held[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) held[k][i] = HAS(p, k) ? (float)gamma[start(p, k) + i] : 0.0f;
+#define GAMMA(k, i) held[k][i]
+#else
+#define GAMMA(k, i) (float)gamma[start(p, k) + (i)]
+#endif
+    const u64 step = (u64)blocks * ROWS;
     u32 turn = 0;
-    for (u64 first = (u64)blockIdx.x * ROWS; first < rows; first += (u64)blocks * ROWS, turn ^= 1) {
+    load(next, (u64)blockIdx.x * ROWS + p.slot);
+    for (u64 first = (u64)blockIdx.x * ROWS; first < rows; first += step, turn ^= 1) {
         const u64 row = first + p.slot;
         const bool there = row < rows;
-        const float rstd = there ? rstd_of[row] : 0.0f;
-        elem_v hd[NV];
-        stream_v hh[NV], hr[NV];
-#pragma unroll
-        for (int k = 0; k < NV; k++)
-            if (there && HAS(p, k)) {
-                const u64 at = row * C + start(p, k);
-                hd[k] = *(const elem_v*)(dy + at);
-                hh[k] = *(const stream_v*)(h + at);
-                if (dh) hr[k] = *(const stream_v*)(dh + at);
-            }
+        const Row r = next;
+        if (T < 1024) load(next, row + step);
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; k++)
@@ -249,8 +339,8 @@ extern "C" __global__ __launch_bounds__(T) void rows_backward(u64 rows, u32 bloc
 #pragma unroll
                 for (int i = 0; i < V; i++)
                     if (counts(p, k, i)) {
-                        const float t = (float)AT(hd[k], i) * ((float)AT(hh[k], i) * rstd);
-                        sum += t * (float)gamma[start(p, k) + i];
+                        const float t = (float)AT(r.dy[k], i) * ((float)AT(r.h[k], i) * r.rstd);
+                        sum += t * GAMMA(k, i);
                         share[k][i] += t;
                     }
         u32 none = 0;
@@ -264,15 +354,16 @@ extern "C" __global__ __launch_bounds__(T) void rows_backward(u64 rows, u32 bloc
                 stream_v more;
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const float xh = (float)AT(hh[k], i) * rstd;
-                    float d = ((float)AT(hd[k], i) * (float)gamma[start(p, k) + i] - xh * mean) * rstd;
-                    if (dh) d += (float)AT(hr[k], i);
+                    const float xh = (float)AT(r.h[k], i) * r.rstd;
+                    float d = ((float)AT(r.dy[k], i) * GAMMA(k, i) - xh * mean) * r.rstd;
+                    if (MORE) d += (float)AT(r.dh[k], i);
                     AT(out, i) = (elem_t)d;
                     AT(more, i) = (stream_t)d;
                 }
                 if (dx) STORE((elem_v*)(dx + at), out);
                 if (dresidual) STORE((stream_v*)(dresidual + at), more);
             }
+        if (T == 1024) load(next, row + step);
     }
     // rows side by side: first those of a wave, then the waves' one after the other
 #if L < 64
@@ -301,18 +392,26 @@ extern "C" __global__ __launch_bounds__(T) void rows_backward(u64 rows, u32 bloc
         if (groups > 1) __syncthreads();
     }
 }
+#define BACKWARD(name, more) \
+    extern "C" __global__ __launch_bounds__(T) void name(u64 rows, u32 blocks, const elem_t* dy, const stream_t* h, const param_t* gamma, const float* rstd, const stream_t* dh, elem_t* dx, stream_t* dresidual, float* parts) { backward<more>(rows, blocks, dy, h, gamma, rstd, dh, dx, dresidual, parts); }
+BACKWARD(rows_backward, false)
+#if RESIDUAL
+BACKWARD(rows_backward_more, true)   // with what reaches h from elsewhere
+#endif
 
-// dgamma[c] = the sum of `count` shares: 64 columns to a workgroup, the shares dealt to its 16 waves.
+// dgamma[c] = the sum of `count` shares: 16 columns to a workgroup, the shares dealt to its 64 rows of threads.
 extern "C" __global__ __launch_bounds__(1024) void rows_fold(const float* __restrict__ parts, u32 count, float* __restrict__ dgamma) {
-    __shared__ float part[16][64];
-    const u32 column = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + column;
+    __shared__ float part[16][16];
+    const u32 column = threadIdx.x & 15u, row = threadIdx.x >> 4, c = blockIdx.x * 16 + column;
     float s = 0.0f;
     if (c < C)
 #pragma unroll 8
-        for (u32 n = wave; n < count; n += 16) s += parts[(u64)n * C + c];
-    part[wave][column] = s;
+        for (u32 n = row; n < count; n += 64) s += parts[(u64)n * C + c];
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if ((threadIdx.x & 63u) < 16) part[threadIdx.x >> 6][column] = s;
     __syncthreads();
-    if (wave == 0 && c < C) {
+    if (threadIdx.x < 16 && c < C) {
         for (u32 w = 1; w < 16; w++) s += part[w][column];
         dgamma[c] = s;
     }
@@ -331,14 +430,14 @@ int pow2_ceil(int64_t x) {
 int row_alignment(int64_t bytes) { return (int)std::min<int64_t>(16, bytes & -bytes); }
 int value_bytes(int dtype) { return (int)dtype_bits(dtype) / 8; }
 
-std::string definitions(const RowProblem& pr, const RowTiling& t, bool stream_out) {
+std::string definitions(const RowProblem& pr, const RowTiling& t) {
     std::ostringstream s;
     s << "#define C " << pr.columns << "\n#define V " << t.vec << "\n#define NV " << t.vectors << "\n#define L " << t.lanes << "\n#define T " << t.threads
       << "\n#define BF16 " << (pr.dtype == HE_BF16) << "\n#define F16 " << (pr.dtype == HE_F16) << "\n#define STREAM_SAME "
       << (pr.stream_dtype() == pr.dtype) << "\n#define PARAM_SAME " << (pr.param_dtype == pr.dtype) << "\n#define RESIDUAL " << pr.residual()
-      << "\n#define TO_I8 " << pr.to_i8 << "\n#define NORM " << pr.norm << "\n#define PITCH " << quantized_pitch(pr.columns) << "ull\n#define EPS "
-      << strfmt("%.9ef", (double)pr.epsilon) << "\n#define X_ALIGN " << row_alignment(pr.columns * value_bytes(pr.dtype)) << "\n#define H_ALIGN "
-      << row_alignment(pr.columns * value_bytes(pr.stream_dtype())) << "\n#define STREAM_OUT " << stream_out << "\n";
+      << "\n#define TO_I8 " << pr.to_i8 << "\n#define PITCH " << quantized_pitch(pr.columns) << "ull\n#define EPS "
+      << strfmt("%.9ef", (double)pr.epsilon) << "\n#define X_ALIGN " << std::min(t.vec * value_bytes(pr.dtype), row_alignment(pr.columns * value_bytes(pr.dtype))) << "\n#define H_ALIGN "
+      << std::min(t.vec * value_bytes(pr.stream_dtype()), row_alignment(pr.columns * value_bytes(pr.stream_dtype()))) << "\n";
     return s.str();
 }
 
@@ -346,12 +445,14 @@ std::string definitions(const RowProblem& pr, const RowTiling& t, bool stream_ou
 
 std::string RowTiling::describe() const { return strfmt("vec=%d vectors=%d lanes=%d threads=%d", vec, vectors, lanes, threads); }
 
-RowTiling plan_rows(const RowProblem& pr, int values) {
+RowTiling plan_rows(const RowProblem& pr) {
+    // 16 bytes of the wider type in an access, and two accesses of each operand to a thread (one to four are within 5% of each other on 8192 x 4096 and 2000 x
+    // 1024, in bf16 and f32; eight, a row to a wave, take 51.5 instead of 47.4 us).
     RowTiling t;
-    t.vec = 16 / value_bytes(pr.dtype);
+    t.vec = 16 / std::max(value_bytes(pr.dtype), value_bytes(pr.stream_dtype()));
     while (t.vec > pr.columns) t.vec /= 2;
     const int64_t vectors = (pr.columns + t.vec - 1) / t.vec;
-    t.lanes = std::min(1024, pow2_ceil((vectors * t.vec + values - 1) / values));
+    t.lanes = std::min(1024, pow2_ceil((vectors + 1) / 2));
     t.vectors = (int)((vectors + t.lanes - 1) / t.lanes);
     t.threads = std::max(256, t.lanes);
     return t;
@@ -367,27 +468,20 @@ RmsNorm::RmsNorm(const RowProblem& pr) : pr_(pr) {
     HE_REQUIRE(pr.param_dtype == HE_F32 || pr.param_dtype == pr.dtype, HE_ERR_INVALID, "rms norm: gamma is f32 or of the operand's type, not %s",
                dtype_name(pr.param_dtype));
     HE_REQUIRE(std::isfinite(pr.epsilon) && pr.epsilon >= 0, HE_ERR_INVALID, "rms norm: epsilon %g", (double)pr.epsilon);
-    few_ = plan_rows(pr, 8);
-    many_ = plan_rows(pr, tuning::get_int("HELIUM_HIP_ROWS_VALUES", 16));
-    back_ = plan_rows(pr, tuning::get_int("HELIUM_HIP_ROWS_BACK_VALUES", 16));
-    const std::string few = definitions(pr, few_, false) + kCommon + kForward;
-    const std::string many = definitions(pr, many_, true) + kCommon + kForward;
-    const std::string back = definitions(pr, back_, true) + kCommon + kBackward;
+    tiling_ = plan_rows(pr);
+    const std::string text = definitions(pr, tiling_) + kCommon, back = text + kBackward;
     const bool has_back = pr.norm && !pr.to_i8;
-    auto compiled = std::async(std::launch::async, [&] { (void)rtc_compile(many, "rows_forward", {}); });
-    auto back_compiled = std::async(std::launch::async, [&] { if (has_back) (void)rtc_compile(back, "rows_backward", {}); });
-    few_kernel_ = std::make_unique<JitKernel>(few, "rows_forward");
+    auto compiled = std::async(std::launch::async, [&] { if (has_back) (void)rtc_compile(back, "rows_backward", {}); });
+    source_ = text + kBytes + (pr.norm ? kForward : kQuantize);
+    forward_ = std::make_unique<JitKernel>(source_, pr.norm ? "rows_forward" : "rows_quantize");
     compiled.get();
-    many_kernel_ = std::make_unique<JitKernel>(many, "rows_forward");
-    back_compiled.get();
-    source_ = few + "\n" + many;
-    describe_ = std::string(pr.norm ? "rms_norm" : "quantize_rows") + " few rows: " + few_.describe() + "\nmany rows: " + many_.describe();
     if (has_back) {
-        back_kernel_ = std::make_unique<JitKernel>(back, "rows_backward");
-        fold_kernel_ = std::make_unique<JitKernel>(back, "rows_fold");
+        backward_ = std::make_unique<JitKernel>(back, "rows_backward");
+        if (pr.residual()) backward_more_ = std::make_unique<JitKernel>(back, "rows_backward_more");
+        fold_ = std::make_unique<JitKernel>(back, "rows_fold");
         source_ += "\n" + back;
-        describe_ += "\nbackward: " + back_.describe();
     }
+    describe_ = std::string(pr.norm ? "rms_norm " : "quantize_rows ") + tiling_.describe();
 }
 
 RmsNorm::~RmsNorm() { scratch_.release(); }
@@ -398,8 +492,6 @@ void check_tensor(const char* what, const void* p, int64_t alignment) {
     HE_REQUIRE(p && ((uintptr_t)p & (alignment - 1)) == 0, HE_ERR_INVALID, "%s is null or not aligned to %lld bytes", what, (long long)alignment);
 }
 }  // namespace
-
-const RowTiling& RmsNorm::forward_tiling(int64_t rows) const { return rows <= 4 * kCUs ? few_ : many_; }
 
 void RmsNorm::forward(int64_t rows, const void* x, const void* gamma, const void* residual, void* new_residual, void* y, float* rstd, float* scales,
                       hipStream_t stream) {
@@ -416,18 +508,19 @@ void RmsNorm::forward(int64_t rows, const void* x, const void* gamma, const void
     check_tensor("y", y, pr_.to_i8 ? 16 : align);
     HE_REQUIRE(((uintptr_t)rstd & 3) == 0, HE_ERR_INVALID, "rstd is not aligned to 4 bytes");
     if (pr_.to_i8) check_tensor("the list of scales", scales, 4);
-    const RowTiling& t = forward_tiling(rows);
+    const RowTiling& t = tiling_;
     const uint64_t blocks = ((uint64_t)rows + t.rows() - 1) / t.rows();
     HE_REQUIRE(blocks < kThreads / t.threads, HE_ERR_UNSUPPORTED, "%lld rows are too many for one launch", (long long)rows);
     uint64_t count = (uint64_t)rows;
     const uint32_t grid[3] = {(uint32_t)blocks, 1, 1}, block[3] = {(uint32_t)t.threads, 1, 1};
     void* args[] = {&count, &x, &gamma, &residual, &new_residual, &y, &rstd, &scales};
-    (&t == &few_ ? few_kernel_ : many_kernel_)->launch(grid, block, 0, stream, args, true);
+    void* quantize_args[] = {&count, &x, &y, &scales};
+    forward_->launch(grid, block, 0, stream, pr_.norm ? args : quantize_args, true);
 }
 
 void RmsNorm::backward(int64_t rows, const void* dy, const void* h, const void* gamma, const float* rstd, const void* dh, void* dx, void* dresidual,
                        float* dgamma, hipStream_t stream) {
-    HE_REQUIRE(back_kernel_, HE_ERR_UNSUPPORTED, "rms norm: an output in 8 bits has no gradient");
+    HE_REQUIRE(backward_, HE_ERR_UNSUPPORTED, "rms norm: an output in 8 bits has no gradient");
     HE_REQUIRE(rows >= 0, HE_ERR_INVALID, "%lld rows", (long long)rows);
     HE_REQUIRE(pr_.residual() || (!dh && !dresidual), HE_ERR_INVALID, "rms norm: made without a residual");
     check_tensor("dgamma", dgamma, 4);
@@ -442,19 +535,21 @@ void RmsNorm::backward(int64_t rows, const void* dy, const void* h, const void* 
         if (dx) check_tensor("dx", dx, align);
         if (dresidual) check_tensor("the residual's gradient", dresidual, stream_align);
     }
-    const uint64_t most = (uint64_t)kCUs * tuning::get_int("HELIUM_HIP_ROWS_BACK_PER_CU", 2);
-    uint32_t blocks = (uint32_t)std::min<uint64_t>(most, ((uint64_t)rows + back_.rows() - 1) / back_.rows());
+    // (one workgroup to a CU where it has one row at a time, otherwise two: 8192 x 4096 bf16 50.6 and 52.5 us, 1517 x 2867 16.4 and 17.5; 8192 x 1024 f32 20.0 and
+    // 19.0, 30000 x 256 bf16 15.3 and 14.6. Four: 57.0, 21.2, 20.4, 15.4)
+    const uint64_t most = (uint64_t)kCUs * tuning::get_int("HELIUM_HIP_ROWS_PER_CU", tiling_.rows() == 1 ? 1 : 2);
+    uint32_t blocks = (uint32_t)std::min<uint64_t>(most, ((uint64_t)rows + tiling_.rows() - 1) / tiling_.rows());
     uint64_t count = (uint64_t)rows;
-    const uint32_t grid[3] = {blocks, 1, 1}, block[3] = {(uint32_t)back_.threads, 1, 1};
-    const uint32_t fold_grid[3] = {(uint32_t)((pr_.columns + 63) / 64), 1, 1}, fold_block[3] = {1024, 1, 1};
+    const uint32_t grid[3] = {blocks, 1, 1}, block[3] = {(uint32_t)tiling_.threads, 1, 1};
+    const uint32_t fold_grid[3] = {(uint32_t)((pr_.columns + 15) / 16), 1, 1}, fold_block[3] = {1024, 1, 1};
     std::lock_guard<std::mutex> lk(mu_);
     // (one workgroup's share is the sum already)
     float* parts = blocks == 1 ? dgamma : scratch_.get(most * pr_.columns, 0, stream).floats;
     void* args[] = {&count, &blocks, &dy, &h, &gamma, &rstd, &dh, &dx, &dresidual, &parts};
-    if (blocks) back_kernel_->launch(grid, block, 0, stream, args, blocks == 1);
+    if (blocks) (dh ? backward_more_ : backward_)->launch(grid, block, 0, stream, args, blocks == 1);
     if (blocks == 1) return;
     void* fold_args[] = {&parts, &blocks, &dgamma};
-    fold_kernel_->launch(fold_grid, fold_block, 0, stream, fold_args, true);
+    fold_->launch(fold_grid, fold_block, 0, stream, fold_args, true);
 }
 
 }  // namespace he

@@ -32,8 +32,7 @@ struct RowTiling {
     int rows() const { return threads / lanes; }
     std::string describe() const;
 };
-// values: as many as a lane holds at most, where 1024 lanes are enough for that.
-RowTiling plan_rows(const RowProblem& pr, int values);
+RowTiling plan_rows(const RowProblem& pr);
 
 class RmsNorm {
 public:
@@ -47,11 +46,10 @@ public:
     const std::string& describe() const { return describe_; }
 
 private:
-    const RowTiling& forward_tiling(int64_t rows) const;
     RowProblem pr_;
-    RowTiling few_, many_, back_;
+    RowTiling tiling_;
     std::string source_, describe_;
-    std::unique_ptr<JitKernel> few_kernel_, many_kernel_, back_kernel_, fold_kernel_;
+    std::unique_ptr<JitKernel> forward_, backward_, backward_more_, fold_;
     std::mutex mu_;  // a backward pass's launches follow each other on their stream: they share the stream's scratch
     ReduceScratch scratch_;
 };

@@ -2,11 +2,10 @@
 import ctypes as C
 
 from . import _ffi
-from ._ffi import check, lib
+from ._ffi import address as _at, addresses as _list, check, lib
 from .device import _h
-from .group_norm import _at
-from .muon import _LIST, _list
 
+_LIST = C.POINTER(C.c_void_p)
 _ffi._sig("he_gradient_clip_create", C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int), C.c_int)
 _ffi._sig("he_gradient_clip_destroy", C.c_void_p)
 _ffi._sig("he_gradient_norm", C.c_void_p, _LIST, C.c_int, C.c_void_p, C.c_void_p)

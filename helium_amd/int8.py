@@ -2,9 +2,8 @@
 import ctypes as C
 
 from . import _ffi
-from ._ffi import check, lib
+from ._ffi import address as _at, check, lib
 from .device import _h
-from .group_norm import _at
 
 _ffi._sig("he_quantized_pitch", C.c_int64, restype=C.c_int64)
 _ffi._sig("he_quantize_rows_create", C.POINTER(C.c_void_p), C.c_int64, C.c_int)

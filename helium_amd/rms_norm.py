@@ -2,9 +2,8 @@
 import ctypes as C
 
 from . import _ffi
-from ._ffi import check, lib
+from ._ffi import address as _at, check, lib
 from .device import _h
-from .group_norm import _at
 
 _ffi._sig("he_rms_norm_create", C.POINTER(C.c_void_p), C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float)
 _ffi._sig("he_rms_norm_destroy", C.c_void_p)

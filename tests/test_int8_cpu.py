@@ -42,46 +42,48 @@ def emulated(op, host, dtype, shape, shares):
     """What the kernels of one of the shapes make of a call."""
     tokens, channels, columns = len(host["x"]), len(host["weights"]), host["x"].shape[1]
     said = dict(re.findall(r"(\w+)=(\w+)", op.describe(tokens)))
-    assert int(said["shape"]) == shape
-    stream, threads, grid = "blocks_n" in said, int(said["threads"]), int(said["grid"])
-    text = SHIM + op.source.split("//// shape\n")[1 + shape]
-    call = f"Call c{{x, w, xs, ws, {'bias' if host['bias'] is not None else 'nullptr'}, y, {tokens}, {channels}, {columns}}};"
-    params = "const u8* x, const float* xs, const u8* w, const float* ws, const float* bias, out_t* y"
-    kernel = "int8_stream(c)" if stream else f"int8_product(c, {grid}, {said['shares']}, parked)"
-    text += f"\nextern \"C\" void emu({params}, i32x4* parked) {{ {call} {kernel}; }}\n"
-    if not stream and shares > 1:
-        text += f"extern \"C\" void emu_join({params}, const i32x4* parked) {{ {call} int8_join(c, {grid}, {said['shares']}, parked); }}\n"
+    assert int(said["shape"]) == shape and int(said["shares"]) == shares
+    threads, grid, wide = int(said["threads"]), int(said["grid"]), -(-channels // 4) * 4
+    texts = op.source.split("//// shape\n")[1:]
+    bias = "bias" if host["bias"] is not None else "nullptr"
+    wrapper = f"""
+extern "C" void emu(const u8* x, const float* xs, const u8* w, const float* ws, const float* bias, out_t* y, int* parked) {{
+    Call c{{x, w, xs, ws, {bias}, y, {tokens}, {channels}, {columns}, {grid}, {shares}, {wide}, parked}};
+    ENTRY_OF(c);
+}}
+"""
     given = [(host[k], 0) for k in FIELDS] + [(host["bias"] if host["bias"] is not None else np.zeros(1, np.float32), 0)]
-    y = np.empty((tokens, channels), np.float32 if dtype == "f32" else np.uint16)
-    parked = np.zeros(grid * int(said["shares"]) * np.prod([int(n) for n in said.get("tile", "1x1").split("x")]) if shares > 1 else 1, np.int32)
-    y, parked = run_kernel(text, "emu", grid, threads, given + [(y, 1), (parked, 2)], grid_y=int(said["shares"]))
-    if int(said["shares"]) > 1:
-        y, = run_kernel(text, "emu_join", grid, threads, given + [(y, 1), (parked, 0)])
+    y, parked = np.empty((tokens, channels), np.float32 if dtype == "f32" else np.uint16), np.zeros((shares if shares > 1 else 0, tokens, wide), np.int32)
+    entry = "int8_stream" if "blocks_n" in said else "int8_product"
+    y, parked = run_kernel(SHIM + texts[shape] + wrapper.replace("ENTRY_OF", entry), "emu", grid, threads, given + [(y, 1), (parked, 2)], grid_y=shares)
+    if shares > 1:
+        y, = run_kernel(SHIM + texts[-1] + wrapper.replace("ENTRY_OF", "int8_join"), "emu", -(-tokens * wide // 4 // 256), 256, given + [(y, 1), (parked, 0)])
     return y
 
 
-def shapes():
-    """The number of shapes, from the source of one product."""
-    return ha.Int8Matmul(16, 16, "f32").source.count("//// shape\n")
+SHAPES, TILES = 9, 4
 
 
-# tiles of every third size, streams of every one (k-th size, shape)
-PAIRS = [(k, shape) for shape in range(6) for k in range(len(SMALL)) if shape > 2 or (shape + k) % 3 == 0]
+# (size, shape): every shape at two or three sizes
+PAIRS = [(k, shape) for shape in range(SHAPES) for k in range(len(SMALL)) if (shape + k) % 3 == 0]
 
 
 @pytest.mark.parametrize("k,shape", PAIRS)
 def test_the_kernels_match_the_oracle(monkeypatch, k, shape):
     tokens, columns, channels = SMALL[k]
-    dtype, shares = ("f32", "bf16", "f16")[k % 3], 1 + (k % 2) * (shape in (1, 2))
+    dtype = ("f32", "bf16", "f16")[k % 3]
     monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
-    monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", "1")
     host = inputs(tokens, columns, channels, bias=k % 2, seed=k)
-    y = emulated(ha.Int8Matmul(columns, channels, dtype), host, dtype, shape, shares)
+    y = emulated(ha.Int8Matmul(columns, channels, dtype), host, dtype, shape, 1)
     check(host, dtype, to_f32(y, dtype))
 
 
-@pytest.mark.parametrize("shape,tokens,columns,channels,shares", [(2, 70, 700, 130, 1), (2, 70, 1400, 70, 3), (1, 130, 400, 130, 1)])
-def test_several_tiles_and_rounds_of_the_ring(monkeypatch, shape, tokens, columns, channels, shares):
+@pytest.mark.parametrize("shape,tokens,columns,channels,shares", [
+    (0, 20, 1100, 300, 1), (1, 130, 400, 130, 1), (1, 9, 2100, 70, 4), (2, 140, 1300, 70, 1), (2, 30, 1300, 70, 2), (3, 70, 700, 130, 1), (3, 70, 2100, 70, 4),
+    (4, 5, 9000, 18, 4), (7, 70, 8192, 17, 2), (6, 40, 5000, 33, 2), (8, 70, 2500, 66, 1),
+])
+def test_several_tiles_shares_and_rounds_of_the_ring(monkeypatch, shape, tokens, columns, channels, shares):
     monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
     monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
     host = inputs(tokens, columns, channels, bias=True, seed=9)
@@ -96,14 +98,20 @@ def test_the_oracles_product_is_exact():
     assert np.allclose(oracle.product(*[host[k] for k in FIELDS], host["bias"]), want, rtol=1e-14)
 
 
-def test_every_shape_has_a_launch_for_every_call():
-    assert shapes() == 6
-    for inputs_, channels in ((1, 1), (4096, 4096), (131071, 17), (512, 1 << 20)):
-        op = ha.Int8Matmul(inputs_, channels, "bf16")
-        for tokens in (1, 15, 16, 17, 64, 65, 200, 1000, 5000):
-            said = dict(re.findall(r"(\w+)=(\w+)", op.describe(tokens)))
-            assert int(said["grid"]) >= 1 and int(said["shares"]) >= 1
-            assert int(said["shares"]) == 1 or (int(said["grid"]) * int(said["shares"]) <= 512 and int(said["shares"]) <= -(-inputs_ // 128))
+def test_every_call_is_cut():
+    op = ha.Int8Matmul(16, 16, "f32")
+    assert op.source.count("//// shape\n") == SHAPES + 1 and op.source.count("int8_product(Call") == TILES
+    used = set()
+    for columns in (1, 100, 1000, 4096, 16384, 131071):
+        for channels in (1, 17, 300, 1024, 4096, 16384, 1 << 20):
+            op = ha.Int8Matmul(columns, channels, "bf16")
+            for tokens in (1, 15, 16, 17, 33, 48, 49, 64, 65, 100, 128, 200, 333, 512, 1000, 5000):
+                said = dict(re.findall(r"(\w+)=([\w.]+)", op.describe(tokens)))
+                used.add(int(said["shape"]))
+                shares = int(said["shares"])
+                assert int(said["grid"]) >= 1 and shares >= 1
+                assert shares == 1 or (shares * tokens * (channels + 3) <= 1 << 23 and shares <= -(-columns // 512) and float(said["estimate"]) > 0)
+    assert used == set(range(SHAPES))   # (nothing is built that no call takes)
 
 
 @pytest.mark.parametrize("kwargs,says", [

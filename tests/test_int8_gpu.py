@@ -36,9 +36,9 @@ def test_products_match_the_oracle(gpu, k):
     check(host, dtype, to_f32(multiply(ha.Int8Matmul(columns, channels, dtype), host, dtype), dtype))
 
 
-@pytest.mark.parametrize("size", [(70, 700, 130), (300, 513, 520), (257, 4096, 300)])
-@pytest.mark.parametrize("shares", [1, 3])
-@pytest.mark.parametrize("shape", range(6))
+@pytest.mark.parametrize("size", [(70, 700, 130), (300, 513, 520), (257, 8192, 300), (33, 9000, 77)])
+@pytest.mark.parametrize("shares", [1, 2, 4])
+@pytest.mark.parametrize("shape", range(9))
 def test_every_shape_and_cut(gpu, monkeypatch, shape, shares, size):
     monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
     monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
@@ -108,9 +108,10 @@ def test_a_quantized_layer(gpu, tokens):
 
 
 def test_calls_on_streams_that_overlap(gpu, monkeypatch):
-    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", "3")
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", "4")
     monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", "4")
     op = ha.Int8Matmul(3000, 128, "f32")
+    assert "shares=4" in op.describe(130)
     cases = [inputs(130, 3000, 128, False, seed=s) for s in (3, 4)]
     want = [multiply(op, h, "f32") for h in cases]
     streams = [ha.Stream(), ha.Stream()]

@@ -48,14 +48,9 @@ def test_the_oracles_whole_numbers_are_the_nearest_ones():
             assert q[r, c] == round(127 * Fraction(float(v)) / a)   # (ties to even)
 
 
-def tilings(text, columns):
-    """What each part of a description says, and the sources in the same order."""
-    return [dict((k, int(n)) for k, n in re.findall(r"(\w+)=(\d+)", line)) for line in text.splitlines()]
-
-
 def parts(op):
-    sources = ["#define C " + s for s in op.source.split("#define C ")[1:]]
-    return list(zip(tilings(op.description, op.columns), sources))
+    """How rows are cut, and the texts of forward (or quantisation) and backward."""
+    return {k: int(n) for k, n in re.findall(r"(\w+)=(\d+)", op.description)}, ["#define C " + s for s in op.source.split("#define C ")[1:]]
 
 
 def pointers(names, types, given):
@@ -73,25 +68,26 @@ BACKWARD_TYPES = dict(zip(BACKWARD, ("const elem_t*", "const stream_t*", "const 
 def emulated_forward(tiling, text, rows, buffers):
     """buffers: by name (array, mode)"""
     params, args = pointers(FORWARD, FORWARD_TYPES, buffers)
-    text += f"\nextern \"C\" void emu_forward(const u64* rows, {params}) {{ rows_forward(*rows, {args}); }}\n"
+    call = f"rows_forward(*rows, {args})" if "gamma" in buffers else "rows_quantize(*rows, x, (u8*)y, scales)"
+    text += f"\nextern \"C\" void emu_forward(const u64* rows, {params}) {{ {call}; }}\n"
     given = [buffers[n] for n in FORWARD if n in buffers]
     side = tiling["threads"] // tiling["lanes"]
     got = run_kernel(text, "emu_forward", -(-rows // side), tiling["threads"], [(np.array([rows], np.uint64), 0)] + given)
     return dict(zip([n for n in FORWARD if n in buffers and buffers[n][1]], got))
 
 
-def emulated_backward(tiling, text, rows, columns, blocks, buffers):
+def emulated_backward(tiling, back, rows, columns, blocks, buffers):
     buffers = dict(buffers, parts=(np.zeros((blocks, columns), np.float32), 1))
     params, args = pointers(BACKWARD, BACKWARD_TYPES, buffers)
     text += f"""
-extern "C" void emu_backward(const u64* rows, const u32* blocks, {params}) {{ rows_backward(*rows, *blocks, {args}); }}
+extern "C" void emu_backward(const u64* rows, const u32* blocks, {params}) {{ rows_backward{"_more" if "dh" in buffers else ""}(*rows, *blocks, {args}); }}
 extern "C" void emu_fold(const float* parts, const u32* count, float* dgamma) {{ rows_fold(parts, *count, dgamma); }}
 """
     count = (np.array([blocks], np.uint32), 0)
     given = [buffers[n] for n in BACKWARD if n in buffers]
     got = run_kernel(text, "emu_backward", blocks, tiling["threads"], [(np.array([rows], np.uint64), 0), count] + given)
     got = dict(zip([n for n in BACKWARD if n in buffers and buffers[n][1]], got))
-    got["dgamma"], = run_kernel(text, "emu_fold", (columns + 63) // 64, 1024, [(got["parts"], 0), count, (np.zeros(columns, np.float32), 1)])
+    got["dgamma"], = run_kernel(text, "emu_fold", (columns + 15) // 16, 1024, [(got["parts"], 0), count, (np.zeros(columns, np.float32), 1)])
     return got
 
 
@@ -104,21 +100,19 @@ def test_the_kernels_match_the_oracle(shape, dtype, residual, same):
     param = dtype if same else "f32"
     host, v = inputs(rows, columns, dtype, residual, param, seed=columns)
     norm = ha.RmsNorm(columns, dtype, residual_dtype=residual, param_dtype=param, epsilon=EPSILON)
-    ops = parts(norm)
-    for tiling, text in ops[columns > 1000:2]:   # (few rows: as many, with more threads to each)
-        buffers = {"x": (host["x"], 0), "gamma": (host["gamma"], 0), "y": (np.empty_like(host["x"]), 1), "rstd": (np.empty(rows, np.float32), 1)}
-        if residual:
-            buffers.update(residual=(host["residual"], 0), new_residual=(np.empty_like(host["h"]), 1))
-        got = emulated_forward(tiling, text, rows, buffers)
-        check_forward(dtype, v, to_f32(got["y"], dtype), got["rstd"])
-        assert not residual or np.array_equal(got["new_residual"], host["h"])
-    tiling, text = ops[2]
+    tiling, (forward, back) = parts(norm)
+    buffers = {"x": (host["x"], 0), "gamma": (host["gamma"], 0), "y": (np.empty_like(host["x"]), 1), "rstd": (np.empty(rows, np.float32), 1)}
+    if residual:
+        buffers.update(residual=(host["residual"], 0), new_residual=(np.empty_like(host["h"]), 1))
+    got = emulated_forward(tiling, forward, rows, buffers)
+    check_forward(dtype, v, to_f32(got["y"], dtype), got["rstd"])
+    assert not residual or np.array_equal(got["new_residual"], host["h"])
     buffers = {k: (host[k], 0) for k in ("dy", "h", "gamma", "rstd")}
     buffers["dx"] = (np.empty_like(host["x"]), 1)
     if residual:
         buffers.update(dh=(host["dh"], 0), dresidual=(np.empty_like(host["h"]), 1))
     for blocks in (1, 3)[columns > 1000:]:
-        got = emulated_backward(tiling, text, rows, columns, blocks, buffers)
+        got = emulated_backward(tiling, back, rows, columns, blocks, buffers)
         check_backward(dtype, residual, v, to_f32(got["dx"], dtype), to_f32(got["dresidual"], residual) if residual else None, got["dgamma"], rows)
 
 
@@ -126,13 +120,13 @@ def test_the_kernels_match_the_oracle(shape, dtype, residual, same):
 def test_the_norm_into_8_bits_matches_the_oracle(shape, dtype, residual, same):
     rows, columns = shape
     host, v = inputs(rows, columns, dtype, residual, "f32", seed=columns + 1)
-    for tiling, text in parts(ha.RmsNorm(columns, dtype, residual_dtype=residual, output="i8", epsilon=EPSILON)):
-        buffers = {"x": (host["x"], 0), "gamma": (host["gamma"], 0), "y": (np.empty((rows, pitch(columns)), np.int8), 1), "scales": (np.empty(rows, np.float32), 1)}
-        if residual:
-            buffers.update(residual=(host["residual"], 0), new_residual=(np.empty_like(host["h"]), 1))
-        got = emulated_forward(tiling, text, rows, buffers)
-        check_quantized_norm(v, got["y"], got["scales"])
-        assert not residual or np.array_equal(got["new_residual"], host["h"])
+    tiling, (text,) = parts(ha.RmsNorm(columns, dtype, residual_dtype=residual, output="i8", epsilon=EPSILON))
+    buffers = {"x": (host["x"], 0), "gamma": (host["gamma"], 0), "y": (np.empty((rows, pitch(columns)), np.int8), 1), "scales": (np.empty(rows, np.float32), 1)}
+    if residual:
+        buffers.update(residual=(host["residual"], 0), new_residual=(np.empty_like(host["h"]), 1))
+    got = emulated_forward(tiling, text, rows, buffers)
+    check_quantized_norm(v, got["y"], got["scales"])
+    assert not residual or np.array_equal(got["new_residual"], host["h"])
 
 
 def borders(rows, columns, dtype, seed):
@@ -159,10 +153,10 @@ def test_quantized_rows_are_the_oracles(shape, dtype):
     rows, columns = shape
     x = borders(rows, columns, dtype, columns)
     want, scales = oracle_int8.quantize(to_f32(x, dtype))
-    for tiling, text in parts(ha.QuantizeRows(columns, dtype)):
-        got = emulated_forward(tiling, text, rows, {"x": (x, 0), "y": (np.empty((rows, pitch(columns)), np.int8), 1), "scales": (np.empty(rows, np.float32), 1)})
-        assert np.array_equal(got["y"][:, :columns], want) and not got["y"][:, columns:].any()
-        assert np.array_equal(got["scales"], scales, equal_nan=True)
+    tiling, (text,) = parts(ha.QuantizeRows(columns, dtype))
+    got = emulated_forward(tiling, text, rows, {"x": (x, 0), "y": (np.empty((rows, pitch(columns)), np.int8), 1), "scales": (np.empty(rows, np.float32), 1)})
+    assert np.array_equal(got["y"][:, :columns], want) and not got["y"][:, columns:].any()
+    assert np.array_equal(got["scales"], scales, equal_nan=True)
 
 
 @pytest.mark.parametrize("epsilon", [0.0, 1.0, 2.0 ** -149])
