@@ -76,7 +76,7 @@ def emulated_forward(tiling, text, rows, buffers):
     return dict(zip([n for n in FORWARD if n in buffers and buffers[n][1]], got))
 
 
-def emulated_backward(tiling, back, rows, columns, blocks, buffers):
+def emulated_backward(tiling, text, rows, columns, blocks, buffers):
     buffers = dict(buffers, parts=(np.zeros((blocks, columns), np.float32), 1))
     params, args = pointers(BACKWARD, BACKWARD_TYPES, buffers)
     text += f"""
