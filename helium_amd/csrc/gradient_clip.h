@@ -18,10 +18,11 @@ struct ClipTensor {
     uint32_t dtype;
     uint64_t bytes;
 };
-// Tensors whose addresses one launch takes: their chunks, of 16 KB each, are dealt to `blocks` workgroups, whose sums lie from `first_sum` on.
+// Tensors whose addresses one launch takes: their chunks, of 16 KB each, are dealt to `blocks` workgroups, whose sums lie from `first_sum` on; the
+// first `passing` chunks are read past the caches, which later ones fill.
 struct ClipGroup {
     size_t first, count;
-    uint32_t chunks, blocks, first_sum;
+    uint32_t chunks, blocks, first_sum, passing;
 };
 
 class GradientClip {

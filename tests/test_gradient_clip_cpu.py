@@ -40,10 +40,10 @@ def groups_of(clip):
     return [{k: int(v) for k, v in re.findall(r"(\w+)=(\d+)", line)} for line in clip.description.splitlines()[1:]]
 
 
-def emulated(clip, host, most, in_place=False):
+def emulated(clip, host, most, in_place=False, passing=0):
     """out and norm of a call, by its launches one after the other."""
     table, groups = np.frombuffer(clip.table(), TABLE), groups_of(clip)
-    sums = np.concatenate([run_group(clip, table, g, host) for g in groups]) if groups else np.zeros(0)
+    sums = np.concatenate([run_group(clip, table, g, host, passing) for g in groups]) if groups else np.zeros(0)
     norm = np.zeros(1, np.float32)
     got = [None] * len(host)
     for g in reversed(groups):
@@ -56,7 +56,7 @@ def emulated(clip, host, most, in_place=False):
         fill = "".join(f"o.in[{k}] = {'o' if in_place else 'i'}{k}; o.out[{k}] = o{k}; " for k in range(g["count"]))
         text = SHIM + clip.source + f"""
 extern "C" void emu({params}const Tensor* t, const double* sums, float* norm) {{
-    Both o{{}}; {fill} clip_scale(o, t, {g["count"]}, {g["chunks"]}, sums, {len(sums)}, {most!r}f, norm);
+    Both o{{}}; {fill} clip_scale(o, t, {g["count"]}, {g["chunks"]}, {passing}, sums, {len(sums)}, {most!r}f, norm);
 }}
 """
         of = host[g["first"]:g["first"] + g["count"]]
@@ -66,13 +66,13 @@ extern "C" void emu({params}const Tensor* t, const double* sums, float* norm) {{
     return got, norm[0], sums
 
 
-def run_group(clip, table, g, host):
+def run_group(clip, table, g, host, passing=0):
     if not g["blocks"]:
         return np.zeros(0)
     params = "".join(f"const u8* i{k}, " for k in range(g["count"]))
     fill = "".join(f"o.in[{k}] = i{k}; " for k in range(g["count"]))
     text = SHIM + clip.source + f"""
-extern "C" void emu({params}const Tensor* t, double* sums) {{ Inputs o{{}}; {fill} clip_squares(o, t, {g["count"]}, {g["chunks"]}, sums); }}
+extern "C" void emu({params}const Tensor* t, double* sums) {{ Inputs o{{}}; {fill} clip_squares(o, t, {g["count"]}, {g["chunks"]}, {passing}, sums); }}
 """
     of = host[g["first"]:g["first"] + g["count"]]
     return run_kernel(text, "emu", g["blocks"], 256, [(h, 0) for h in of] + [(table[g["first"]:g["first"] + g["count"]], 0), (np.zeros(g["blocks"]), 1)])[0]
@@ -84,7 +84,7 @@ def test_the_kernels_match_the_oracle(k, most):
     sizes, dtypes = GROUPS[k]
     host, values = inputs(sizes, dtypes, 0.3, seed=k)
     clip = ha.GradientClip(sizes, dtypes)
-    got, norm, sums = emulated(clip, host, most)
+    got, norm, sums = emulated(clip, host, most, passing=k % 2)
     check(dtypes, values, most, got, norm)
     text = SHIM + clip.source + f"\nextern \"C\" void emu(const double* sums, float* norm) {{ clip_norm(sums, {len(sums)}, norm); }}\n"
     check_norm(values, run_kernel(text, "emu", 1, 256, [(sums, 0), (np.zeros(1, np.float32), 1)])[0][0])
@@ -113,7 +113,12 @@ def test_workgroups_are_dealt_by_the_work():
     clip = ha.GradientClip([1 << 28] * 130 + [16], "bf16")
     groups = groups_of(clip)
     assert len(groups) == 2 and groups[0]["first_sum"] == 0 and groups[1]["first_sum"] == groups[0]["blocks"]
-    assert sum(g["blocks"] for g in groups) <= 2048 and groups[0]["blocks"] > 60 * groups[1]["blocks"] > 0
+    assert sum(g["blocks"] for g in groups) <= 1025 and groups[0]["blocks"] > 60 * groups[1]["blocks"] > 0
+    # (192 MB stay in the caches: 12288 chunks from the end)
+    chunks = [128 << 15, (2 << 15) + 1]
+    assert [g["passing"] for g in groups] == [chunks[0], chunks[1] - 12288]
+    groups = groups_of(ha.GradientClip([1 << 20] * 128 + [1 << 20], "f32"))
+    assert [g["passing"] for g in groups] == [129 * 256 - 12288, 0]
     assert groups_of(ha.GradientClip([3, 4], "f32"))[0]["blocks"] == 2
     table = np.frombuffer(clip.table(), TABLE)
     assert np.array_equal(table["first"][:3], [0, 1 << 15, 2 << 15]) and table["bytes"][130] == 32
