@@ -7,14 +7,14 @@ The convolutions, the loss and their gradients are recorded helium-ir graphs; gr
 step of the filters are calls on the tensors those graphs read and write. Group norm, unlike the batch norm of harness/resnet.py, has
 no running statistics and one behaviour in training and use, and its gradients here are its own rules instead of the some sixty recorded ops.
 The other parameters (gamma, beta, the linear layer) are trained by plain gradient steps, as a matrix's orthogonalised update
-has no meaning for vectors.
+has no meaning for vectors. With `max_norm` all gradients are clipped by their norm together before the steps.
 
 Everything that one step makes stays on the device; only the loss comes back. `execute_graph` works on streams of the library's own, the operators on the
 caller's (here the default one), so the two wait for each other with device.synchronize() at every change.
 """
 import numpy as np
 
-from helium_amd import GroupNorm, Muon, device
+from helium_amd import GradientClip, GroupNorm, Muon, device
 from helium_amd.backend import Tensor, execute_graph
 
 from . import autodiff as ad
@@ -79,10 +79,11 @@ class Stage:
 
 
 class Classifier:
-    """channels: of the image, then of each stage's result. dtype: of images, activations and flows; parameters are f32."""
+    """channels: of the image, then of each stage's result. dtype: of images, activations and flows; parameters are f32. max_norm: what the norm
+    of all gradients together is clipped to, None for no clipping."""
 
     def __init__(self, batch, extent, channels, groups, classes, dtype="bf16", precision="f32_f32", seed=66, learning_rate=0.02,
-                 momentum=0.95, weight_decay=0.01, other_rate=0.1):
+                 momentum=0.95, weight_decay=0.01, other_rate=0.1, max_norm=None):
         rng = np.random.default_rng(seed)
         self.dtype, self.settings = dtype, dict(learning_rate=learning_rate, momentum=momentum, weight_decay=weight_decay)
         self.stages = [Stage(rng, batch, extent, i, o, groups, dtype, "silu" if k == SILU_STAGE else "relu", k == 0)
@@ -105,19 +106,27 @@ class Classifier:
         self.head_graph = G.g
         self.loss = G.g.new_output(loss.raw.node)
         self.d_activation = G.g.new_output(grads[activation.id].into_data_type(dtype).node)
-        self.new_linear = G.g.new_output((ad.Tensor(linear.value.raw) - ad.Tensor(grads[linear.id]) * other_rate).raw.node)
+        # (a gradient that is to be clipped leaves the graph, and the step follows with that of the others)
+        self.max_norm = max_norm
+        if max_norm is None:
+            self.new_linear = G.g.new_output((ad.Tensor(linear.value.raw) - ad.Tensor(grads[linear.id]) * other_rate).raw.node)
+        else:
+            self.d_linear = G.g.new_output(grads[linear.id].node)
         self.head_feeds = {n: Tensor.from_numpy(a, "f32", a.size) for n, a in G.feeds.items()}
 
-        # the step of gamma and beta of all stages
+        # the step of gamma and beta of all stages, and of the linear layer where its gradient is clipped
         G = ad.Graph()
         self.affine_in, self.affine_out = [], []
-        for s in self.stages:
-            for _ in ("gamma", "beta"):
-                value, gradient = (ad.Tensor(ad.Raw(G, G.g.new_input([s.norm.channels], "f32"))) for _ in range(2))
-                self.affine_in += [value.raw.node, gradient.raw.node]
-                self.affine_out.append(G.g.new_output((value - gradient * other_rate).raw.node))
+        for extents in [[s.norm.channels] for s in self.stages for _ in ("gamma", "beta")] + ([] if max_norm is None else [[last, classes]]):
+            value, gradient = (ad.Tensor(ad.Raw(G, G.g.new_input(extents, "f32"))) for _ in range(2))
+            self.affine_in += [value.raw.node, gradient.raw.node]
+            self.affine_out.append(G.g.new_output((value - gradient * other_rate).raw.node))
         self.affine_graph = G.g
         self.affine_feeds = {n: Tensor.from_numpy(a, "f32", a.size) for n, a in G.feeds.items()}
+        if max_norm is not None:
+            sizes = [s.filter_shape[0] * s.filter_shape[1] for s in self.stages] + [s.norm.channels for s in self.stages for _ in range(2)] + [weights.size]
+            self.clip = GradientClip(sizes, [dtype] * len(self.stages) + ["f32"] * (2 * len(self.stages) + 1))
+            self.norm = Tensor.from_numpy(np.zeros(1, np.float32), "f32", 1)
 
     def graphs(self):
         return [g for s in self.stages for g in (s.forward_graph, s.backward_graph)] + [self.head_graph, self.affine_graph]
@@ -128,15 +137,29 @@ class Classifier:
         for s in self.stages:
             x = s.forward(x)
         got = execute_graph(self.head_graph, {**self.head_feeds, **dict(zip(self.head_in, (x, self.linear, labels)))})
-        flow, self.next_linear = got[self.d_activation], got[self.new_linear]
+        flow = got[self.d_activation]
+        if self.max_norm is None:
+            self.next_linear = got[self.new_linear]
+        else:
+            self.linear_gradient = got[self.d_linear]
         for s in reversed(self.stages):
             flow = s.backward(flow)
         return float(got[self.loss].to_numpy()[0])
+
+    def all_gradients(self):
+        """Of the filters, of gamma and beta of each stage, and of the linear layer, where gradients are clipped."""
+        return [s.filter_gradient for s in self.stages] + [t for s in self.stages for t in (s.d_gamma, s.d_beta)] + [self.linear_gradient]
 
     def step(self, image, labels):
         """One training step; returns the loss before it."""
         loss = self.gradients(image, labels)
         feeds = [t for s in self.stages for t in (s.gamma, s.d_gamma, s.beta, s.d_beta)]
+        if self.max_norm is not None:
+            gradients = self.all_gradients()
+            device.synchronize()
+            self.clip.clip(gradients, gradients, self.max_norm, self.norm)
+            device.synchronize()
+            feeds += [self.linear, self.linear_gradient]
         got = execute_graph(self.affine_graph, {**self.affine_feeds, **dict(zip(self.affine_in, feeds))})
         device.synchronize()
         filters, momenta = [s.filter for s in self.stages], [s.momentum for s in self.stages]
@@ -144,7 +167,7 @@ class Classifier:
         device.synchronize()
         for k, s in enumerate(self.stages):
             s.gamma, s.beta = got[self.affine_out[2 * k]], got[self.affine_out[2 * k + 1]]
-        self.linear = self.next_linear
+        self.linear = self.next_linear if self.max_norm is None else got[self.affine_out[-1]]
         return loss
 
 
