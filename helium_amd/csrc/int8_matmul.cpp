@@ -15,8 +15,7 @@ namespace {
 // ---- device text ---------------------------------------------------------------------------------------------------
 // y[t][n] = (sum over k of x[t][k] w[n][k]) x_scale[t] w_scale[n] + bias[n]. The sums are whole numbers in 32 bits and exact (fewer than 2^17
 // products of at most 2^14), so that no cut of a sum changes a result. The definitions ahead of the text hold the type of the result (BF16, F16)
-// and the shape: of tiles TN, TM, WAVES_N, WAVES_M, STAGES, AHEAD; of streams BN, BM, WAVES,
-// STEPS (of 64 bytes of k, on their way at a time, twice).
+// and the shape: of tiles TN, TM, WAVES_N, WAVES_M, STAGES, AHEAD; of streams BN, BM, WAVES, STEPS (of 64 bytes of k, on their way at a time, twice).
 //
 // Weights are the instruction's rows and tokens its columns: a lane then has four neighbouring channels of one token at a time.
 const char* kCommon = R"HIP(
@@ -57,8 +56,9 @@ struct Call {
 __device__ __forceinline__ i32x4* parked_at(const Call& c, u32 share, u32 m, u32 n) {
     return (i32x4*)(c.parked + ((u64)share * c.tokens + m) * c.parked_pitch + n);
 }
-// One rounding of the sum to f32, one of each product, one of the bias' addition, and that to the result's type.
-__device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale) { return (float)sum * x_scale * w_scale; }
+// One rounding of the sum to f32, one of its product with the token's scale, one with the channel's and the bias added, and that to the result's type: the same
+// in every shape and cut.
+__device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale, float bias) { return __builtin_fmaf((float)sum * x_scale, w_scale, bias); }
 typedef out_t out4_any __attribute__((ext_vector_type(4), aligned(sizeof(out_t))));
 __device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 sum) {
     const float x_scale = c.x_scales[m];
@@ -67,7 +67,7 @@ __device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 su
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const u32 of = n + k < c.channels ? n + k : c.channels - 1;
-        out[k] = (out_t)(scaled(sum[k], x_scale, c.w_scales[of]) + (c.bias ? c.bias[of] : 0.0f));
+        out[k] = (out_t)scaled(sum[k], x_scale, c.w_scales[of], c.bias ? c.bias[of] : 0.0f);
     }
     if (n + 4 <= c.channels) *(out4_any*)to = out;
     else
@@ -79,6 +79,11 @@ __device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 su
 
 // Tiles. Rows of 128 bytes of k go from memory straight into a ring of STAGES k-tiles in LDS and from there, 16 bytes to a lane, into the
 // matrix instructions (32 x 32 x 32).
+//
+// 256 x 256: 4096 x 4096 x 4096 64 to 66 us (2100 TOPS; the instructions alone would take 31 at the 2.1 GHz that such products run at), 10 of them beginning and
+// end: results leave when no sums are left to hide them. Per k-tile a CU reads 192 KB of LDS and writes 64, 2048 clocks, as many as its instructions
+// take, and both together take 1.75 us (3700 clocks). Waves of 64 x 128, four along the channels, 64 us, 128 x 64 66, 32 x 256 71; raised priority for the
+// instructions 69; four waves of 128 x 128 69.
 const char* kTile = R"HIP(
 #define WTN (TN / WAVES_N)
 #define WTM (TM / WAVES_M)
@@ -105,6 +110,7 @@ struct False { static constexpr int value = 0; constexpr operator bool() const {
 // What a wave stores of its sums: 32 tokens at a time through its strip, so that whole vectors of channels go out.
 __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Call& c, u32 n0, u32 m0, const float* w_scales, const float* bias, out_t* strip) {
     const u32 lane = threadIdx.x & 63u, half = lane >> 5;
+    const bool past = (u64)c.tokens * c.channels >= (1u << 21);   // (results of 4 MB and more bypass the caches: 4096 x 4096 x 4096 67.5 -> 66.5 us)
 #pragma unroll
     for (int j = 0; j < MB; j++) {
         const u32 m = m0 + j * 32 + (lane & 31u);
@@ -117,7 +123,7 @@ __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Ca
                 const f32x4 ws = *(const f32x4*)(w_scales + n), b = *(const f32x4*)(bias + n);
                 out4 out;
 #pragma unroll
-                for (int k = 0; k < 4; k++) out[k] = (out_t)(scaled(acc[i][j][e * 4 + k], x_scale, ws[k]) + b[k]);
+                for (int k = 0; k < 4; k++) out[k] = (out_t)scaled(acc[i][j][e * 4 + k], x_scale, ws[k], b[k]);
                 *(out4*)(strip + (lane & 31u) * STRIP_PITCH + n) = out;
             }
         // (the strip is the wave's own: what it wrote is there when its LDS accesses are done, which the reads' own waits see to)
@@ -131,11 +137,12 @@ __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Ca
             const out_v out = *(const out_v*)(strip + token * STRIP_PITCH + n);
             if (m0 + j * 32 + token >= c.tokens) continue;
             out_t* to = c.y + (u64)(m0 + j * 32 + token) * c.channels + n0 + n;
-            if (n0 + n + PER <= c.channels) *(out_any*)to = out;
-            else
+            if (n0 + n + PER > c.channels) {
 #pragma unroll
                 for (u32 k = 0; k < PER; k++)
                     if (n0 + n + k < c.channels) to[k] = out[k];
+            } else if (past) __builtin_nontemporal_store(out, (out_any*)to);
+            else *(out_any*)to = out;
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -328,6 +335,8 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 
 // Streams. Reading the weights once is nearly all there is to do for few tokens, so they go straight into registers, as many loads on their way as
 // there is room for; the tokens come out of the L2. The matrix instructions (16 x 16 x 64) are far from being a bound.
+//
+// One token, 4096 x 4096: 5.6 us, 3 of them a launch; 8192 inputs, 16384 channels (134 MB, more than the caches hold with two others) 25 us (5.3 TB/s).
 const char* kStream = R"HIP(
 extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     __shared__ __attribute__((aligned(16))) int sums[WAVES][BM * 16][BN * 16 + 4];
@@ -486,6 +495,9 @@ struct CallArg {
 struct Int8Kernels {
     std::string source;
     std::unique_ptr<JitKernel> product[kCount], join;
+    std::mutex mu;  // a call's two launches follow each other on their stream: they share the stream's scratch, which all products have in common
+    ReduceScratch scratch;
+    ~Int8Kernels() { scratch.release(); }
 
     explicit Int8Kernels(int dtype) {
         std::vector<std::string> texts(kCount);
@@ -548,8 +560,6 @@ Int8Matmul::Int8Matmul(const Int8Problem& pr) : pr_(pr) {
     kernels_ = Int8Kernels::of(pr.dtype);
 }
 
-Int8Matmul::~Int8Matmul() { scratch_.release(); }
-
 const std::string& Int8Matmul::source() const { return kernels_->source; }
 
 void Int8Matmul::multiply(int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales, const float* bias, void* y,
@@ -579,8 +589,8 @@ void Int8Matmul::multiply(int64_t tokens, const void* x, const float* x_scales, 
         return;
     }
     const uint32_t join_grid[3] = {(uint32_t)cut(tokens * (int64_t)cut(pr_.channels, 4), 256), 1, 1}, join_block[3] = {256, 1, 1};
-    std::lock_guard<std::mutex> lk(mu_);
-    call.parked = (int32_t*)scratch_.get(kMostParked, 0, stream).floats;
+    std::lock_guard<std::mutex> lk(kernels_->mu);
+    call.parked = (int32_t*)kernels_->scratch.get(kMostParked, 0, stream).floats;
     kernels_->product[c.shape]->launch(grid, block, 0, stream, args);
     kernels_->join->launch(join_grid, join_block, 0, stream, args, true);
 }

@@ -44,7 +44,6 @@ struct Int8Kernels;
 class Int8Matmul {
 public:
     explicit Int8Matmul(const Int8Problem& pr);
-    ~Int8Matmul();
     void multiply(int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales, const float* bias, void* y,
                   hipStream_t stream);
     const std::string& source() const;
@@ -53,8 +52,6 @@ public:
 private:
     Int8Problem pr_;
     std::shared_ptr<Int8Kernels> kernels_;
-    std::mutex mu_;  // a call's launches follow each other on their stream: they share the stream's scratch
-    ReduceScratch scratch_;
 };
 
 }  // namespace he

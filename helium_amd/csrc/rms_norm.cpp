@@ -97,7 +97,8 @@ template <bool SUM, bool MOST> __device__ __forceinline__ void over_row(float& s
     }
 #endif
 }
-#define STORE(p, v) __builtin_nontemporal_store(v, p)
+// (a macro: a template's parameter would lose the vectors' alignment)
+#define STORE(past, p, v) do { if (past) __builtin_nontemporal_store(v, p); else *(p) = (v); } while (0)
 )HIP";
 
 // 8 bits. Adding 1.5 * 2^23 to a value within +-2^22 rounds it to a whole number, which the sum's last bits are (1.5 * 2^52 in 64 bits).
@@ -123,9 +124,13 @@ __device__ __forceinline__ void store_padding(u8* row, const Lane& p) {
 // A row is read once and held in registers; its sum of squares (and the largest |h gamma|) are joined over its lanes, and the results
 // are written. In 8 bits: with p = h gamma and P = max |p|, q = rint(127 p / P) needs no 1 / rms, which goes into the scale,
 // rstd P / 127, alone.
+//
+// Bound by memory: 8192 x 4096 bf16 with a residual 47.1 us (5.7 TB/s, the rate of a copy), into 8 bits 2048 x 4096 10.6 us (5.5 TB/s); f32 residuals beside
+// 16-bit operands, 2000 x 16384, 71 us (5.5 TB/s; 90 with accesses of 16 bytes of the narrower type). One row of 4096: a launch, 2.5 us.
 const char* kForward = R"HIP(
-extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const elem_t* x, const param_t* __restrict__ gamma, const stream_t* residual,
-                                                             stream_t* new_residual, void* y, float* __restrict__ rstd_out, float* __restrict__ scales) {
+// PAST: results bypass the caches
+template <bool PAST> __device__ __forceinline__ void forward(u64 rows, const elem_t* x, const param_t* __restrict__ gamma, const stream_t* residual,
+                                                            stream_t* new_residual, void* y, float* __restrict__ rstd_out, float* __restrict__ scales) {
     __shared__ float red[WAVES][2];
     const Lane p = lane();
     const u64 row = (u64)blockIdx.x * ROWS + p.slot;
@@ -179,7 +184,7 @@ extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const ele
     // (not before all lanes have what they read: a ragged row's last two vectors overlap, and the new residual may lie in the old one's place)
 #pragma unroll
     for (int k = 0; k < NV; k++)
-        if (there && HAS(p, k)) STORE((stream_v*)(new_residual + row * C + start(p, k)), hr[k]);
+        if (there && HAS(p, k)) STORE(PAST, (stream_v*)(new_residual + row * C + start(p, k)), hr[k]);
 #endif
     const float rstd = 1.0f / sqrtf(sum / (float)C + EPS);
     if (rstd_out && there && p.l == 0) rstd_out[row] = rstd;
@@ -211,16 +216,22 @@ extern "C" __global__ __launch_bounds__(T) void rows_forward(u64 rows, const ele
             elem_v out;
 #pragma unroll
             for (int i = 0; i < V; i++) AT(out, i) = (elem_t)(h[k][i] * rstd * weight[k][i]);
-            STORE((elem_v*)((elem_t*)y + row * C + c), out);
+            STORE(PAST, (elem_v*)((elem_t*)y + row * C + c), out);
         }
 #endif
 }
+#define FORWARD(name, past) \
+    extern "C" __global__ __launch_bounds__(T) void name(u64 rows, const elem_t* x, const param_t* gamma, const stream_t* residual, stream_t* new_residual, void* y, float* rstd, float* scales) { forward<past>(rows, x, gamma, residual, new_residual, y, rstd, scales); }
+FORWARD(rows_forward, true)
+FORWARD(rows_forward_few, false)   // results that stay in the caches for whoever reads them next
 )HIP";
 
 // q = rint(127 x / A), exactly, ties to even. 127 / A is taken in two parts, and x times both is added up with one rounding: a quotient in the
 // middle of two whole numbers (x = A / 2 has one) is a value of the type, and so comes out as itself. Any other one is further from the middle
 // than it is off: x = a 2^i and A = b 2^j with whole a and b give a distance of at least 1 / (2 a) of x / A, where the error is 2^-16 of that
 // in f32 (a has 8 or 11 bits) and 2^-45 in f64 (24 bits).
+//
+// 4096 x 4096 bf16 10.9 us (4.6 TB/s), f32 14.9 (5.6 TB/s). Deciding by the remainder instead was bound by its arithmetic: 17.7 us.
 const char* kQuantize = R"HIP(
 #if BF16 || F16
 typedef float wide_t;
@@ -285,7 +296,10 @@ extern "C" __global__ __launch_bounds__(T) void rows_quantize(u64 rows, const el
 )HIP";
 
 // With xh = h rstd and flow = dy gamma: dh' = dh + rstd (flow - xh mean(flow xh)), dgamma = sum over the rows of dy xh. A workgroup goes through rows
-// `gridDim.x` apart and keeps its share of dgamma in registers; `rows_fold` adds up the workgroups' shares. The order is fixed.
+// `blocks` apart and keeps its share of dgamma in registers; `rows_fold` adds up the workgroups' shares. The order is fixed.
+//
+// Bound by memory: 8192 x 4096 bf16 with the residual's gradient 50.8 us with the fold (5.3 TB/s); with the next row's loads under conditions, or with
+// gamma's loads in between, 57 to 60: the counter of loads then runs to zero before each row.
 const char* kBackward = R"HIP(
 template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 blocks, const elem_t* dy, const stream_t* h, const param_t* __restrict__ gamma,
                                                              const float* __restrict__ rstd_of, const stream_t* dh, elem_t* dx, stream_t* dresidual,
@@ -314,7 +328,7 @@ template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 bloc
         }
     };
     // (gamma stays as well: a load between a row's and the next row's would be waited for with both)
-    #if T < 1024
+#if T < 1024
     float held[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; k++)
@@ -360,8 +374,8 @@ template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 bloc
                     AT(out, i) = (elem_t)d;
                     AT(more, i) = (stream_t)d;
                 }
-                if (dx) STORE((elem_v*)(dx + at), out);
-                if (dresidual) STORE((stream_v*)(dresidual + at), more);
+                if (dx) STORE(true, (elem_v*)(dx + at), out);
+                if (dresidual) STORE(true, (stream_v*)(dresidual + at), more);
             }
         if (T == 1024) load(next, row + step);
     }
@@ -474,6 +488,7 @@ RmsNorm::RmsNorm(const RowProblem& pr) : pr_(pr) {
     auto compiled = std::async(std::launch::async, [&] { if (has_back) (void)rtc_compile(back, "rows_backward", {}); });
     source_ = text + kBytes + (pr.norm ? kForward : kQuantize);
     forward_ = std::make_unique<JitKernel>(source_, pr.norm ? "rows_forward" : "rows_quantize");
+    if (pr.norm) forward_few_ = std::make_unique<JitKernel>(source_, "rows_forward_few");
     compiled.get();
     if (has_back) {
         backward_ = std::make_unique<JitKernel>(back, "rows_backward");
@@ -515,7 +530,9 @@ void RmsNorm::forward(int64_t rows, const void* x, const void* gamma, const void
     const uint32_t grid[3] = {(uint32_t)blocks, 1, 1}, block[3] = {(uint32_t)t.threads, 1, 1};
     void* args[] = {&count, &x, &gamma, &residual, &new_residual, &y, &rstd, &scales};
     void* quantize_args[] = {&count, &x, &y, &scales};
-    forward_->launch(grid, block, 0, stream, pr_.norm ? args : quantize_args, true);
+    // (results of 4 MB and more in 16 bits bypass the caches: 8192 x 4096 48.6 -> 47.1 us; asking in the kernel cost as much again)
+    const bool few = pr_.norm && rows * pr_.columns < (1 << 21);
+    (few ? forward_few_ : forward_)->launch(grid, block, 0, stream, pr_.norm ? args : quantize_args, true);
 }
 
 void RmsNorm::backward(int64_t rows, const void* dy, const void* h, const void* gamma, const float* rstd, const void* dh, void* dx, void* dresidual,

@@ -49,7 +49,7 @@ private:
     RowProblem pr_;
     RowTiling tiling_;
     std::string source_, describe_;
-    std::unique_ptr<JitKernel> forward_, backward_, backward_more_, fold_;
+    std::unique_ptr<JitKernel> forward_, forward_few_, backward_, backward_more_, fold_;
     std::mutex mu_;  // a backward pass's launches follow each other on their stream: they share the stream's scratch
     ReduceScratch scratch_;
 };

@@ -572,8 +572,9 @@ typedef struct he_int8_matmul_s* he_int8_matmul_t;
  * device. */
 int he_int8_matmul_create(he_int8_matmul_t* matmul, int64_t inputs, int64_t channels, int dtype);
 /* x and weights are aligned to 16 bytes, everything else to its own type; bias may be NULL; y shares no memory with the operands. At most 2^24
- * tokens; there may be none. The first call on a stream that shares out its sums allocates scratch for it, later ones allocate nothing; calls on several
- * streams may overlap. Captured graphs that may run at the same time are captured on streams of their own, or from handles of their own. */
+ * tokens; there may be none. The first call on a stream that shares out its sums (he_int8_matmul_describe says which do) allocates 16 MB for it, which all
+ * products of a result type have in common; later ones allocate nothing. Calls on several streams may overlap; captured graphs that may run at the same time are
+ * captured on streams of their own. */
 int he_int8_matmul(he_int8_matmul_t matmul, int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales,
                    const float* bias, void* y, he_stream_t stream);
 /* The generated HIP source of all shapes, and how a call with so many tokens is cut (at most `capacity` bytes of text). */

@@ -48,6 +48,18 @@ def test_every_shape_and_cut(gpu, monkeypatch, shape, shares, size):
     check(host, dtype, to_f32(multiply(ha.Int8Matmul(columns, channels, dtype), host, dtype), dtype))
 
 
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_no_cut_changes_a_bit(gpu, monkeypatch, tokens):
+    host = inputs(tokens, 8300, 130, bias=True, seed=6)
+    op = ha.Int8Matmul(8300, 130, "f32")
+    want = multiply(op, host, "f32")
+    for shape in range(9):
+        for shares in (1, 2, 4):
+            monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+            monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
+            assert np.array_equal(multiply(op, host, "f32"), want), (shape, shares)
+
+
 @pytest.mark.parametrize("tokens,columns,channels", [(1, 8192, 64), (40, 6000, 64), (300, 9000, 300)])
 def test_the_largest_sums_are_exact(gpu, tokens, columns, channels):
     """Every product 127 * 127, and sums far beyond the 24 bits of f32 (of which the result keeps the first)."""

@@ -68,7 +68,7 @@ BACKWARD_TYPES = dict(zip(BACKWARD, ("const elem_t*", "const stream_t*", "const 
 def emulated_forward(tiling, text, rows, buffers):
     """buffers: by name (array, mode)"""
     params, args = pointers(FORWARD, FORWARD_TYPES, buffers)
-    call = f"rows_forward(*rows, {args})" if "gamma" in buffers else "rows_quantize(*rows, x, (u8*)y, scales)"
+    call = f"rows_forward_few(*rows, {args})" if "gamma" in buffers else "rows_quantize(*rows, x, (u8*)y, scales)"
     text += f"\nextern \"C\" void emu_forward(const u64* rows, {params}) {{ {call}; }}\n"
     given = [buffers[n] for n in FORWARD if n in buffers]
     side = tiling["threads"] // tiling["lanes"]
