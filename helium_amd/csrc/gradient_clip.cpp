@@ -167,7 +167,8 @@ extern "C" __global__ __launch_bounds__(256) void clip_scale(Both o, const Tenso
         else load<false>(h, o.in[t] + at, left);
         if (k == blockIdx.x) {
             const double n = norm_of(sums, sum_count, waves), c = (double)most / (n + 1e-6);
-            by = (float)(c > 1.0 ? 1.0 : c);   // (a norm that is NaN makes everything so)
+            // (a norm that is NaN makes everything so, unless nothing is to be clipped)
+            by = most == __builtin_inff() || c > 1.0 ? 1.0f : (float)c;
             if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
         }
         // (nothing to do in place where nothing is clipped)

@@ -52,7 +52,7 @@ class GradientClip:
         check(lib.he_gradient_norm(self.handle, a, n, _at(norm), _h(stream)))
 
     def clip(self, gradients, out, most, norm=None, stream=None):
-        """out[k] = gradients[k] * min(1, most / (norm + 1e-6)); it may be gradients[k]. norm receives the norm before clipping."""
+        """out[k] = gradients[k] * min(1, most / (norm + 1e-6)); it may be gradients[k], but results share no memory. norm receives the norm before clipping."""
         (a, n), (b, m) = _list(gradients), _list(out)
         if n != m:
             raise ValueError(f"{n} gradients and {m} results")

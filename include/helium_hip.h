@@ -540,8 +540,8 @@ int he_rms_norm_forward(he_rms_norm_t norm, int64_t rows, const void* x, const v
 /* dy: of y; h, rstd: as the forward pass had them; dh: what reaches h from its other readers, NULL for nothing. The gradient of h, which is
  * that of x and of the residual, goes to dx (dtype) and dresidual (residual_dtype), of which one may be NULL; dx may be dy, or h where their types are the same,
  * and dresidual may be dh or h. dgamma [columns] is f32, summed over the rows in a fixed order, zero without rows. Not with to_i8. The first call
- * on a stream allocates scratch for it, later ones allocate nothing; calls on several streams may overlap. Captured graphs that may run at the
- * same time are captured on streams of their own, or from handles of their own. */
+ * on a stream allocates scratch for it, later ones allocate nothing; calls on several streams may overlap. A captured call works in the
+ * scratch of the stream it was captured on, wherever it is replayed: what may run at the same time is captured on streams of its own, or from handles of its own. */
 int he_rms_norm_backward(he_rms_norm_t norm, int64_t rows, const void* dy, const void* h, const void* gamma, const float* rstd, const void* dh,
                          void* dx, void* dresidual, float* dgamma, he_stream_t stream);
 const char* he_rms_norm_source(he_rms_norm_t norm);
@@ -558,7 +558,8 @@ int64_t he_quantized_pitch(int64_t columns);
 
 typedef struct he_quantize_rows_s* he_quantize_rows_t;
 /* scale = A / 127 with A the largest |x| of the row, q = the whole number nearest to 127 x / A, ties to even. A row of zeros has scale 0; one that is
- * not finite throughout has scale NaN and zeros (products with it are NaN). dtype: of x, HE_F32, HE_BF16 or HE_F16; at most 32768 columns. */
+ * not finite throughout has scale NaN and zeros (products with it are NaN). dtype: of x, HE_F32, HE_BF16 or HE_F16; at most 32768 columns. q shares no memory with x. Alignment as
+ * in section 10. */
 int he_quantize_rows_create(he_quantize_rows_t* quantize, int64_t columns, int dtype);
 int he_quantize_rows(he_quantize_rows_t quantize, int64_t rows, const void* x, void* q, float* scales, he_stream_t stream);
 const char* he_quantize_rows_source(he_quantize_rows_t quantize);
@@ -573,8 +574,8 @@ typedef struct he_int8_matmul_s* he_int8_matmul_t;
 int he_int8_matmul_create(he_int8_matmul_t* matmul, int64_t inputs, int64_t channels, int dtype);
 /* x and weights are aligned to 16 bytes, everything else to its own type; bias may be NULL; y shares no memory with the operands. At most 2^24
  * tokens; there may be none. The first call on a stream that shares out its sums (he_int8_matmul_describe says which do) allocates 16 MB for it, which all
- * products of a result type have in common; later ones allocate nothing. Calls on several streams may overlap; captured graphs that may run at the same time are
- * captured on streams of their own. */
+ * products of a result type have in common; later ones allocate nothing. Calls on several streams may overlap. A captured call works in the scratch of the stream
+ * it was captured on, wherever it is replayed: what may run at the same time is captured on streams of its own. */
 int he_int8_matmul(he_int8_matmul_t matmul, int64_t tokens, const void* x, const float* x_scales, const void* weights, const float* weight_scales,
                    const float* bias, void* y, he_stream_t stream);
 /* The generated HIP source of all shapes, and how a call with so many tokens is cut (at most `capacity` bytes of text). */
@@ -592,12 +593,13 @@ typedef struct he_gradient_clip_s* he_gradient_clip_t;
 int he_gradient_clip_create(he_gradient_clip_t* clip, const int64_t* sizes, const int* dtypes, int count);
 /* norm[0] = sqrt(sum of the squares of all values), added up in 64 bits in a fixed order. A list of `count` device addresses in host memory,
  * each aligned to its own type; that of a tensor without values may be NULL. The first call on a stream allocates workspace for it, later ones allocate
- * nothing; calls on several streams may overlap. Captured graphs that may run at the same time are captured on streams of their own, or from
- * handles of their own. */
+ * nothing; calls on several streams may overlap. A captured call works in the workspace of the stream it was captured on, wherever it is replayed: what
+ * may run at the same time is captured on streams of its own, or from handles of its own. */
 int he_gradient_norm(he_gradient_clip_t clip, const void* const* gradients, int count, float* norm, he_stream_t stream);
 /* out[k] = gradients[k] * min(1, most / (norm + 1e-6)), rounded once to its type, and the norm (before clipping) in norm[0], which may be NULL. out[k] may be
- * gradients[k]; otherwise it shares no memory with any of them. most is 0 or more, infinity for no clipping. A norm that is NaN makes every result NaN, an infinite one
- * zeros (NaN where a value is infinite): norm[0] tells. */
+ * gradients[k]; otherwise it shares no memory with any of them, and results share none with each other (a gradient that is listed twice in place would be scaled
+ * twice). most is 0 or more; with infinity results are the gradients, whatever their norm. Otherwise a norm that is NaN makes every result NaN, an infinite one zeros (NaN
+ * where a value is infinite): norm[0] tells. */
 int he_gradient_clip(he_gradient_clip_t clip, const void* const* gradients, void* const* out, int count, float most, float* norm,
                      he_stream_t stream);
 /* The generated HIP source, how the tensors are cut, and the table the kernels read, for inspection and tests. */

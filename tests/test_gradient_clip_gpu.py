@@ -86,6 +86,17 @@ def test_norms_that_are_not_finite_are_told(gpu):
             assert np.isinf(norm) and np.isnan(got[0][77]) and not np.delete(got[0], 77).any() and not to_f32(got[1], "bf16").any()
 
 
+def test_nothing_is_clipped_to_infinity(gpu):
+    host, values = inputs([3000, 40], ["f32", "bf16"], 0.3, seed=8)
+    clip = ha.GradientClip([3000, 40], ["f32", "bf16"])
+    for bad in (0.5, np.nan, np.inf):
+        host[0][77] = bad
+        for in_place in (False, True):
+            got, norm = clipped(clip, host, np.inf, in_place)
+            assert all(np.array_equal(g, h, equal_nan=True) for g, h in zip(got, host))
+            assert np.isfinite(norm) == np.isfinite(bad)
+
+
 def test_results_are_the_same_from_call_to_call_and_overlapping_streams(gpu):
     sizes, dtypes = [300_000, 11, 5000], ["f32", "bf16", "f16"]
     clip = ha.GradientClip(sizes, dtypes)
