@@ -78,8 +78,7 @@ extern "C" void emu({params}const Tensor* t, double* sums) {{ Inputs o{{}}; {fil
     return run_kernel(text, "emu", g["blocks"], 256, [(h, 0) for h in of] + [(table[g["first"]:g["first"] + g["count"]], 0), (np.zeros(g["blocks"]), 1)])[0]
 
 
-@pytest.mark.parametrize("k", range(len(GROUPS)))
-@pytest.mark.parametrize("most", [0.5, 1e6])
+@pytest.mark.parametrize("k,most", [(k, most) for k in range(len(GROUPS)) for most in (0.5, 1e6) if len(GROUPS[k][0]) < 100 or most == 0.5])
 def test_the_kernels_match_the_oracle(k, most):
     sizes, dtypes = GROUPS[k]
     host, values = inputs(sizes, dtypes, 0.3, seed=k)

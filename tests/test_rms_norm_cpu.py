@@ -111,9 +111,8 @@ def test_the_kernels_match_the_oracle(shape, dtype, residual, same):
     buffers["dx"] = (np.empty_like(host["x"]), 1)
     if residual:
         buffers.update(dh=(host["dh"], 0), dresidual=(np.empty_like(host["h"]), 1))
-    for blocks in (1, 3)[columns > 1000:]:
-        got = emulated_backward(tiling, back, rows, columns, blocks, buffers)
-        check_backward(dtype, residual, v, to_f32(got["dx"], dtype), to_f32(got["dresidual"], residual) if residual else None, got["dgamma"], rows)
+    got = emulated_backward(tiling, back, rows, columns, 3, buffers)   # (of fewer rows, workgroups without any leave zeros)
+    check_backward(dtype, residual, v, to_f32(got["dx"], dtype), to_f32(got["dresidual"], residual) if residual else None, got["dgamma"], rows)
 
 
 @pytest.mark.parametrize("shape,dtype,residual,same", [c for c in CASES if c[0][1] < 2000][2::2])
