@@ -60,15 +60,23 @@ __device__ __forceinline__ i32x4* parked_at(const Call& c, u32 share, u32 m, u32
 // in every shape and cut.
 __device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale, float bias) { return __builtin_fmaf((float)sum * x_scale, w_scale, bias); }
 typedef out_t out4_any __attribute__((ext_vector_type(4), aligned(sizeof(out_t))));
-__device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 sum) {
-    const float x_scale = c.x_scales[m];
-    out_t* to = c.y + (u64)m * c.channels + n;
-    out4_any out;
+struct Scales { float x, w[4], bias[4]; };   // of a token and four channels, of which the last may be missing
+__device__ __forceinline__ Scales scales_of(const Call& c, u32 m, u32 n) {
+    Scales s;
+    s.x = c.x_scales[m < c.tokens ? m : c.tokens - 1];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         const u32 of = n + k < c.channels ? n + k : c.channels - 1;
-        out[k] = (out_t)scaled(sum[k], x_scale, c.w_scales[of], c.bias ? c.bias[of] : 0.0f);
+        s.w[k] = c.w_scales[of];
+        s.bias[k] = c.bias ? c.bias[of] : 0.0f;
     }
+    return s;
+}
+__device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 sum, const Scales& s) {
+    out_t* to = c.y + (u64)m * c.channels + n;
+    out4_any out;
+#pragma unroll
+    for (int k = 0; k < 4; k++) out[k] = (out_t)scaled(sum[k], s.x, s.w[k], s.bias[k]);
     if (n + 4 <= c.channels) *(out4_any*)to = out;
     else
 #pragma unroll
@@ -80,10 +88,10 @@ __device__ __forceinline__ void store_four(const Call& c, u32 m, u32 n, i32x4 su
 // Tiles. Rows of 128 bytes of k go from memory straight into a ring of STAGES k-tiles in LDS and from there, 16 bytes to a lane, into the
 // matrix instructions (32 x 32 x 32).
 //
-// 256 x 256: 4096 x 4096 x 4096 64 to 66 us (2100 TOPS; the instructions alone would take 31 at the 2.1 GHz that such products run at), 10 of them beginning and
-// end: results leave when no sums are left to hide them. Per k-tile a CU reads 192 KB of LDS and writes 64, 2048 clocks, as many as its instructions
-// take, and both together take 1.75 us (3700 clocks). Waves of 64 x 128, four along the channels, 64 us, 128 x 64 66, 32 x 256 71; raised priority for the
-// instructions 69; four waves of 128 x 128 69.
+// 256 x 256: 4096 x 4096 x 4096 62 us (2220 TOPS), 8192 x 8192 x 8192 449 (2450). The instructions alone, on zeros, take 25 us of the 62, on numbers like the
+// operands' 40: the card lowers its clock under them. Loads alone take 39, reads of LDS 10; without the reads it is 62 as well, without the loads 55; some
+// 10 us are beginning and end, where results leave that no sums hide. Waves of 64 x 128, four along the channels or two, 62 us, four waves of
+// 128 x 128 65; tiles of 128 x 256 70, 192 x 192 77.
 const char* kTile = R"HIP(
 #define WTN (TN / WAVES_N)
 #define WTM (TM / WAVES_M)
@@ -98,23 +106,17 @@ const char* kTile = R"HIP(
 // a wave's strip of 32 tokens; two rows are apart by what a token's pair of lanes writes, so that they meet different banks
 #define STRIP_PITCH (WTN + 8)
 #define STRIP_VALUES (32 * STRIP_PITCH)
-#define STRIP_BYTES (STRIP_VALUES * WAVES_N * WAVES_M * (int)sizeof(out_t))
-#define LDS_BYTES (STAGES * STAGE_BYTES > STRIP_BYTES ? STAGES * STAGE_BYTES : STRIP_BYTES)
-
-__device__ __attribute__((aligned(16))) const u32 nothing[4] = {0, 0, 0, 0};   // what lies behind a row's end
+#define STRIPS ((WAVES_N * WAVES_M + STAGES - 1) / STAGES)   /* in a stage's room */
+static_assert(STRIPS * STRIP_VALUES * sizeof(out_t) <= STAGE_BYTES, "");
 
 struct Fragments { i32x4 w[NB], x[MB]; };
-struct True { static constexpr int value = 1; constexpr operator bool() const { return true; } };
-struct False { static constexpr int value = 0; constexpr operator bool() const { return false; } };
 
 // What a wave stores of its sums: 32 tokens at a time through its strip, so that whole vectors of channels go out.
-__device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Call& c, u32 n0, u32 m0, const float* w_scales, const float* bias, out_t* strip) {
+__device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Call& c, u32 n0, u32 m0, const float (&x_scales)[MB], const float* w_scales, const float* bias, out_t* strip) {
     const u32 lane = threadIdx.x & 63u, half = lane >> 5;
     const bool past = (u64)c.tokens * c.channels >= (1u << 21);   // (results of 4 MB and more bypass the caches: 4096 x 4096 x 4096 67.5 -> 66.5 us)
 #pragma unroll
     for (int j = 0; j < MB; j++) {
-        const u32 m = m0 + j * 32 + (lane & 31u);
-        const float x_scale = c.x_scales[m < c.tokens ? m : c.tokens - 1];
 #pragma unroll
         for (int i = 0; i < NB; i++)
 #pragma unroll
@@ -123,7 +125,7 @@ __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Ca
                 const f32x4 ws = *(const f32x4*)(w_scales + n), b = *(const f32x4*)(bias + n);
                 out4 out;
 #pragma unroll
-                for (int k = 0; k < 4; k++) out[k] = (out_t)scaled(acc[i][j][e * 4 + k], x_scale, ws[k], b[k]);
+                for (int k = 0; k < 4; k++) out[k] = (out_t)scaled(acc[i][j][e * 4 + k], x_scales[j], ws[k], b[k]);
                 *(out4*)(strip + (lane & 31u) * STRIP_PITCH + n) = out;
             }
         // (the strip is the wave's own: what it wrote is there when its LDS accesses are done, which the reads' own waits see to)
@@ -149,14 +151,6 @@ __device__ __forceinline__ void store_sums(const i32x16 (&acc)[NB][MB], const Ca
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
-// The scales and the bias of the tile's channels, in LDS: 1 and 0 where there are none.
-__device__ __forceinline__ void load_channels(const Call& c, u32 n0, float* w_scales, float* bias) {
-    for (u32 n = threadIdx.x; n < TN; n += WAVES_N * WAVES_M * 64) {
-        const bool there = n0 + n < c.channels;
-        w_scales[n] = there ? c.w_scales[n0 + n] : 1.0f;
-        bias[n] = there && c.bias ? c.bias[n0 + n] : 0.0f;
-    }
-}
 // Which tile a block makes. Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: an XCD takes neighbours, in groups of
 // four rows of tiles, whose weights and tokens they share.
 __device__ __forceinline__ void place(const Call& c, u32& tn, u32& tm) {
@@ -167,37 +161,114 @@ __device__ __forceinline__ void place(const Call& c, u32& tn, u32& tm) {
     tn = in / high;
 }
 
+// What a wave fetches of a k-tile. Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads meet different
+// banks, the chunk (l % 8) ^ (row / 2 % 8) of its 128 bytes: two rows fill the 64 banks, so rows two apart must differ. (A tile that ends beyond an
+// operand loads its last row there: sums that nothing stores. Behind a row's end its last chunk is loaded once more: what is read there of the tokens
+// counts as zeros.)
+struct Source { u32 wave, chunks, off[LOADS], chunk[2]; };
+// What it reads of a stage: the first of its rows of weights and of tokens, its half of a k-step's chunks, and where those lie.
+struct Reader { u32 w_at, x_at, half, swz; };
+__device__ __forceinline__ void fetch(u8* stage, const u8* w, const u8* x, const Source& s, u32 kt) {
+    u32 behind[2];   // by how many chunks a lane's lies behind the row's last, which it loads then
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const u32 last = s.chunks - 1, mine = kt * 8 + s.chunk[e];
+        behind[e] = mine > last ? mine - last : 0;
+    }
+#pragma unroll
+    for (int l = 0; l < LOADS; l++) {
+        const u32 row = (s.wave * LOADS + l) * 8;   // of the weights, then of the tokens
+        const u8* src = (row < TN ? w : x) + (u64)kt * ROW + (s.off[l] - behind[l & 1] * 16);
+        __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(stage + row * ROW), 16, 0, 0);
+    }
+}
+__device__ __forceinline__ void read(const u8* stage, const Reader& r, int kk, Fragments& g, bool whole, u32 chunks_left) {
+    const u8 *w = stage + r.w_at, *x = stage + r.x_at;
+    const u32 at = ((kk * 2 + r.half) ^ r.swz) * 16;
+#pragma unroll
+    for (int i = 0; i < NB; i++) g.w[i] = *(const i32x4*)(w + i * 32 * ROW + at);
+#pragma unroll
+    for (int j = 0; j < MB; j++) {
+        g.x[j] = *(const i32x4*)(x + j * 32 * ROW + at);
+        if (!whole && kk * 2 + r.half >= chunks_left) g.x[j] = i32x4{0, 0, 0, 0};
+    }
+}
+__device__ __forceinline__ void multiply(const Fragments& g, i32x16 (&acc)[NB][MB]) {
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) acc[i][j] = MFMA_32(g.w[i], g.x[j], acc[i][j]);
+}
+// One k-tile, from `from`; the one to come goes to `to`. The loop is rotated by AHEAD k-steps: the matrix instructions that the last k-tile left over cover
+// the barrier's way, the first reads of this one and the loads of the one to come; the reads of further steps are issued between the instructions of
+// those before. The order is asked for, since the compiler by itself reads, waits and multiplies in turn.
+//
+// Each stage is an array of its own, and the calls of a round of the ring name theirs: only so does the compiler know that a direct load does not write where
+// a read looks. Otherwise it has the reads wait for all loads that are on their way: 4096 x 4096 x 4096 66 us for 62, 512 x 4096 x 4096 17.9 for 14.7.
+template <bool MORE> __device__ __forceinline__ void k_tile(const u8* from, u8* to, const u8* w, const u8* x, const Source& s, const Reader& r, u32 kt, Fragments (&f)[2][AHEAD],
+                                                           i32x16 (&acc)[NB][MB]) {
+    // This wave's loads of the k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'. No wave still reads the
+    // stage that is filled next. (The bare barrier: __syncthreads() would wait for all loads.)
+    __builtin_amdgcn_s_waitcnt(WAIT_LOADS(MORE ? (STAGES - 2) * LOADS : 0));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int g = 0; g < 4 / AHEAD; g++) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) read(from, r, g * AHEAD + k, f[g & 1][k], MORE, s.chunks - kt * 8);
+        if (g == 0 && MORE) fetch(to, w, x, s, kt + STAGES - 1);
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) multiply(f[(g & 1) ^ 1][k], acc);
+        if (g == 0) {
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+            for (int n = 0; n < AHEAD * MMAS; n++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+                for (int l = n * LOADS / (AHEAD * MMAS); l < (n + 1) * LOADS / (AHEAD * MMAS); l++)
+                    if (MORE) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < AHEAD * MMAS; n++) {
+                // (reads behind the first instruction: the wait for its operands is for all reads before it)
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (n * 2 < AHEAD * READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (n * 2 + 1 < AHEAD * READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
+    }
+}
+
 extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS void int8_product(Call c) {
-    __shared__ __attribute__((aligned(16))) u8 lds[LDS_BYTES];
+    __shared__ __attribute__((aligned(16))) u8 s0[STAGE_BYTES], s1[STAGE_BYTES];
+#if STAGES > 2
+    __shared__ __attribute__((aligned(16))) u8 s2[STAGE_BYTES];
+#else
+    u8* const s2 = s1;
+#endif
+#if STAGES > 3
+    __shared__ __attribute__((aligned(16))) u8 s3[STAGE_BYTES];
+#else
+    u8* const s3 = s2;   // (the last)
+#endif
     __shared__ __attribute__((aligned(16))) float w_scales[TN], bias[TN];
     const u32 lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave_n = wave / WAVES_M, wave_m = wave % WAVES_M;
     u32 tn, tm;
     place(c, tn, tm);
     const u32 n0 = tn * TN, m0 = tm * TM;
-    const u8 *w_rows = c.w + (u64)n0 * c.pitch, *x_rows = c.x + (u64)m0 * c.pitch;
-    const u32 k_tiles = (c.pitch + ROW - 1) / ROW, chunks = c.pitch / 16;
-    const u32 k_begin = (u32)((u64)k_tiles * blockIdx.y / c.shares), k_end = (u32)((u64)k_tiles * (blockIdx.y + 1) / c.shares);
-    // Direct loads: lane l of the load of rows 8 r .. 8 r + 7 takes row l / 8 and, so that fragment reads meet different banks, the chunk
-    // (l % 8) ^ (row / 2 % 8) of its 128 bytes: two rows fill the 64 banks, so rows two apart must differ. (A tile that ends beyond an
-    // operand loads its last row there: sums that nothing stores.)
-    u32 off[LOADS], chunk[2] = {(lane & 7u) ^ (lane >> 4), (lane & 7u) ^ (4u + (lane >> 4))};
+    const u32 k_tiles = (c.pitch + ROW - 1) / ROW, halvings = __builtin_ctz(c.shares);   // (shares are a power of two)
+    const u32 k_begin = k_tiles * blockIdx.y >> halvings, k_end = k_tiles * (blockIdx.y + 1) >> halvings;
+    const u8 *w = c.w + (u64)n0 * c.pitch, *x = c.x + (u64)m0 * c.pitch;
+    Source source{wave, c.pitch / 16, {}, {(lane & 7u) ^ (lane >> 4), (lane & 7u) ^ (4u + (lane >> 4))}};
 #pragma unroll
     for (int l = 0; l < LOADS; l++) {
-        const u32 row = (wave * LOADS + l) * 8;   // of the weights, then of the tokens
-        const u32 of = row < TN ? row : row - TN, last = (row < TN ? c.channels - n0 : c.tokens - m0) - 1, mine = of + (lane >> 3);
-        off[l] = (mine < last ? mine : last) * c.pitch + chunk[l & 1] * 16;
+        const u32 row = (wave * LOADS + l) * 8, of = row < TN ? row : row - TN, last = (row < TN ? c.channels - n0 : c.tokens - m0) - 1, mine = of + (lane >> 3);
+        source.off[l] = (mine < last ? mine : last) * c.pitch + source.chunk[l & 1] * 16;
     }
-    auto fetch = [&](u32 kt, u32 slot) {
-        u8* base = lds + slot * STAGE_BYTES;
-        const bool whole = kt * 8 + 8 <= chunks;
-#pragma unroll
-        for (int l = 0; l < LOADS; l++) {
-            const u32 row = (wave * LOADS + l) * 8;
-            const u8* src = (row < TN ? w_rows : x_rows) + (u64)kt * ROW + off[l];
-            if (!whole && kt * 8 + chunk[l & 1] >= chunks) src = (const u8*)nothing;
-            __builtin_amdgcn_global_load_lds((const GLOBAL_AS u32*)src, (LDS_AS u32*)(base + row * ROW), 16, 0, 0);
-        }
-    };
+    const u32 frag_row = lane & 31u, half = lane >> 5;
+    const Reader reader{(wave_n * WTN + frag_row) * ROW, (TN + wave_m * WTM + frag_row) * ROW, half, lane >> 1 & 7u};
     i32x16 acc[NB][MB];
 #pragma unroll
     for (int i = 0; i < NB; i++)
@@ -205,36 +276,6 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
         for (int j = 0; j < MB; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-    const u32 frag_row = lane & 31u, half = lane >> 5, swz = lane >> 1 & 7u;
-    auto read = [&](Fragments& g, const u8* stage, int kk) {
-        const u8 *w = stage + (wave_n * WTN + frag_row) * ROW, *x = stage + (TN + wave_m * WTM + frag_row) * ROW;
-        const u32 at = ((kk * 2 + half) ^ swz) * 16;
-#pragma unroll
-        for (int i = 0; i < NB; i++) g.w[i] = *(const i32x4*)(w + i * 32 * ROW + at);
-#pragma unroll
-        for (int j = 0; j < MB; j++) g.x[j] = *(const i32x4*)(x + j * 32 * ROW + at);
-    };
-    auto multiply = [&](const Fragments& g) {
-#pragma unroll
-        for (int i = 0; i < NB; i++)
-#pragma unroll
-            for (int j = 0; j < MB; j++) acc[i][j] = MFMA_32(g.w[i], g.x[j], acc[i][j]);
-    };
-    u32 slot = 0;
-    // This wave's loads of a k-tile have landed (those of the STAGES - 2 behind it may be on their way), then the other waves'. No wave still reads the
-    // stage that is filled next. (The bare barrier: __syncthreads() would wait for all loads.)
-    auto meet = [&](auto more) {
-        if (more) __builtin_amdgcn_s_waitcnt(WAIT_LOADS((STAGES - 2) * LOADS));
-        else __builtin_amdgcn_s_waitcnt(WAIT_LOADS(0));
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    };
-    auto fetch_ahead = [&](u32 kt) { fetch(kt + STAGES - 1, slot + STAGES - 1 < STAGES ? slot + STAGES - 1 : slot - 1); };
-    const u32 k_count = k_end - k_begin, ahead = STAGES - 1 < k_count ? STAGES - 1 : k_count;
-    load_channels(c, n0, w_scales, bias);
-    for (u32 s = 0; s < ahead; s++) fetch(k_begin + s, s);
-    u32 kt = k_begin;
     Fragments f[2][AHEAD];
 #pragma unroll
     for (int s = 0; s < AHEAD; s++) {
@@ -243,75 +284,46 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 #pragma unroll
         for (int j = 0; j < MB; j++) f[1][s].x[j] = i32x4{0, 0, 0, 0};
     }
-#if AHEAD == 1
-    // The loop is rotated by a k-step: the matrix instructions that the last k-tile left over cover the barrier's way, the
-    // first reads of this one and the loads of the one to come; each further step's reads are issued between the instructions of
-    // the step before. The order is asked for, since the compiler by itself reads, waits and multiplies in turn.
-    auto k_tile = [&](u32 kt, auto more) {
-        meet(more);
-        const u8* stage = lds + slot * STAGE_BYTES;
-        read(f[0][0], stage, 0);
-        if (more) fetch_ahead(kt);
-        multiply(f[1][0]);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    // The scales and the bias, asked for before the k-tiles, so that nothing waits for them.
+    const u32 n = n0 + threadIdx.x % TN, n_at = n < c.channels ? n : c.channels - 1;
+    const float my_scale = c.w_scales[n_at], my_bias = c.bias ? c.bias[n_at] : 0.0f;
+    float x_scales[MB];
 #pragma unroll
-        for (int n = 0; n < MMAS; n++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-#pragma unroll
-            for (int l = n * LOADS / MMAS; l < (n + 1) * LOADS / MMAS; l++)
-                if (more) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-        }
-#pragma unroll
-        for (int kk = 1; kk < 4; kk++) {
-            read(f[kk & 1][0], stage, kk);
-            multiply(f[(kk & 1) ^ 1][0]);
-#pragma unroll
-            for (int n = 0; n < MMAS; n++) {
-                // (reads behind the first instruction: the wait for its operands is for all reads before it)
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                if (n * 2 < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                if (n * 2 + 1 < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-        }
-        slot = slot + 1 < STAGES ? slot + 1 : 0;
-    };
-    for (; kt + ahead < k_end; kt++) k_tile(kt, True());
-    for (; kt < k_end; kt++) k_tile(kt, False());
-    multiply(f[1][0]);
-#else
-    // A wave of a small tile has few matrix instructions to a k-step, fewer than an LDS read takes to come: the loop is rotated by a whole
-    // k-tile, whose instructions cover the barrier and all reads of the next one.
-    auto k_tile = [&](u32 kt, auto more, auto odd) {
-        constexpr int now = decltype(odd)::value;
-        meet(more);
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) read(f[now][kk], lds + slot * STAGE_BYTES, kk);
-        if (more) fetch_ahead(kt);
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) multiply(f[now ^ 1][kk]);
-        slot = slot + 1 < STAGES ? slot + 1 : 0;
-        // (all reads and loads first)
-        __builtin_amdgcn_sched_group_barrier(0x100, 4 * READS, 0);
-        if (more) __builtin_amdgcn_sched_group_barrier(0x020, LOADS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 4 * MMAS, 0);
-    };
-    auto either = [&](u32 kt, auto more) {
-        if ((kt - k_begin) & 1) k_tile(kt, more, True());
-        else k_tile(kt, more, False());
-    };
-    for (; kt + ahead + 1 < k_end; kt += 2) {
-        k_tile(kt, True(), False());
-        k_tile(kt + 1, True(), True());
+    for (int j = 0; j < MB; j++) {
+        const u32 m = m0 + wave_m * WTM + j * 32 + frag_row;
+        x_scales[j] = c.x_scales[m < c.tokens ? m : c.tokens - 1];
     }
-    for (; kt + ahead < k_end; kt++) either(kt, True());
-    for (; kt < k_end; kt++) either(kt, False());
-    if (k_count & 1)
+    // Whole rounds of the ring, each call with its own stages (see k_tile); what is left takes them as they come.
+    const u32 k_count = k_end - k_begin, ahead = STAGES - 1 < k_count ? STAGES - 1 : k_count;
+    u32 kt = k_begin;
+    if (k_count >= 2 * STAGES - 1) {
+        fetch(s0, w, x, source, kt);
+        if (STAGES > 2) fetch(s1, w, x, source, kt + 1);
+        if (STAGES > 3) fetch(s2, w, x, source, kt + 2);
+        do {
+            k_tile<true>(s0, s3, w, x, source, reader, kt, f, acc);
+            k_tile<true>(s1, s0, w, x, source, reader, kt + 1, f, acc);
+            if (STAGES > 2) k_tile<true>(s2, s1, w, x, source, reader, kt + 2, f, acc);
+            if (STAGES > 3) k_tile<true>(s3, s2, w, x, source, reader, kt + 3, f, acc);
+            kt += STAGES;
+        } while (kt + 2 * STAGES - 1 <= k_end);
+    } else {
+        if (ahead > 0) fetch(s0, w, x, source, kt);
+        if (STAGES > 2 && ahead > 1) fetch(s1, w, x, source, kt + 1);
+        if (STAGES > 3 && ahead > 2) fetch(s2, w, x, source, kt + 2);
+    }
+    u8 *from = s0, *to = s3;
+    for (; kt + ahead < k_end; kt++) {
+        k_tile<true>(from, to, w, x, source, reader, kt, f, acc);
+        to = from;
+        from = from == s0 ? s1 : from == s1 ? s2 : s3;
+    }
+    for (; kt < k_end; kt++) {
+        k_tile<false>(from, to, w, x, source, reader, kt, f, acc);
+        from = from == s3 ? s0 : from == s0 ? s1 : from == s1 ? s2 : s3;
+    }
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) multiply(f[0][kk]);
-    else
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) multiply(f[1][kk]);
-#endif
+    for (int s = 0; s < AHEAD; s++) multiply(f[1][s], acc);
 
     if (c.shares > 1) {
 #pragma unroll
@@ -327,8 +339,9 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
         }
         return;
     }
+    if (threadIdx.x < TN) w_scales[threadIdx.x] = my_scale, bias[threadIdx.x] = my_bias;
     __syncthreads();   // the operand stages become the waves' strips
-    store_sums(acc, c, n0 + wave_n * WTN, m0 + wave_m * WTM, w_scales + wave_n * WTN, bias + wave_n * WTN, (out_t*)lds + wave * STRIP_VALUES);
+    store_sums(acc, c, n0 + wave_n * WTN, m0 + wave_m * WTM, x_scales, w_scales + wave_n * WTN, bias + wave_n * WTN, (out_t*)(wave % STAGES == 0 ? s0 : wave % STAGES == 1 ? s1 : wave % STAGES == 2 ? s2 : s3) + wave / STAGES * STRIP_VALUES);
 }
 
 )HIP";
@@ -336,7 +349,7 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 // Streams. Reading the weights once is nearly all there is to do for few tokens, so they go straight into registers, as many loads on their way as
 // there is room for; the tokens come out of the L2. The matrix instructions (16 x 16 x 64) are far from being a bound.
 //
-// One token, 4096 x 4096: 5.6 us, 3 of them a launch; 8192 inputs, 16384 channels (134 MB, more than the caches hold with two others) 25 us (5.3 TB/s).
+// One token, 4096 x 4096: 5.5 us (5.7 where the scales are read when the sums are there), 3 of them a launch; 8192 inputs, 16384 channels (134 MB, more than the caches hold with two others) 25 us (5.3 TB/s).
 const char* kStream = R"HIP(
 extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     __shared__ __attribute__((aligned(16))) int sums[WAVES][BM * 16][BN * 16 + 4];
@@ -344,6 +357,10 @@ extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     const u32 n0 = blockIdx.x % tiles_n * (BN * 16), m0 = blockIdx.x / tiles_n * (BM * 16);
     // (the waves take turns along k, STEPS steps each: together they read long pieces of a row)
     const u32 chunks = c.pitch / 16, groups = (c.pitch + 64 * STEPS - 1) / (64 * STEPS), part = blockIdx.y * WAVES + wave, parts = c.shares * WAVES;
+    // (four channels to a thread, whose scales are there when the sums are)
+    static_assert(BM * 16 * BN * 4 <= WAVES * 64, "");
+    const u32 j = threadIdx.x / (BN * 4), i = threadIdx.x % (BN * 4) * 4, m = m0 + j, n = n0 + i;
+    const Scales scales = scales_of(c, m, n);
     const u8 *w[BN], *x[BM];
 #pragma unroll
     for (int i = 0; i < BN; i++) {
@@ -399,16 +416,12 @@ extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
 #pragma unroll
         for (int j = 0; j < BM; j++) *(i32x4*)&sums[wave][j * 16 + (lane & 15u)][i * 16 + (lane >> 4) * 4] = acc[i][j];
     __syncthreads();
-    // (four channels to a thread)
-    for (u32 e = threadIdx.x; e < BM * 16 * BN * 4; e += WAVES * 64) {
-        const u32 j = e / (BN * 4), i = e % (BN * 4) * 4, m = m0 + j, n = n0 + i;
-        if (m >= c.tokens || n >= c.channels) continue;
-        i32x4 sum = *(const i32x4*)&sums[0][j][i];
+    if (j >= BM * 16 || m >= c.tokens || n >= c.channels) return;
+    i32x4 sum = *(const i32x4*)&sums[0][j][i];
 #pragma unroll
-        for (int v = 1; v < WAVES; v++) sum += *(const i32x4*)&sums[v][j][i];
-        if (c.shares > 1) *parked_at(c, blockIdx.y, m, n) = sum;
-        else store_four(c, m, n, sum);
-    }
+    for (int v = 1; v < WAVES; v++) sum += *(const i32x4*)&sums[v][j][i];
+    if (c.shares > 1) *parked_at(c, blockIdx.y, m, n) = sum;
+    else store_four(c, m, n, sum, scales);
 }
 )HIP";
 
@@ -419,10 +432,11 @@ extern "C" __global__ __launch_bounds__(256) void int8_join(Call c) {
     const u64 at = (u64)blockIdx.x * 256 + threadIdx.x;
     if (at >= (u64)c.tokens * fours) return;
     const u32 m = (u32)(at / fours), n = (u32)(at % fours) * 4;
+    const Scales scales = scales_of(c, m, n);
     i32x4 sum = *parked_at(c, 0, m, n);
 #pragma unroll 4
     for (u32 s = 1; s < c.shares; s++) sum += *parked_at(c, s, m, n);
-    store_four(c, m, n, sum);
+    store_four(c, m, n, sum, scales);
 }
 )HIP";
 
@@ -431,14 +445,14 @@ constexpr uint64_t kCUs = 256;
 constexpr uint64_t kMostParked = 1 << 22;  // sums of all shares together, for which the scratch has room
 
 // What the choice goes by (cut_of below), from products of 1 to 8192 tokens: microseconds of a call, of a k-tile in a workgroup that has a CU to itself and
-// on full CUs, and of beginning and ending a workgroup there. The small tiles, whose waves
-// have few matrix instructions to a k-step, read a whole k-tile ahead: 1024 x 4096 x 4096 28.1 -> 25.9 us with 64 x 128 (128 x 128 24.6), 512 tokens
-// 22.6 -> 17.9, 2048 x 1024 x 1024 7.4 -> 6.8. Of 256 x 256 four waves along the channels read less from LDS than two: 66.4 -> 64.
+// on full CUs, and of beginning and ending a workgroup there. The small tiles, whose waves have few matrix instructions to a k-step, read two steps ahead
+// (1024 x 4096 x 4096 with 128 x 128 22.9 -> 21.2 us); 256 x 256 has no registers for that (61.7, and 63.1 with the spills). Waves of 64 x 32 in a 64 x 128
+// tile 13.95 us with 512 x 4096 x 4096, of 32 x 64 14.7; four stages of 64 x 64 rather than three 9.4 for 10.7 with 128 x 4096 x 4096.
 const Int8Shape kShapes[] = {
-    {256, 256, 4, 2, 2, 1, 1, 9.0, 1.24, 1.76, 6.5},
-    {128, 128, 2, 4, 4, 1, 4, 5.2, 0.46, 0.61, 3.3},
-    {64, 128, 2, 2, 3, 2, 4, 3.6, 0.42, 0.60, 3.2},
-    {64, 64, 2, 2, 3, 3, 4, 3.5, 0.33, 0.43, 2.0},
+    {256, 256, 4, 2, 2, 1, 1, 8.3, 1.03, 1.57, 9.5},
+    {128, 128, 2, 4, 4, 1, 2, 4.3, 0.37, 0.56, 2.8},
+    {64, 128, 1, 4, 3, 2, 2, 3.6, 0.29, 0.61, 1.7},
+    {64, 64, 2, 2, 4, 2, 2, 3.1, 0.20, 0.39, 1.1},
     {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 1, 8, 4},
     {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 2, 8, 4},
     {0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 1, 3, 8, 2},

@@ -20,7 +20,7 @@ struct Int8Problem {
 // of a workgroup share the sums of 16 blocks_n channels of 16 blocks_m tokens and read their operands straight into registers.
 struct Int8Shape {
     int tile_n = 0, tile_m = 0, waves_n = 0, waves_m = 0, stages = 0, per_cu = 1;  // of tiles
-    int ahead = 1;  // k-steps whose operands are read from LDS ahead of the matrix instructions: 1, or all 4 of a k-tile
+    int ahead = 1;  // k-steps whose operands are read from LDS ahead of the matrix instructions: 1 or 2 (a k-tile has 4)
     double base = 0, alone = 0, full = 0, round = 0;  // microseconds: of a call; of a k-tile on a CU of its own, and on a full one; of another round of workgroups
     int blocks_n = 0, blocks_m = 0, waves = 0, steps = 0;  // of streams
     bool stream() const { return blocks_n > 0; }

@@ -48,6 +48,17 @@ def test_every_shape_and_cut(gpu, monkeypatch, shape, shares, size):
     check(host, dtype, to_f32(multiply(ha.Int8Matmul(columns, channels, dtype), host, dtype), dtype))
 
 
+@pytest.mark.parametrize("shape", range(4))
+def test_every_count_of_k_tiles(gpu, monkeypatch, shape):
+    """None to several rounds of a tile's ring, and what is left behind the last; rows that end inside a k-tile."""
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", "1")
+    for count in range(1, 18):
+        columns = count * 128 - (0, 1, 127, 112, 50)[count % 5]
+        host = inputs(150, columns, 270, bias=True, seed=count)
+        check(host, "f32", multiply(ha.Int8Matmul(columns, 270, "f32"), host, "f32"))
+
+
 @pytest.mark.parametrize("tokens", [40, 300])
 def test_no_cut_changes_a_bit(gpu, monkeypatch, tokens):
     host = inputs(tokens, 8300, 130, bias=True, seed=6)
