@@ -242,10 +242,10 @@ def _product(inputs, channels, dtype):
 
 
 @functools.lru_cache(maxsize=16)
-def _clip(shapes, dtype):
+def _clip(sizes, dtype):
     import helium_amd as ha
 
-    return ha.GradientClip(_sizes({"shapes": shapes}), dtype)
+    return ha.GradientClip(sizes, dtype)
 
 
 def _at(*tensors):
@@ -268,7 +268,7 @@ def run(s):
         y = _plain_product(s, *_plain_quantize(_plain_rms(h, s["gamma"])[0]))
         return {"y": y, "h": h} if "residual" in s else {"y": y}
     if kind == "clip":
-        _clip(case["shapes"], case["dtype"]).clip(_at(*s["gradients"]), _at(*s["clipped"]), MOST_NORM, s["norm"].data_ptr())
+        _clip(_sizes(case), case["dtype"]).clip(_at(*s["gradients"]), _at(*s["clipped"]), MOST_NORM, s["norm"].data_ptr())
         return {"clipped": s["flat"], "norm": s["norm"]}
     if kind == "norm":
         op = _rms_norm(case["columns"], case["dtype"], case["residual"], "same")
