@@ -560,8 +560,9 @@ void RmsNorm::backward(int64_t rows, const void* dy, const void* h, const void* 
     const uint32_t grid[3] = {blocks, 1, 1}, block[3] = {(uint32_t)tiling_.threads, 1, 1};
     const uint32_t fold_grid[3] = {(uint32_t)((pr_.columns + 15) / 16), 1, 1}, fold_block[3] = {1024, 1, 1};
     std::lock_guard<std::mutex> lk(mu_);
-    // (one workgroup's share is the sum already)
-    float* parts = blocks == 1 ? dgamma : scratch_.get(most * pr_.columns, 0, stream).floats;
+    // (asked for whatever the rows are, so that a stream's first call is the one that allocates; one workgroup's share is the sum already)
+    float* const scratch = scratch_.get(most * pr_.columns, 0, stream).floats;
+    float* parts = blocks == 1 ? dgamma : scratch;
     void* args[] = {&count, &blocks, &dy, &h, &gamma, &rstd, &dh, &dx, &dresidual, &parts};
     if (blocks) (dh ? backward_more_ : backward_)->launch(grid, block, 0, stream, args, blocks == 1);
     if (blocks == 1) return;

@@ -540,7 +540,8 @@ int he_rms_norm_forward(he_rms_norm_t norm, int64_t rows, const void* x, const v
 /* dy: of y; h, rstd: as the forward pass had them; dh: what reaches h from its other readers, NULL for nothing. The gradient of h, which is
  * that of x and of the residual, goes to dx (dtype) and dresidual (residual_dtype), of which one may be NULL; dx may be dy, or h where their types are the same,
  * and dresidual may be dh or h. dgamma [columns] is f32, summed over the rows in a fixed order, zero without rows. Not with to_i8. The first call
- * on a stream allocates scratch for it, later ones allocate nothing; calls on several streams may overlap. A captured call works in the
+ * on a stream allocates scratch for it, whatever its rows, later ones allocate nothing (code is loaded by the first call that needs it, which may be a captured one);
+ * calls on several streams may overlap. A captured call works in the
  * scratch of the stream it was captured on, wherever it is replayed: what may run at the same time is captured on streams of its own, or from handles of its own. */
 int he_rms_norm_backward(he_rms_norm_t norm, int64_t rows, const void* dy, const void* h, const void* gamma, const float* rstd, const void* dh,
                          void* dx, void* dresidual, float* dgamma, he_stream_t stream);

@@ -200,3 +200,36 @@ def test_a_captured_call_replays(gpu):
         assert np.array_equal(y.cpu().numpy(), want[0]) and np.array_equal(q.cpu().numpy(), want[2])
         for a, b in zip((dr, dgamma), want[1]):
             assert np.array_equal(a.cpu().numpy(), b)
+
+
+def test_later_calls_on_a_stream_allocate_nothing_whatever_their_rows(gpu):
+    """The first call is of one row, which needs no workgroup's shares; what follows is captured, of more rows than workgroups."""
+    torch = pytest.importorskip("torch")
+    rows, columns = 1000, 32760   # (the scratch of 256 workgroups is 33 MB)
+    norm = ha.RmsNorm(columns, "bf16", epsilon=EPSILON)
+    host, _ = inputs(rows, columns, "bf16", None, "f32", seed=11)
+    want = run_backward(norm, rows, host, None)
+    norm = ha.RmsNorm(columns, "bf16", epsilon=EPSILON)
+    t = {k: torch.from_numpy(host[k].copy()).cuda() for k in ("dy", "h", "gamma", "rstd")}
+    dx, dgamma = torch.zeros_like(t["dy"]), torch.zeros(columns, device="cuda")
+    s = ha.Stream()
+    stream = torch.cuda.ExternalStream(ha._ffi.lib.he_stream_raw(s.handle))
+    call = lambda n: norm.backward(n, *[a.data_ptr() for a in (*t.values(), dx, dgamma)], stream=s)  # noqa: E731
+    torch.cuda.synchronize()
+    call(1)
+    stream.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    call(300)
+    stream.synchronize()
+    assert torch.cuda.mem_get_info()[0] > free - (16 << 20)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call(rows)
+    for _ in range(3):
+        dx.fill_(7)
+        dgamma.fill_(7)
+        call(2)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(dx.cpu().numpy(), want[0]) and np.array_equal(dgamma.cpu().numpy(), want[2])
