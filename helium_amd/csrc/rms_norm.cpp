@@ -554,7 +554,7 @@ void RmsNorm::backward(int64_t rows, const void* dy, const void* h, const void* 
     }
     // (one workgroup to a CU where it has one row at a time, otherwise two: 8192 x 4096 bf16 50.6 and 52.5 us, 1517 x 2867 16.4 and 17.5; 8192 x 1024 f32 20.0 and
     // 19.0, 30000 x 256 bf16 15.3 and 14.6. Four: 57.0, 21.2, 20.4, 15.4)
-    const uint64_t most = (uint64_t)kCUs * tuning::get_int("HELIUM_HIP_ROWS_PER_CU", tiling_.rows() == 1 ? 1 : 2);
+    const uint64_t most = (uint64_t)kCUs * (tiling_.rows() == 1 ? 1 : 2);
     uint32_t blocks = (uint32_t)std::min<uint64_t>(most, ((uint64_t)rows + tiling_.rows() - 1) / tiling_.rows());
     uint64_t count = (uint64_t)rows;
     const uint32_t grid[3] = {blocks, 1, 1}, block[3] = {(uint32_t)tiling_.threads, 1, 1};

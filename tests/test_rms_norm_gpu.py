@@ -233,3 +233,15 @@ def test_later_calls_on_a_stream_allocate_nothing_whatever_their_rows(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert np.array_equal(dx.cpu().numpy(), want[0]) and np.array_equal(dgamma.cpu().numpy(), want[2])
+
+
+def test_the_number_of_workgroups_is_not_the_environments(gpu, monkeypatch):
+    """(A stream's scratch is sized by it.)"""
+    rows, columns = 3000, 515
+    norm = ha.RmsNorm(columns, "f32", epsilon=EPSILON)
+    host, _ = inputs(rows, columns, "f32", None, "f32", seed=12)
+    want = run_backward(norm, rows, host, None)
+    for value in ("0", "4"):
+        monkeypatch.setenv("HELIUM_HIP_ROWS_PER_CU", value)
+        for a, b in zip(run_backward(norm, rows, host, None), want):
+            assert np.array_equal(a, b)
