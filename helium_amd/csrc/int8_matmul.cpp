@@ -548,12 +548,12 @@ std::string Int8Cut::describe() const {
 // Of all shapes and numbers of shares the one with the least estimate. A share is at least four k-tiles long, or what a stream's waves need to have four
 // steps of it each.
 Int8Cut plan_int8(const Int8Problem& pr, int64_t tokens) {
-    const int forced = tuning::get_int("HELIUM_HIP_INT8_SHAPE", 0), forced_shares = tuning::get_int("HELIUM_HIP_INT8_SHARES", 0);
-    Int8Cut best = cut_of(pr, tokens, forced ? std::min(forced, kCount) - 1 : 0, 1);
+    const int forced = std::clamp(tuning::get_int("HELIUM_HIP_INT8_SHAPE", 0), 0, kCount), forced_shares = tuning::get_int("HELIUM_HIP_INT8_SHARES", 0);
+    Int8Cut best = cut_of(pr, tokens, forced ? forced - 1 : 0, 1);
     if (forced_shares) best.estimate = 1e30;
     for (int k = 0; k < kCount; k++) {
         const Int8Shape& t = kShapes[k];
-        if (forced ? k != std::min(forced, kCount) - 1 : t.stream() && t.blocks_m != (int)std::min<uint64_t>(4, cut(tokens, 16))) continue;
+        if (forced ? k != forced - 1 : t.stream() && t.blocks_m != (int)std::min<uint64_t>(4, cut(tokens, 16))) continue;
         const uint64_t least = t.stream() ? (uint64_t)t.waves * 256 : 512;  // bytes of k
         for (uint32_t shares = 1; shares <= 16; shares *= 2) {
             if (shares > 1 && ((uint64_t)shares * tokens * parked_pitch(pr) > kMostParked || (uint64_t)quantized_pitch(pr.inputs) < least * shares)) break;

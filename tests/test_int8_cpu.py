@@ -114,6 +114,16 @@ def test_every_call_is_cut():
     assert used == set(range(SHAPES))   # (nothing is built that no call takes)
 
 
+def test_shapes_that_there_are_none_of_are_not_forced(monkeypatch):
+    op = ha.Int8Matmul(700, 130, "f32")
+    want = op.describe(70)
+    for shape in ("-1", "-20", "0", "none"):
+        monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", shape)
+        assert op.describe(70) == want
+    monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", "1000")
+    assert f"shape={SHAPES - 1} " in op.describe(70)
+
+
 @pytest.mark.parametrize("kwargs,says", [
     (dict(inputs=0), "0 inputs"),
     (dict(channels=-1), "-1 channels"),
