@@ -127,11 +127,15 @@ __device__ __forceinline__ void store_padding(u8* row, const Lane& p) {
 //
 // Bound by memory: 8192 x 4096 bf16 with a residual 47.1 us (5.7 TB/s, the rate of a copy), into 8 bits 2048 x 4096 10.6 us (5.5 TB/s); f32 residuals beside
 // 16-bit operands, 2000 x 16384, 71 us (5.5 TB/s; 90 with accesses of 16 bytes of the narrower type). One row of 4096: a launch, 2.5 us.
+//
+// A sum of squares that f32 cannot hold (from values of some 1e17 on in long rows, of 1.8e19 in any; without an epsilon to speak of, of values below 1e-15) is taken
+// again of the values times a power of two; other rows' results are as they would be without it.
 const char* kForward = R"HIP(
+__device__ __forceinline__ bool beyond(float sum) { return !(sum < __builtin_inff()) || (EPS < 0x1p-80f && sum < 0x1p-90f); }
 // PAST: results bypass the caches
 template <bool PAST> __device__ __forceinline__ void forward(u64 rows, const elem_t* x, const param_t* __restrict__ gamma, const stream_t* residual,
                                                             stream_t* new_residual, void* y, float* __restrict__ rstd_out, float* __restrict__ scales) {
-    __shared__ float red[WAVES][2];
+    __shared__ float red[2][WAVES][2];
     const Lane p = lane();
     const u64 row = (u64)blockIdx.x * ROWS + p.slot;
     const bool there = row < rows;
@@ -179,14 +183,47 @@ template <bool PAST> __device__ __forceinline__ void forward(u64 rows, const ele
             }
         }
     }
-    over_row<true, TO_I8>(sum, most, red);
+    over_row<true, TO_I8>(sum, most, red[0]);
 #if RESIDUAL
     // (not before all lanes have what they read: a ragged row's last two vectors overlap, and the new residual may lie in the old one's place)
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (there && HAS(p, k)) STORE(PAST, (stream_v*)(new_residual + row * C + start(p, k)), hr[k]);
 #endif
-    const float rstd = 1.0f / sqrtf(sum / (float)C + EPS);
+    float rstd = 1.0f / sqrtf(sum / (float)C + EPS);
+    // (the same answer in all threads that meet in over_row: those of a wave, or of a workgroup)
+#if L > 64
+    bool again = false;
+#pragma unroll
+    for (u32 r = 0; r < ROWS; r++) {
+        float s = 0.0f;
+#pragma unroll
+        for (u32 w = 0; w < WAVES_OF_ROW; w++) s += red[0][r * WAVES_OF_ROW + w][0];
+        again = again || beyond(s);
+    }
+#else
+    const bool again = __any(there && beyond(sum));
+#endif
+    if (again) {
+        const float by = sum < 1.0f ? 0x1p100f : 0x1p-80f;
+        float squares = 0.0f;
+        u32 none = 0;
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (there && HAS(p, k))
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (counts(p, k, i)) {
+#if RESIDUAL
+                        const float v = (float)AT(hr[k], i) * by;
+#else
+                        const float v = (float)AT(hx[k], i) * by;
+#endif
+                        squares += v * v;
+                    }
+        over_row<true, false>(squares, none, red[1]);
+        if (beyond(sum)) rstd = by / sqrtf(squares / (float)C + EPS * by * by);
+    }
     if (rstd_out && there && p.l == 0) rstd_out[row] = rstd;
 #if TO_I8
     const Steps s = steps_of(most);

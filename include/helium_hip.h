@@ -528,7 +528,8 @@ typedef struct he_rms_norm_s* he_rms_norm_t;
 /* Rows of `columns` values (at most 32768), row-major and packed; how many there are is each call's. h = x + residual, rounded to the
  * residual's type, or x itself without one; rstd = 1 / sqrt(mean of h^2 + epsilon); y = h * rstd * gamma[c]. dtype: HE_F32, HE_BF16 or
  * HE_F16, of x, y and their gradients; residual_dtype: HE_F32 or dtype, or -1: there is no residual; param_dtype: of gamma, HE_F32 or
- * dtype. Arithmetic and sums are f32 (squares of values beyond 1e19 overflow). to_i8: y is quantised as section 11 has it, a row's scale
+ * dtype. Arithmetic and sums are f32; h and rstd have to be in its range (without an epsilon, rows below 1e-38 have a rstd that is not; squares and their
+ * sums need not be). to_i8: y is quantised as section 11 has it, h * gamma being in range too (where it is infinite the row has scale NaN), a row's scale
  * being the largest |y| / 127; q may differ from the correctly rounded one by 1 where y / scale is next to the middle of two whole numbers.
  * Compiles the kernels; needs no device. */
 int he_rms_norm_create(he_rms_norm_t* norm, int64_t columns, int dtype, int residual_dtype, int param_dtype, int to_i8, float epsilon);

@@ -48,6 +48,16 @@ static inline float __shfl_xor(float v, int mask, int width) {
     WAVE_BAR();
     return r;
 }
+static int g_any[1024];
+static inline int __any(int p) {
+    unsigned tid = threadIdx.x;
+    g_any[tid] = p != 0;
+    WAVE_BAR();
+    int r = 0;
+    for (unsigned l = 0; l < 64; l++) r |= g_any[(tid & ~63u) + l];
+    WAVE_BAR();
+    return r;
+}
 static inline int __float_as_int(float f) { int i; memcpy(&i, &f, 4); return i; }
 static inline unsigned __float_as_uint(float f) { unsigned i; memcpy(&i, &f, 4); return i; }
 static inline float atomicAdd(float* a, float v) {

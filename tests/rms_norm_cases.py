@@ -80,3 +80,38 @@ def check_backward(dtype, residual, v, dx, dresidual, dgamma, rows_per_block):
     # a lane's rows, the lanes and waves side by side (10 at most), then 16 chains over 512 workgroups
     depth = rows_per_block + 10 + 32 + 16 + 4
     within(dgamma, wgamma, depth * U * (dy * xh).sum(axis=0), "dgamma")
+
+
+# rows, columns, x's type, the residual's, epsilon: several rows to a wave, to a workgroup, one row to a workgroup
+BEYOND = [(9, 20, "f32", None, 1e-5), (70, 21, "bf16", "f32", 0.0), (3, 64, "f32", "f32", 0.0), (7, 300, "bf16", "bf16", 1e-5), (9, 700, "f32", None, 0.0),
+          (5, 1203, "bf16", "f32", 0.0), (4, 1203, "f32", "f32", 1e-5), (5, 2056, "bf16", None, 0.0)]
+
+
+def beyond(rows, columns, dtype, residual, epsilon, seed):
+    """Rows whose squares or sums of squares f32 cannot hold, too large and, without an epsilon, too small ones, between ordinary rows; gamma is f32."""
+    host, v = inputs(rows, columns, dtype, residual, "f32", seed)
+    sizes = np.array([1, 3e17, 1, 1e19, 1e25, 1e37] if epsilon else [1, 1e-15, 3e18, 1e-25, 1e-34, 1, 1e36])[np.arange(rows) % (6 if epsilon else 7), None]
+    for k, t in (("x", dtype), ("residual", residual)):
+        if t:
+            host[k] = to_storage(v[k] * sizes, t)
+            v[k] = to_f32(host[k], t)
+    stream = residual or dtype
+    host["h"] = to_storage(v["x"] + v["residual"], stream) if residual else host["x"]
+    v["h"] = to_f32(host["h"], stream)
+    assert np.isfinite(v["h"]).all() and (np.abs(v["h"]).max(axis=1) > 0).all()
+    return host, v
+
+
+def check_beyond(dtype, v, epsilon, y, rstd):
+    """As check_forward has it: the factor that the values are taken times is a power of two."""
+    want, wrstd = oracle.forward(v["h"], v["gamma"], epsilon)
+    assert wrstd.min() > 2.0 ** -125 and wrstd.max() < 2.0 ** 126
+    within(rstd, wrstd, (DEPTH / 2 + 4) * U * wrstd, "rstd")
+    within(y, want, rounded((DEPTH / 2 + 8) * U * np.abs(want), want, dtype), "y")
+
+
+def check_quantized_beyond(v, epsilon, q, scales):
+    want, _ = oracle.forward(v["h"], v["gamma"], epsilon)
+    most = np.abs(want).max(axis=1)
+    within(scales, most / 127, (DEPTH / 2 + 12) * U * most / 127, "scales")
+    within(q[:, :v["h"].shape[1]].astype(np.float64), 127 * want / most[:, None], 0.5 + 127 * 6 * U, "q")

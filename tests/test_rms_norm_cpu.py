@@ -12,7 +12,7 @@ from helium_amd import _ffi
 from helium_amd.int8 import pitch
 from oracle import int8 as oracle_int8
 from oracle import rms_norm as oracle
-from rms_norm_cases import EPSILON, SHAPES, TYPES, check_backward, check_forward, check_quantized_norm, inputs
+from rms_norm_cases import BEYOND, EPSILON, SHAPES, TYPES, beyond, check_backward, check_beyond, check_forward, check_quantized_beyond, check_quantized_norm, inputs
 
 
 def test_the_oracles_gradients_are_those_of_its_forward_pass():
@@ -231,3 +231,22 @@ def test_operands_are_checked_before_any_launch():
     assert _ffi.lib.he_quantize_rows_create(None, 64, _ffi.F32) == _ffi.ERR_INVALID
     assert _ffi.lib.he_quantize_rows(None, 1, *[None] * 4) == _ffi.ERR_INVALID
     assert _ffi.lib.he_quantize_rows_destroy(None) == _ffi.OK
+
+
+@pytest.mark.parametrize("rows,columns,dtype,residual,epsilon", BEYOND)
+@pytest.mark.parametrize("output", ["same", "i8"])
+def test_rows_whose_squares_are_beyond_f32(rows, columns, dtype, residual, epsilon, output):
+    host, v = beyond(rows, columns, dtype, residual, epsilon, seed=columns)
+    tiling, (text, *_) = parts(ha.RmsNorm(columns, dtype, residual_dtype=residual, output=output, epsilon=epsilon))
+    buffers = {"x": (host["x"], 0), "gamma": (host["gamma"], 0), "rstd": (np.empty(rows, np.float32), 1)}
+    buffers["y"] = (np.empty_like(host["x"]) if output == "same" else np.empty((rows, pitch(columns)), np.int8), 1)
+    if output == "i8":
+        buffers["scales"] = (np.empty(rows, np.float32), 1)
+    if residual:
+        buffers.update(residual=(host["residual"], 0), new_residual=(np.empty_like(host["h"]), 1))
+    got = emulated_forward(tiling, text, rows, buffers)
+    assert not residual or np.array_equal(got["new_residual"], host["h"])
+    if output == "same":
+        check_beyond(dtype, v, epsilon, to_f32(got["y"], dtype), got["rstd"])
+    else:
+        check_quantized_beyond(v, epsilon, got["y"], got["scales"])

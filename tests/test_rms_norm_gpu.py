@@ -7,7 +7,7 @@ from device_arrays import Array, at, empty
 from group_norm_cases import to_f32, to_storage
 from helium_amd.int8 import pitch
 from oracle import int8 as oracle_int8
-from rms_norm_cases import EPSILON, LARGE, SHAPES, TYPES, check_backward, check_forward, check_quantized_norm, inputs
+from rms_norm_cases import BEYOND, EPSILON, LARGE, SHAPES, TYPES, beyond, check_backward, check_beyond, check_forward, check_quantized_beyond, check_quantized_norm, inputs
 from test_rms_norm_cpu import borders
 
 pytestmark = pytest.mark.gpu
@@ -245,3 +245,16 @@ def test_the_number_of_workgroups_is_not_the_environments(gpu, monkeypatch):
         monkeypatch.setenv("HELIUM_HIP_ROWS_PER_CU", value)
         for a, b in zip(run_backward(norm, rows, host, None), want):
             assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("rows,columns,dtype,residual,epsilon", BEYOND + [(40, 4096, "bf16", "bf16", 1e-5), (40, 12290, "f32", None, 0.0), (9, 32767, "bf16", "f32", 0.0), (700, 4096, "f32", "f32", 0.0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rows_whose_squares_are_beyond_f32(gpu, rows, columns, dtype, residual, epsilon, in_place):
+    host, v = beyond(rows, columns, dtype, residual, epsilon, seed=columns)
+    y, h, rstd, _ = run_forward(ha.RmsNorm(columns, dtype, residual_dtype=residual, epsilon=epsilon), rows, host, residual, in_place=in_place)
+    check_beyond(dtype, v, epsilon, to_f32(y, dtype), rstd)
+    assert not residual or np.array_equal(h, host["h"])
+    if not in_place:
+        q, h, _, scales = run_forward(ha.RmsNorm(columns, dtype, residual_dtype=residual, output="i8", epsilon=epsilon), rows, host, residual, to_i8=True)
+        check_quantized_beyond(v, epsilon, q, scales)
+        assert not residual or np.array_equal(h, host["h"])
