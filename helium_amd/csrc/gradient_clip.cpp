@@ -106,15 +106,15 @@ __device__ __forceinline__ double squares(const Held& h, u32 dtype, double sum) 
         }
     return sum + other;
 }
-__device__ __forceinline__ void scale(Held& h, u32 dtype, float by) {
+template <class F> __device__ __forceinline__ void scale(Held& h, u32 dtype, F by) {
 #pragma unroll
     for (int k = 0; k < VECTORS; k++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const u32 word = h.v[k][e];
-            if (dtype == F32_T) h.v[k][e] = bits_of(of_bits(word) * by);
-            else if (dtype == BF16_T) h.v[k][e] = bf16_bits(of_bits(word << 16) * by) | bf16_bits(of_bits(word & 0xffff0000u) * by) << 16;
-            else h.v[k][e] = f16_bits(f16_value(word) * by) | f16_bits(f16_value(word >> 16) * by) << 16;
+            if (dtype == F32_T) h.v[k][e] = bits_of((float)(of_bits(word) * by));
+            else if (dtype == BF16_T) h.v[k][e] = bf16_bits((float)(of_bits(word << 16) * by)) | bf16_bits((float)(of_bits(word & 0xffff0000u) * by)) << 16;
+            else h.v[k][e] = f16_bits((float)(f16_value(word) * by)) | f16_bits((float)(f16_value(word >> 16) * by)) << 16;
         }
 }
 // (`passing`: chunks of the group that no later launch finds in a cache)
@@ -159,6 +159,7 @@ extern "C" __global__ __launch_bounds__(256) void clip_scale(Both o, const Tenso
     __shared__ double waves[4];
     const Begins begins = begins_of(tensors, count);
     float by = 1.0f;
+    double exact_by = 1.0;
     for (u32 k = blockIdx.x; k < chunks; k += gridDim.x) {
         const u32 c = chunks - 1 - k, t = tensor_of(begins, c), dtype = tensors[t].dtype;
         const u64 at = (u64)(c - tensors[t].first) * CHUNK, left = tensors[t].bytes - at;
@@ -169,11 +170,14 @@ extern "C" __global__ __launch_bounds__(256) void clip_scale(Both o, const Tenso
             const double n = norm_of(sums, sum_count, waves), c = (double)most / (n + 1e-6);
             // (a norm that is NaN makes everything so, unless nothing is to be clipped)
             by = most == __builtin_inff() || c > 1.0 ? 1.0f : (float)c;
+            exact_by = c;
             if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
         }
         // (nothing to do in place where nothing is clipped)
         if (by == 1.0f && o.in[t] == o.out[t]) continue;
-        if (by != 1.0f) scale(h, dtype, by);
+        // (a factor near the end of f32's range, or beyond it, is taken in f64: of huge gradients there it leaves ordinary values)
+        if (by < 0x1p-100f) scale(h, dtype, exact_by);
+        else if (by != 1.0f) scale(h, dtype, by);
         store(h, o.out[t] + at, left);
     }
 }

@@ -598,10 +598,11 @@ int he_gradient_clip_create(he_gradient_clip_t* clip, const int64_t* sizes, cons
  * nothing; calls on several streams may overlap. A captured call works in the workspace of the stream it was captured on, wherever it is replayed: what
  * may run at the same time is captured on streams of its own, or from handles of its own. */
 int he_gradient_norm(he_gradient_clip_t clip, const void* const* gradients, int count, float* norm, he_stream_t stream);
-/* out[k] = gradients[k] * min(1, most / (norm + 1e-6)), rounded once to its type, and the norm (before clipping) in norm[0], which may be NULL. out[k] may be
- * gradients[k]; otherwise it shares no memory with any of them, and results share none with each other (a gradient that is listed twice in place would be scaled
- * twice). most is 0 or more; with infinity results are the gradients, whatever their norm. Otherwise a norm that is NaN makes every result NaN, an infinite one zeros (NaN
- * where a value is infinite): norm[0] tells. */
+/* out[k] = gradients[k] * min(1, most / (norm + 1e-6)), and the norm (before clipping) in norm[0], which may be NULL. The factor is rounded to f32 (below 2^-100 it stays in 64
+ * bits), its product with a value to the result's type, at once or by way of f32. out[k] may be gradients[k]; otherwise it shares no memory with any of them, and results share none with
+ * each other (a gradient that is listed twice in place would be scaled twice). most is 0 or more; with infinity results are the gradients, whatever their norm. Otherwise a norm that
+ * is NaN makes every result NaN, an infinite one zeros (NaN where a value is infinite): norm[0] tells, but a finite norm that f32 cannot hold is infinite there as well, beside results
+ * that are scaled as they should be. */
 int he_gradient_clip(he_gradient_clip_t clip, const void* const* gradients, void* const* out, int count, float most, float* norm,
                      he_stream_t stream);
 /* The generated HIP source, how the tensors are cut, and the table the kernels read, for inspection and tests. */

@@ -89,6 +89,17 @@ def test_the_kernels_match_the_oracle(k, most):
     check_norm(values, run_kernel(text, "emu", 1, 256, [(sums, 0), (np.zeros(1, np.float32), 1)])[0][0])
 
 
+@pytest.mark.parametrize("size,most", [(1e37, 1e-3), (1e37, 1e-6), (3e36, 1e-30), (1e30, 1e-3)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_factors_that_f32_holds_with_few_bits_or_none(size, most, in_place):
+    """(most / norm is below 2^-126, where f32 has fewer than 24 bits, in all but the last.)"""
+    sizes, dtypes = [700, 300, 5000], ["f32", "bf16", "f32"]
+    host, values = inputs(sizes, dtypes, size, seed=12)
+    most = float(np.float32(most))   # (as the call has it)
+    got, _, _ = emulated(ha.GradientClip(sizes, dtypes), host, most, in_place=in_place)
+    check(dtypes, values, most, got)
+
+
 def test_results_may_take_the_gradients_places():
     sizes, dtypes = GROUPS[1]
     host, values = inputs(sizes, dtypes, 0.3, seed=9)

@@ -56,6 +56,20 @@ def test_the_norm_neither_vanishes_nor_overflows(gpu, size):
     check(dtypes, values, 1.0, got, norm)
 
 
+@pytest.mark.parametrize("size,most", [(1e37, 1e-3), (1e37, 1e-6), (3e36, 1e-30), (1e30, 1e-3)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_factors_that_f32_holds_with_few_bits_or_none(gpu, size, most, in_place):
+    sizes, dtypes = [70_000, 301, 50_001], ["f32", "bf16", "f32"]
+    host, values = inputs(sizes, dtypes, size, seed=12)
+    most = float(np.float32(most))   # (as the call has it)
+    got, norm = clipped(ha.GradientClip(sizes, dtypes), host, most, in_place)
+    check(dtypes, values, most, got)
+    if oracle.norm(values) > np.finfo(np.float32).max:   # (beyond which f32 has infinity)
+        assert np.isposinf(norm)
+    else:
+        check_norm(values, norm)
+
+
 def test_no_values_and_zeros(gpu):
     norm = empty((1,), np.float32)
     for sizes in ([], [0, 0]):
