@@ -43,6 +43,9 @@ typedef out_t out_any __attribute__((ext_vector_type(PER), aligned(sizeof(out_t)
 #define MFMA_16(a, b, c) __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0)
 #define LDS_AS __attribute__((address_space(3)))
 #define GLOBAL_AS __attribute__((address_space(1)))
+#define AS_F32(f) asm("" : "+v"(f))
+#else
+#define AS_F32(f)
 #endif
 struct Call {
     const u8 *x, *w;
@@ -57,8 +60,14 @@ __device__ __forceinline__ i32x4* parked_at(const Call& c, u32 share, u32 m, u32
     return (i32x4*)(c.parked + ((u64)share * c.tokens + m) * c.parked_pitch + n);
 }
 // One rounding of the sum to f32, one of its product with the token's scale, one with the channel's and the bias added, and that to the result's type: the same
-// in every shape and cut.
-__device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale, float bias) { return __builtin_fmaf((float)sum * x_scale, w_scale, bias); }
+// in every shape and cut. (To f16 the compiler would take the last two as one where it can, some channels of a tile among them.)
+__device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale, float bias) {
+    float f = __builtin_fmaf((float)sum * x_scale, w_scale, bias);
+#if F16
+    AS_F32(f);
+#endif
+    return f;
+}
 typedef out_t out4_any __attribute__((ext_vector_type(4), aligned(sizeof(out_t))));
 struct Scales { float x, w[4], bias[4]; };   // of a token and four channels, of which the last may be missing
 __device__ __forceinline__ Scales scales_of(const Call& c, u32 m, u32 n) {

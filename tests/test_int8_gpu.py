@@ -171,3 +171,37 @@ def test_a_captured_call_replays(gpu, tokens):
         graph.replay()
         torch.cuda.synchronize()
         assert np.array_equal(y.cpu().numpy(), want)
+
+
+# 16-wave streams take 4096 bytes of k to a share, others 2048, tiles 512
+@pytest.mark.parametrize("size", [(70, 16500, 130), (33, 16390, 77), (257, 17000, 300)])
+@pytest.mark.parametrize("shares", [2, 4])
+@pytest.mark.parametrize("shape", range(9))
+def test_every_shape_and_cut_is_the_one_that_is_named(gpu, monkeypatch, shape, shares, size):
+    tokens, columns, channels = size
+    dtype = DTYPES[(shape + 1) % 3]
+    host = inputs(tokens, columns, channels, bias=True, seed=shape)
+    op, results = ha.Int8Matmul(columns, channels, dtype), []
+    for of in (1, shares):
+        monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+        monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(of))
+        assert f" shape={shape} " in op.describe(tokens) and f" shares={of} " in op.describe(tokens)
+        results.append(multiply(op, host, dtype))
+    check(host, dtype, to_f32(results[0], dtype))
+    assert np.array_equal(*results)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_no_cut_of_long_sums_changes_a_bit(gpu, monkeypatch, tokens, dtype):
+    host = inputs(tokens, 16600, 130, bias=True, seed=6)
+    host["x_scales"] *= np.float32(2e-4)   # (results that f16 has too)
+    op = ha.Int8Matmul(16600, 130, dtype)
+    want = multiply(op, host, dtype)
+    assert np.isfinite(to_f32(want, dtype)).all()
+    for shape in range(9):
+        for shares in (1, 2, 4):
+            monkeypatch.setenv("HELIUM_HIP_INT8_SHAPE", str(shape + 1))
+            monkeypatch.setenv("HELIUM_HIP_INT8_SHARES", str(shares))
+            assert f" shape={shape} " in op.describe(tokens) and f" shares={shares} " in op.describe(tokens)
+            assert np.array_equal(multiply(op, host, dtype), want), (shape, shares)
