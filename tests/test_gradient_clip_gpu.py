@@ -1,4 +1,6 @@
 """Gradient clipping through the C ABI on the GPU against the 64-bit oracle, by itself and in a training step."""
+import re
+
 import numpy as np
 import pytest
 
@@ -177,3 +179,17 @@ def test_a_training_step_of_a_normalised_layer(gpu):
     check(["f32", "f32"], gradients, 1.0, [dweight.back(), dgamma.back()])
     want, _ = oracle_muon.step(dweight.back(), momentum, weight, 0.1, 0.9, 0.0, True)
     assert np.allclose(d["weight"].back(), want, atol=1e-5)
+
+
+def test_more_than_the_caches_keep_in_several_groups(gpu):
+    """The first group's first chunks are read past the caches, its others and the second group's are not."""
+    sizes = [830_000 + 7 * k for k in range(128)] + [900_001, 0, 33, 1_000_003, 5] + [50_009] * 60 + [70_001, 1]
+    dtypes = ["bf16"] * 140 + ["f16"] * 53 + ["f32"] * 2
+    clip = ha.GradientClip(sizes, dtypes)
+    (chunks, passing), (_, none) = [(int(a), int(b)) for a, b in re.findall(r"chunks=(\d+) blocks=\d+ first_sum=\d+ passing=(\d+)", clip.description)]
+    assert 0 < passing < chunks and none == 0
+    host, values = inputs(sizes, dtypes, 0.01, seed=13)
+    got, norm = clipped(clip, host, 0.5)
+    check(dtypes, values, 0.5, got, norm)
+    again, same = clipped(clip, host, 0.5, in_place=True)
+    assert same == norm and all(np.array_equal(a, b) for a, b in zip(again, got))

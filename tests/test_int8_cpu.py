@@ -154,3 +154,16 @@ def test_operands_are_checked_before_any_launch():
     with pytest.raises(ha.HeliumError):
         op.describe(0)
     assert _ffi.lib.he_int8_matmul_destroy(None) == _ffi.OK
+
+
+def test_shared_sums_fit_their_scratch():
+    """(2^22 sums of 32 bits: rows of channels in fours, of every share.)"""
+    most = 0
+    for columns in (512, 1000, 4096, 9000, 16384, 131071):
+        for channels in (1, 3, 64, 130, 1001, 1024, 4097, 20000, 1 << 20):
+            op = ha.Int8Matmul(columns, channels, "bf16")
+            for tokens in (1, 2, 7, 16, 33, 64, 65, 100, 127, 200, 255, 333, 511, 777, 1024, 3000, 5000, 20000, 1 << 20):
+                shares = int(re.search(r" shares=(\d+)", op.describe(tokens))[1])
+                if shares > 1:
+                    most = max(most, shares * tokens * -(-channels // 4) * 4)
+    assert 1 << 20 < most <= 1 << 22
