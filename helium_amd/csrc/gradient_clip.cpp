@@ -22,7 +22,7 @@ constexpr size_t kMostTensors = 65536;
 //
 // Bound by memory: everything is read twice and written once. The second launch goes through the chunks in the opposite order, so that it begins with
 // what the first one read last; of more than the Infinity Cache (256 MB) holds, only the last 192 MB are read so that they stay there, and results never are
-// written so. 24 x 4096 x 4096 bf16: squares 125 us (6.5 TB/s), scaling 268 (6.0 TB/s); in the same order 419 us together, without the distinction 408. The
+// written so. 24 x 4096 x 4096 bf16: squares 125 to 135 us (6.0 to 6.5 TB/s), scaling 268 (6.0 TB/s); in the same order 419 us together, without the distinction 408. The
 // 65 tensors (47 MB) of a classifier 26.5 us; with 2048 workgroups 29.7, and results that stay in the caches cost another 1 (40 x 1000 x 1000 bf16: 42.8 and 51.3).
 const char* kText = R"HIP(
 typedef unsigned char u8;

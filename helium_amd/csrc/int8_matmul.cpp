@@ -358,7 +358,8 @@ extern "C" __global__ __launch_bounds__(WAVES_N * WAVES_M * 64) KERNEL_ATTRS voi
 // Streams. Reading the weights once is nearly all there is to do for few tokens, so they go straight into registers, as many loads on their way as
 // there is room for; the tokens come out of the L2. The matrix instructions (16 x 16 x 64) are far from being a bound.
 //
-// One token, 4096 x 4096: 5.5 us (5.7 where the scales are read when the sums are there), 3 of them a launch; 8192 inputs, 16384 channels (134 MB, more than the caches hold with two others) 25 us (5.3 TB/s).
+// One token, 4096 x 4096: 5.4 us (5.7 where the scales are read when the sums are there), 3 of them a launch, and 6.2 with weights that are in no cache; such weights of 8192 inputs and 16384
+// channels (134 MB) 24.6 us (5.5 TB/s), of 28672 channels 40.1 (5.9 TB/s), where the estimate below takes tiles of 64 x 64, in 31.0 and 43.6.
 const char* kStream = R"HIP(
 extern "C" __global__ __launch_bounds__(WAVES * 64) void int8_stream(Call c) {
     __shared__ __attribute__((aligned(16))) int sums[WAVES][BM * 16][BN * 16 + 4];
@@ -453,7 +454,7 @@ constexpr uint64_t kThreads = 1ull << 32;  // a launch has fewer
 constexpr uint64_t kCUs = 256;
 constexpr uint64_t kMostParked = 1 << 22;  // sums of all shares together, for which the scratch has room
 
-// What the choice goes by (cut_of below), from products of 1 to 8192 tokens: microseconds of a call, of a k-tile in a workgroup that has a CU to itself and
+// What the choice goes by (cut_of below), of tiles from products of 33 to 8192 tokens: microseconds of a call, of a k-tile in a workgroup that has a CU to itself and
 // on full CUs, and of beginning and ending a workgroup there. The small tiles, whose waves have few matrix instructions to a k-step, read two steps ahead
 // (1024 x 4096 x 4096 with 128 x 128 22.9 -> 21.2 us); 256 x 256 has no registers for that (61.7, and 63.1 with the spills). Waves of 64 x 32 in a 64 x 128
 // tile 13.95 us with 512 x 4096 x 4096, of 32 x 64 14.7; four stages of 64 x 64 rather than three 9.4 for 10.7 with 128 x 4096 x 4096.
@@ -486,6 +487,18 @@ int64_t parked_pitch(const Int8Problem& pr) { return (int64_t)cut(pr.channels, 4
 
 // How long a call would take, in microseconds. Streams: a CU reads 36 KB in one, of weights and tokens alike, the weights come out of memory at 6 TB/s at
 // best, and a workgroup that follows another on its CU takes a while to begin and end. Shares cost a second launch.
+//
+// Tiles have no such bound by memory here, so that for a token or two of large layers they are taken for faster than they are. In us, weights in no cache, each side's best but
+// for the tiles' shares, which are the chosen ones:
+//   inputs, channels    1 token: tiles, stream    8 tokens: tiles, stream
+//   4096, 14336                  14.2    14.1               14.3    16.3
+//   4096, 28672                  26.8    23.3               27.2    28.4
+//   4096, 128256                 91      87                 95      111
+//   8192, 8192                   18.4    14.0               18.8    16.2
+//   8192, 16384                  31.0    24.6               30.8    29.5
+//   8192, 28672                  43.6    40.1               43.8    49.9
+//   14336, 4096                  15.1    12.9               15.4    15.2
+// (4096 and 4096 are the stream's: 6.2, tiles 8.6.)
 Int8Cut cut_of(const Int8Problem& pr, int64_t tokens, int shape, uint32_t shares) {
     const Int8Shape& t = kShapes[shape];
     Int8Cut c;

@@ -126,7 +126,8 @@ __device__ __forceinline__ void store_padding(u8* row, const Lane& p) {
 // rstd P / 127, alone.
 //
 // Bound by memory: 8192 x 4096 bf16 with a residual 47.1 us (5.7 TB/s, the rate of a copy), into 8 bits 2048 x 4096 10.6 us (5.5 TB/s); f32 residuals beside
-// 16-bit operands, 2000 x 16384, 71 us (5.5 TB/s; 90 with accesses of 16 bytes of the narrower type). One row of 4096: a launch, 2.5 us.
+// 16-bit operands, 2000 x 16384, 71 us (5.5 TB/s; 90 with accesses of 16 bytes of the narrower type). One row of 4096: a launch, 2.5 us. Rows beyond 16384 with an f32 operand do not
+// fit a thread's 128 registers and keep some 400 bytes of theirs in scratch memory: 1000 x 32768 f32 354 us, with a residual 441 (46 and 92 at the rate of a copy).
 //
 // A sum of squares that f32 cannot hold (from values of some 1e17 on in long rows, of 1.8e19 in any; without an epsilon to speak of, of values below 1e-15) is taken
 // again of the values times a power of two; other rows' results are as they would be without it.
@@ -336,7 +337,8 @@ extern "C" __global__ __launch_bounds__(T) void rows_quantize(u64 rows, const el
 // `blocks` apart and keeps its share of dgamma in registers; `rows_fold` adds up the workgroups' shares. The order is fixed.
 //
 // Bound by memory: 8192 x 4096 bf16 with the residual's gradient 50.8 us with the fold (5.3 TB/s); with the next row's loads under conditions, or with
-// gamma's loads in between, 57 to 60: the counter of loads then runs to zero before each row.
+// gamma's loads in between, 57 to 60: the counter of loads then runs to zero before each row. Rows of 1024 threads, which are not asked for ahead: 4096 x 5120 bf16 beside an f32
+// stream 69.6 us (59 at the rate of a copy), 4096 x 8192 102 (94), 1500 x 16384 bf16 52.5 (34.5); 1000 x 32768 f32, whose values do not fit the registers either, 236 (92).
 const char* kBackward = R"HIP(
 template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 blocks, const elem_t* dy, const stream_t* h, const param_t* __restrict__ gamma,
                                                              const float* __restrict__ rstd_of, const stream_t* dh, elem_t* dx, stream_t* dresidual,
@@ -349,7 +351,8 @@ template <bool MORE> __device__ __forceinline__ void backward(u64 rows, u32 bloc
     for (int k = 0; k < NV; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) share[k][i] = 0.0f;
-    // A row's operands are asked for while the row before is worked on, where a thread has the registers (1024 threads have 128 each). The loads are
+    // A row's operands are asked for while the row before is worked on, but for rows of 1024 threads: those have 128 registers each, which is too few for the widest rows (with
+    // the prefetch, 16384 bf16 with dh and 16384 f32 spill; 8192 beside an f32 stream would fit in 100, and are not told apart). The loads are
     // the same for every thread and row, from the last one's place where there is none: loads under a condition would be waited for at once.
     struct Row { elem_v dy[NV]; stream_v h[NV], dh[NV]; float rstd; } next;
     auto load = [&](Row& r, u64 row) {
@@ -450,7 +453,8 @@ BACKWARD(rows_backward, false)
 BACKWARD(rows_backward_more, true)   // with what reaches h from elsewhere
 #endif
 
-// dgamma[c] = the sum of `count` shares: 16 columns to a workgroup, the shares dealt to its 64 rows of threads.
+// dgamma[c] = the sum of `count` shares: 16 columns to a workgroup, the shares dealt to its 64 rows of threads. 256 shares of 4096 columns 4.7 us; 16 columns are half a line of 128
+// bytes, and the workgroups that have its halves run on different XCDs: 8.4 MB are fetched of 4.2.
 extern "C" __global__ __launch_bounds__(1024) void rows_fold(const float* __restrict__ parts, u32 count, float* __restrict__ dgamma) {
     __shared__ float part[16][16];
     const u32 column = threadIdx.x & 15u, row = threadIdx.x >> 4, c = blockIdx.x * 16 + column;

@@ -571,8 +571,8 @@ int he_quantize_rows_destroy(he_quantize_rows_t quantize);
 typedef struct he_int8_matmul_s* he_int8_matmul_t;
 /* y[t][n] = x_scales[t] * weight_scales[n] * (sum over k of x[t][k] weights[n][k]) + bias[n]: x and weights are quantised matrices of `inputs`
  * columns (fewer than 2^17), weights with a row for each of `channels` (at most 2^24); how many tokens there are is each call's. Sums are exact, in
- * 32-bit whole numbers; y is row-major and packed, of dtype (HE_F32, HE_BF16 or HE_F16), rounded once from f32. Compiles the kernels; needs no
- * device. */
+ * 32-bit whole numbers; y is row-major and packed, of dtype (HE_F32, HE_BF16 or HE_F16), rounded once from f32: the sum times x_scales[t], which has to
+ * be in f32's range, times weight_scales[n], plus bias[n]. Compiles the kernels; needs no device. */
 int he_int8_matmul_create(he_int8_matmul_t* matmul, int64_t inputs, int64_t channels, int dtype);
 /* x and weights are aligned to 16 bytes, everything else to its own type; bias may be NULL; y shares no memory with the operands. At most 2^24
  * tokens; there may be none. The first call on a stream that shares out its sums (he_int8_matmul_describe says which do) allocates 16 MB for it, which all
